@@ -856,6 +856,96 @@ int mnx_channel_outer_stack_f32(const float* y, const float* const* s, int32_t L
 int mnx_channel_outer_stack_bwd_f32(const float* grad, const float* y, const float* const* s, int32_t L, int64_t E,
                                     int32_t F, float* grad_y, float* const* grad_s, mnx_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Training step: layer norm (forward, backward, second order) and AdamW.    */
+/* The reference takes both from torch (nn.LayerNorm between MACE's           */
+/* interactions, src/molzoo/mace.py:487-544; optimizer.step() of its trainer, */
+/* src/molix/core/steps/train_step.py:86).                                     */
+/* Element types of tensors that need not be float32:                         */
+#define MNX_F32 0
+#define MNX_BF16 1
+#define MNX_F16 2
+/* ------------------------------------------------------------------------ */
+/* Layer norm over the last axis of rows x width values, rows ldx (ldg, ldu)  */
+/* elements apart, unit stride within a row; outputs are contiguous.  dtype   */
+/* is the type of every rows x width array, wdtype that of the vectors of     */
+/* width values; sums are in float32.  weight and bias may be NULL (1 and 0). */
+/*   y = (x - mean) rstd weight + bias,  rstd = 1 / sqrt(var + eps)            */
+/* stats [2][rows] float32: mean, rstd, as the backward reads them.           */
+/* bwd: NULL outputs are skipped.  bwd2: the derivatives of                    */
+/* <seed_x, grad_x> + <seed_w, grad_weight> + <seed_b, grad_bias> with respect */
+/* to grad, x and weight (NULL dweight is skipped; seed_w and seed_b may be    */
+/* NULL).  Both sum over the rows in a fixed order.                            */
+/* 1 <= width <= MNX_LAYER_NORM_MAX_WIDTH; rows = 0 gives zero sums.           */
+/* ------------------------------------------------------------------------ */
+#define MNX_LAYER_NORM_MAX_WIDTH (1 << 24)
+int mnx_layer_norm_fwd(const void* x, int64_t ldx, int64_t rows, int64_t width, const void* weight,
+                       const void* bias, double eps, int32_t dtype, int32_t wdtype, void* y, float* stats,
+                       mnx_stream_t stream);
+size_t mnx_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width);
+int mnx_layer_norm_bwd(const void* grad, int64_t ldg, const void* x, int64_t ldx, int64_t rows, int64_t width,
+                       const void* weight, int32_t dtype, int32_t wdtype, const float* stats, void* grad_x,
+                       void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                       mnx_stream_t stream);
+int mnx_layer_norm_bwd2(const void* grad, int64_t ldg, const void* x, int64_t ldx, const void* seed_x, int64_t ldu,
+                        const void* seed_w, const void* seed_b, int64_t rows, int64_t width, const void* weight,
+                        int32_t dtype, int32_t wdtype, const float* stats, void* dgrad, void* dx, void* dweight,
+                        void* workspace, size_t workspace_bytes, mnx_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* 2-norm of `count` tensors together (float32 on the device; squares summed  */
+/* in float64, fixed order).  Arrays of tensors are host arrays of `count`    */
+/* entries; numel may be 0 (its pointer is then not read).                     */
+/* ------------------------------------------------------------------------ */
+#define MNX_OPTIM_MAX_ELEMENTS ((int64_t)1 << 36) /* of one tensor */
+size_t mnx_grad_norm_workspace_bytes(const int64_t* numel, int64_t count);
+int mnx_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtype, int64_t count, float* norm,
+                  void* workspace, size_t workspace_bytes, mnx_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* One AdamW step over `count` tensors (decoupled weight decay):               */
+/*   g = s grad, s = min(1, max_norm / (norm + 1e-6)), negative to maximise    */
+/*   step += 1;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2   */
+/*   p = p (1 - lr weight_decay)                                               */
+/*       - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)    */
+/* Parameters and gradients of one tensor share its dtype; all arithmetic is   */
+/* float32.  state_bits 32: exp_avgs and exp_avg_sqs point to float32.         */
+/* state_bits 8: they point to one byte an element, and bases to an int16 pair */
+/* (first, second moment) per 256 elements.  A code c stands for the float32   */
+/* with the bits (base + c) << 20, 0 for c = 0; a first moment's top bit is    */
+/* the sign (0x80: NaN).  Codes are rounded with a dither hashed from seed,    */
+/* the tensor's number, its step and the element's number.                     */
+/* max_norm < 0: no clipping.  norm_in (device) is the norm to clip by, NULL:  */
+/* that of grads.  norm_out (device, or NULL) receives it.  skip_nonfinite: a  */
+/* norm that is not finite leaves everything as it is.  lr_device (or NULL)    */
+/* holds the learning rate in place of lr.                                      */
+/* ------------------------------------------------------------------------ */
+typedef struct mnx_adamw_args {
+    int64_t count;
+    void* const* params;
+    const void* const* grads;
+    void* const* exp_avgs;
+    void* const* exp_avg_sqs;
+    int16_t* const* bases;
+    float* const* steps; /* device, one value each */
+    const int64_t* numel;
+    const int32_t* dtype;
+    int32_t state_bits, maximize, skip_nonfinite;
+    uint32_t seed;
+    double lr, beta1, beta2, eps, weight_decay, max_norm;
+    const float* lr_device;
+    const float* norm_in;
+    float* norm_out;
+    void* workspace;
+    size_t workspace_bytes;
+} mnx_adamw_args;
+size_t mnx_adamw_workspace_bytes(const int64_t* numel, int64_t count);
+int mnx_adamw_step(const mnx_adamw_args* args, mnx_stream_t stream);
+/* The moments that 8-bit states stand for, in float32. */
+int mnx_adamw8_moments(const void* const* exp_avgs, const void* const* exp_avg_sqs, int16_t* const* bases,
+                       const int64_t* numel, int64_t count, float* const* out_avgs, float* const* out_avg_sqs,
+                       mnx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

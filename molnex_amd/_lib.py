@@ -152,6 +152,17 @@ SIGNATURES = {
     "mnx_edge_tp_proj_fwd_f32": (C.c_int, [c_i32, vp, c_i32, vp, vp, vp, vp, vp, c_i64, vp, vp]),
     "mnx_edge_tp_proj_bwd_f32": (C.c_int, [c_i32, vp, c_i32, vp, vp, vp, vp, vp, vp, c_i64, vp, vp, vp, vp, vp, vp,
                                            c_sz, vp]),
+    "mnx_layer_norm_fwd": (C.c_int, [vp, c_i64, c_i64, c_i64, vp, vp, c_f64, c_i32, c_i32, vp, vp, vp]),
+    "mnx_layer_norm_bwd_workspace_bytes": (c_sz, [c_i64, c_i64]),
+    "mnx_layer_norm_bwd": (C.c_int, [vp, c_i64, vp, c_i64, c_i64, c_i64, vp, c_i32, c_i32, vp, vp, vp, vp, vp, c_sz,
+                                     vp]),
+    "mnx_layer_norm_bwd2": (C.c_int, [vp, c_i64, vp, c_i64, vp, c_i64, vp, vp, c_i64, c_i64, vp, c_i32, c_i32, vp, vp,
+                                      vp, vp, vp, c_sz, vp]),
+    "mnx_grad_norm_workspace_bytes": (c_sz, [vp, c_i64]),
+    "mnx_grad_norm": (C.c_int, [vp, vp, vp, c_i64, vp, vp, c_sz, vp]),
+    "mnx_adamw_workspace_bytes": (c_sz, [vp, c_i64]),
+    "mnx_adamw_step": (C.c_int, [vp, vp]),
+    "mnx_adamw8_moments": (C.c_int, [vp, vp, vp, vp, c_i64, vp, vp, vp]),
 }
 
 

@@ -30,6 +30,7 @@ Ops
 ``molix::pme_energy``           PME energy of a periodic system: real-space, reciprocal and self terms in one op each way
 ``molix::pair_features``        radial features, both atoms' type embeddings and the envelope of each edge (Allegro)
 ``molix::residual_blocks``      weight blocks of a residual linear layer (Allegro's layer tail)
+``molix::layer_norm``           layer norm over the last axis, with its backward and second-order ops (``training.py``)
 ``molix::segment_sum``          weighted segment sum of rows by segment id (scatter_sum / MessageAggregation)
 """
 
@@ -3124,3 +3125,5 @@ segment_sum.register_autograd(_seg_backward, setup_context=_seg_setup)
 
 # second-order formulas (autograd of the backward ops): registered on import, after every op above
 from . import second_order  # noqa: E402,F401
+# layer norm and AdamW
+from . import training  # noqa: E402,F401

@@ -1,0 +1,40 @@
+"""Layer norm with the signature of ``torch.nn.functional.layer_norm``, by the ``molix::layer_norm`` kernels."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+from torch import Tensor, ops
+
+from ...training import DTYPES, LAYER_NORM_MAX_WIDTH
+
+
+def layer_norm(input: Tensor, normalized_shape, weight: Tensor | None = None, bias: Tensor | None = None,
+               eps: float = 1e-5) -> Tensor:
+    """Norm over the trailing axes ``normalized_shape``, in float32 whatever the type, with derivatives of any order.
+
+    The kernels take float32, bfloat16 and float16 with weights of that type or float32; other types (float64
+    models) go to torch.  Under autocast it computes and returns float32, as torch's does.  GPU tensors only."""
+    if input.device.type != "cuda":
+        raise RuntimeError(f"layer_norm runs on the GPU only (got a {input.device} tensor)")
+    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
+    lead = input.dim() - len(shape)
+    if not shape or lead < 0 or tuple(input.shape[lead:]) != shape:
+        raise ValueError(f"layer_norm: input of shape {tuple(input.shape)} does not end in {shape}")
+    for t in (weight, bias):
+        if t is not None and tuple(t.shape) != shape:
+            raise ValueError(f"layer_norm: weight and bias must be {shape}, got {tuple(t.shape)}")
+    if torch.is_autocast_enabled("cuda") and input.dtype in DTYPES:
+        input = input.float()
+        weight, bias = (t.float() if t is not None and t.dtype in DTYPES else t for t in (weight, bias))
+    types = {t.dtype for t in (weight, bias) if t is not None}
+    width = math.prod(shape)
+    if (input.dtype not in DTYPES or len(types) > 1 or not types <= {input.dtype, torch.float32}
+            or not 1 <= width <= LAYER_NORM_MAX_WIDTH):
+        return torch.nn.functional.layer_norm(input, shape, weight, bias, eps)
+    if len(shape) == 1:
+        return ops.molix.layer_norm(input, weight, bias, float(eps))[0]
+    flat = [t if t is None else t.reshape(width) for t in (weight, bias)]
+    y = ops.molix.layer_norm(input.reshape(*input.shape[:lead], width), *flat, float(eps))[0]
+    return y.reshape(input.shape)

@@ -1,3 +1,4 @@
 from .locality import NeighborList
+from .norm import LayerNorm
 
-__all__ = ["NeighborList"]
+__all__ = ["NeighborList", "LayerNorm"]

@@ -25,6 +25,7 @@ from pydantic import BaseModel, ConfigDict, Field
 
 from ..config import config
 from ..irreps import Irreps
+from ..molix.nn.norm import LayerNorm
 from ..molrep.embedding.angular import SphericalHarmonics
 from ..molrep.embedding.cutoff import CosineCutoff, PolynomialCutoff
 from ..molrep.embedding.node import ContinuousEmbeddingSpec, DiscreteEmbeddingSpec, JointEmbedding
@@ -169,7 +170,7 @@ class MACE(nn.Module):
             ElementUpdate(hidden_dim=irreps_dim, num_species=num_elements)
             for _ in range(max(num_interactions - 1, 0))])
         self.layer_norms = nn.ModuleList([
-            nn.LayerNorm(irreps_dim) if layer_norm else nn.Identity() for _ in range(max(num_interactions - 1, 0))])
+            LayerNorm(irreps_dim) if layer_norm else nn.Identity() for _ in range(max(num_interactions - 1, 0))])
 
     def _build_literal(self, F, S, num_bessel, l_max, L, correlation, avg_num_neighbors, hidden_irreps):
         hidden = Irreps(hidden_irreps)

@@ -1,0 +1,575 @@
+"""The AdamW step over many tensors (molix.F.adamw_step, adamw8_step) and the gradients' norm, against the formula in
+float64, and the optimizer class against torch.optim.AdamW.
+
+Tolerances, u = 2^-24.  m = b1 m + (1 - b1) g: three roundings and the rounded constants, of terms |b1 m| and
+|(1 - b1) g s|: 4 u of their magnitudes, and 2 u more for a clip factor s; v likewise with g^2, 6 u and 4 u more.
+p: p (1 - lr wd) is off by 2 u |p|; the update lr/(1 - b1^t) m / (sqrt(v)/sqrt(1 - b2^t) + eps) by 16 u of
+itself with m's magnitudes in the place of |m| (a square root, a reciprocal and a division of 1 unit or so each, half
+of v's error, three rounded constants); one rounding of the result.  Parameters of 16 bits add half a unit of their
+last place, eps / 2.
+8-bit codes: the float64 value is compared with the code's, and may differ by one code only where the dither's
+threshold is met within 1e-4 of a step (a float32 moment is within 2^-20 of a step of its float64 value).
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from molnex_amd.molix import F
+from molnex_amd.molix.optim import AdamW
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+HALF = {torch.float32: 0.0, torch.bfloat16: torch.finfo(torch.bfloat16).eps / 2, torch.float16: torch.finfo(torch.float16).eps / 2}
+H = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.05)
+B = 256
+
+
+def make(sizes, dtype=torch.float32, seed=0, bits=32, scale=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    rnd = lambda n: torch.randn(n, generator=g, device=DEV)  # noqa: E731
+    dts = dtype if isinstance(dtype, list) else [dtype] * len(sizes)
+    p = [rnd(n).to(d) for n, d in zip(sizes, dts)]
+    gr = [(scale * rnd(n) * torch.exp(rnd(n))).to(d) for n, d in zip(sizes, dts)]
+    steps = [torch.tensor(float(3 * i % 50), device=DEV) for i in range(len(sizes))]
+    if bits == 32:
+        return p, gr, [0.3 * rnd(n) for n in sizes], [rnd(n) ** 2 for n in sizes], steps
+    rng = np.random.default_rng(seed)
+    codes = lambda n: torch.from_numpy(rng.integers(0, 256, n, dtype=np.uint8)).to(DEV)  # noqa: E731
+    m, v = [codes(n) for n in sizes], [codes(n) for n in sizes]
+    for t in m:
+        t[t == 128] = 0  # NaN
+    # exponents around 2^-10 and 2^-14, so that steps of the moments and of the gradients are of a size
+    bases = [torch.from_numpy(np.stack([rng.integers(117 * 8, 119 * 8, -(-n // B)) - 127,
+                                        rng.integers(113 * 8, 115 * 8, -(-n // B)) - 255], 1).astype(np.int16)).to(DEV)
+             for n in sizes]
+    return p, gr, m, v, bases, steps
+
+
+def reference(p, g, m, v, t, h, factor=1.0, clipped=False, maximize=False):
+    """(p, m, v) after the step in float64, and the bounds of their errors."""
+    b1, b2 = h["betas"]
+    p, g, m, v = (x.double() for x in (p, g, m, v))
+    g = g * factor * (-1 if maximize else 1)
+    more = 2 if clipped else 0
+    new_m, mags = b1 * m + (1 - b1) * g, b1 * m.abs() + (1 - b1) * g.abs()
+    new_v = b2 * v + (1 - b2) * g * g
+    denom = (new_v / (1 - b2 ** t)).sqrt() + h["eps"]
+    size = h["lr"] / (1 - b1 ** t)
+    new_p = p * (1 - h["lr"] * h["weight_decay"]) - size * new_m / denom
+    bound_p = 3 * U * p.abs() + (20 + more) * U * size * mags / denom + U * new_p.abs()
+    return (new_p, bound_p), (new_m, (4 + more) * U * mags), (new_v, (6 + 2 * more) * U * new_v)
+
+
+def close(got, ref, bound, half=0.0):
+    tiny = 2.0 ** -149 if half == 0 else 2.0 ** -25
+    err, limit = (got.double() - ref).abs(), bound + half * ref.abs() + tiny
+    assert bool((err <= limit).all()), float((err / limit).max())
+
+
+def run_32(data, **kw):
+    p, g, m, v, s = ([t.clone() for t in ts] for ts in data)
+    norm = F.adamw_step(p, g, m, v, s, **{**H, **kw})
+    for a, b in zip(g, data[1]):
+        assert torch.equal(a.nan_to_num(), b.nan_to_num())  # clipping does not rewrite them
+    return norm, p, m, v, s
+
+
+def check_32(data, norm=None, max_norm=None, maximize=False, **kw):
+    got, p, m, v, s = run_32(data, max_norm=max_norm, maximize=maximize, **kw)
+    true = math.sqrt(sum(float(t.double().pow(2).sum()) for t in data[1]))
+    factor = 1.0 if max_norm is None else min(1.0, max_norm / (true + 1e-6))
+    if max_norm is not None:
+        assert got.shape == () and abs(float(got) - true) <= 2 * U * true
+    for i in range(len(p)):
+        t = float(data[4][i]) + 1
+        assert float(s[i]) == t
+        (rp, bp), (rm, bm), (rv, bv) = reference(data[0][i], data[1][i], data[2][i], data[3][i], t, {**H, **kw}, factor,
+                                                 max_norm is not None, maximize)
+        close(p[i], rp, bp, HALF[p[i].dtype])
+        close(m[i], rm, bm)
+        close(v[i], rv, bv)
+
+
+SIZES = [[1], [5], [256], [257], [8191, 8192, 8193], [3, 0, 70_001, 1, 4096], [16_385, 2, 100_000]]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_step(sizes, dtype):
+    check_32(make(sizes, dtype))
+    check_32(make(sizes, dtype, 1), max_norm=0.5)
+
+
+def test_many_tensors():
+    """More tensors than a launch takes, of mixed types."""
+    dts = [torch.float32, torch.bfloat16, torch.float16]
+    n = 1100
+    data = make([1 + (37 * i) % 700 for i in range(n)], [dts[i % 3] for i in range(n)])
+    check_32(data, max_norm=1.0)
+    check_32(data)
+
+
+@pytest.mark.parametrize("kw", [dict(maximize=True), dict(weight_decay=0.0), dict(betas=(0.0, 0.0)), dict(eps=1e-3),
+                                dict(max_norm=1e9), dict(max_norm=0.0), dict(lr=0.0)])
+def test_options(kw):
+    check_32(make([300, 17, 5000]), **kw)
+
+
+def test_zero_gradients_decay_only():
+    p, g, m, v, s = make([1000])
+    z = [torch.zeros(1000, device=DEV)]
+    _, pn, mn, vn, _ = run_32((p, z, z, z, s), max_norm=1.0)
+    assert torch.equal(pn[0], p[0] * torch.tensor(1 - H["lr"] * H["weight_decay"], device=DEV))
+    assert torch.equal(mn[0], z[0]) and torch.equal(vn[0], z[0])
+
+
+def test_learning_rate_on_the_device():
+    data = make([500, 77])
+    a, b = run_32(data), run_32(data, lr=torch.tensor(H["lr"], device=DEV, dtype=torch.float64))
+    for x, y in zip(a[1], b[1]):
+        assert float((x - y).abs().max()) <= 8 * U * float(x.abs().max())  # lr rounded to float32
+    c = run_32(data, lr=torch.tensor(H["lr"], dtype=torch.float64))
+    assert all(torch.equal(x, y) for x, y in zip(a[1], c[1]))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_gradients_that_are_not_finite(bad):
+    data = make([3000, 40, 9000])
+    data[1][2][1234] = bad
+    norm, p, m, v, s = run_32(data, skip_nonfinite=True, max_norm=1.0)
+    assert not math.isfinite(float(norm))
+    for got, old in zip((p, m, v, s), (data[0], data[2], data[3], data[4])):
+        assert all(torch.equal(a, b) for a, b in zip(got, old))
+    _, p, m, v, s = run_32(data)  # without either, that element alone
+    _, pc, mc, vc, _ = run_32((data[0], [t.nan_to_num(0, 0, 0) for t in data[1]], *data[2:]))
+    assert bool(p[2][1234].isnan()) and not bool(m[2][1234].isfinite())
+    for a, b in ((p, pc), (m, mc), (v, vc)):
+        a[2][1234] = b[2][1234] = 0
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    _, p, *_ = run_32(data, max_norm=1.0)  # clipped by it, as clip_grad_norm_ does
+    assert bool(p[0].isnan().any()) == math.isnan(bad)
+    ok, pf, *_ = run_32(make([3000]), skip_nonfinite=True)
+    assert math.isfinite(float(ok)) and not torch.equal(pf[0], make([3000])[0][0])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_unaligned_and_permuted_tensors(bits):
+    """Views at odd offsets, and parameters whose memory order is not row by row, step as their copies do."""
+    n = 60 * 70
+    p, g, m, v, *rest = make([n, n], bits=bits)
+    shift = lambda t: torch.cat([t.new_zeros(1), t])[1:]  # noqa: E731
+    a = [[shift(t) for t in ts] for ts in (p, g, m, v)]
+    step = F.adamw_step if bits == 32 else F.adamw8_step
+    rest_a, rest_b = ([[t.clone() for t in ts] for ts in rest] for _ in range(2))
+    b = [[t.clone() for t in ts] for ts in (p, g, m, v)]
+    step(*a, *rest_a, **H)
+    step(*b, *rest_b, **H)
+    for x, y in zip(a[0] + a[2] + a[3], b[0] + b[2] + b[3]):
+        assert torch.equal(x, y)
+    # the same memory seen as a transposed matrix; the gradient row by row, so it has to be laid out
+    c = [[t.clone().view(70, 60).t() for t in ts] for ts in (p, g, m, v)]
+    c[1] = [t.contiguous() for t in c[1]]
+    step(*c, *[[t.clone() for t in ts] for ts in rest], **H)
+    for x, y in zip(c[0] + c[2] + c[3], b[0] + b[2] + b[3]):
+        assert torch.equal(x.t().reshape(-1), y)
+    # a parameter with gaps
+    gap = torch.zeros(n, 2, device=DEV)[:, 0]
+    gap.copy_(p[0])
+    d = [[gap], [g[0].clone()], [m[0].clone()], [v[0].clone()]]
+    step(*d, *[[ts[0].clone()] for ts in rest], **H)
+    assert torch.equal(gap, b[0][0])
+
+
+def test_norm():
+    for data in (make([1]), make([5, 70_000, 0, 3], [torch.float32, torch.bfloat16, torch.float16, torch.float32]),
+                 make([100 + i for i in range(400)])):
+        ref = math.sqrt(sum(float(t.double().pow(2).sum()) for t in data[1]))
+        assert abs(float(F.grad_norm(data[1])) - ref) <= 2 * U * ref
+        assert torch.equal(F.grad_norm(data[1]), F.grad_norm(data[1]))
+    big = [torch.full((1000,), 1e25, device=DEV)]  # squares beyond float32
+    assert abs(float(F.grad_norm(big)) / (1e25 * 1000 ** 0.5) - 1) <= 4 * U
+    assert float(F.grad_norm([])) == 0
+    w = torch.randn(50, 60, device=DEV)
+    for t in (w.t(), w[::2, ::3]):
+        ref = float(t.double().norm())
+        assert abs(float(F.grad_norm([t])) - ref) <= 2 * U * ref
+
+
+def test_large_tensor():
+    """One tensor of more than 2^31 elements: its first and last elements."""
+    n = (1 << 31) + 4099
+    p, g = torch.zeros(n, device=DEV, dtype=torch.bfloat16), torch.zeros(n, device=DEV, dtype=torch.bfloat16)
+    m, v = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+    ends = [slice(0, 5000), slice(n - 5000, n)]
+    data = make([5000, 5000], torch.bfloat16)
+    for e, a, b, c, d in zip(ends, *data[:4]):
+        p[e], g[e], m[e], v[e] = a, b, c, d
+    s = [torch.tensor(4.0, device=DEV)]
+    norm = F.adamw_step([p], [g], [m], [v], s, max_norm=1.0, **H)
+    true = math.sqrt(sum(float(t.double().pow(2).sum()) for t in data[1]))
+    assert abs(float(norm) - true) <= 2 * U * true
+    for k, e in enumerate(ends):
+        (rp, bp), (rm, bm), (rv, bv) = reference(*(data[i][k] for i in range(4)), 5.0, H, min(1, 1 / (true + 1e-6)), True)
+        close(p[e], rp, bp, HALF[torch.bfloat16])
+        close(m[e], rm, bm)
+        close(v[e], rv, bv)
+    assert float(p[5000:n - 5000:1017].abs().max()) == 0
+
+
+# ---------------------------------------------------------------------------
+# 8-bit states
+# ---------------------------------------------------------------------------
+
+
+def value(k):
+    octave = np.maximum(k >> 3, 1)
+    return np.ldexp((k - 8 * (octave - 1)) / 8.0, octave - 127)
+
+
+def decode(codes, bases, signed):
+    c = codes.cpu().numpy().astype(np.int64)
+    base = np.repeat(bases.cpu().numpy().astype(np.int64), B)[:len(c)]
+    size = c & 127 if signed else c
+    got = np.where(size > 0, value(base + size), 0.0)
+    if signed:
+        got = np.where(c == 128, np.nan, np.where(c > 127, -got, got))
+    return torch.from_numpy(got).to(DEV)
+
+
+def mix(x):
+    x = np.asarray(x, dtype=np.uint64) & np.uint64(0xFFFFFFFF)
+    for shift, factor in ((15, 0x6A09E667), (13, 0xBB67AE85)):
+        x = ((x ^ (x >> np.uint64(shift))) * np.uint64(factor)) & np.uint64(0xFFFFFFFF)
+    return x ^ (x >> np.uint64(16))
+
+
+def dither(seed, number, step, index):
+    key = mix(mix([(seed * 0x3C6EF373 + number * 0xA54FF53B) & 0xFFFFFFFF]) + np.uint64(step * 0x510E527F & 0xFFFFFFFF))
+    h = mix(key + ((np.asarray(index, dtype=np.uint64) & np.uint64(0xFFFFFFFF)) * np.uint64(0x9E3779B1) & np.uint64(0xFFFFFFFF)))
+    return (h & np.uint64(0xFFFF)).astype(np.float64), (h >> np.uint64(16)).astype(np.float64)
+
+
+def check_codes(codes, base, x, draw, most, up):
+    """codes and base (numpy) of one tensor against the float64 moments x."""
+    pad = lambda a: np.pad(a, (0, -len(a) % B)).reshape(-1, B)  # noqa: E731
+    z, chance = pad(np.abs(x)), (pad(draw) + 0.5) / 65536
+    part, e = np.frexp(z.astype(np.float32).astype(np.float64))
+    key = lambda part, e: np.where(part > 0, np.floor((2 * part - 1) * 8) + 8 * (e + 126), 0).astype(np.int64)  # noqa: E731
+    base = base.astype(np.int64)[:, None]
+    want = np.maximum(key(part, e).max(1, keepdims=True) + 1 - most, 0)
+    assert np.abs(base - want).max() <= 1 and (base != want).mean() <= 1e-3
+    k = np.maximum(key(*np.frexp(z)), base)
+    low = np.where(k > base, value(k), 0.0)
+    share = (z - low) / (value(k + 1) - low)
+    if up:
+        lifted, edge = np.where(k > base, share >= 1 - chance, z > 0), np.where(k > base, np.abs(share - 1 + chance), 1)
+    else:
+        lifted = np.where(k > base, share >= 1 - chance, share > chance)
+        edge = np.where(k > base, np.abs(share - 1 + chance), np.abs(share - chance))
+    code = np.where(lifted, k + 1, np.where(k > base, k, base)) - base
+    off = pad(codes.astype(np.int64) & 127 if not up else codes.astype(np.int64)) - np.where(z > 0, code, 0)
+    assert np.abs(off).max() <= 1 and np.all((off == 0) | (edge < 1e-4) | (share < 1e-4) | (share > 1 - 1e-4))
+    assert (off != 0).mean() <= 1e-3
+    return z
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sizes", [[1], [255, 256, 257], [3, 0, 70_001, 1, 4096], [100_000]])
+def test_8bit_step(sizes, dtype):
+    p, g, m, v, bases, steps = make(sizes, dtype, bits=8, scale=1e-2)
+    new = [[t.clone() for t in ts] for ts in (p, g, m, v, bases, steps)]
+    clip = dtype == torch.float16
+    norm = F.adamw8_step(*new, seed=12345, max_norm=0.05 if clip else None, **H)
+    factor = min(1.0, 0.05 / (float(norm) + 1e-6)) if clip else 1.0
+    back = F.adamw8_moments(*new[2:5])
+    for i, n in enumerate(sizes):
+        t = float(steps[i]) + 1
+        assert float(new[5][i]) == t
+        if not n:
+            continue
+        old_m, old_v = decode(m[i], bases[i][:, 0], True), decode(v[i], bases[i][:, 1], False)
+        (rp, bp), (rm, bm), (rv, bv) = reference(p[i], g[i], old_m, old_v, t, H, factor, clip)
+        close(new[0][i], rp, bp, HALF[dtype])
+        dm, dv = dither(12345, i, int(t), np.arange(n))
+        b = new[4][i].cpu().numpy()
+        z = check_codes(new[2][i].cpu().numpy(), b[:, 0], rm.cpu().numpy(), dm, 127, False)
+        signs = np.sign(back[0][i].cpu().numpy())
+        assert np.all((signs == 0) | (signs == np.sign(rm.cpu().numpy()))) and z.shape
+        check_codes(new[3][i].cpu().numpy(), b[:, 1], rv.cpu().numpy(), dv, 255, True)
+        for got, codes, col in ((back[0][i], new[2][i], 0), (back[1][i], new[3][i], 1)):
+            assert torch.equal(got.double(), decode(codes, new[4][i][:, col], col == 0))
+
+
+def test_8bit_first_step_and_zero_blocks():
+    """From zero states: blocks without gradients stay zero, and no zero second moment meets a first one."""
+    n = 4 * B
+    p, g = torch.randn(n, device=DEV), torch.randn(n, device=DEV)
+    g[B:2 * B] = 0
+    g[2 * B:3 * B] *= 10.0 ** torch.linspace(-18, 0, B, device=DEV)
+    state = [torch.zeros(n, dtype=torch.uint8, device=DEV), torch.zeros(n, dtype=torch.uint8, device=DEV),
+             torch.zeros(4, 2, dtype=torch.int16, device=DEV), torch.zeros((), device=DEV)]
+    old = p.clone()
+    for _ in range(3):
+        F.adamw8_step([p], [g], *[[t] for t in state], lr=1e-3, weight_decay=0.0)
+        m, v = (t[0] for t in F.adamw8_moments(*[[t] for t in state[:3]]))
+        assert float(m[B:2 * B].abs().max()) == float(v[B:2 * B].abs().max()) == 0
+        assert bool((v[(g * g) > 1e-44] > 0).all())
+    assert torch.equal(p[B:2 * B], old[B:2 * B])
+    # steps of a constant gradient are lr each; v's code may be 12.5 % off and m's 12.5 %, from the second step on
+    assert float((p - old).abs().max()) <= 3 * 1e-3 * 1.3
+
+
+def test_8bit_moments_are_unbiased():
+    """2000 steps with fresh gradients: the mean of v over the elements stays that of a float32 v.  Dithering leaves v
+    with a relative deviation of about sqrt(0.125 / 2) = 25 %, over 16384 elements 0.2 % of their mean; 2 % is ten
+    times that.  m's mean square exceeds the float32 one's by its rounding noise, at most (0.125^2 / 6) / (1 - 0.81)
+    = 1.4 % of itself: within 5 %."""
+    n, steps = 16384, 2000
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    scale = torch.exp(torch.randn(n, generator=gen, device=DEV))
+    p8, p32 = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+    s8 = [torch.zeros(n, dtype=torch.uint8, device=DEV), torch.zeros(n, dtype=torch.uint8, device=DEV),
+          torch.zeros(n // B, 2, dtype=torch.int16, device=DEV), torch.zeros((), device=DEV)]
+    s32 = [torch.zeros(n, device=DEV), torch.zeros(n, device=DEV), torch.zeros((), device=DEV)]
+    for k in range(steps):
+        g = scale * torch.randn(n, generator=gen, device=DEV)
+        F.adamw8_step([p8], [g], *[[t] for t in s8], lr=1e-3, seed=1)
+        F.adamw_step([p32], [g], *[[t] for t in s32], lr=1e-3)
+    m, v = (t[0] for t in F.adamw8_moments(*[[t] for t in s8[:3]]))
+    assert abs(float((v / s32[1]).mean()) - 1) <= 0.02
+    ratio = float((m / scale).square().mean() / (s32[0] / scale).square().mean())
+    assert abs(ratio - 1) <= 0.05
+
+
+def test_8bit_gradient_that_is_not_finite():
+    """Its element becomes NaN; the block's others keep sound moments."""
+    n = 2 * B
+    p, g, m, v, bases, steps = make([n], bits=8, scale=1e-2)
+    clean = [[t.clone() for t in ts] for ts in (p, g, m, v, bases, steps)]
+    bad = [[t.clone() for t in ts] for ts in (p, g, m, v, bases, steps)]
+    for at, what in ((3, float("nan")), (100, float("inf")), (300, 3e25)):  # the last: its square overflows
+        bad[1][0][at] = what
+        clean[1][0][at] = 0
+    for s in (clean, bad):
+        F.adamw8_step(*s, lr=1e-3)
+    (mb,), (vb,) = F.adamw8_moments(*bad[2:5])
+    (mc,), (vc,) = F.adamw8_moments(*clean[2:5])
+    at = torch.tensor([3, 100, 300], device=DEV)
+    rest = torch.ones(n, dtype=torch.bool, device=DEV)
+    rest[at] = False
+    assert bool(mb[at].isnan().all()) and bool(mb[rest].isfinite().all()) and bool(vb.isfinite().all())
+    # bases may differ where the clean element was its block's largest: within two codes
+    assert float(((vb - vc)[rest] / vc[rest]).abs().max()) <= 0.26
+    assert torch.equal(bad[0][0][rest], clean[0][0][rest])
+
+
+def test_8bit_seeds_and_repeats():
+    data = make([5000], bits=8, scale=1e-2)
+    def run(seed):
+        s = [[t.clone() for t in ts] for ts in data]
+        F.adamw8_step(*s, lr=1e-3, seed=seed)
+        return [t[0] for t in s]
+    a, b, c = run(7), run(7), run(8)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert torch.equal(a[0], c[0]) and not torch.equal(a[3], c[3])
+
+
+def test_8bit_large_tensor():
+    """Elements beyond 2^31 and 2^32 of one tensor."""
+    n = (1 << 32) + 3 * B + 5
+    p, g = torch.zeros(n, device=DEV, dtype=torch.bfloat16), torch.zeros(n, device=DEV, dtype=torch.bfloat16)
+    m, v = (torch.zeros(n, device=DEV, dtype=torch.uint8) for _ in range(2))
+    bases = torch.zeros(-(-n // B), 2, dtype=torch.int16, device=DEV)
+    at = n - (2 * B + 5)
+    data = make([2 * B + 5], torch.bfloat16, scale=1e-2)
+    p[at:], g[at:] = data[0][0], data[1][0]
+    s = torch.zeros((), device=DEV)
+    F.adamw8_step([p], [g], [m], [v], [bases], [s], seed=3, **H)
+    zero = torch.zeros(2 * B + 5, device=DEV)
+    (rp, bp), (rm, _), (rv, _) = reference(data[0][0], data[1][0], zero, zero, 1.0, H)
+    close(p[at:], rp, bp, HALF[torch.bfloat16])
+    dm, dv = dither(3, 0, 1, np.arange(at, n))
+    b = bases[at // B:].cpu().numpy()
+    check_codes(m[at:].cpu().numpy(), b[:, 0], rm.cpu().numpy(), dm, 127, False)
+    check_codes(v[at:].cpu().numpy(), b[:, 1], rv.cpu().numpy(), dv, 255, True)
+
+
+# ---------------------------------------------------------------------------
+# Streams, graphs, the optimizer
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_graph(bits):
+    data = make([700, 33, 20_000], bits=bits, scale=1e-2)
+    kw = dict(H, max_norm=0.1, skip_nonfinite=True)
+    step = F.adamw_step if bits == 32 else F.adamw8_step
+    captured, eager = ([[t.clone() for t in ts] for ts in data] for _ in range(2))
+    grads = captured[1]
+    eager[1] = grads
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*captured, **kw)
+    torch.cuda.current_stream().wait_stream(side)
+    step(*eager, **kw)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = step(*captured, **kw)
+    for k in range(4):
+        for t in grads:
+            t.normal_()
+        if k == 2:
+            grads[1][0] = float("inf")
+        graph.replay()
+        torch.cuda.synchronize()
+        other = step(*eager, **kw)
+        assert torch.equal(norm, other)
+        for a, b in zip(captured, eager):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def _model(seed, dtype=torch.float32):
+    torch.manual_seed(seed)
+    return torch.nn.Sequential(torch.nn.Linear(40, 100), torch.nn.SiLU(), torch.nn.Linear(100, 7)).to(DEV, dtype)
+
+
+def _grads(model, k):
+    x = torch.randn(64, 40, device=DEV, generator=torch.Generator(device=DEV).manual_seed(k))
+    for p in model.parameters():
+        p.grad = None
+    model(x.to(next(model.parameters()).dtype)).square().mean().backward()
+
+
+def test_optimizer_against_torch():
+    """Twenty steps of a small network, clipped: torch's clip_grad_norm_ and AdamW.  Each step's parameters differ by
+    a few units of the update (20 u lr a step), far below 1e-6."""
+    a, b = _model(0), _model(0)
+    oa = AdamW([{"params": a[0].parameters()}, {"params": a[2].parameters(), "lr": 3e-3, "weight_decay": 0.0}], lr=1e-3,
+               max_norm=0.05)
+    ob = torch.optim.AdamW([{"params": b[0].parameters()}, {"params": b[2].parameters(), "lr": 3e-3, "weight_decay": 0.0}],
+                           lr=1e-3)
+    sched = [torch.optim.lr_scheduler.StepLR(o, 7, 0.5) for o in (oa, ob)]
+    for k in range(20):
+        _grads(a, k)
+        for p, q in zip(a.parameters(), b.parameters()):  # the same gradients: Adam amplifies their noise
+            q.grad = p.grad.clone()
+        before = [p.grad.clone() for p in a.parameters()]
+        oa.step()
+        assert all(torch.equal(p.grad, g) for p, g in zip(a.parameters(), before))
+        norm = torch.nn.utils.clip_grad_norm_(b.parameters(), 0.05)
+        assert abs(float(oa.grad_norm) - float(norm)) <= 1e-6 * float(norm)
+        ob.step()
+        for s in sched:
+            s.step()
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert float((p - q).abs().max()) <= 1e-6
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_optimizer_state_dict(bits, dtype):
+    """A saved and loaded optimizer goes on bit for bit; 8-bit codes stay codes, float32 moments of 16-bit parameters
+    stay float32."""
+    a = _model(1, dtype)
+    oa = AdamW(a.parameters(), state_bits=bits, min_8bit_size=500, seed=9)
+    for k in range(3):
+        _grads(a, k)
+        oa.step()
+    b = _model(2, dtype)
+    b.load_state_dict(a.state_dict())
+    ob = AdamW(b.parameters(), state_bits=bits, min_8bit_size=500, seed=9)
+    ob.load_state_dict(oa.state_dict())
+    kinds = {s["exp_avg"].dtype for s in ob.state.values()}
+    assert kinds == ({torch.float32} if bits == 32 else {torch.float32, torch.uint8})
+    for k in range(3, 6):
+        for m, o in ((a, oa), (b, ob)):
+            _grads(m, k)
+            o.step()
+    assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters()))
+    for s in ob.state.values():
+        assert s["step"].device.type == "cuda" and float(s["step"]) == 6
+
+
+def test_optimizer_loads_torch_state():
+    a, b = _model(3), _model(3)
+    ob = torch.optim.AdamW(b.parameters())
+    for k in range(2):
+        _grads(b, k)
+        ob.step()
+    a.load_state_dict(b.state_dict())
+    oa = AdamW(a.parameters())
+    oa.load_state_dict(ob.state_dict())
+    _grads(b, 5)
+    for p, q in zip(a.parameters(), b.parameters()):
+        p.grad = q.grad.clone()
+    oa.step(), ob.step()
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert float((p - q).abs().max()) <= 1e-7
+
+
+def test_optimizer_closure_missing_gradients_and_versions():
+    model = _model(4)
+    opt = AdamW(model.parameters(), state_bits=8, min_8bit_size=1000, max_norm=1.0)
+    _grads(model, 0)
+    model[0].bias.grad = None
+    kept, version = model[0].bias.clone(), model[0].weight._version
+    loss = opt.step(lambda: model(torch.ones(3, 40, device=DEV)).sum())
+    assert loss.requires_grad and torch.equal(model[0].bias, kept) and model[0].weight._version > version
+    assert model[0].bias not in opt.state and opt.state[model[0].weight]["exp_avg"].dtype == torch.uint8
+    assert opt.state[model[2].bias]["exp_avg"].dtype == torch.float32
+    opt.zero_grad()
+    opt.step()  # nothing to do
+    x = torch.ones(2, 40, device=DEV, requires_grad=True)
+    y = model(x).square().sum()
+    _g = torch.autograd.grad(y, model[2].weight, retain_graph=True)[0]
+    model[2].weight.grad = _g
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_refusals():
+    p, g, m, v, s = make([300])
+    with pytest.raises(ValueError):
+        F.adamw_step(p, g, m, v, [], **H)
+    with pytest.raises(ValueError):
+        F.adamw_step(p, [g[0][:100]], m, v, s, **H)
+    with pytest.raises(ValueError):
+        F.adamw_step(p, [g[0].half()], m, v, s, **H)
+    with pytest.raises(ValueError):
+        F.adamw_step(p, g, [m[0].half()], v, s, **H)
+    with pytest.raises(ValueError):
+        F.adamw_step(p, g, m, v, [s[0].double()], **H)
+    with pytest.raises(ValueError):
+        F.adamw_step(p * 2, g * 2, m * 2, v * 2, s * 2, **H)
+    with pytest.raises(ValueError):
+        F.adamw_step(p, g, m, v, s, **{**H, "betas": (1.0, 0.9)})
+    with pytest.raises(ValueError):
+        F.adamw_step(p, g, m, v, s, max_norm=-1.0, **H)
+    with pytest.raises(ValueError):
+        F.adamw_step(p, g, m, v, s, max_norm=1.0, grad_norm=torch.zeros((), device=DEV, dtype=torch.float64), **H)
+    with pytest.raises(TypeError):
+        F.adamw_step([p[0].double()], [g[0].double()], m, v, s, **H)
+    with pytest.raises(RuntimeError):
+        F.adamw_step([p[0].cpu()], [g[0].cpu()], m, v, s, **H)
+    with pytest.raises(RuntimeError):
+        F.adamw_step(p, [g[0].to_sparse()], m, v, s, **H)
+    with pytest.raises(ValueError):
+        F.adamw_step([p[0].view(20, 15).t()], [g[0].view(20, 15).t()], [m[0].view(15, 20)], [v[0].view(15, 20)], s, **H)
+    p8, g8, m8, v8, b8, s8 = make([300], bits=8)
+    with pytest.raises(ValueError):
+        F.adamw8_step(p8, g8, m8, v8, [b8[0][:1]], s8, **H)
+    with pytest.raises(ValueError):
+        F.adamw8_step(p8, g8, m, v, b8, s8, **H)
+    with pytest.raises(ValueError):
+        F.adamw8_moments(m8, v8, b8, out=([m[0]], [v[0][:5]]))
+    with pytest.raises(RuntimeError):
+        F.grad_norm([torch.ones(3)])
+    for bad in (dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0), dict(max_norm=-2.0), dict(state_bits=16)):
+        with pytest.raises(ValueError):
+            AdamW(_model(0).parameters(), **bad)
