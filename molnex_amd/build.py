@@ -2,7 +2,8 @@
 
 Plain ``hipcc`` invocations (no CMake): each ``csrc/*.hip`` / ``*.cpp`` is
 compiled to an object in parallel, then linked into one shared library that
-exports the C ABI of ``include/molnex.h``.  ``python -m molnex_amd.build``.
+exports the C ABI of ``include/molnex.h``; the ops registered in C++ are compiled
+with g++ and linked to it.  ``python -m molnex_amd.build``.
 """
 
 from __future__ import annotations
@@ -53,6 +54,39 @@ def _compile(src: str) -> str:
     return f"{src}: {time.time() - t0:.1f}s"
 
 
+# the ops registered in C++: host code against torch's headers, linked to the library above
+TORCH_SOURCE = "torch_ops.cpp"
+TORCH_LIB = os.path.join(LIBDIR, "libmolnex_torch.so")
+
+
+def _compile_torch() -> str:
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-c", "-D__HIP_PLATFORM_AMD__=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for path in [*include_paths(), os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")]:
+        cmd += ["-isystem", path]
+    obj = os.path.join(BUILD, "torch_ops.o")
+    t0 = time.time()
+    r = subprocess.run(cmd + [os.path.join(CSRC, TORCH_SOURCE), "-o", obj], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {TORCH_SOURCE}\n{r.stdout}\n{r.stderr}")
+    return f"{TORCH_SOURCE}: {time.time() - t0:.1f}s"
+
+
+def _link_torch() -> None:
+    from torch.utils.cpp_extension import library_paths
+
+    tmp = TORCH_LIB + ".tmp"
+    cmd = ["g++", "-shared", os.path.join(BUILD, "torch_ops.o"), "-o", tmp, "-L", LIBDIR, "-lmolnex_hip",
+           *(f"-L{path}" for path in library_paths()), "-lc10", "-lc10_hip", "-ltorch_cpu", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_LIB)
+
+
 def build(verbose: bool = True) -> str:
     sys.path.insert(0, os.path.dirname(PKG))
     from molnex_amd.csrc import gen_edge_tp, gen_sc, gen_tp, gen_tp_any
@@ -64,7 +98,8 @@ def build(verbose: bool = True) -> str:
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
-        for msg in ex.map(_compile, SOURCES):
+        torch_ops = ex.submit(_compile_torch)
+        for msg in [*ex.map(_compile, SOURCES), torch_ops.result()]:
             if verbose:
                 print("  built", msg, flush=True)
     objs = [os.path.join(BUILD, os.path.splitext(s)[0] + ".o") for s in SOURCES]
@@ -74,8 +109,9 @@ def build(verbose: bool = True) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    _link_torch()
     if verbose:
-        print("  linked", LIB, flush=True)
+        print("  linked", LIB, "and", TORCH_LIB, flush=True)
     return LIB
 
 

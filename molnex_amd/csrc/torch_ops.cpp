@@ -1,0 +1,594 @@
+// torch.ops.molix.layer_norm* and the AdamW ops, registered in C++ over the C ABI of include/molnex.h.
+//
+// These are called once or more per layer and step, on tensors small enough that the host bounds them, and AdamW's
+// arguments are lists of every parameter.  Registered from Python (molnex_amd/_ops.py), a 700 x 128 layer norm forward
+// and backward took 179 us, most of it the autograd engine's thread and the caller passing the interpreter's lock to
+// and fro, and a step over 60 tensors 119 us, the time to ask each tensor its type, layout and address.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <algorithm>
+#include <optional>
+#include <tuple>
+#include <vector>
+
+#include "../../include/molnex.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void check(int rc, const char* what) {
+    if (rc != MNX_OK) TORCH_CHECK(false, what, " failed (status ", rc, "): ", mnx_last_error());
+}
+
+mnx_stream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+// -1 for a type the kernels do not take.
+int dtype_of(at::ScalarType t) {
+    switch (t) {
+        case at::kFloat: return MNX_F32;
+        case at::kBFloat16: return MNX_BF16;
+        case at::kHalf: return MNX_F16;
+        default: return -1;
+    }
+}
+
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+const void* data(const OptTensor& t) { return given(t) ? t->const_data_ptr() : nullptr; }
+void* out(const Tensor& t) { return t.numel() ? t.mutable_data_ptr() : nullptr; }
+OptTensor contiguous(const OptTensor& t) { return given(t) ? OptTensor(t->contiguous()) : std::nullopt; }
+
+// ---------------------------------------------------------------------------
+// Layer norm
+// ---------------------------------------------------------------------------
+
+struct Shape {
+    int64_t rows, width;
+    int dtype, wdtype;
+};
+
+Shape norm_shape(const char* name, const Tensor& x, const OptTensor& weight, const OptTensor& bias) {
+    TORCH_CHECK(x.is_cuda(), "molix::", name, " runs on the GPU only (got a ", x.device(), " tensor)");
+    Shape s{0, 0, dtype_of(x.scalar_type()), -1};
+    TORCH_CHECK_TYPE(s.dtype >= 0, "molix::", name, ": float32, bfloat16 or float16, got ", x.scalar_type());
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= MNX_LAYER_NORM_MAX_WIDTH, "molix::", name,
+                      ": the last axis must have 1 to ", MNX_LAYER_NORM_MAX_WIDTH, " values, got ", x.sizes());
+    s.width = x.size(-1);
+    s.rows = x.numel() / s.width;
+    for (const auto* t : {&weight, &bias}) {
+        if (!given(*t)) continue;
+        TORCH_CHECK_VALUE((*t)->dim() == 1 && (*t)->size(0) == s.width, "molix::", name,
+                          ": weight and bias must be (", s.width, ",), got ", (*t)->sizes());
+        const int d = dtype_of((*t)->scalar_type());
+        TORCH_CHECK_TYPE((d == s.dtype || d == MNX_F32) && (s.wdtype < 0 || s.wdtype == d) &&
+                             (*t)->device() == x.device(),
+                         "molix::", name, ": weight and bias share one type, ", x.scalar_type(),
+                         " or float32, and x's device");
+        s.wdtype = d;
+    }
+    if (s.wdtype < 0) s.wdtype = s.dtype;
+    return s;
+}
+
+// A tensor's rows in place where they are evenly spaced (a column block of a wider matrix), else a contiguous copy.
+struct Rows {
+    Tensor t;
+    int64_t ld;
+    Rows(const Tensor& x, int64_t width) : t(x), ld(width) {
+        if (x.is_contiguous()) return;
+        if (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= width) ld = x.stride(0);
+        else t = x.contiguous();
+    }
+    const void* ptr() const { return t.numel() ? t.const_data_ptr() : nullptr; }
+};
+
+void check_stats(const char* name, const Tensor& stats, const Tensor& x, int64_t rows) {
+    TORCH_CHECK_VALUE(stats.scalar_type() == at::kFloat && stats.dim() == 2 && stats.size(0) == 2 &&
+                          stats.size(1) == rows && stats.device() == x.device(),
+                      "molix::", name, ": stats float32 (2, ", rows, ")");
+}
+
+void check_like(const char* name, const char* what, const Tensor& t, const Tensor& x) {
+    TORCH_CHECK_VALUE(t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.device() == x.device(),
+                      "molix::", name, ": ", what, " must be ", x.scalar_type(), " ", x.sizes(), " like x, got ",
+                      t.scalar_type(), " ", t.sizes());
+}
+
+std::tuple<Tensor, Tensor> layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+    const Shape s = norm_shape("layer_norm", x, weight, bias);
+    const c10::DeviceGuard guard(x.device());
+    const Rows xs(x, s.width);
+    const OptTensor w = contiguous(weight), b = contiguous(bias);
+    Tensor y = at::empty(x.sizes(), x.options()), stats = at::empty({2, s.rows}, x.options().dtype(at::kFloat));
+    check(mnx_layer_norm_fwd(xs.ptr(), xs.ld, s.rows, s.width, data(w), data(b), eps, s.dtype, s.wdtype, out(y),
+                             static_cast<float*>(out(stats)), stream_of(x)),
+          "layer_norm");
+    return {y, stats};
+}
+
+Tensor vector_like(const Tensor& x, const OptTensor& t, bool needed) {
+    return at::empty({needed ? x.size(-1) : 0}, given(t) ? t->options() : x.options());
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& grad, const Tensor& x, const OptTensor& weight,
+                                                       const OptTensor& bias, const Tensor& stats, double eps,
+                                                       bool need_x, bool need_w, bool need_b) {
+    (void)eps;  // higher orders read it
+    const char* name = "layer_norm_backward";
+    const Shape s = norm_shape(name, x, weight, bias);
+    check_like(name, "grad", grad, x);
+    check_stats(name, stats, x, s.rows);
+    TORCH_CHECK_VALUE((!need_w || given(weight)) && (!need_b || given(bias)), "molix::", name,
+                      ": the gradient of a weight or bias that is not there");
+    const c10::DeviceGuard guard(x.device());
+    const Rows xs(x, s.width), g(grad, s.width);
+    const OptTensor w = contiguous(weight);
+    const Tensor st = stats.contiguous();
+    Tensor gx = need_x ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+    Tensor gw = vector_like(x, weight, need_w), gb = vector_like(x, bias, need_b);
+    Tensor ws;
+    size_t bytes = 0;
+    if (need_w || need_b) {
+        bytes = mnx_layer_norm_bwd_workspace_bytes(s.rows, s.width);
+        ws = at::empty({int64_t(bytes)}, x.options().dtype(at::kByte));
+    }
+    check(mnx_layer_norm_bwd(g.ptr(), g.ld, xs.ptr(), xs.ld, s.rows, s.width, data(w), s.dtype, s.wdtype,
+                             st.const_data_ptr<float>(), out(gx), out(gw), out(gb), bytes ? out(ws) : nullptr, bytes,
+                             stream_of(x)),
+          "layer_norm backward");
+    return {gx, gw, gb};
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward2(const Tensor& grad, const Tensor& x, const OptTensor& weight,
+                                                        const Tensor& stats, double eps, const OptTensor& seed_x,
+                                                        const OptTensor& seed_w, const OptTensor& seed_b,
+                                                        bool need_w) {
+    (void)eps;
+    const char* name = "layer_norm_backward2";
+    Shape s = norm_shape(name, x, weight, std::nullopt);
+    check_like(name, "grad", grad, x);
+    check_stats(name, stats, x, s.rows);
+    if (given(seed_x)) check_like(name, "seed_x", *seed_x, x);
+    if (!given(weight) && (given(seed_w) || given(seed_b)))
+        s.wdtype = dtype_of((given(seed_w) ? seed_w : seed_b)->scalar_type());
+    for (const auto* t : {&seed_w, &seed_b})
+        TORCH_CHECK_VALUE(!given(*t) || ((*t)->dim() == 1 && (*t)->size(0) == s.width && (*t)->device() == x.device() &&
+                                         dtype_of((*t)->scalar_type()) == s.wdtype && s.wdtype >= 0),
+                          "molix::", name, ": seed_w and seed_b like the weight");
+    TORCH_CHECK_VALUE(!need_w || given(weight), "molix::", name, ": the derivative of a weight that is not there");
+    const c10::DeviceGuard guard(x.device());
+    const Rows xs(x, s.width), g(grad, s.width), u(given(seed_x) ? *seed_x : at::zeros_like(xs.t), s.width);
+    const OptTensor w = contiguous(weight), p = contiguous(seed_w), q = contiguous(seed_b);
+    const Tensor st = stats.contiguous();
+    Tensor dg = at::empty(x.sizes(), x.options()), dx = at::empty(x.sizes(), x.options());
+    Tensor dw = vector_like(x, weight, need_w);
+    const size_t bytes = mnx_layer_norm_bwd_workspace_bytes(s.rows, s.width);
+    Tensor ws = at::empty({int64_t(bytes)}, x.options().dtype(at::kByte));
+    check(mnx_layer_norm_bwd2(g.ptr(), g.ld, xs.ptr(), xs.ld, u.ptr(), u.ld, data(p), data(q), s.rows, s.width,
+                              data(w), s.dtype, s.wdtype, st.const_data_ptr<float>(), out(dg), out(dx), out(dw),
+                              out(ws), bytes, stream_of(x)),
+          "layer_norm second order");
+    return {dg, dx, dw};
+}
+
+// The ops through the dispatcher: differentiable where the caller's mode has gradients on.
+template <typename F>
+auto op(const char* name) {
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+auto layer_norm_op() {
+    static auto o = op<decltype(layer_norm)>("molix::layer_norm");
+    return o;
+}
+auto layer_norm_backward_op() {
+    static auto o = op<decltype(layer_norm_backward)>("molix::layer_norm_backward");
+    return o;
+}
+auto layer_norm_backward2_op() {
+    static auto o = op<decltype(layer_norm_backward2)>("molix::layer_norm_backward2");
+    return o;
+}
+
+bool wants_grad(const OptTensor& t) { return given(t) && t->requires_grad(); }
+OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+Tensor or_undefined(const OptTensor& t) { return given(t) ? *t : Tensor(); }
+
+class LayerNorm : public torch::autograd::Function<LayerNorm> {
+  public:
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias,
+                                 double eps) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [y, stats] = layer_norm_op().call(x, weight, bias, eps);
+        ctx->save_for_backward({x, or_undefined(weight), or_undefined(bias), stats});
+        ctx->saved_data["eps"] = eps;
+        ctx->mark_non_differentiable({stats});
+        return {y, stats};
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &b = saved[2];
+        // edges are numbered over the tensors that were there
+        const bool nx = ctx->needs_input_grad(0), nw = w.defined() && ctx->needs_input_grad(1);
+        const bool nb = b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1);
+        if (!grads[0].defined() || !(nx || nw || nb)) return {Tensor(), Tensor(), Tensor(), Tensor()};
+        auto [gx, gw, gb] = layer_norm_backward_op().call(grads[0], x, optional(w), optional(b), saved[3],
+                                                          ctx->saved_data["eps"].toDouble(), nx, nw, nb);
+        return {nx ? gx : Tensor(), nw ? gw : Tensor(), nb ? gb : Tensor(), Tensor()};
+    }
+};
+
+std::tuple<Tensor, Tensor> layer_norm_autograd(const Tensor& x, const OptTensor& weight, const OptTensor& bias,
+                                               double eps) {
+    if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias))) {
+        auto r = LayerNorm::apply(x, weight, bias, eps);
+        return {r[0], r[1]};
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    return layer_norm_op().call(x, weight, bias, eps);
+}
+
+class LayerNormBackward : public torch::autograd::Function<LayerNormBackward> {
+  public:
+    static variable_list forward(AutogradContext* ctx, const Tensor& grad, const Tensor& x, const OptTensor& weight,
+                                 const OptTensor& bias, const Tensor& stats, double eps, bool need_x, bool need_w,
+                                 bool need_b) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [gx, gw, gb] = layer_norm_backward_op().call(grad, x, weight, bias, stats, eps, need_x, need_w, need_b);
+        ctx->save_for_backward({grad, x, or_undefined(weight), stats});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["needed"] = int64_t(need_x) | int64_t(need_w) << 1 | int64_t(need_b) << 2;
+        ctx->set_materialize_grads(false);
+        return {gx, gw, gb};
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& seeds) {
+        variable_list none(9);
+        const auto saved = ctx->get_saved_variables();
+        const Tensor& w = saved[2];
+        const bool ng = ctx->needs_input_grad(0), nx = ctx->needs_input_grad(1);
+        const bool nw = w.defined() && ctx->needs_input_grad(2);
+        const int64_t needed = ctx->saved_data["needed"].toInt();
+        OptTensor seed[3];
+        bool any = false;
+        for (int k = 0; k < 3; ++k) {
+            if (needed >> k & 1) seed[k] = optional(seeds[k]);
+            any |= given(seed[k]);
+        }
+        if (!any || !(ng || nx || nw)) return none;
+        auto [dg, dx, dw] = layer_norm_backward2_op().call(saved[0], saved[1], optional(w), saved[3],
+                                                           ctx->saved_data["eps"].toDouble(), seed[0], seed[1],
+                                                           seed[2], nw);
+        if (ng) none[0] = dg;
+        if (nx) none[1] = dx;
+        if (nw) none[2] = dw;
+        return none;
+    }
+};
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_autograd(const Tensor& grad, const Tensor& x,
+                                                                const OptTensor& weight, const OptTensor& bias,
+                                                                const Tensor& stats, double eps, bool need_x,
+                                                                bool need_w, bool need_b) {
+    if (at::GradMode::is_enabled() && (grad.requires_grad() || x.requires_grad() || wants_grad(weight))) {
+        auto r = LayerNormBackward::apply(grad, x, weight, bias, stats, eps, need_x, need_w, need_b);
+        return {r[0], r[1], r[2]};
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    return layer_norm_backward_op().call(grad, x, weight, bias, stats, eps, need_x, need_w, need_b);
+}
+
+// Third and higher orders: the second order as differentiable torch operations in float32.
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward2_autograd(const Tensor& grad, const Tensor& x,
+                                                                 const OptTensor& weight, const Tensor& stats,
+                                                                 double eps, const OptTensor& seed_x,
+                                                                 const OptTensor& seed_w, const OptTensor& seed_b,
+                                                                 bool need_w) {
+    bool tracked = grad.requires_grad() || x.requires_grad();
+    for (const auto* t : {&weight, &seed_x, &seed_w, &seed_b}) tracked |= wants_grad(*t);
+    if (!at::GradMode::is_enabled() || !tracked) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return layer_norm_backward2_op().call(grad, x, weight, stats, eps, seed_x, seed_w, seed_b, need_w);
+    }
+    const int64_t D = x.size(-1);
+    const Tensor g2 = grad.reshape({-1, D}).to(at::kFloat), x2 = x.reshape({-1, D}).to(at::kFloat);
+    const Tensor u = given(seed_x) ? seed_x->reshape({-1, D}).to(at::kFloat) : at::zeros_like(x2);
+    const Tensor w = given(weight) ? weight->to(at::kFloat) : at::ones({D}, x2.options());
+    const Tensor xc = x2 - x2.mean(1, true), r = (xc.square().mean(1, true) + eps).rsqrt(), h = xc * r;
+    const auto J = [&](const Tensor& a) { return r * (a - a.mean(1, true) - h * (a * h).mean(1, true)); };
+    const Tensor a = g2 * w, ju = J(u);
+    Tensor dg = w * ju;
+    Tensor dx = -r * ((a * h).mean(1, true) * ju + (u * h).mean(1, true) * J(a)) - r * h * (ju * a).mean(1, true);
+    if (given(seed_w)) {
+        const Tensor p = seed_w->to(at::kFloat);
+        dg = dg + p * h;
+        dx = dx + J(g2 * p);
+    }
+    if (given(seed_b)) dg = dg + seed_b->to(at::kFloat);
+    Tensor dw = need_w ? (g2 * ju).sum(0).to(weight->scalar_type()) : at::empty({0}, x.options());
+    return {dg.to(x.scalar_type()).reshape(x.sizes()), dx.to(x.scalar_type()).reshape(x.sizes()), dw};
+}
+
+// ---------------------------------------------------------------------------
+// AdamW
+// ---------------------------------------------------------------------------
+
+constexpr int64_t kStateBlock = 256;
+
+at::Device gpu_of(const char* name, at::TensorList ts) {
+    TORCH_CHECK(ts[0].is_cuda(), "molix::", name, " runs on the GPU only (got a ", ts[0].device(), " tensor)");
+    return ts[0].device();
+}
+
+void check_values(const char* name, const char* what, const Tensor& t, at::Device device) {
+    TORCH_CHECK(t.layout() == at::kStrided, "molix::", name, ": ", what, " must be dense, got ", t.layout());
+    TORCH_CHECK(t.device() == device, "molix::", name, ": ", what, " on ", t.device(), ", others on ", device);
+    TORCH_CHECK_TYPE(dtype_of(t.scalar_type()) >= 0, "molix::", name, ": ", what,
+                     " float32, bfloat16 or float16, got ", t.scalar_type());
+}
+
+Tensor grad_norm(at::TensorList grads) {
+    if (grads.empty()) return at::zeros({});
+    const at::Device device = gpu_of("grad_norm", grads);
+    const c10::DeviceGuard guard(device);
+    std::vector<Tensor> kept;
+    std::vector<const void*> ptrs;
+    std::vector<int64_t> numel;
+    std::vector<int32_t> dtype;
+    for (const Tensor& g : grads) {
+        check_values("grad_norm", "gradients", g, device);
+        const bool whole = g.is_non_overlapping_and_dense();
+        if (!whole) kept.push_back(g.contiguous());
+        ptrs.push_back((whole ? g : kept.back()).const_data_ptr());
+        numel.push_back(g.numel());
+        dtype.push_back(dtype_of(g.scalar_type()));
+    }
+    const auto f32 = grads[0].options().dtype(at::kFloat);
+    const size_t bytes = mnx_grad_norm_workspace_bytes(numel.data(), int64_t(numel.size()));
+    Tensor norm = at::empty({}, f32), ws = at::empty({int64_t(bytes)}, f32.dtype(at::kByte));
+    check(mnx_grad_norm(ptrs.data(), numel.data(), dtype.data(), int64_t(ptrs.size()), static_cast<float*>(out(norm)),
+                        out(ws), bytes, stream_of(norm)),
+          "grad_norm");
+    return norm;
+}
+
+struct Options {
+    double lr, beta1, beta2, eps, weight_decay;
+    bool maximize;
+    std::optional<double> max_norm;
+    bool skip_nonfinite;
+    int64_t seed;
+};
+
+// Returns the norm that was used; without one, an empty tensor.
+Tensor step(const char* name, int bits, at::TensorList params, at::TensorList grads, at::TensorList exp_avgs,
+            at::TensorList exp_avg_sqs, at::TensorList bases, at::TensorList steps, const OptTensor& lr,
+            const OptTensor& norm_in, const Options& o) {
+    const size_t count = params.size();
+    TORCH_CHECK_VALUE(grads.size() == count && exp_avgs.size() == count && exp_avg_sqs.size() == count &&
+                          steps.size() == count && (bits == 32 || bases.size() == count),
+                      "molix::", name, ": lists of ", count, ", ", grads.size(), ", ", exp_avgs.size(), ", ",
+                      exp_avg_sqs.size(), " and ", steps.size(), " tensors");
+    TORCH_CHECK_VALUE(o.beta1 >= 0 && o.beta1 < 1 && o.beta2 >= 0 && o.beta2 < 1 && o.eps >= 0, "molix::", name,
+                      ": betas (", o.beta1, ", ", o.beta2, "), eps ", o.eps);
+    TORCH_CHECK_VALUE(!o.max_norm || *o.max_norm >= 0, "molix::", name, ": max_norm ", o.max_norm.value_or(0));
+    const bool uses_norm = o.max_norm.has_value() || o.skip_nonfinite;
+    if (!count) return given(norm_in) ? *norm_in : uses_norm ? at::zeros({}) : at::empty({0});
+    const at::Device device = gpu_of(name, params);
+    const c10::DeviceGuard guard(device);
+    const at::ScalarType moment = bits == 32 ? at::kFloat : at::kByte;
+
+    std::vector<void*> p_ptr(count), m_ptr(count), v_ptr(count);
+    std::vector<const void*> g_ptr(count);
+    std::vector<int16_t*> b_ptr(count);
+    std::vector<float*> s_ptr(count);
+    std::vector<int64_t> numel(count);
+    std::vector<int32_t> dtype(count);
+    std::vector<Tensor> kept;                          // gradients laid out like their parameters
+    std::vector<std::pair<const Tensor*, Tensor>> gaps;  // parameters with gaps and their copies
+    for (size_t i = 0; i < count; ++i) {
+        const Tensor &p = params[i], &g = grads[i], &m = exp_avgs[i], &v = exp_avg_sqs[i], &s = steps[i];
+        check_values(name, "parameters", p, device);
+        TORCH_CHECK(g.layout() == at::kStrided, "molix::", name, ": sparse gradients are not supported");
+        TORCH_CHECK_VALUE(g.scalar_type() == p.scalar_type() && g.sizes() == p.sizes() && g.device() == device,
+                          "molix::", name, ": gradient ", i, " is ", g.scalar_type(), " ", g.sizes(), " on ",
+                          g.device(), ", its parameter ", p.scalar_type(), " ", p.sizes(), " on ", device);
+        TORCH_CHECK_VALUE(m.scalar_type() == moment && v.scalar_type() == moment && m.sizes() == p.sizes() &&
+                              v.sizes() == p.sizes() && m.device() == device && v.device() == device,
+                          "molix::", name, ": the moments of tensor ", i, " must be ", moment,
+                          " of its shape and device");
+        TORCH_CHECK_VALUE(s.scalar_type() == at::kFloat && s.numel() == 1 && s.device() == device, "molix::", name,
+                          ": step ", i, " must be one float32 on ", device);
+        if (bits == 8) {
+            const Tensor& b = bases[i];
+            const int64_t blocks = (p.numel() + kStateBlock - 1) / kStateBlock;
+            TORCH_CHECK_VALUE(b.scalar_type() == at::kShort && b.dim() == 2 && b.size(0) == blocks && b.size(1) == 2 &&
+                                  b.is_contiguous() && b.device() == device,
+                              "molix::", name, ": bases ", i, " must be contiguous int16 (", blocks, ", 2) on ",
+                              device);
+            b_ptr[i] = static_cast<int16_t*>(out(b));
+        }
+        const Tensor *pp = &p, *gg = &g;
+        if (!(p.is_contiguous() && g.is_contiguous() && m.is_contiguous() && v.is_contiguous())) {
+            if (!p.is_non_overlapping_and_dense()) {
+                gaps.emplace_back(&p, p.detach().contiguous());
+                pp = &gaps.back().second;
+            }
+            TORCH_CHECK_VALUE(m.strides() == pp->strides() && v.strides() == pp->strides(), "molix::", name,
+                              ": the moments of tensor ", i,
+                              " must have its strides (contiguous where the tensor has gaps)");
+            if (g.strides() != pp->strides()) {
+                kept.push_back(at::empty_strided(pp->sizes(), pp->strides(), g.options()).copy_(g.detach()));
+                gg = &kept.back();
+            }
+        }
+        p_ptr[i] = out(*pp);
+        g_ptr[i] = gg->numel() ? gg->const_data_ptr() : nullptr;
+        m_ptr[i] = out(m);
+        v_ptr[i] = out(v);
+        s_ptr[i] = static_cast<float*>(out(s));
+        numel[i] = p.numel();
+        dtype[i] = dtype_of(p.scalar_type());
+    }
+    std::vector<void*> order;
+    for (void* p : p_ptr)
+        if (p) order.push_back(p);
+    std::sort(order.begin(), order.end());
+    TORCH_CHECK_VALUE(std::adjacent_find(order.begin(), order.end()) == order.end(), "molix::", name,
+                      ": a parameter is given twice");
+
+    mnx_adamw_args a{};
+    a.count = int64_t(count);
+    a.params = p_ptr.data();
+    a.grads = g_ptr.data();
+    a.exp_avgs = m_ptr.data();
+    a.exp_avg_sqs = v_ptr.data();
+    a.bases = bits == 8 ? b_ptr.data() : nullptr;
+    a.steps = s_ptr.data();
+    a.numel = numel.data();
+    a.dtype = dtype.data();
+    a.state_bits = bits;
+    a.maximize = o.maximize;
+    a.skip_nonfinite = o.skip_nonfinite;
+    a.seed = uint32_t(o.seed);
+    a.lr = o.lr;
+    a.beta1 = o.beta1;
+    a.beta2 = o.beta2;
+    a.eps = o.eps;
+    a.weight_decay = o.weight_decay;
+    a.max_norm = o.max_norm.value_or(-1.0);
+    Tensor rate;
+    if (given(lr)) {
+        TORCH_CHECK_VALUE(lr->numel() == 1 && lr->device() == device, "molix::", name,
+                          ": lr must be a number or one value on ", device);
+        rate = lr->detach().to(at::kFloat);
+        a.lr_device = rate.const_data_ptr<float>();
+    }
+    const auto f32 = params[0].options().dtype(at::kFloat).requires_grad(false);
+    Tensor norm;
+    if (given(norm_in)) {
+        TORCH_CHECK_VALUE(norm_in->numel() == 1 && norm_in->scalar_type() == at::kFloat && norm_in->device() == device,
+                          "molix::", name, ": grad_norm must be one float32 on ", device);
+        a.norm_in = norm_in->const_data_ptr<float>();
+    } else if (uses_norm) {
+        norm = at::empty({}, f32);
+        a.norm_out = static_cast<float*>(out(norm));
+    }
+    a.workspace_bytes = mnx_adamw_workspace_bytes(a.numel, a.count);
+    Tensor ws = at::empty({int64_t(a.workspace_bytes)}, f32.dtype(at::kByte));
+    a.workspace = out(ws);
+    check(mnx_adamw_step(&a, stream_of(ws)), name);
+    for (auto& [p, copy] : gaps) p->detach().copy_(copy);
+    for (const at::TensorList& l : {params, exp_avgs, exp_avg_sqs, steps, bases})
+        for (const Tensor& t : l) t.unsafeGetTensorImpl()->bump_version();
+    return norm.defined() ? norm : at::empty({0}, f32);
+}
+
+Tensor adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs, at::TensorList exp_avg_sqs,
+                  at::TensorList steps, double lr, double beta1, double beta2, double eps, double weight_decay,
+                  bool maximize, std::optional<double> max_norm, const OptTensor& grad_norm, bool skip_nonfinite,
+                  const OptTensor& lr_tensor) {
+    return step("adamw_step", 32, params, grads, exp_avgs, exp_avg_sqs, {}, steps, lr_tensor, grad_norm,
+                {lr, beta1, beta2, eps, weight_decay, maximize, max_norm, skip_nonfinite, 0});
+}
+
+Tensor adamw8_step(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs, at::TensorList exp_avg_sqs,
+                   at::TensorList bases, at::TensorList steps, double lr, double beta1, double beta2, double eps,
+                   double weight_decay, bool maximize, std::optional<double> max_norm, const OptTensor& grad_norm,
+                   bool skip_nonfinite, const OptTensor& lr_tensor, int64_t seed) {
+    return step("adamw8_step", 8, params, grads, exp_avgs, exp_avg_sqs, bases, steps, lr_tensor, grad_norm,
+                {lr, beta1, beta2, eps, weight_decay, maximize, max_norm, skip_nonfinite, seed});
+}
+
+void adamw8_moments(at::TensorList exp_avgs, at::TensorList exp_avg_sqs, at::TensorList bases, at::TensorList out_avgs,
+                    at::TensorList out_avg_sqs) {
+    const char* name = "adamw8_moments";
+    const size_t count = exp_avgs.size();
+    TORCH_CHECK_VALUE(exp_avg_sqs.size() == count && bases.size() == count && out_avgs.size() == count &&
+                          out_avg_sqs.size() == count,
+                      "molix::", name, ": lists of ", count, ", ", exp_avg_sqs.size(), ", ", bases.size(), ", ",
+                      out_avgs.size(), " and ", out_avg_sqs.size(), " tensors");
+    if (!count) return;
+    const at::Device device = gpu_of(name, exp_avgs);
+    const c10::DeviceGuard guard(device);
+    std::vector<const void*> m_ptr(count), v_ptr(count);
+    std::vector<int16_t*> b_ptr(count);
+    std::vector<float*> om_ptr(count), ov_ptr(count);
+    std::vector<int64_t> numel(count);
+    for (size_t i = 0; i < count; ++i) {
+        const Tensor &m = exp_avgs[i], &v = exp_avg_sqs[i], &b = bases[i];
+        TORCH_CHECK_VALUE(m.scalar_type() == at::kByte && v.scalar_type() == at::kByte && m.sizes() == v.sizes() &&
+                              m.strides() == v.strides() && m.is_non_overlapping_and_dense() &&
+                              m.device() == device && v.device() == device,
+                          "molix::", name, ": the moments of tensor ", i, " must be dense uint8 of one layout");
+        const int64_t blocks = (m.numel() + kStateBlock - 1) / kStateBlock;
+        TORCH_CHECK_VALUE(b.scalar_type() == at::kShort && b.dim() == 2 && b.size(0) == blocks && b.size(1) == 2 &&
+                              b.is_contiguous() && b.device() == device,
+                          "molix::", name, ": bases ", i, " must be contiguous int16 (", blocks, ", 2) on ", device);
+        for (const Tensor* t : {&out_avgs[i], &out_avg_sqs[i]})
+            TORCH_CHECK_VALUE(t->scalar_type() == at::kFloat && t->sizes() == m.sizes() &&
+                                  t->strides() == m.strides() && t->device() == device,
+                              "molix::", name, ": out of tensor ", i, " must be float32 of its shape and strides");
+        m_ptr[i] = m.const_data_ptr();
+        v_ptr[i] = v.const_data_ptr();
+        b_ptr[i] = static_cast<int16_t*>(out(b));
+        om_ptr[i] = static_cast<float*>(out(out_avgs[i]));
+        ov_ptr[i] = static_cast<float*>(out(out_avg_sqs[i]));
+        numel[i] = m.numel();
+    }
+    check(mnx_adamw8_moments(m_ptr.data(), v_ptr.data(), b_ptr.data(), numel.data(), int64_t(count), om_ptr.data(),
+                             ov_ptr.data(), stream_of(exp_avgs[0])),
+          name);
+    for (const at::TensorList& l : {out_avgs, out_avg_sqs})
+        for (const Tensor& t : l) t.unsafeGetTensorImpl()->bump_version();
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(molix, m) {
+    const std::vector<at::Tag> tags{at::Tag::pt2_compliant_tag};
+    m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor)", tags);
+    m.def("layer_norm_backward(Tensor grad, Tensor x, Tensor? weight, Tensor? bias, Tensor stats, float eps, "
+          "bool need_x, bool need_w, bool need_b) -> (Tensor, Tensor, Tensor)",
+          tags);
+    m.def("layer_norm_backward2(Tensor grad, Tensor x, Tensor? weight, Tensor stats, float eps, Tensor? seed_x, "
+          "Tensor? seed_w, Tensor? seed_b, bool need_w) -> (Tensor, Tensor, Tensor)",
+          tags);
+    m.def("grad_norm(Tensor[] grads) -> Tensor", tags);
+    m.def("adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avgs, Tensor(c!)[] exp_avg_sqs, "
+          "Tensor(d!)[] steps, float lr, float beta1, float beta2, float eps, float weight_decay, bool maximize, "
+          "float? max_norm, Tensor? grad_norm, bool skip_nonfinite, Tensor? lr_tensor) -> Tensor",
+          tags);
+    m.def("adamw8_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avgs, Tensor(c!)[] exp_avg_sqs, "
+          "Tensor(d!)[] bases, Tensor(e!)[] steps, float lr, float beta1, float beta2, float eps, "
+          "float weight_decay, bool maximize, float? max_norm, Tensor? grad_norm, bool skip_nonfinite, "
+          "Tensor? lr_tensor, int seed) -> Tensor",
+          tags);
+    m.def("adamw8_moments(Tensor[] exp_avgs, Tensor[] exp_avg_sqs, Tensor[] bases, Tensor(a!)[] out_avgs, "
+          "Tensor(b!)[] out_avg_sqs) -> ()",
+          tags);
+}
+
+TORCH_LIBRARY_IMPL(molix, CUDA, m) {
+    m.impl("layer_norm", layer_norm);
+    m.impl("layer_norm_backward", layer_norm_backward);
+    m.impl("layer_norm_backward2", layer_norm_backward2);
+    m.impl("grad_norm", grad_norm);
+    m.impl("adamw_step", adamw_step);
+    m.impl("adamw8_step", adamw8_step);
+    m.impl("adamw8_moments", adamw8_moments);
+}
+
+TORCH_LIBRARY_IMPL(molix, Autograd, m) {
+    m.impl("layer_norm", layer_norm_autograd);
+    m.impl("layer_norm_backward", layer_norm_backward_autograd);
+    m.impl("layer_norm_backward2", layer_norm_backward2_autograd);
+    // no gradients: they write into leaves (their versions rise) or read gradients
+    for (const char* name : {"grad_norm", "adamw_step", "adamw8_step", "adamw8_moments"})
+        m.impl(name, torch::CppFunction::makeFallthrough());
+}

@@ -5,9 +5,11 @@ from __future__ import annotations
 import math
 
 import torch
-from torch import Tensor, ops
+from torch import Tensor
 
 from ...training import DTYPES, LAYER_NORM_MAX_WIDTH
+
+_layer_norm = torch.ops.molix.layer_norm.default
 
 
 def layer_norm(input: Tensor, normalized_shape, weight: Tensor | None = None, bias: Tensor | None = None,
@@ -34,7 +36,7 @@ def layer_norm(input: Tensor, normalized_shape, weight: Tensor | None = None, bi
             or not 1 <= width <= LAYER_NORM_MAX_WIDTH):
         return torch.nn.functional.layer_norm(input, shape, weight, bias, eps)
     if len(shape) == 1:
-        return ops.molix.layer_norm(input, weight, bias, float(eps))[0]
+        return _layer_norm(input, weight, bias, eps)[0]
     flat = [t if t is None else t.reshape(width) for t in (weight, bias)]
-    y = ops.molix.layer_norm(input.reshape(*input.shape[:lead], width), *flat, float(eps))[0]
+    y = _layer_norm(input.reshape(*input.shape[:lead], width), *flat, eps)[0]
     return y.reshape(input.shape)
