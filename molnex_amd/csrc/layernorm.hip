@@ -7,109 +7,398 @@
 //     dg = w J u + p h + q,   dw = sum over rows of g J u,
 //     dx = J(p g) - r (alpha J u + ups J a) - r h mean(u J a)
 // Every sum is in float32; the variance is the mean square about the mean, not a difference of moments.
+//
+// Each array is read or written once, and the bytes bound every kernel here (8 to 40 operations a value).  A row is
+// held in the registers of TPR threads, VPL vectors of 16 bytes each: its sums, and then its results, come from
+// there.  A workgroup has several such groups of threads, takes rows in turn, and keeps the weights in registers.  The
+// backward kernels sum over the rows they take in registers too and leave one partial row of sums a workgroup, which a
+// second launch joins, so nothing is read again and the order of the sums is fixed.
 #include "elem.h"
+#include "wave.h"
 
 namespace mnx {
 
-__device__ __forceinline__ float wave_sum(float v) {
-    for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off);
-    return v;
+template <int DT>
+constexpr int kVec = DT == kF32 ? 4 : 8;  // values of a vector of 16 bytes
+
+// Vectors are read at the alignment of a value (rows of an odd width start anywhere).
+template <int DT>
+struct Vec {
+    typedef typename Elem<DT>::T T;
+    typedef T Packed __attribute__((ext_vector_type(kVec<DT>), aligned(sizeof(T))));
+};
+
+// Columns c .. c + kVec - 1 of a row of `width` values; 0 past its end.
+template <int DT>
+__device__ __forceinline__ void load_vec(const typename Elem<DT>::T* p, int c, int width, float (&v)[kVec<DT>]) {
+    if (c + kVec<DT> <= width) {
+        const auto t = *reinterpret_cast<const typename Vec<DT>::Packed*>(p + c);
+#pragma unroll
+        for (int e = 0; e < kVec<DT>; ++e) v[e] = float(t[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kVec<DT>; ++e) v[e] = c + e < width ? float(p[c + e]) : 0.0f;
+    }
+}
+template <int DT>
+__device__ __forceinline__ void store_vec(typename Elem<DT>::T* p, int c, int width, const float (&v)[kVec<DT>]) {
+    using T = typename Elem<DT>::T;
+    if (c + kVec<DT> <= width) {
+        typename Vec<DT>::Packed t;
+#pragma unroll
+        for (int e = 0; e < kVec<DT>; ++e) t[e] = T(v[e]);
+        *reinterpret_cast<typename Vec<DT>::Packed*>(p + c) = t;
+    } else {
+#pragma unroll
+        for (int e = 0; e < kVec<DT>; ++e)
+            if (c + e < width) p[c + e] = T(v[e]);
+    }
+}
+// Values of a vector of weights; `none` where there is no vector and past the end 0.
+template <int N>
+__device__ __forceinline__ void load_weights(const void* p, int c, int width, int dtype, float none, float (&v)[N]) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = c + e < width ? (p ? load_elem(p, c + e, dtype) : none) : 0.0f;
 }
 
-// One wavefront per row, the row read again for each sum.
+// K sums over the TPR threads of a group, on all of them.  More than a wavefront joins through `lds` (K floats a
+// wavefront, two sets used in turn so that one barrier a call suffices).
+template <int TPR, int K>
+__device__ __forceinline__ void group_sum(float (&s)[K], float* lds, int& turn) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if constexpr (TPR >= 16) s[k] += dpp_partner<8>(s[k]);
+        s[k] += dpp_partner<4>(s[k]);
+        s[k] += dpp_partner<2>(s[k]);
+        s[k] += dpp_partner<1>(s[k]);
+        if constexpr (TPR >= 32) {
+            float z = s[k];
+            pair_sum_swap16(s[k], z);
+        }
+        if constexpr (TPR >= 64) {
+            float z = s[k];
+            pair_sum_swap32(s[k], z);
+        }
+    }
+    if constexpr (TPR > 64) {
+        constexpr int W = TPR / 64;
+        float* set = lds + turn * W * K;
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int k = 0; k < K; ++k) set[(threadIdx.x >> 6) * K + k] = s[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            s[k] = set[k];
+#pragma unroll
+            for (int i = 1; i < W; ++i) s[k] += set[i * K + k];
+        }
+    }
+}
+
+template <int DT, int TPR, int VPL, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_ln_fwd(const typename Elem<DT>::T* x, int64_t rows, int width,
+                                                    int64_t ldx, const void* w, const void* b, int wdt, float eps,
+                                                    typename Elem<DT>::T* y, float* stats) {
+    constexpr int V = kVec<DT>, G = THREADS / TPR;
+    __shared__ float lds[2 * THREADS / 64];
+    int turn = 0;
+    const int t = threadIdx.x % TPR;
+    float wv[VPL][V], bv[VPL][V];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        load_weights(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
+        load_weights(b, (j * TPR + t) * V, width, wdt, 0.0f, bv[j]);
+    }
+    const float inv = 1.0f / width;
+    for (int64_t row = int64_t(blockIdx.x) * G + threadIdx.x / TPR; row < rows; row += int64_t(gridDim.x) * G) {
+        float v[VPL][V], s[1] = {0};
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) load_vec<DT>(x + row * ldx, (j * TPR + t) * V, width, v[j]);
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[0] += v[j][e];
+        group_sum<TPR>(s, lds, turn);
+        const float mu = s[0] * inv;
+        s[0] = 0;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                v[j][e] = (j * TPR + t) * V + e < width ? v[j][e] - mu : 0.0f;
+                s[0] += v[j][e] * v[j][e];
+            }
+        group_sum<TPR>(s, lds, turn);
+        const float r = 1.0f / sqrtf(s[0] * inv + eps);
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[j][e] = v[j][e] * r * wv[j][e] + bv[j][e];
+            store_vec<DT>(y + row * width, (j * TPR + t) * V, width, v[j]);
+        }
+        if (t == 0) {
+            stats[row] = mu;
+            stats[rows + row] = r;
+        }
+    }
+}
+
+// Sums over the rows that the groups of a workgroup took: `acc` of each thread's columns, joined over the groups into
+// row blockIdx.x of partial (.., N, width), or as the results where there is one workgroup.
+template <int DT, int TPR, int VPL, int N, int THREADS>
+__device__ __forceinline__ void join_groups(const float (&acc)[N][VPL][kVec<DT>], float* lds, int width,
+                                            float* partial, void* const (&result)[N], int wdt) {
+    constexpr int V = kVec<DT>, G = THREADS / TPR, C = TPR * V;  // columns of a vector index
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < V; ++e) lds[n * THREADS * V + threadIdx.x * V + e] = acc[n][j][e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < N * C; i += THREADS) {
+            const int n = i / C, c = i % C, col = j * C + c;
+            if (col >= width) continue;
+            float s = lds[n * THREADS * V + c];
+            for (int g = 1; g < G; ++g) s += lds[n * THREADS * V + g * C + c];
+            if (gridDim.x > 1) partial[(int64_t(blockIdx.x) * N + n) * width + col] = s;
+            else if (result[n]) store_elem(result[n], col, wdt, s);
+        }
+    }
+}
+
+template <int DT, int TPR, int VPL, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_ln_bwd(const typename Elem<DT>::T* g, int64_t ldg,
+                                                    const typename Elem<DT>::T* x, int64_t ldx, int64_t rows,
+                                                    int width, const void* w, int wdt, const float* stats,
+                                                    typename Elem<DT>::T* gx, float* partial, void* gw, void* gb,
+                                                    int sums) {
+    constexpr int V = kVec<DT>, G = THREADS / TPR;
+    extern __shared__ float lds[];
+    int turn = 0;
+    const int t = threadIdx.x % TPR;
+    float wv[VPL][V], acc[2][VPL][V] = {};
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) load_weights(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
+    const float inv = 1.0f / width;
+    for (int64_t row = int64_t(blockIdx.x) * G + threadIdx.x / TPR; row < rows; row += int64_t(gridDim.x) * G) {
+        float h[VPL][V], a[VPL][V], s[2] = {0, 0};
+        const float mu = stats[row], r = stats[rows + row];
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            load_vec<DT>(x + row * ldx, (j * TPR + t) * V, width, h[j]);
+            load_vec<DT>(g + row * ldg, (j * TPR + t) * V, width, a[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {  // past the end a and wv are 0, and h is not stored
+                h[j][e] = (h[j][e] - mu) * r;
+                acc[0][j][e] += a[j][e] * h[j][e];
+                acc[1][j][e] += a[j][e];
+                a[j][e] *= wv[j][e];
+                s[0] += a[j][e];
+                s[1] += a[j][e] * h[j][e];
+            }
+        if (!gx) continue;
+        group_sum<TPR>(s, lds, turn);
+        const float sa = s[0] * inv, sah = s[1] * inv;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) a[j][e] = r * (a[j][e] - sa - h[j][e] * sah);
+            store_vec<DT>(gx + row * width, (j * TPR + t) * V, width, a[j]);
+        }
+    }
+    if (sums) join_groups<DT, TPR, VPL, 2, THREADS>(acc, lds, width, partial, {gw, gb}, wdt);
+}
+
+template <int DT, int TPR, int VPL, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_ln_bwd2(const typename Elem<DT>::T* g, int64_t ldg,
+                                                     const typename Elem<DT>::T* x, int64_t ldx,
+                                                     const typename Elem<DT>::T* u, int64_t ldu, int64_t rows,
+                                                     int width, const void* w, const void* p, const void* q, int wdt,
+                                                     const float* stats, typename Elem<DT>::T* dg,
+                                                     typename Elem<DT>::T* dx, float* partial, void* dw, int sums) {
+    constexpr int V = kVec<DT>, G = THREADS / TPR;
+    extern __shared__ float lds[];
+    int turn = 0;
+    const int t = threadIdx.x % TPR;
+    float wv[VPL][V], pv[VPL][V], qv[VPL][V], acc[1][VPL][V] = {};
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        load_weights(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
+        load_weights(p, (j * TPR + t) * V, width, wdt, 0.0f, pv[j]);
+        load_weights(q, (j * TPR + t) * V, width, wdt, 0.0f, qv[j]);
+    }
+    const float inv = 1.0f / width;
+    for (int64_t row = int64_t(blockIdx.x) * G + threadIdx.x / TPR; row < rows; row += int64_t(gridDim.x) * G) {
+        float h[VPL][V], gv[VPL][V], uv[VPL][V], s[7] = {};
+        const float mu = stats[row], r = stats[rows + row];
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            load_vec<DT>(x + row * ldx, (j * TPR + t) * V, width, h[j]);
+            load_vec<DT>(g + row * ldg, (j * TPR + t) * V, width, gv[j]);
+            load_vec<DT>(u + row * ldu, (j * TPR + t) * V, width, uv[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {  // past the end gv, uv and the weights are 0
+                h[j][e] = (h[j][e] - mu) * r;
+                const float a = gv[j][e] * wv[j][e], b = gv[j][e] * pv[j][e];
+                s[0] += a;
+                s[1] += a * h[j][e];
+                s[2] += uv[j][e];
+                s[3] += uv[j][e] * h[j][e];
+                s[4] += uv[j][e] * a;
+                s[5] += b;
+                s[6] += b * h[j][e];
+            }
+        group_sum<TPR>(s, lds, turn);
+        const float sa = s[0] * inv, sah = s[1] * inv, su = s[2] * inv, suh = s[3] * inv, sua = s[4] * inv;
+        const float sb = s[5] * inv, sbh = s[6] * inv;
+        const float phi = r * (sua - su * sa - suh * sah);  // mean(u J a)
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float hv = h[j][e], gg = gv[j][e];
+                const float ju = r * (uv[j][e] - su - hv * suh), ja = r * (gg * wv[j][e] - sa - hv * sah);
+                const float jb = r * (gg * pv[j][e] - sb - hv * sbh);
+                acc[0][j][e] += gg * ju;
+                gv[j][e] = wv[j][e] * ju + pv[j][e] * hv + qv[j][e];
+                uv[j][e] = jb - r * (sah * ju + suh * ja) - r * hv * phi;
+            }
+            store_vec<DT>(dg + row * width, (j * TPR + t) * V, width, gv[j]);
+            store_vec<DT>(dx + row * width, (j * TPR + t) * V, width, uv[j]);
+        }
+    }
+    if (sums) join_groups<DT, TPR, VPL, 1, THREADS>(acc, lds, width, partial, {dw}, wdt);
+}
+
+// Joins the workgroups' sums: partial (parts, N, width).  64 columns a workgroup, its 16 wavefronts each a
+// sixteenth of the parts.
+__global__ __launch_bounds__(1024) void k_ln_join(const float* partial, int parts, int N, int width, int wdt, void* r0,
+                                                  void* r1) {
+    __shared__ float part[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t all = int64_t(N) * width, col = int64_t(blockIdx.x) * 64 + lane;
+    float s = 0;
+    if (col < all)
+        for (int i = wave; i < parts; i += 16) s += partial[i * all + col];
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave || col >= all) return;
+    for (int i = 1; i < 16; ++i) s += part[i][lane];
+    void* r = col < width ? r0 : r1;
+    if (r) store_elem(r, col < width ? col : col - width, wdt, s);
+}
+
+// Rows too wide for a workgroup's registers: a workgroup takes a row and reads it again for each sum (from L2: a row is
+// at most a few hundred KB where many are in flight), and the column sums are a launch of their own.
 template <int DT>
-__global__ __launch_bounds__(256) void k_ln_fwd(const typename Elem<DT>::T* x, int64_t rows, int width, int64_t ldx,
+__global__ __launch_bounds__(256) void k_ln_fwd_wide(const typename Elem<DT>::T* x, int64_t rows, int width, int64_t ldx,
                                                 const void* w, const void* b, int wdt, float eps,
                                                 typename Elem<DT>::T* y, float* stats) {
     using T = typename Elem<DT>::T;
-    const int lane = threadIdx.x & 63;
-    const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const T* xr = x + row * ldx;
-    const float inv = 1.0f / width;
-    float s = 0;
-    for (int c = lane; c < width; c += 64) s += float(xr[c]);
-    const float mu = wave_sum(s) * inv;
-    s = 0;
-    for (int c = lane; c < width; c += 64) {
-        const float d = float(xr[c]) - mu;
-        s += d * d;
-    }
-    const float r = 1.0f / sqrtf(wave_sum(s) * inv + eps);
-    for (int c = lane; c < width; c += 64) {
-        const float h = (float(xr[c]) - mu) * r;
-        y[row * width + c] = T(h * (w ? load_elem(w, c, wdt) : 1.0f) + (b ? load_elem(b, c, wdt) : 0.0f));
-    }
-    if (lane == 0) {
-        stats[row] = mu;
-        stats[rows + row] = r;
+    __shared__ float lds[2 * 4 * 7];
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T* xr = x + row * ldx;
+        const float inv = 1.0f / width;
+        float s[1] = {0};
+        for (int c = threadIdx.x; c < width; c += 256) s[0] += float(xr[c]);
+        group_sum<256>(s, lds, turn);
+        const float mu = s[0] * inv;
+        s[0] = 0;
+        for (int c = threadIdx.x; c < width; c += 256) {
+            const float d = float(xr[c]) - mu;
+            s[0] += d * d;
+        }
+        group_sum<256>(s, lds, turn);
+        const float r = 1.0f / sqrtf(s[0] * inv + eps);
+        for (int c = threadIdx.x; c < width; c += 256) {
+            const float h = (float(xr[c]) - mu) * r;
+            y[row * width + c] = T(h * (w ? load_elem(w, c, wdt) : 1.0f) + (b ? load_elem(b, c, wdt) : 0.0f));
+        }
+        if (threadIdx.x == 0) {
+            stats[row] = mu;
+            stats[rows + row] = r;
+        }
     }
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void k_ln_bwd(const typename Elem<DT>::T* g, int64_t ldg,
+__global__ __launch_bounds__(256) void k_ln_bwd_wide(const typename Elem<DT>::T* g, int64_t ldg,
                                                 const typename Elem<DT>::T* x, int64_t ldx, int64_t rows, int width,
                                                 const void* w, int wdt, const float* stats,
                                                 typename Elem<DT>::T* gx) {
     using T = typename Elem<DT>::T;
-    const int lane = threadIdx.x & 63;
-    const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const T *xr = x + row * ldx, *gr = g + row * ldg;
-    const float mu = stats[row], r = stats[rows + row], inv = 1.0f / width;
-    float sa = 0, sah = 0;
-    for (int c = lane; c < width; c += 64) {
-        const float a = float(gr[c]) * (w ? load_elem(w, c, wdt) : 1.0f);
-        sa += a;
-        sah += a * ((float(xr[c]) - mu) * r);
-    }
-    sa = wave_sum(sa) * inv;
-    sah = wave_sum(sah) * inv;
-    for (int c = lane; c < width; c += 64) {
-        const float a = float(gr[c]) * (w ? load_elem(w, c, wdt) : 1.0f), h = (float(xr[c]) - mu) * r;
-        gx[row * width + c] = T(r * (a - sa - h * sah));
+    __shared__ float lds[2 * 4 * 7];
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T *xr = x + row * ldx, *gr = g + row * ldg;
+        const float mu = stats[row], r = stats[rows + row], inv = 1.0f / width;
+        float s[2] = {0, 0};
+        for (int c = threadIdx.x; c < width; c += 256) {
+            const float a = float(gr[c]) * (w ? load_elem(w, c, wdt) : 1.0f);
+            s[0] += a;
+            s[1] += a * ((float(xr[c]) - mu) * r);
+        }
+        group_sum<256>(s, lds, turn);
+        const float sa = s[0] * inv, sah = s[1] * inv;
+        for (int c = threadIdx.x; c < width; c += 256) {
+            const float a = float(gr[c]) * (w ? load_elem(w, c, wdt) : 1.0f), h = (float(xr[c]) - mu) * r;
+            gx[row * width + c] = T(r * (a - sa - h * sah));
+        }
     }
 }
 
-// Second order, row part; mean(u) and mean(u h) are left for the column sums.
+// Second order, row part; mean(u) and mean(u h) go to the column sums.
 template <int DT>
-__global__ __launch_bounds__(256) void k_ln_bwd2(const typename Elem<DT>::T* g, int64_t ldg,
+__global__ __launch_bounds__(256) void k_ln_bwd2_wide(const typename Elem<DT>::T* g, int64_t ldg,
                                                  const typename Elem<DT>::T* x, int64_t ldx,
                                                  const typename Elem<DT>::T* u, int64_t ldu, int64_t rows, int width,
                                                  const void* w, const void* p, const void* q, int wdt,
                                                  const float* stats, typename Elem<DT>::T* dg,
                                                  typename Elem<DT>::T* dx, float* usums) {
     using T = typename Elem<DT>::T;
-    const int lane = threadIdx.x & 63;
-    const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const T *xr = x + row * ldx, *gr = g + row * ldg, *ur = u + row * ldu;
-    const float mu = stats[row], r = stats[rows + row], inv = 1.0f / width;
-    float sa = 0, sah = 0, su = 0, suh = 0, sua = 0, sb = 0, sbh = 0;
-    for (int c = lane; c < width; c += 64) {
-        const float gv = gr[c], h = (float(xr[c]) - mu) * r, uv = ur[c];
-        const float a = gv * (w ? load_elem(w, c, wdt) : 1.0f), b = p ? gv * load_elem(p, c, wdt) : 0.0f;
-        sa += a;
-        sah += a * h;
-        su += uv;
-        suh += uv * h;
-        sua += uv * a;
-        sb += b;
-        sbh += b * h;
-    }
-    sa = wave_sum(sa) * inv, sah = wave_sum(sah) * inv, su = wave_sum(su) * inv, suh = wave_sum(suh) * inv;
-    sua = wave_sum(sua) * inv, sb = wave_sum(sb) * inv, sbh = wave_sum(sbh) * inv;
-    const float phi = r * (sua - su * sa - suh * sah);  // mean(u J a)
-    for (int c = lane; c < width; c += 64) {
-        const float gv = gr[c], h = (float(xr[c]) - mu) * r, uv = ur[c], wv = w ? load_elem(w, c, wdt) : 1.0f;
-        const float pv = p ? load_elem(p, c, wdt) : 0.0f, a = gv * wv;
-        const float ju = r * (uv - su - h * suh), ja = r * (a - sa - h * sah), jb = r * (gv * pv - sb - h * sbh);
-        dg[row * width + c] = T(wv * ju + pv * h + (q ? load_elem(q, c, wdt) : 0.0f));
-        dx[row * width + c] = T(jb - r * (sah * ju + suh * ja) - r * h * phi);
-    }
-    if (lane == 0) {
-        usums[row] = su;
-        usums[rows + row] = suh;
+    __shared__ float lds[2 * 4 * 7];
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T *xr = x + row * ldx, *gr = g + row * ldg, *ur = u + row * ldu;
+        const float mu = stats[row], r = stats[rows + row], inv = 1.0f / width;
+        float s[7] = {};
+        for (int c = threadIdx.x; c < width; c += 256) {
+            const float gv = gr[c], h = (float(xr[c]) - mu) * r, uv = ur[c];
+            const float a = gv * (w ? load_elem(w, c, wdt) : 1.0f), b = p ? gv * load_elem(p, c, wdt) : 0.0f;
+            s[0] += a;
+            s[1] += a * h;
+            s[2] += uv;
+            s[3] += uv * h;
+            s[4] += uv * a;
+            s[5] += b;
+            s[6] += b * h;
+        }
+        group_sum<256>(s, lds, turn);
+        const float sa = s[0] * inv, sah = s[1] * inv, su = s[2] * inv, suh = s[3] * inv, sua = s[4] * inv;
+        const float sb = s[5] * inv, sbh = s[6] * inv;
+        const float phi = r * (sua - su * sa - suh * sah);  // mean(u J a)
+        for (int c = threadIdx.x; c < width; c += 256) {
+            const float gv = gr[c], h = (float(xr[c]) - mu) * r, uv = ur[c], wv = w ? load_elem(w, c, wdt) : 1.0f;
+            const float pv = p ? load_elem(p, c, wdt) : 0.0f, a = gv * wv;
+            const float ju = r * (uv - su - h * suh), ja = r * (a - sa - h * sah), jb = r * (gv * pv - sb - h * sbh);
+            dg[row * width + c] = T(wv * ju + pv * h + (q ? load_elem(q, c, wdt) : 0.0f));
+            dx[row * width + c] = T(jb - r * (sah * ju + suh * ja) - r * h * phi);
+        }
+        if (threadIdx.x == 0) {
+            usums[row] = su;
+            usums[rows + row] = suh;
+        }
     }
 }
 
@@ -138,46 +427,75 @@ __global__ __launch_bounds__(256) void k_ln_cols(const typename Elem<DT>::T* g, 
     }
 }
 
-__global__ __launch_bounds__(256) void k_ln_cols_join(const float* partial, int strips, int width, int wdt, void* gw,
-                                                      void* gb) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= width) return;
-    float s0 = 0, s1 = 0;
-    for (int s = 0; s < strips; ++s) {
-        s0 += partial[int64_t(2 * s) * width + c];
-        s1 += partial[int64_t(2 * s + 1) * width + c];
-    }
-    if (gw) store_elem(gw, c, wdt, s0);
-    if (gb) store_elem(gb, c, wdt, s1);
+// A variant by the vectors of a row: as few threads a row as hold it in up to `Most` values each, a wavefront at most
+// where that is enough, so that its sums need no barrier (8192 x 1024 fp32: MEASURE).  Calls f(TPR, VPL) with
+// the two as integral constants; false where no variant holds the row.
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+template <typename F>
+static void with_type(int dtype, F&& f) {
+    if (dtype == kF32) f(Int<kF32>());
+    else if (dtype == kBF16) f(Int<kBF16>());
+    else f(Int<kF16>());
 }
 
+template <int DT, int Most, typename F>
+static bool ln_variant(int64_t width, F&& f) {
+    constexpr int V = kVec<DT>;
+    const int64_t nv = ceil_div(width, V);
+    if (nv <= 8) return f(Int<8>(), Int<1>()), true;
+    if (nv <= 16) return f(Int<16>(), Int<1>()), true;
+    if (nv <= 32) return f(Int<32>(), Int<1>()), true;
+    if (nv <= 64) return f(Int<64>(), Int<1>()), true;
+    if (nv <= 128) return f(Int<64>(), Int<2>()), true;
+    if constexpr (Most / V >= 4) {
+        if (nv <= 192) return f(Int<64>(), Int<3>()), true;
+        if (nv <= 256) return f(Int<64>(), Int<4>()), true;
+    }
+    if constexpr (Most / V >= 8)
+        if (nv <= 512) return f(Int<64>(), Int<8>()), true;
+    if (nv <= 256) return f(Int<256>(), Int<1>()), true;
+    if (nv <= 512) return f(Int<256>(), Int<2>()), true;
+    if constexpr (Most / V >= 4)
+        if (nv <= 1024) return f(Int<256>(), Int<4>()), true;
+    if (nv <= 1024) return f(Int<512>(), Int<2>()), true;
+    if constexpr (Most / V >= 4)
+        if (nv <= 2048) return f(Int<512>(), Int<4>()), true;
+    return false;
+}
+
+// Values of a row a thread holds at most: forward (three arrays of them in registers), backward (five), second order
+// (seven).
+constexpr int kLnMost = 32, kLnMost1 = 32, kLnMost2 = 16;
+constexpr int kLnParts = 512;  // workgroups of the backward kernels at most, so rows of partial sums
+constexpr int ln_threads(int tpr) { return tpr > 64 ? tpr : 512; }  // of their workgroups
+
+// Strips of rows of the wide form's column sums.
 static int ln_strips(int64_t rows) { return int(std::max<int64_t>(1, std::min<int64_t>(256, rows / 64))); }
+
+// Workgroups of a backward kernel whose workgroup takes `groups` rows at a time.
+static int64_t ln_parts(const void* kernel, int threads, int64_t rows, int groups) {
+    const int64_t need = std::min<int64_t>(std::max<int64_t>(ceil_div(rows, groups), 1), kLnParts);
+    return device_fill_grid(kernel, threads, need);
+}
+
+constexpr int64_t kLnWideGrid = 1 << 16;
+static size_t ln_partial_floats(int64_t rows, int64_t width) {
+    return size_t(std::min<int64_t>(std::max<int64_t>(rows, 1), kLnParts)) * 2 * size_t(width);
+}
 
 static int ln_check(const char* what, int64_t rows, int64_t width, int dtype, int wdtype) {
     MNX_REQUIRE(elem_valid(dtype) && elem_valid(wdtype), "%s: unknown element type", what);
     MNX_REQUIRE(rows >= 0 && width >= 1 && width <= MNX_LAYER_NORM_MAX_WIDTH, "%s: rows >= 0, 1 <= width <= %d", what,
                 MNX_LAYER_NORM_MAX_WIDTH);
-    MNX_REQUIRE(rows <= (int64_t(1) << 32), "%s: too many rows", what);
+    MNX_REQUIRE(rows <= (int64_t(1) << 40), "%s: too many rows", what);
     return MNX_OK;
 }
 
 }  // namespace mnx
 
 using namespace mnx;
-
-#define LN_DISPATCH(dtype, CALL)          \
-    do {                                  \
-        if ((dtype) == kF32) {            \
-            constexpr int DT = kF32;      \
-            CALL;                         \
-        } else if ((dtype) == kBF16) {    \
-            constexpr int DT = kBF16;     \
-            CALL;                         \
-        } else {                          \
-            constexpr int DT = kF16;      \
-            CALL;                         \
-        }                                 \
-    } while (0)
 
 extern "C" {
 
@@ -187,29 +505,43 @@ int mnx_layer_norm_fwd(const void* x, int64_t ldx, int64_t rows, int64_t width, 
     if (int rc = ln_check("layer norm", rows, width, dtype, wdtype)) return rc;
     if (rows == 0) return MNX_OK;
     MNX_REQUIRE(x && y && stats && ldx >= width, "layer norm: null pointer or ldx < width");
-    LN_DISPATCH(dtype, (k_ln_fwd<DT><<<ceil_div(rows, 4), 256, 0, stream>>>(
-                           static_cast<const Elem<DT>::T*>(x), rows, int(width), ldx, weight, bias, wdtype, float(eps),
-                           static_cast<Elem<DT>::T*>(y), stats)));
+    int64_t grid = 0;
+    with_type(dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        using T = typename Elem<DT>::T;
+        const T* xs = static_cast<const T*>(x);
+        T* ys = static_cast<T*>(y);
+        const bool held = ln_variant<DT, kLnMost>(width, [&](auto tpr, auto vpl) {
+            constexpr int TPR = decltype(tpr)::value, VPL = decltype(vpl)::value, THREADS = TPR > 256 ? TPR : 256;
+            const auto kernel = k_ln_fwd<DT, TPR, VPL, THREADS>;
+            grid = device_fill_grid(reinterpret_cast<const void*>(kernel), THREADS, ceil_div(rows, THREADS / TPR));
+            if (grid > 0)
+                kernel<<<grid, THREADS, 0, stream>>>(xs, rows, int(width), ldx, weight, bias, wdtype, float(eps), ys,
+                                                     stats);
+        });
+        if (!held) {
+            grid = std::min<int64_t>(rows, kLnWideGrid);
+            k_ln_fwd_wide<DT><<<grid, 256, 0, stream>>>(xs, rows, int(width), ldx, weight, bias, wdtype, float(eps), ys,
+                                                        stats);
+        }
+    });
+    MNX_REQUIRE(grid > 0, "layer norm: device query failed");
     MNX_CHECK_LAUNCH();
     return MNX_OK;
 }
 
 size_t mnx_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width) {
     Workspace ws{nullptr, 0};
-    ws.take<float>(size_t(ln_strips(rows)) * 2 * size_t(std::max<int64_t>(width, 1)));
-    ws.take<float>(size_t(std::max<int64_t>(rows, 0)) * 2);
+    rows = std::max<int64_t>(rows, 0);
+    ws.take<float>(ln_partial_floats(rows, std::max<int64_t>(width, 1)));
+    ws.take<float>(size_t(rows) * 2);
     return ws.used;
 }
 
-static int ln_cols(const void* g, int64_t ldg, const void* x, int64_t ldx, const void* u, int64_t ldu, int64_t rows,
-                   int64_t width, int dtype, int wdtype, const float* stats, const float* usums, float* partial,
-                   void* gw, void* gb, mnx_stream_t stream) {
-    const int strips = ln_strips(rows);
-    LN_DISPATCH(dtype, (k_ln_cols<DT><<<dim3(ceil_div(width, 64), strips), 256, 0, stream>>>(
-                           static_cast<const Elem<DT>::T*>(g), ldg, static_cast<const Elem<DT>::T*>(x), ldx,
-                           static_cast<const Elem<DT>::T*>(u), ldu, rows, int(width), stats, usums, partial)));
-    MNX_CHECK_LAUNCH();
-    k_ln_cols_join<<<ceil_div(width, 256), 256, 0, stream>>>(partial, strips, int(width), wdtype, gw, gb);
+// `parts` rows of sums in `partial`, joined into the results.
+static int ln_join(const float* partial, int64_t parts, int N, int64_t width, int wdtype, void* r0, void* r1,
+                   mnx_stream_t stream) {
+    k_ln_join<<<ceil_div(N * width, 64), 1024, 0, stream>>>(partial, int(parts), N, int(width), wdtype, r0, r1);
     MNX_CHECK_LAUNCH();
     return MNX_OK;
 }
@@ -222,18 +554,41 @@ int mnx_layer_norm_bwd(const void* grad, int64_t ldg, const void* x, int64_t ldx
     if (int rc = ln_check("layer norm backward", rows, width, dtype, wdtype)) return rc;
     MNX_REQUIRE(rows == 0 || (grad && x && stats && ldg >= width && ldx >= width),
                 "layer norm backward: null pointer or a row stride below the width");
-    if (rows && grad_x) {
-        LN_DISPATCH(dtype, (k_ln_bwd<DT><<<ceil_div(rows, 4), 256, 0, stream>>>(
-                               static_cast<const Elem<DT>::T*>(grad), ldg, static_cast<const Elem<DT>::T*>(x), ldx,
-                               rows, int(width), weight, wdtype, stats, static_cast<Elem<DT>::T*>(grad_x))));
-        MNX_CHECK_LAUNCH();
-    }
-    if (!grad_weight && !grad_bias) return MNX_OK;
-    Workspace ws{static_cast<char*>(workspace), workspace_bytes};
-    float* partial = ws.take<float>(size_t(ln_strips(rows)) * 2 * width);
-    if (!workspace || !ws.fits()) return set_error(MNX_ERR_WORKSPACE, "layer norm backward: workspace too small");
-    return ln_cols(grad, ldg, x, ldx, nullptr, 0, rows, width, dtype, wdtype, stats, nullptr, partial, grad_weight,
-                   grad_bias, stream);
+    const bool sums = grad_weight || grad_bias;
+    if (!sums && (!rows || !grad_x)) return MNX_OK;
+    float* partial = static_cast<float*>(workspace);
+    if (sums && (!workspace || workspace_bytes < mnx_layer_norm_bwd_workspace_bytes(rows, width)))
+        return set_error(MNX_ERR_WORKSPACE, "layer norm backward: workspace too small");
+    int64_t parts = 0;
+    bool held = true;
+    with_type(dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        using T = typename Elem<DT>::T;
+        const T *gs = static_cast<const T*>(grad), *xs = static_cast<const T*>(x);
+        T* gx = static_cast<T*>(grad_x);
+        held = ln_variant<DT, DT == kF32 ? kLnMost1 : kLnMost1 / 2>(width, [&](auto tpr, auto vpl) {
+            constexpr int TPR = decltype(tpr)::value, VPL = decltype(vpl)::value, THREADS = ln_threads(TPR);
+            const auto kernel = k_ln_bwd<DT, TPR, VPL, THREADS>;
+            const size_t lds = size_t(2) * THREADS * kVec<DT> * sizeof(float);
+            parts = ln_parts(reinterpret_cast<const void*>(kernel), THREADS, rows, THREADS / TPR);
+            if (parts > 0)
+                kernel<<<parts, THREADS, lds, stream>>>(gs, ldg, xs, ldx, rows, int(width), weight, wdtype, stats, gx,
+                                                        partial, grad_weight, grad_bias, sums);
+        });
+        if (!held) {
+            if (rows && gx)
+                k_ln_bwd_wide<DT><<<std::min<int64_t>(rows, kLnWideGrid), 256, 0, stream>>>(
+                    gs, ldg, xs, ldx, rows, int(width), weight, wdtype, stats, gx);
+            parts = ln_strips(rows);
+            if (sums)
+                k_ln_cols<DT><<<dim3(ceil_div(width, 64), parts), 256, 0, stream>>>(
+                    gs, ldg, xs, ldx, nullptr, 0, rows, int(width), stats, nullptr, partial);
+        }
+    });
+    MNX_REQUIRE(parts > 0, "layer norm backward: device query failed");
+    MNX_CHECK_LAUNCH();
+    if (!sums || (held && parts == 1)) return MNX_OK;
+    return ln_join(partial, parts, 2, width, wdtype, grad_weight, grad_bias, stream);
 }
 
 int mnx_layer_norm_bwd2(const void* grad, int64_t ldg, const void* x, int64_t ldx, const void* seed_x, int64_t ldu,
@@ -245,21 +600,42 @@ int mnx_layer_norm_bwd2(const void* grad, int64_t ldg, const void* x, int64_t ld
     MNX_REQUIRE(rows == 0 || (grad && x && seed_x && stats && dgrad && dx && ldg >= width && ldx >= width &&
                               ldu >= width),
                 "layer norm second order: null pointer or a row stride below the width");
+    if (!rows && !dweight) return MNX_OK;
     Workspace ws{static_cast<char*>(workspace), workspace_bytes};
-    float* partial = ws.take<float>(size_t(ln_strips(rows)) * 2 * width);
+    float* partial = ws.take<float>(ln_partial_floats(rows, width));
     float* usums = ws.take<float>(size_t(rows) * 2);
     if (!workspace || !ws.fits()) return set_error(MNX_ERR_WORKSPACE, "layer norm second order: workspace too small");
-    if (rows) {
-        LN_DISPATCH(dtype, (k_ln_bwd2<DT><<<ceil_div(rows, 4), 256, 0, stream>>>(
-                               static_cast<const Elem<DT>::T*>(grad), ldg, static_cast<const Elem<DT>::T*>(x), ldx,
-                               static_cast<const Elem<DT>::T*>(seed_x), ldu, rows, int(width), weight, seed_w, seed_b,
-                               wdtype, stats, static_cast<Elem<DT>::T*>(dgrad), static_cast<Elem<DT>::T*>(dx),
-                               usums)));
-        MNX_CHECK_LAUNCH();
-    }
-    if (!dweight) return MNX_OK;
-    return ln_cols(grad, ldg, x, ldx, seed_x, ldu, rows, width, dtype, wdtype, stats, usums, partial, dweight, nullptr,
-                   stream);
+    int64_t parts = 0;
+    bool held = true;
+    with_type(dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        using T = typename Elem<DT>::T;
+        const T *gs = static_cast<const T*>(grad), *xs = static_cast<const T*>(x), *us = static_cast<const T*>(seed_x);
+        T *dg = static_cast<T*>(dgrad), *dxs = static_cast<T*>(dx);
+        held = ln_variant<DT, kLnMost2>(width, [&](auto tpr, auto vpl) {
+            constexpr int TPR = decltype(tpr)::value, VPL = decltype(vpl)::value, THREADS = ln_threads(TPR);
+            const auto kernel = k_ln_bwd2<DT, TPR, VPL, THREADS>;
+            const size_t lds = size_t(THREADS) * kVec<DT> * sizeof(float);
+            parts = ln_parts(reinterpret_cast<const void*>(kernel), THREADS, rows, THREADS / TPR);
+            if (parts > 0)
+                kernel<<<parts, THREADS, lds, stream>>>(gs, ldg, xs, ldx, us, ldu, rows, int(width), weight, seed_w,
+                                                        seed_b, wdtype, stats, dg, dxs, partial, dweight, !!dweight);
+        });
+        if (!held) {
+            if (rows)
+                k_ln_bwd2_wide<DT><<<std::min<int64_t>(rows, kLnWideGrid), 256, 0, stream>>>(
+                    gs, ldg, xs, ldx, us, ldu, rows, int(width), weight, seed_w, seed_b, wdtype, stats, dg, dxs, usums);
+            parts = ln_strips(rows);
+            if (dweight)
+                k_ln_cols<DT><<<dim3(ceil_div(width, 64), parts), 256, 0, stream>>>(
+                    gs, ldg, xs, ldx, us, ldu, rows, int(width), stats, usums, partial);
+        }
+    });
+    MNX_REQUIRE(parts > 0, "layer norm second order: device query failed");
+    MNX_CHECK_LAUNCH();
+    if (!dweight || (held && parts == 1)) return MNX_OK;
+    // the wide form leaves (strips, 2, width) with the sums in the first half
+    return ln_join(partial, parts, held ? 1 : 2, width, wdtype, dweight, nullptr, stream);
 }
 
 }  // extern "C"
