@@ -54,11 +54,25 @@ __device__ __forceinline__ void store_vec(typename Elem<DT>::T* p, int c, int wi
             if (c + e < width) p[c + e] = T(v[e]);
     }
 }
-// Values of a vector of weights; `none` where there is no vector and past the end 0.
-template <int N>
-__device__ __forceinline__ void load_weights(const void* p, int c, int width, int dtype, float none, float (&v)[N]) {
+// Values of a vector of weights, of the rows' type or float32; `none` where there is no vector, 0 past the end.
+template <int DT>
+__device__ __forceinline__ void load_weights(const void* p, int c, int width, int dtype, float none,
+                                             float (&v)[kVec<DT>]) {
+    constexpr int V = kVec<DT>;
+    if (!p) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = c + e < width ? (p ? load_elem(p, c + e, dtype) : none) : 0.0f;
+        for (int e = 0; e < V; ++e) v[e] = c + e < width ? none : 0.0f;
+    } else if (DT == kF32 || dtype == DT) {
+        load_vec<DT>(static_cast<const typename Elem<DT>::T*>(p), c, width, v);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; k += 4) {
+            float f[4];
+            load_vec<kF32>(static_cast<const float*>(p), c + k, width, f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[k + e] = f[e];
+        }
+    }
 }
 
 // K sums over the TPR threads of a group, on all of them.  More than a wavefront joins through `lds` (K floats a
@@ -108,8 +122,8 @@ __global__ __launch_bounds__(THREADS) void k_ln_fwd(const typename Elem<DT>::T* 
     float wv[VPL][V], bv[VPL][V];
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-        load_weights(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
-        load_weights(b, (j * TPR + t) * V, width, wdt, 0.0f, bv[j]);
+        load_weights<DT>(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
+        load_weights<DT>(b, (j * TPR + t) * V, width, wdt, 0.0f, bv[j]);
     }
     const float inv = 1.0f / width;
     for (int64_t row = int64_t(blockIdx.x) * G + threadIdx.x / TPR; row < rows; row += int64_t(gridDim.x) * G) {
@@ -182,7 +196,7 @@ __global__ __launch_bounds__(THREADS) void k_ln_bwd(const typename Elem<DT>::T* 
     const int t = threadIdx.x % TPR;
     float wv[VPL][V], acc[2][VPL][V] = {};
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) load_weights(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
+    for (int j = 0; j < VPL; ++j) load_weights<DT>(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
     const float inv = 1.0f / width;
     for (int64_t row = int64_t(blockIdx.x) * G + threadIdx.x / TPR; row < rows; row += int64_t(gridDim.x) * G) {
         float h[VPL][V], a[VPL][V], s[2] = {0, 0};
@@ -230,9 +244,9 @@ __global__ __launch_bounds__(THREADS) void k_ln_bwd2(const typename Elem<DT>::T*
     float wv[VPL][V], pv[VPL][V], qv[VPL][V], acc[1][VPL][V] = {};
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-        load_weights(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
-        load_weights(p, (j * TPR + t) * V, width, wdt, 0.0f, pv[j]);
-        load_weights(q, (j * TPR + t) * V, width, wdt, 0.0f, qv[j]);
+        load_weights<DT>(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
+        load_weights<DT>(p, (j * TPR + t) * V, width, wdt, 0.0f, pv[j]);
+        load_weights<DT>(q, (j * TPR + t) * V, width, wdt, 0.0f, qv[j]);
     }
     const float inv = 1.0f / width;
     for (int64_t row = int64_t(blockIdx.x) * G + threadIdx.x / TPR; row < rows; row += int64_t(gridDim.x) * G) {
@@ -280,20 +294,22 @@ __global__ __launch_bounds__(THREADS) void k_ln_bwd2(const typename Elem<DT>::T*
     if (sums) join_groups<DT, TPR, VPL, 1, THREADS>(acc, lds, width, partial, {dw}, wdt);
 }
 
-// Joins the workgroups' sums: partial (parts, N, width).  64 columns a workgroup, its 16 wavefronts each a
-// sixteenth of the parts.
+// Joins the workgroups' sums: partial (parts, N, width).  16 columns a workgroup, each thread every 64th part of one:
+// the sums of 512 parts are 8 loads deep, and a narrow row still gives many workgroups.
 __global__ __launch_bounds__(1024) void k_ln_join(const float* partial, int parts, int N, int width, int wdt, void* r0,
                                                   void* r1) {
-    __shared__ float part[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t all = int64_t(N) * width, col = int64_t(blockIdx.x) * 64 + lane;
+    __shared__ float part[64][16];
+    const int c = threadIdx.x & 15, group = threadIdx.x >> 4;
+    const int64_t all = int64_t(N) * width, col = int64_t(blockIdx.x) * 16 + c;
     float s = 0;
     if (col < all)
-        for (int i = wave; i < parts; i += 16) s += partial[i * all + col];
-    part[wave][lane] = s;
+#pragma unroll 8
+        for (int i = group; i < parts; i += 64) s += partial[i * all + col];
+    part[group][c] = s;
     __syncthreads();
-    if (wave || col >= all) return;
-    for (int i = 1; i < 16; ++i) s += part[i][lane];
+    if (group || col >= all) return;
+#pragma unroll
+    for (int i = 1; i < 64; ++i) s += part[i][c];
     void* r = col < width ? r0 : r1;
     if (r) store_elem(r, col < width ? col : col - width, wdt, s);
 }
@@ -442,25 +458,29 @@ static void with_type(int dtype, F&& f) {
 
 template <int DT, int Most, typename F>
 static bool ln_variant(int64_t width, F&& f) {
-    constexpr int V = kVec<DT>;
-    const int64_t nv = ceil_div(width, V);
+    constexpr int M = Most / kVec<DT>;
+    const int64_t nv = ceil_div(width, kVec<DT>);
     if (nv <= 8) return f(Int<8>(), Int<1>()), true;
     if (nv <= 16) return f(Int<16>(), Int<1>()), true;
     if (nv <= 32) return f(Int<32>(), Int<1>()), true;
+    if constexpr (M >= 3)
+        if (nv <= 48) return f(Int<16>(), Int<3>()), true;
     if (nv <= 64) return f(Int<64>(), Int<1>()), true;
+    if constexpr (M >= 3)
+        if (nv <= 96) return f(Int<32>(), Int<3>()), true;
     if (nv <= 128) return f(Int<64>(), Int<2>()), true;
-    if constexpr (Most / V >= 4) {
+    if constexpr (M >= 3)
         if (nv <= 192) return f(Int<64>(), Int<3>()), true;
+    if constexpr (M >= 4)
         if (nv <= 256) return f(Int<64>(), Int<4>()), true;
-    }
-    if constexpr (Most / V >= 8)
+    if constexpr (M >= 8)
         if (nv <= 512) return f(Int<64>(), Int<8>()), true;
     if (nv <= 256) return f(Int<256>(), Int<1>()), true;
     if (nv <= 512) return f(Int<256>(), Int<2>()), true;
-    if constexpr (Most / V >= 4)
+    if constexpr (M >= 4)
         if (nv <= 1024) return f(Int<256>(), Int<4>()), true;
     if (nv <= 1024) return f(Int<512>(), Int<2>()), true;
-    if constexpr (Most / V >= 4)
+    if constexpr (M >= 4)
         if (nv <= 2048) return f(Int<512>(), Int<4>()), true;
     return false;
 }
@@ -541,7 +561,7 @@ size_t mnx_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width) {
 // `parts` rows of sums in `partial`, joined into the results.
 static int ln_join(const float* partial, int64_t parts, int N, int64_t width, int wdtype, void* r0, void* r1,
                    mnx_stream_t stream) {
-    k_ln_join<<<ceil_div(N * width, 64), 1024, 0, stream>>>(partial, int(parts), N, int(width), wdtype, r0, r1);
+    k_ln_join<<<ceil_div(N * width, 16), 1024, 0, stream>>>(partial, int(parts), N, int(width), wdtype, r0, r1);
     MNX_CHECK_LAUNCH();
     return MNX_OK;
 }
