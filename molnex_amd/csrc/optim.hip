@@ -6,7 +6,9 @@
 //
 // The tensors' addresses travel in the kernels' arguments (a table of up to kTensors entries a launch), so a call
 // copies nothing to the device and can be captured in a graph; the step counts t, the norm and what follows from
-// them stay on the device.  A workgroup takes a chunk of one tensor.
+// them stay on the device.  A workgroup takes a chunk of one tensor, four elements a thread and vector.
+//
+// Bytes bound it: an element takes 28 (32-bit states, float32) or 16 (8-bit) and 4 more for the norm.
 //
 // 8-bit states: 256 elements of a tensor share two bases (int16).  A code c stands for the float32 with the bits
 // (base + c) << 20, exponent and 3 bits of mantissa, zero for c = 0: 7 bits of magnitude and a sign for m, 8 bits for
@@ -26,7 +28,15 @@ constexpr int kTensors = 64;       // tensors of one update launch: the table st
 constexpr int kNormTensors = 160;  // tensors of one norm launch
 constexpr int kStepTensors = 480;  // tensors of one launch of the step counts
 constexpr int kBlock = 256;        // elements of a block of 8-bit states
-constexpr int kChunk = 8192;       // elements a workgroup takes
+
+// Elements that a workgroup takes: a power of two of whole blocks for its four wavefronts.  Small calls are cut finer, so
+// that they reach every compute unit and no thread has several vectors to wait for; 8192 keeps what a workgroup reads
+// first (its tensor's entry and scalars) below a few per cent of its time.
+inline int chunk_of(int64_t total) {
+    int chunk = 1024;
+    while (chunk < 8192 && total / chunk > 2048) chunk *= 2;
+    return chunk;
+}
 
 struct AdamwTable {
     void* p[kTensors];
@@ -38,6 +48,7 @@ struct AdamwTable {
     uint32_t start[kTensors + 1];  // first chunk of each tensor
     uint8_t dtype[kTensors];
     int count, first;              // tensors here, number of the first one in the call
+    int chunk;
 };
 
 struct NormTable {
@@ -45,7 +56,7 @@ struct NormTable {
     int64_t n[kNormTensors];
     uint32_t start[kNormTensors + 1];
     uint8_t dtype[kNormTensors];
-    int count;
+    int count, chunk;
     int64_t out;  // place of the first chunk's partial sum
 };
 
@@ -79,38 +90,119 @@ __device__ __forceinline__ int find_tensor(const uint32_t* start, int count, uin
     return __builtin_amdgcn_readfirstlane(at - 1);
 }
 
-// Sums over the workgroup of 256, valid on thread 0.
+// Four consecutive elements, at the alignment of one; past `end` they are 0 and not stored.
+template <int DT>
+struct Four {
+    typedef typename Elem<DT>::T T;
+    typedef T Packed __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+};
+template <int DT>
+__device__ __forceinline__ void load4(const void* base, int64_t e, int64_t end, float (&v)[4]) {
+    const auto* p = static_cast<const typename Elem<DT>::T*>(base);
+    if (e + 4 <= end) {
+        const auto t = *reinterpret_cast<const typename Four<DT>::Packed*>(p + e);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = float(t[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = e + k < end ? float(p[e + k]) : 0.0f;
+    }
+}
+template <int DT>
+__device__ __forceinline__ void store4(void* base, int64_t e, int64_t end, const float (&v)[4]) {
+    using T = typename Elem<DT>::T;
+    auto* p = static_cast<T*>(base);
+    if (e + 4 <= end) {
+        typename Four<DT>::Packed t;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t[k] = T(v[k]);
+        *reinterpret_cast<typename Four<DT>::Packed*>(p + e) = t;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (e + k < end) p[e + k] = T(v[k]);
+    }
+}
+
+typedef uint32_t PackedU32 __attribute__((aligned(1)));
+typedef uint32_t Bases __attribute__((aligned(2)));  // m's base in the low half, v's in the high
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int64_t e, int64_t end) {
+    if (e + 4 <= end) return *reinterpret_cast<const PackedU32*>(p + e);
+    uint32_t c = 0;
+    for (int k = 0; k < 4; ++k)
+        if (e + k < end) c |= uint32_t(p[e + k]) << 8 * k;
+    return c;
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, int64_t e, int64_t end, uint32_t c) {
+    if (e + 4 <= end) {
+        *reinterpret_cast<PackedU32*>(p + e) = c;
+    } else {
+        for (int k = 0; k < 4; ++k)
+            if (e + k < end) p[e + k] = uint8_t(c >> 8 * k);
+    }
+}
+
+// The chunk that a workgroup takes.
+struct Chunk {
+    int tensor;
+    int64_t begin, end;
+};
+template <typename Table>
+__device__ __forceinline__ Chunk chunk_at(const Table& t, uint32_t at) {
+    const int i = find_tensor(t.start, t.count, at);
+    const int64_t begin = int64_t(at - t.start[i]) * t.chunk;
+    return {i, begin, min(t.n[i], begin + t.chunk)};
+}
+
+// Sums over the workgroup, on every thread.
+template <int THREADS>
 __device__ __forceinline__ double block_sum(double v) {
-    __shared__ double part[4];
+    __shared__ double part[THREADS / 64];
     for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = (part[0] + part[1]) + (part[2] + part[3]);
+    v = part[0];
+    for (int i = 1; i < THREADS / 64; ++i) v += part[i];
     __syncthreads();
     return v;
 }
 
 // Squares are summed in float64: no overflow where the norm itself has none, and the same last bits whatever the
 // order of the chunks.
-__global__ __launch_bounds__(256) void k_sumsq(const NormTable t, double* partial) {
-    const int i = find_tensor(t.start, t.count, blockIdx.x);
-    const int64_t begin = int64_t(blockIdx.x - t.start[i]) * kChunk, end = min(t.n[i], begin + kChunk);
-    double s = 0;
-    for (int64_t e = begin + threadIdx.x; e < end; e += 256) {
-        const double g = load_elem(t.g[i], e, t.dtype[i]);
-        s += g * g;
+template <int DT>
+__device__ __forceinline__ double sum_squares(const void* g, const Chunk& c) {
+    constexpr int U = 4;
+    double s[U] = {};
+    for (int64_t e = c.begin + threadIdx.x * 4; e < c.end; e += U * 1024) {
+        float v[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u) load4<DT>(g, e + u * 1024, c.end, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[u] = __builtin_fma(double(v[u][k]), double(v[u][k]), s[u]);
     }
-    s = block_sum(s);
+    return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+__global__ __launch_bounds__(256) void k_sumsq(const NormTable t, double* partial) {
+    const Chunk c = chunk_at(t, blockIdx.x);
+    const void* g = t.g[c.tensor];
+    const int dt = t.dtype[c.tensor];
+    const double s = block_sum<256>(dt == kF32    ? sum_squares<kF32>(g, c)
+                                    : dt == kBF16 ? sum_squares<kBF16>(g, c)
+                                                  : sum_squares<kF16>(g, c));
     if (threadIdx.x == 0) partial[t.out + blockIdx.x] = s;
 }
 
 __device__ __forceinline__ double sum_partial(const double* partial, int64_t chunks) {
     double s = 0;
-    for (int64_t i = threadIdx.x; i < chunks; i += 256) s += partial[i];
-    return block_sum(s);
+#pragma unroll 8
+    for (int64_t i = threadIdx.x; i < chunks; i += 1024) s += partial[i];
+    return block_sum<1024>(s);
 }
 
-__global__ __launch_bounds__(256) void k_norm(const double* partial, int64_t chunks, float* norm) {
+__global__ __launch_bounds__(1024) void k_norm(const double* partial, int64_t chunks, float* norm) {
     const double s = sum_partial(partial, chunks);
     if (threadIdx.x == 0) *norm = float(sqrt(s));
 }
@@ -124,7 +216,7 @@ __device__ __forceinline__ uint32_t mix(uint32_t x) {
 }
 
 // The step counts and everything that the update takes from them and from the norm, in float64.
-__global__ __launch_bounds__(256) void k_adamw_prepare(const StepTable t, const double* partial, int64_t chunks,
+__global__ __launch_bounds__(1024) void k_adamw_prepare(const StepTable t, const double* partial, int64_t chunks,
                                                        const float* norm_in, float* norm_out, double max_norm,
                                                        int skip_nonfinite, int maximize, double lr, const float* lr_dev,
                                                        double b1, double b2, double wd, uint32_t seed,
@@ -145,7 +237,7 @@ __global__ __launch_bounds__(256) void k_adamw_prepare(const StepTable t, const 
     }
     if (skip) return;
     if (lr_dev) lr = *lr_dev;
-    for (int i = threadIdx.x; i < t.count; i += 256) {
+    for (int i = threadIdx.x; i < t.count; i += 1024) {
         const float step = *t.step[i] + 1.0f;
         *t.step[i] = step;
         TensorScalars s;
@@ -168,20 +260,49 @@ __device__ __forceinline__ float updated(const Hyper& h, const TensorScalars& s,
     return p * s.decay - s.size * a.m / (sqrtf(a.v) * s.inv_root + h.eps);
 }
 
+template <int DT>
+__device__ __forceinline__ void update32(const AdamwTable& t, const Chunk& c, const Hyper& h, const TensorScalars& s,
+                                         float scale) {
+    constexpr int U = 2;  // vectors of each array in flight
+    const void* gs = t.g[c.tensor];
+    void *ps = t.p[c.tensor], *ms = t.m[c.tensor], *vs = t.v[c.tensor];
+    for (int64_t e = c.begin + threadIdx.x * 4; e < c.end; e += U * 1024) {
+        float p[U][4], g[U][4], m[U][4], v[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            load4<DT>(gs, e + u * 1024, c.end, g[u]);
+            load4<DT>(ps, e + u * 1024, c.end, p[u]);
+            load4<kF32>(ms, e + u * 1024, c.end, m[u]);
+            load4<kF32>(vs, e + u * 1024, c.end, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const Moments a = moments(h, m[u][k], v[u][k], g[u][k] * scale);
+                p[u][k] = updated(h, s, p[u][k], a);
+                m[u][k] = a.m;
+                v[u][k] = a.v;
+            }
+            store4<DT>(ps, e + u * 1024, c.end, p[u]);
+            store4<kF32>(ms, e + u * 1024, c.end, m[u]);
+            store4<kF32>(vs, e + u * 1024, c.end, v[u]);
+        }
+    }
+}
+
+// Chunks are taken from the last to the first: the norm read them from the first to the last, so the latest gradients
+// are still in the 256 MB cache.
 __global__ __launch_bounds__(256) void k_adamw(const AdamwTable t, const Hyper h, const CallScalars* call,
                                                const TensorScalars* tensors) {
     if (call->skip) return;
-    const int i = find_tensor(t.start, t.count, blockIdx.x);
-    const int64_t begin = int64_t(blockIdx.x - t.start[i]) * kChunk, end = min(t.n[i], begin + kChunk);
-    const TensorScalars s = tensors[t.first + i];
+    const Chunk c = chunk_at(t, gridDim.x - 1 - blockIdx.x);
+    const TensorScalars s = tensors[t.first + c.tensor];
     const float scale = call->scale;
-    float *m = static_cast<float*>(t.m[i]), *v = static_cast<float*>(t.v[i]);
-    for (int64_t e = begin + threadIdx.x; e < end; e += 256) {
-        const Moments a = moments(h, m[e], v[e], load_elem(t.g[i], e, t.dtype[i]) * scale);
-        store_elem(t.p[i], e, t.dtype[i], updated(h, s, load_elem(t.p[i], e, t.dtype[i]), a));
-        m[e] = a.m;
-        v[e] = a.v;
-    }
+    const int dt = t.dtype[c.tensor];
+    if (dt == kF32) update32<kF32>(t, c, h, s, scale);
+    else if (dt == kBF16) update32<kBF16>(t, c, h, s, scale);
+    else update32<kF16>(t, c, h, s, scale);
 }
 
 constexpr int kTopM = 127, kTopV = 255, kNanM = 0x80;
@@ -213,68 +334,127 @@ __device__ __forceinline__ uint32_t encode_v(float v, int base, uint32_t dither)
 }
 __device__ __forceinline__ int base_of(uint32_t largest, int top) { return max(int(largest >> 20) + 1 - top, 0); }
 
+__device__ __forceinline__ uint32_t max_partner(uint32_t v, int partner) { return max(v, uint32_t(partner)); }
+// On every lane.
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-    for (int off = 32; off; off >>= 1) v = max(v, uint32_t(__shfl_xor(int(v), off)));
-    return v;
+    v = max_partner(v, __builtin_amdgcn_update_dpp(0, int(v), 0x140, 0xf, 0xf, false));
+    v = max_partner(v, __builtin_amdgcn_update_dpp(0, int(v), 0x141, 0xf, 0xf, false));
+    v = max_partner(v, __builtin_amdgcn_update_dpp(0, int(v), 0x1b, 0xf, 0xf, false));
+    v = max_partner(v, __builtin_amdgcn_update_dpp(0, int(v), 0xb1, 0xf, 0xf, false));
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(r[0], r[1]);
+    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(r[0], r[1]);
 }
 
-// A wavefront takes a block of 256 elements, four to a lane.
+__device__ __forceinline__ bool finite_bits(uint32_t magnitude) { return magnitude < 0x7F800000u; }
+
+// A wavefront takes a block of 256 elements, four to a lane, and two blocks at a time.
+template <int DT>
+__device__ __forceinline__ void update8(const AdamwTable& t, const Chunk& c, const Hyper& h, const TensorScalars& s,
+                                        float scale) {
+    constexpr int U = 2;
+    const int lane = threadIdx.x & 63;
+    const void* gs = t.g[c.tensor];
+    void* ps = t.p[c.tensor];
+    uint8_t *ms = static_cast<uint8_t*>(t.m[c.tensor]), *vs = static_cast<uint8_t*>(t.v[c.tensor]);
+    Bases* bs = reinterpret_cast<Bases*>(t.bases[c.tensor]);
+    for (int64_t b = c.begin + (threadIdx.x >> 6) * kBlock; b < c.end; b += U * 4 * kBlock) {
+        float p[U][4], g[U][4];
+        uint32_t cm[U], cv[U], base[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = b + u * 4 * kBlock, e = at + lane * 4;
+            load4<DT>(gs, e, c.end, g[u]);
+            load4<DT>(ps, e, c.end, p[u]);
+            cm[u] = load_codes(ms, e, c.end);
+            cv[u] = load_codes(vs, e, c.end);
+            base[u] = at < c.end ? bs[at / kBlock] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = b + u * 4 * kBlock, e = at + lane * 4;
+            if (at >= c.end) break;
+            const int bm = int16_t(base[u]), bv = int16_t(base[u] >> 16);
+            Moments a[4];
+            bool finite[4];
+            uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {  // past the end the codes and the gradient are 0, and so are the moments
+                a[k] = moments(h, decode_m(cm[u] >> 8 * k & 255, bm), decode_v(cv[u] >> 8 * k & 255, bv),
+                               g[u][k] * scale);
+                p[u][k] = updated(h, s, p[u][k], a[k]);
+                const uint32_t um = __float_as_uint(a[k].m) & 0x7FFFFFFFu, uv = __float_as_uint(a[k].v);
+                finite[k] = finite_bits(um) && finite_bits(uv);
+                top_m = max(top_m, finite[k] ? um : 0);
+                top_v = max(top_v, finite[k] ? uv : 0);
+            }
+            store4<DT>(ps, e, c.end, p[u]);
+            const int nm = base_of(wave_max(top_m), kTopM), nv = base_of(wave_max(top_v), kTopV);
+            uint32_t om = 0, ov = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t r = mix(s.key + uint32_t(e + k) * 0x9E3779B1u);
+                om |= (finite[k] ? encode_m(a[k].m, nm, r & 0xFFFF) : kNanM) << 8 * k;
+                ov |= (finite[k] ? encode_v(a[k].v, nv, r >> 16) : kTopV) << 8 * k;
+            }
+            store_codes(ms, e, c.end, om);
+            store_codes(vs, e, c.end, ov);
+            if (lane == 0) bs[at / kBlock] = uint32_t(nm) | uint32_t(nv) << 16;
+        }
+    }
+}
+
 __global__ __launch_bounds__(256) void k_adamw8(const AdamwTable t, const Hyper h, const CallScalars* call,
                                                 const TensorScalars* tensors) {
     if (call->skip) return;
-    const int i = find_tensor(t.start, t.count, blockIdx.x);
-    const int64_t begin = int64_t(blockIdx.x - t.start[i]) * kChunk, n = t.n[i], end = min(n, begin + kChunk);
-    const TensorScalars s = tensors[t.first + i];
+    const Chunk c = chunk_at(t, gridDim.x - 1 - blockIdx.x);
+    const TensorScalars s = tensors[t.first + c.tensor];
     const float scale = call->scale;
-    uint8_t *cm = static_cast<uint8_t*>(t.m[i]), *cv = static_cast<uint8_t*>(t.v[i]);
-    const int lane = threadIdx.x & 63;
-    for (int64_t b = begin + (threadIdx.x >> 6) * kBlock; b < end; b += 4 * kBlock) {
-        int16_t* bases = t.bases[i] + b / kBlock * 2;
-        const int bm = bases[0], bv = bases[1];
-        Moments a[4];
-        uint32_t top_m = 0, top_v = 0;
-        for (int k = 0; k < 4; ++k) {
-            const int64_t e = b + lane * 4 + k;
-            a[k] = {0, 0};
-            if (e >= n) continue;
-            a[k] = moments(h, decode_m(cm[e], bm), decode_v(cv[e], bv), load_elem(t.g[i], e, t.dtype[i]) * scale);
-            store_elem(t.p[i], e, t.dtype[i], updated(h, s, load_elem(t.p[i], e, t.dtype[i]), a[k]));
-            const uint32_t um = __float_as_uint(a[k].m) & 0x7FFFFFFFu, uv = __float_as_uint(a[k].v);
-            if (um < 0x7F800000u && uv < 0x7F800000u) {
-                top_m = max(top_m, um);
-                top_v = max(top_v, uv);
-            }
-        }
-        const int nm = base_of(wave_max(top_m), kTopM), nv = base_of(wave_max(top_v), kTopV);
-        for (int k = 0; k < 4; ++k) {
-            const int64_t e = b + lane * 4 + k;
-            if (e >= n) continue;
-            const uint32_t r = mix(s.key + uint32_t(e) * 0x9E3779B1u);
-            const bool finite = (__float_as_uint(a[k].m) & 0x7FFFFFFFu) < 0x7F800000u &&
-                                __float_as_uint(a[k].v) < 0x7F800000u;
-            cm[e] = finite ? encode_m(a[k].m, nm, r & 0xFFFF) : kNanM;
-            cv[e] = finite ? encode_v(a[k].v, nv, r >> 16) : kTopV;
-        }
-        if (lane == 0) bases[0] = int16_t(nm), bases[1] = int16_t(nv);
-    }
+    const int dt = t.dtype[c.tensor];
+    if (dt == kF32) update8<kF32>(t, c, h, s, scale);
+    else if (dt == kBF16) update8<kBF16>(t, c, h, s, scale);
+    else update8<kF16>(t, c, h, s, scale);
 }
 
 // The moments that 8-bit states stand for: t.p and t.g receive m and v in float32.
 __global__ __launch_bounds__(256) void k_adamw8_moments(const AdamwTable t) {
-    const int i = find_tensor(t.start, t.count, blockIdx.x);
-    const int64_t begin = int64_t(blockIdx.x - t.start[i]) * kChunk, end = min(t.n[i], begin + kChunk);
-    const uint8_t *cm = static_cast<const uint8_t*>(t.m[i]), *cv = static_cast<const uint8_t*>(t.v[i]);
-    float *m = static_cast<float*>(t.p[i]), *v = static_cast<float*>(const_cast<void*>(t.g[i]));
-    for (int64_t e = begin + threadIdx.x; e < end; e += 256) {
-        const int16_t* bases = t.bases[i] + e / kBlock * 2;
-        m[e] = decode_m(cm[e], bases[0]);
-        v[e] = decode_v(cv[e], bases[1]);
+    constexpr int U = 4;
+    const Chunk c = chunk_at(t, blockIdx.x);
+    const uint8_t *ms = static_cast<const uint8_t*>(t.m[c.tensor]), *vs = static_cast<const uint8_t*>(t.v[c.tensor]);
+    const Bases* bs = reinterpret_cast<const Bases*>(t.bases[c.tensor]);
+    void *mo = t.p[c.tensor], *vo = const_cast<void*>(t.g[c.tensor]);
+    for (int64_t b = c.begin + threadIdx.x * 4; b < c.end; b += U * 1024) {
+        uint32_t cm[U], cv[U], base[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t e = b + u * 1024;
+            cm[u] = load_codes(ms, e, c.end);
+            cv[u] = load_codes(vs, e, c.end);
+            base[u] = e < c.end ? bs[e / kBlock] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float m[4], v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                m[k] = decode_m(cm[u] >> 8 * k & 255, int16_t(base[u]));
+                v[k] = decode_v(cv[u] >> 8 * k & 255, int16_t(base[u] >> 16));
+            }
+            store4<kF32>(mo, b + u * 1024, c.end, m);
+            store4<kF32>(vo, b + u * 1024, c.end, v);
+        }
     }
 }
 
-static int64_t chunks_of(const int64_t* numel, int64_t count) {
+static int chunk_size(const int64_t* numel, int64_t count) {
+    int64_t total = 0;
+    for (int64_t i = 0; i < count; ++i) total += std::max<int64_t>(numel[i], 0);
+    return chunk_of(total);
+}
+static int64_t chunks_of(const int64_t* numel, int64_t count, int chunk) {
     int64_t chunks = 0;
-    for (int64_t i = 0; i < count; ++i) chunks += ceil_div(std::max<int64_t>(numel[i], 0), kChunk);
+    for (int64_t i = 0; i < count; ++i) chunks += ceil_div(std::max<int64_t>(numel[i], 0), chunk);
     return chunks;
 }
 
@@ -293,6 +473,7 @@ static int launch_sumsq(const void* const* grads, const int64_t* numel, const in
                         double* partial, mnx_stream_t stream) {
     NormTable t;
     t.count = 0;
+    t.chunk = chunk_size(numel, count);
     t.out = 0;
     uint32_t chunks = 0;
     auto flush = [&]() -> int {
@@ -308,7 +489,7 @@ static int launch_sumsq(const void* const* grads, const int64_t* numel, const in
     for (int64_t i = 0; i < count; ++i) {
         if (!numel[i]) continue;
         MNX_REQUIRE(grads[i], "gradient norm: tensor %lld is null", (long long)i);
-        const int64_t c = ceil_div(numel[i], kChunk);
+        const int64_t c = ceil_div(numel[i], t.chunk);
         if (t.count == kNormTensors || chunks + c > (1u << 23))
             if (int rc = flush()) return rc;
         t.g[t.count] = grads[i];
@@ -327,7 +508,7 @@ using namespace mnx;
 extern "C" {
 
 size_t mnx_grad_norm_workspace_bytes(const int64_t* numel, int64_t count) {
-    return size_t(std::max<int64_t>(count > 0 && numel ? chunks_of(numel, count) : 0, 1)) * sizeof(double);
+    return size_t(std::max<int64_t>(count > 0 && numel ? chunks_of(numel, count, chunk_size(numel, count)) : 0, 1)) * sizeof(double);
 }
 
 int mnx_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtype, int64_t count, float* norm,
@@ -339,7 +520,7 @@ int mnx_grad_norm(const void* const* grads, const int64_t* numel, const int32_t*
         return set_error(MNX_ERR_WORKSPACE, "gradient norm: workspace too small");
     double* partial = static_cast<double*>(workspace);
     if (int rc = launch_sumsq(grads, numel, dtype, count, partial, stream)) return rc;
-    k_norm<<<1, 256, 0, stream>>>(partial, chunks_of(numel, count), norm);
+    k_norm<<<1, 1024, 0, stream>>>(partial, chunks_of(numel, count, chunk_size(numel, count)), norm);
     MNX_CHECK_LAUNCH();
     return MNX_OK;
 }
@@ -371,7 +552,8 @@ int mnx_adamw_step(const mnx_adamw_args* args, mnx_stream_t stream) {
     Workspace ws{static_cast<char*>(a.workspace), a.workspace_bytes};
     CallScalars* call = ws.take<CallScalars>(1);
     TensorScalars* scalars = ws.take<TensorScalars>(size_t(std::max<int64_t>(a.count, 1)));
-    const int64_t chunks = chunks_of(a.numel, a.count);
+    const int chunk = chunk_size(a.numel, a.count);
+    const int64_t chunks = chunks_of(a.numel, a.count, chunk);
     double* partial = ws.take<double>(size_t(std::max<int64_t>(chunks, 1)));
     if (!a.workspace || !ws.fits()) return set_error(MNX_ERR_WORKSPACE, "adamw: workspace too small");
 
@@ -383,14 +565,15 @@ int mnx_adamw_step(const mnx_adamw_args* args, mnx_stream_t stream) {
         st.first = int(at);
         st.count = int(std::min<int64_t>(kStepTensors, a.count - at));
         for (int i = 0; i < st.count; ++i) st.step[i] = a.steps[at + i];
-        k_adamw_prepare<<<1, 256, 0, stream>>>(st, own_norm ? partial : nullptr, chunks, a.norm_in, a.norm_out,
+        k_adamw_prepare<<<1, 1024, 0, stream>>>(st, own_norm ? partial : nullptr, chunks, a.norm_in, a.norm_out,
                                                a.max_norm, a.skip_nonfinite, a.maximize, a.lr, a.lr_device, a.beta1,
                                                a.beta2, a.weight_decay, a.seed, call, scalars);
         MNX_CHECK_LAUNCH();
     }
     const Hyper h{float(a.beta1), float(1 - a.beta1), float(a.beta2), float(1 - a.beta2), float(a.eps)};
     AdamwTable t;
-    for (int64_t at = 0; at < a.count; at += kTensors) {
+    t.chunk = chunk;
+    for (int64_t at = (a.count - 1) / kTensors * kTensors; at >= 0 && a.count; at -= kTensors) {  // the last ones first
         t.first = int(at);
         t.count = int(std::min<int64_t>(kTensors, a.count - at));
         int64_t c = 0;
@@ -403,7 +586,7 @@ int mnx_adamw_step(const mnx_adamw_args* args, mnx_stream_t stream) {
             t.n[i] = a.numel[at + i];
             t.dtype[i] = uint8_t(a.dtype[at + i]);
             t.start[i] = uint32_t(c);
-            c += ceil_div(t.n[i], kChunk);
+            c += ceil_div(t.n[i], t.chunk);
         }
         t.start[t.count] = uint32_t(c);
         if (!c) continue;
@@ -422,6 +605,7 @@ int mnx_adamw8_moments(const void* const* exp_avgs, const void* const* exp_avg_s
     MNX_REQUIRE(count == 0 || (exp_avgs && exp_avg_sqs && bases && out_avgs && out_avg_sqs),
                 "adamw8 moments: null pointer");
     AdamwTable t;
+    t.chunk = chunk_size(numel, count);
     for (int64_t at = 0; at < count; at += kTensors) {
         t.first = int(at);
         t.count = int(std::min<int64_t>(kTensors, count - at));
@@ -438,7 +622,7 @@ int mnx_adamw8_moments(const void* const* exp_avgs, const void* const* exp_avg_s
             t.n[i] = numel[k];
             t.dtype[i] = kF32;
             t.start[i] = uint32_t(c);
-            c += ceil_div(t.n[i], kChunk);
+            c += ceil_div(t.n[i], t.chunk);
         }
         t.start[t.count] = uint32_t(c);
         if (!c) continue;
