@@ -12,6 +12,7 @@ import concurrent.futures as cf
 import os
 import subprocess
 import sys
+import sysconfig
 import time
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -65,7 +66,8 @@ def _compile_torch() -> str:
 
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-c", "-D__HIP_PLATFORM_AMD__=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-    for path in [*include_paths(), os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")]:
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    for path in [*include_paths(), os.path.join(rocm, "include"), sysconfig.get_paths()["include"]]:
         cmd += ["-isystem", path]
     obj = os.path.join(BUILD, "torch_ops.o")
     t0 = time.time()
@@ -80,7 +82,8 @@ def _link_torch() -> None:
 
     tmp = TORCH_LIB + ".tmp"
     cmd = ["g++", "-shared", os.path.join(BUILD, "torch_ops.o"), "-o", tmp, "-L", LIBDIR, "-lmolnex_hip",
-           *(f"-L{path}" for path in library_paths()), "-lc10", "-lc10_hip", "-ltorch_cpu", "-Wl,-rpath,$ORIGIN"]
+           *(f"-L{path}" for path in library_paths()), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")

@@ -256,8 +256,13 @@ struct Moments {
 __device__ __forceinline__ Moments moments(const Hyper& h, float m, float v, float g) {
     return {m * h.b1 + g * h.w1, v * h.b2 + (g * g) * h.w2};
 }
+// The square root and the reciprocal by the hardware's instructions, a unit of the last place each: the update is lr
+// times a number of the order of one, added to p, and with the exact forms k_adamw8 is bound by them (SQRT_MEASURE).
+// The root's instruction takes no subnormals: a v below 2^-96 is scaled (its root is far below any eps but 0).
 __device__ __forceinline__ float updated(const Hyper& h, const TensorScalars& s, float p, const Moments& a) {
-    return p * s.decay - s.size * a.m / (sqrtf(a.v) * s.inv_root + h.eps);
+    const bool tiny = a.v < 0x1p-96f;
+    const float root = __builtin_amdgcn_sqrtf(tiny ? a.v * 0x1p96f : a.v) * (tiny ? 0x1p-48f : 1.0f);
+    return p * s.decay - s.size * a.m * __builtin_amdgcn_rcpf(root * s.inv_root + h.eps);
 }
 
 template <int DT>

@@ -3,11 +3,18 @@
 // These are called once or more per layer and step, on tensors small enough that the host bounds them, and AdamW's
 // arguments are lists of every parameter.  Registered from Python (molnex_amd/_ops.py), a 700 x 128 layer norm forward
 // and backward took 179 us, most of it the autograd engine's thread and the caller passing the interpreter's lock to
-// and fro, and a step over 60 tensors 119 us, the time to ask each tensor its type, layout and address.
+// and fro, and a step over 60 tensors 119 us, the time to ask each tensor its type, layout and address.  The library
+// is a Python module too, whose functions take the lists of tensors straight to the ops: through torch.ops, each of
+// 300 tensors is boxed first (BOXED_MEASURE).
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -592,3 +599,123 @@ TORCH_LIBRARY_IMPL(molix, Autograd, m) {
     for (const char* name : {"grad_norm", "adamw_step", "adamw8_step", "adamw8_moments"})
         m.impl(name, torch::CppFunction::makeFallthrough());
 }
+
+// ---------------------------------------------------------------------------
+// The Python module: the ops on lists of tensors, called through the dispatcher without boxing
+// ---------------------------------------------------------------------------
+
+namespace {
+
+std::vector<Tensor> tensors(PyObject* o, const char* what) {
+    PyObject* seq = PySequence_Fast(o, "");
+    if (!seq) {
+        PyErr_Clear();
+        TORCH_CHECK_TYPE(false, what, ": a list of tensors, got ", Py_TYPE(o)->tp_name);
+    }
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+    PyObject** items = PySequence_Fast_ITEMS(seq);
+    std::vector<Tensor> got;
+    got.reserve(n);
+    Py_ssize_t i = 0;
+    for (; i < n && THPVariable_Check(items[i]); ++i) got.push_back(THPVariable_Unpack(items[i]));
+    const char* other = i < n ? Py_TYPE(items[i])->tp_name : nullptr;
+    Py_DECREF(seq);
+    TORCH_CHECK_TYPE(!other, what, ": tensors, got ", other ? other : "");
+    return got;
+}
+
+OptTensor tensor_or_none(PyObject* o, const char* what) {
+    if (o == Py_None) return std::nullopt;
+    TORCH_CHECK_TYPE(THPVariable_Check(o), what, ": a tensor or None, got ", Py_TYPE(o)->tp_name);
+    return THPVariable_Unpack(o);
+}
+
+double number(PyObject* o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw python_error();
+    return v;
+}
+
+bool truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw python_error();
+    return v;
+}
+
+struct Released {  // of the interpreter's lock
+    PyThreadState* state = PyEval_SaveThread();
+    ~Released() { PyEval_RestoreThread(state); }
+};
+
+// (bits, params, grads, exp_avgs, exp_avg_sqs, bases, steps, lr, beta1, beta2, eps, weight_decay, maximize, max_norm,
+// grad_norm, skip_nonfinite, lr_tensor, seed); bases and seed for 8 bits
+PyObject* py_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 18, "step: 18 arguments, got ", n);
+    const bool eight = number(a[0]) == 8;
+    const auto params = tensors(a[1], "parameters"), grads = tensors(a[2], "gradients");
+    const auto avgs = tensors(a[3], "first moments"), sqs = tensors(a[4], "second moments");
+    const auto bases = eight ? tensors(a[5], "bases") : std::vector<Tensor>();
+    const auto steps = tensors(a[6], "steps");
+    const double lr = number(a[7]), b1 = number(a[8]), b2 = number(a[9]), eps = number(a[10]), wd = number(a[11]);
+    const bool maximize = truth(a[12]), skip = truth(a[15]);
+    const std::optional<double> max_norm = a[13] == Py_None ? std::nullopt : std::optional<double>(number(a[13]));
+    const OptTensor norm_in = tensor_or_none(a[14], "grad_norm"), rate = tensor_or_none(a[16], "lr");
+    const int64_t seed = eight ? PyLong_AsLongLong(a[17]) : 0;
+    if (PyErr_Occurred()) throw python_error();
+    Tensor norm;
+    {
+        Released r;
+        static auto step32 = op<decltype(adamw_step)>("molix::adamw_step");
+        static auto step8 = op<decltype(adamw8_step)>("molix::adamw8_step");
+        norm = eight ? step8.call(params, grads, avgs, sqs, bases, steps, lr, b1, b2, eps, wd, maximize, max_norm,
+                                  norm_in, skip, rate, seed)
+                     : step32.call(params, grads, avgs, sqs, steps, lr, b1, b2, eps, wd, maximize, max_norm, norm_in,
+                                   skip, rate);
+    }
+    if (norm.dim()) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(norm));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_grad_norm(PyObject*, PyObject* list) {
+    HANDLE_TH_ERRORS
+    const auto grads = tensors(list, "gradients");
+    Tensor norm;
+    {
+        Released r;
+        static auto o = op<decltype(grad_norm)>("molix::grad_norm");
+        norm = o.call(grads);
+    }
+    return THPVariable_Wrap(std::move(norm));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_moments(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 5, "moments: 5 lists, got ", n);
+    const auto avgs = tensors(a[0], "first moments"), sqs = tensors(a[1], "second moments");
+    const auto bases = tensors(a[2], "bases"), om = tensors(a[3], "out"), ov = tensors(a[4], "out");
+    {
+        Released r;
+        static auto o = op<decltype(adamw8_moments)>("molix::adamw8_moments");
+        o.call(avgs, sqs, bases, om, ov);
+    }
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef kMethods[] = {
+    {"step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_step)), METH_FASTCALL,
+     "molix::adamw_step or adamw8_step; the norm, or None"},
+    {"grad_norm", py_grad_norm, METH_O, "molix::grad_norm"},
+    {"moments", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_moments)), METH_FASTCALL,
+     "molix::adamw8_moments"},
+    {nullptr, nullptr, 0, nullptr},
+};
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "libmolnex_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr,
+                       nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit_libmolnex_torch() { return PyModule_Create(&kModule); }

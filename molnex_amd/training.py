@@ -8,7 +8,9 @@ implementations, and holds the functions that ``molix.F`` exports.
 
 from __future__ import annotations
 
+import importlib.util
 import os
+import sys
 
 import torch
 from torch import Tensor
@@ -23,7 +25,13 @@ STATE_BLOCK = 256
 if not os.path.exists(TORCH_LIB_PATH):
     raise _lib.MolnexError(f"molnex torch library not found at {TORCH_LIB_PATH}; build it with "
                            "`python -m molnex_amd.build`")
-torch.ops.load_library(TORCH_LIB_PATH)
+# a Python module whose loading registers the ops, too
+_host = sys.modules.get("libmolnex_torch")
+if _host is None:
+    _spec = importlib.util.spec_from_file_location("libmolnex_torch", TORCH_LIB_PATH)
+    _host = importlib.util.module_from_spec(_spec)
+    _spec.loader.exec_module(_host)
+    sys.modules["libmolnex_torch"] = _host
 
 if "_fakes" in globals():  # a reload of this module
     globals()["_fakes"]._destroy()
@@ -92,17 +100,13 @@ def dense(t: Tensor) -> bool:
     return True
 
 
-_grad_norm = torch.ops.molix.grad_norm.default
-_adamw_step = torch.ops.molix.adamw_step.default
-_adamw8_step = torch.ops.molix.adamw8_step.default
-_adamw8_moments = torch.ops.molix.adamw8_moments.default
-
-
 def grad_norm(grads) -> Tensor:
     """The 2-norm of all of ``grads`` together (float32, 0-dim, on their device; no synchronisation): squares are
     summed in float64 in a fixed order."""
     grads = list(grads)
-    return _grad_norm(grads) if grads else torch.zeros(())
+    if not grads:
+        return torch.zeros(())
+    return torch.ops.molix.grad_norm(grads) if torch.compiler.is_compiling() else _host.grad_norm(grads)
 
 
 def _rate(lr) -> tuple[float, Tensor | None]:
@@ -125,9 +129,13 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
             raise ValueError("molix.adamw_step: no parameters, but other tensors")
         return grad_norm
     rate, lr_tensor = _rate(lr)
-    norm = _adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, rate, betas[0], betas[1], eps, weight_decay,
-                       maximize, max_norm, grad_norm, skip_nonfinite, lr_tensor)
-    return grad_norm if norm.dim() else norm
+    if torch.compiler.is_compiling():
+        norm = torch.ops.molix.adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, rate, betas[0], betas[1], eps,
+                                          weight_decay, maximize, max_norm, grad_norm, skip_nonfinite, lr_tensor)
+        return grad_norm if norm.dim() else norm
+    norm = _host.step(32, params, grads, exp_avgs, exp_avg_sqs, None, steps, rate, betas[0], betas[1], eps,
+                      weight_decay, maximize, max_norm, grad_norm, skip_nonfinite, lr_tensor, 0)
+    return grad_norm if norm is None else norm
 
 
 def adamw8_step(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, lr, betas=(0.9, 0.999), eps=1e-8,
@@ -143,9 +151,14 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, lr, betas
             raise ValueError("molix.adamw8_step: no parameters, but other tensors")
         return grad_norm
     rate, lr_tensor = _rate(lr)
-    norm = _adamw8_step(params, grads, exp_avgs, exp_avg_sqs, bases, steps, rate, betas[0], betas[1], eps, weight_decay,
-                        maximize, max_norm, grad_norm, skip_nonfinite, lr_tensor, seed & 0xFFFFFFFF)
-    return grad_norm if norm.dim() else norm
+    if torch.compiler.is_compiling():
+        norm = torch.ops.molix.adamw8_step(params, grads, exp_avgs, exp_avg_sqs, bases, steps, rate, betas[0],
+                                           betas[1], eps, weight_decay, maximize, max_norm, grad_norm, skip_nonfinite,
+                                           lr_tensor, seed & 0xFFFFFFFF)
+        return grad_norm if norm.dim() else norm
+    norm = _host.step(8, params, grads, exp_avgs, exp_avg_sqs, bases, steps, rate, betas[0], betas[1], eps,
+                      weight_decay, maximize, max_norm, grad_norm, skip_nonfinite, lr_tensor, seed & 0xFFFFFFFF)
+    return grad_norm if norm is None else norm
 
 
 def adamw8_moments(exp_avgs, exp_avg_sqs, bases, out=None) -> tuple[list[Tensor], list[Tensor]]:
@@ -153,5 +166,6 @@ def adamw8_moments(exp_avgs, exp_avg_sqs, bases, out=None) -> tuple[list[Tensor]
     if out is None:
         out = tuple([torch.empty_like(t, dtype=torch.float32) for t in ts] for ts in (exp_avgs, exp_avg_sqs))
     if exp_avgs or exp_avg_sqs:
-        _adamw8_moments(exp_avgs, exp_avg_sqs, bases, *out)
+        call = torch.ops.molix.adamw8_moments if torch.compiler.is_compiling() else _host.moments
+        call(exp_avgs, exp_avg_sqs, bases, *out)
     return out
