@@ -897,7 +897,7 @@ int mnx_layer_norm_bwd2(const void* grad, int64_t ldg, const void* x, int64_t ld
 /* in float64, fixed order).  Arrays of tensors are host arrays of `count`    */
 /* entries; numel may be 0 (its pointer is then not read).                     */
 /* ------------------------------------------------------------------------ */
-#define MNX_OPTIM_MAX_ELEMENTS ((int64_t)1 << 36) /* of one tensor */
+#define MNX_OPTIM_MAX_ELEMENTS ((int64_t)1 << 34) /* of one tensor */
 size_t mnx_grad_norm_workspace_bytes(const int64_t* numel, int64_t count);
 int mnx_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtype, int64_t count, float* norm,
                   void* workspace, size_t workspace_bytes, mnx_stream_t stream);

@@ -29,14 +29,25 @@ constexpr int kNormTensors = 160;  // tensors of one norm launch
 constexpr int kStepTensors = 480;  // tensors of one launch of the step counts
 constexpr int kBlock = 256;        // elements of a block of 8-bit states
 
-// Elements that a workgroup takes: a power of two of whole blocks for its four wavefronts.  Small calls are cut finer, so
-// that they reach every compute unit and no thread has several vectors to wait for; 8192 keeps what a workgroup reads
-// first (its tensor's entry and scalars) below a few per cent of its time.
-inline int chunk_of(int64_t total) {
+// Elements that a workgroup takes.  The update reads all that its chunk has, two vectors of each array a thread, and is
+// done: 128 M fp32 parameters take 645 us so, 656 us with four vectors, and 721 us in chunks of 8192 looped over; 24 M
+// bf16 ones 95, 99 and 117 us, 64 M with 8-bit states 261, 269 and 282 us.
+// The norm's workgroups leave a partial sum each, for one workgroup to add up, and take more; small calls are cut finer,
+// so that they reach every compute unit.
+constexpr int kUpdateVectors = 2, kUpdateChunk = kUpdateVectors * 1024;
+inline int norm_chunk(int64_t total) {
     int chunk = 1024;
-    while (chunk < 8192 && total / chunk > 2048) chunk *= 2;
+    while (chunk < 16384 && total / chunk > 2048) chunk *= 2;
     return chunk;
 }
+
+// Workgroups of a launch at most (of 256 threads each; a grid has fewer than 2^32 threads).
+constexpr int64_t kMostChunks = int64_t(1) << 23;
+static_assert(MNX_OPTIM_MAX_ELEMENTS / kUpdateChunk <= kMostChunks, "a tensor fits a launch");
+
+// Calls that move more than the 256 MB cache holds pass it by: 128 M fp32 parameters take 645 us so against 788 us, 64 M
+// with 8-bit states and their read-back 261 against 307 us; 3.2 M, which fit, 31.9 against 29.9 us.
+constexpr int64_t kCacheBytes = int64_t(256) << 20;
 
 struct AdamwTable {
     void* p[kTensors];
@@ -48,7 +59,6 @@ struct AdamwTable {
     uint32_t start[kTensors + 1];  // first chunk of each tensor
     uint8_t dtype[kTensors];
     int count, first;              // tensors here, number of the first one in the call
-    int chunk;
 };
 
 struct NormTable {
@@ -90,17 +100,21 @@ __device__ __forceinline__ int find_tensor(const uint32_t* start, int count, uin
     return __builtin_amdgcn_readfirstlane(at - 1);
 }
 
-// Four consecutive elements, at the alignment of one; past `end` they are 0 and not stored.
+// Four consecutive elements, at the alignment of one; past `end` they are 0 and not stored.  NT: past the caches, where
+// that is 16 bytes a lane (narrower ones lose by it).
 template <int DT>
 struct Four {
     typedef typename Elem<DT>::T T;
     typedef T Packed __attribute__((ext_vector_type(4), aligned(sizeof(T))));
 };
-template <int DT>
+template <int DT, bool NT = false>
 __device__ __forceinline__ void load4(const void* base, int64_t e, int64_t end, float (&v)[4]) {
     const auto* p = static_cast<const typename Elem<DT>::T*>(base);
     if (e + 4 <= end) {
-        const auto t = *reinterpret_cast<const typename Four<DT>::Packed*>(p + e);
+        typename Four<DT>::Packed t;
+        const auto* q = reinterpret_cast<const typename Four<DT>::Packed*>(p + e);
+        if constexpr (NT && DT == kF32) t = __builtin_nontemporal_load(q);
+        else t = *q;
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = float(t[k]);
     } else {
@@ -108,7 +122,7 @@ __device__ __forceinline__ void load4(const void* base, int64_t e, int64_t end, 
         for (int k = 0; k < 4; ++k) v[k] = e + k < end ? float(p[e + k]) : 0.0f;
     }
 }
-template <int DT>
+template <int DT, bool NT = false>
 __device__ __forceinline__ void store4(void* base, int64_t e, int64_t end, const float (&v)[4]) {
     using T = typename Elem<DT>::T;
     auto* p = static_cast<T*>(base);
@@ -116,7 +130,9 @@ __device__ __forceinline__ void store4(void* base, int64_t e, int64_t end, const
         typename Four<DT>::Packed t;
 #pragma unroll
         for (int k = 0; k < 4; ++k) t[k] = T(v[k]);
-        *reinterpret_cast<typename Four<DT>::Packed*>(p + e) = t;
+        auto* q = reinterpret_cast<typename Four<DT>::Packed*>(p + e);
+        if constexpr (NT && DT == kF32) __builtin_nontemporal_store(t, q);
+        else *q = t;
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -148,10 +164,10 @@ struct Chunk {
     int64_t begin, end;
 };
 template <typename Table>
-__device__ __forceinline__ Chunk chunk_at(const Table& t, uint32_t at) {
+__device__ __forceinline__ Chunk chunk_at(const Table& t, uint32_t at, int chunk) {
     const int i = find_tensor(t.start, t.count, at);
-    const int64_t begin = int64_t(at - t.start[i]) * t.chunk;
-    return {i, begin, min(t.n[i], begin + t.chunk)};
+    const int64_t begin = int64_t(at - t.start[i]) * chunk;
+    return {i, begin, min(t.n[i], begin + chunk)};
 }
 
 // Sums over the workgroup, on every thread.
@@ -186,7 +202,7 @@ __device__ __forceinline__ double sum_squares(const void* g, const Chunk& c) {
 }
 
 __global__ __launch_bounds__(256) void k_sumsq(const NormTable t, double* partial) {
-    const Chunk c = chunk_at(t, blockIdx.x);
+    const Chunk c = chunk_at(t, blockIdx.x, t.chunk);
     const void* g = t.g[c.tensor];
     const int dt = t.dtype[c.tensor];
     const double s = block_sum<256>(dt == kF32    ? sum_squares<kF32>(g, c)
@@ -215,6 +231,14 @@ __device__ __forceinline__ uint32_t mix(uint32_t x) {
     return x ^ (x >> 16);
 }
 
+// b^t of a whole number t by squaring: 24 multiplications deep at most, where the library's pow takes microseconds.
+__device__ __forceinline__ double power(double b, uint32_t t) {
+    double r = 1;
+    for (; t; t >>= 1, b *= b)
+        if (t & 1) r *= b;
+    return r;
+}
+
 // The step counts and everything that the update takes from them and from the norm, in float64.
 __global__ __launch_bounds__(1024) void k_adamw_prepare(const StepTable t, const double* partial, int64_t chunks,
                                                        const float* norm_in, float* norm_out, double max_norm,
@@ -241,8 +265,8 @@ __global__ __launch_bounds__(1024) void k_adamw_prepare(const StepTable t, const
         const float step = *t.step[i] + 1.0f;
         *t.step[i] = step;
         TensorScalars s;
-        s.size = float(lr / (1 - pow(b1, double(step))));
-        s.inv_root = float(1 / sqrt(1 - pow(b2, double(step))));
+        s.size = float(lr / (1 - power(b1, uint32_t(step))));
+        s.inv_root = float(1 / sqrt(1 - power(b2, uint32_t(step))));
         s.decay = float(1 - lr * wd);
         s.key = mix(mix(seed * 0x3C6EF373u + uint32_t(t.first + i) * 0xA54FF53Bu) + uint32_t(step) * 0x510E527Fu);
         tensors[t.first + i] = s;
@@ -257,7 +281,8 @@ __device__ __forceinline__ Moments moments(const Hyper& h, float m, float v, flo
     return {m * h.b1 + g * h.w1, v * h.b2 + (g * g) * h.w2};
 }
 // The square root and the reciprocal by the hardware's instructions, a unit of the last place each: the update is lr
-// times a number of the order of one, added to p, and with the exact forms k_adamw8 is bound by them (SQRT_MEASURE).
+// times a number of the order of one, added to p, and the exact forms are a third of k_adamw8's instructions (then 230
+// against 223 us for 64 M elements, before other steps brought that to 166 us, 6.2 TB/s).
 // The root's instruction takes no subnormals: a v below 2^-96 is scaled (its root is far below any eps but 0).
 __device__ __forceinline__ float updated(const Hyper& h, const TensorScalars& s, float p, const Moments& a) {
     const bool tiny = a.v < 0x1p-96f;
@@ -265,49 +290,49 @@ __device__ __forceinline__ float updated(const Hyper& h, const TensorScalars& s,
     return p * s.decay - s.size * a.m * __builtin_amdgcn_rcpf(root * s.inv_root + h.eps);
 }
 
-template <int DT>
+template <int DT, bool NT>
 __device__ __forceinline__ void update32(const AdamwTable& t, const Chunk& c, const Hyper& h, const TensorScalars& s,
                                          float scale) {
-    constexpr int U = 2;  // vectors of each array in flight
+    constexpr int U = kUpdateVectors;
     const void* gs = t.g[c.tensor];
     void *ps = t.p[c.tensor], *ms = t.m[c.tensor], *vs = t.v[c.tensor];
-    for (int64_t e = c.begin + threadIdx.x * 4; e < c.end; e += U * 1024) {
-        float p[U][4], g[U][4], m[U][4], v[U][4];
+    const int64_t e = c.begin + threadIdx.x * 4;
+    float p[U][4], g[U][4], m[U][4], v[U][4];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            load4<DT>(gs, e + u * 1024, c.end, g[u]);
-            load4<DT>(ps, e + u * 1024, c.end, p[u]);
-            load4<kF32>(ms, e + u * 1024, c.end, m[u]);
-            load4<kF32>(vs, e + u * 1024, c.end, v[u]);
+    for (int u = 0; u < U; ++u) {
+        load4<DT, NT>(gs, e + u * 1024, c.end, g[u]);
+        load4<DT, NT>(ps, e + u * 1024, c.end, p[u]);
+        load4<kF32, NT>(ms, e + u * 1024, c.end, m[u]);
+        load4<kF32, NT>(vs, e + u * 1024, c.end, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const Moments a = moments(h, m[u][k], v[u][k], g[u][k] * scale);
+            p[u][k] = updated(h, s, p[u][k], a);
+            m[u][k] = a.m;
+            v[u][k] = a.v;
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const Moments a = moments(h, m[u][k], v[u][k], g[u][k] * scale);
-                p[u][k] = updated(h, s, p[u][k], a);
-                m[u][k] = a.m;
-                v[u][k] = a.v;
-            }
-            store4<DT>(ps, e + u * 1024, c.end, p[u]);
-            store4<kF32>(ms, e + u * 1024, c.end, m[u]);
-            store4<kF32>(vs, e + u * 1024, c.end, v[u]);
-        }
+        store4<DT, NT>(ps, e + u * 1024, c.end, p[u]);
+        store4<kF32, NT>(ms, e + u * 1024, c.end, m[u]);
+        store4<kF32, NT>(vs, e + u * 1024, c.end, v[u]);
     }
 }
 
 // Chunks are taken from the last to the first: the norm read them from the first to the last, so the latest gradients
 // are still in the 256 MB cache.
+template <bool NT>
 __global__ __launch_bounds__(256) void k_adamw(const AdamwTable t, const Hyper h, const CallScalars* call,
                                                const TensorScalars* tensors) {
     if (call->skip) return;
-    const Chunk c = chunk_at(t, gridDim.x - 1 - blockIdx.x);
+    const Chunk c = chunk_at(t, gridDim.x - 1 - blockIdx.x, kUpdateChunk);
     const TensorScalars s = tensors[t.first + c.tensor];
     const float scale = call->scale;
     const int dt = t.dtype[c.tensor];
-    if (dt == kF32) update32<kF32>(t, c, h, s, scale);
-    else if (dt == kBF16) update32<kBF16>(t, c, h, s, scale);
-    else update32<kF16>(t, c, h, s, scale);
+    if (dt == kF32) update32<kF32, NT>(t, c, h, s, scale);
+    else if (dt == kBF16) update32<kBF16, NT>(t, c, h, s, scale);
+    else update32<kF16, NT>(t, c, h, s, scale);
 }
 
 constexpr int kTopM = 127, kTopV = 255, kNanM = 0x80;
@@ -355,112 +380,125 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 __device__ __forceinline__ bool finite_bits(uint32_t magnitude) { return magnitude < 0x7F800000u; }
 
 // A wavefront takes a block of 256 elements, four to a lane, and two blocks at a time.
-template <int DT>
+template <int DT, bool NT>
 __device__ __forceinline__ void update8(const AdamwTable& t, const Chunk& c, const Hyper& h, const TensorScalars& s,
                                         float scale) {
-    constexpr int U = 2;
+    constexpr int U = kUpdateVectors;
     const int lane = threadIdx.x & 63;
     const void* gs = t.g[c.tensor];
     void* ps = t.p[c.tensor];
     uint8_t *ms = static_cast<uint8_t*>(t.m[c.tensor]), *vs = static_cast<uint8_t*>(t.v[c.tensor]);
     Bases* bs = reinterpret_cast<Bases*>(t.bases[c.tensor]);
-    for (int64_t b = c.begin + (threadIdx.x >> 6) * kBlock; b < c.end; b += U * 4 * kBlock) {
-        float p[U][4], g[U][4];
-        uint32_t cm[U], cv[U], base[U];
+    const int64_t b = c.begin + (threadIdx.x >> 6) * kBlock;
+    float p[U][4], g[U][4];
+    uint32_t cm[U], cv[U], base[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t at = b + u * 4 * kBlock, e = at + lane * 4;
-            load4<DT>(gs, e, c.end, g[u]);
-            load4<DT>(ps, e, c.end, p[u]);
-            cm[u] = load_codes(ms, e, c.end);
-            cv[u] = load_codes(vs, e, c.end);
-            base[u] = at < c.end ? bs[at / kBlock] : 0;
+    for (int u = 0; u < U; ++u) {
+        const int64_t at = b + u * 4 * kBlock, e = at + lane * 4;
+        load4<DT, NT>(gs, e, c.end, g[u]);
+        load4<DT, NT>(ps, e, c.end, p[u]);
+        cm[u] = load_codes(ms, e, c.end);
+        cv[u] = load_codes(vs, e, c.end);
+        base[u] = at < c.end ? bs[at / kBlock] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t at = b + u * 4 * kBlock, e = at + lane * 4;
+        if (at >= c.end) break;
+        const int bm = int16_t(base[u]), bv = int16_t(base[u] >> 16);
+        Moments a[4];
+        bool finite[4];
+        uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // past the end the codes and the gradient are 0, and so are the moments
+            a[k] = moments(h, decode_m(cm[u] >> 8 * k & 255, bm), decode_v(cv[u] >> 8 * k & 255, bv),
+                           g[u][k] * scale);
+            p[u][k] = updated(h, s, p[u][k], a[k]);
+            const uint32_t um = __float_as_uint(a[k].m) & 0x7FFFFFFFu, uv = __float_as_uint(a[k].v);
+            finite[k] = finite_bits(um) && finite_bits(uv);
+            top_m = max(top_m, finite[k] ? um : 0);
+            top_v = max(top_v, finite[k] ? uv : 0);
         }
+        store4<DT, NT>(ps, e, c.end, p[u]);
+        const int nm = base_of(wave_max(top_m), kTopM), nv = base_of(wave_max(top_v), kTopV);
+        uint32_t om = 0, ov = 0;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t at = b + u * 4 * kBlock, e = at + lane * 4;
-            if (at >= c.end) break;
-            const int bm = int16_t(base[u]), bv = int16_t(base[u] >> 16);
-            Moments a[4];
-            bool finite[4];
-            uint32_t top_m = 0, top_v = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {  // past the end the codes and the gradient are 0, and so are the moments
-                a[k] = moments(h, decode_m(cm[u] >> 8 * k & 255, bm), decode_v(cv[u] >> 8 * k & 255, bv),
-                               g[u][k] * scale);
-                p[u][k] = updated(h, s, p[u][k], a[k]);
-                const uint32_t um = __float_as_uint(a[k].m) & 0x7FFFFFFFu, uv = __float_as_uint(a[k].v);
-                finite[k] = finite_bits(um) && finite_bits(uv);
-                top_m = max(top_m, finite[k] ? um : 0);
-                top_v = max(top_v, finite[k] ? uv : 0);
-            }
-            store4<DT>(ps, e, c.end, p[u]);
-            const int nm = base_of(wave_max(top_m), kTopM), nv = base_of(wave_max(top_v), kTopV);
-            uint32_t om = 0, ov = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t r = mix(s.key + uint32_t(e + k) * 0x9E3779B1u);
-                om |= (finite[k] ? encode_m(a[k].m, nm, r & 0xFFFF) : kNanM) << 8 * k;
-                ov |= (finite[k] ? encode_v(a[k].v, nv, r >> 16) : kTopV) << 8 * k;
-            }
-            store_codes(ms, e, c.end, om);
-            store_codes(vs, e, c.end, ov);
-            if (lane == 0) bs[at / kBlock] = uint32_t(nm) | uint32_t(nv) << 16;
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t r = mix(s.key + uint32_t(e + k) * 0x9E3779B1u);
+            om |= (finite[k] ? encode_m(a[k].m, nm, r & 0xFFFF) : kNanM) << 8 * k;
+            ov |= (finite[k] ? encode_v(a[k].v, nv, r >> 16) : kTopV) << 8 * k;
         }
+        store_codes(ms, e, c.end, om);
+        store_codes(vs, e, c.end, ov);
+        if (lane == 0) bs[at / kBlock] = uint32_t(nm) | uint32_t(nv) << 16;
     }
 }
 
+template <bool NT>
 __global__ __launch_bounds__(256) void k_adamw8(const AdamwTable t, const Hyper h, const CallScalars* call,
                                                 const TensorScalars* tensors) {
     if (call->skip) return;
-    const Chunk c = chunk_at(t, gridDim.x - 1 - blockIdx.x);
+    const Chunk c = chunk_at(t, gridDim.x - 1 - blockIdx.x, kUpdateChunk);
     const TensorScalars s = tensors[t.first + c.tensor];
     const float scale = call->scale;
     const int dt = t.dtype[c.tensor];
-    if (dt == kF32) update8<kF32>(t, c, h, s, scale);
-    else if (dt == kBF16) update8<kBF16>(t, c, h, s, scale);
-    else update8<kF16>(t, c, h, s, scale);
+    if (dt == kF32) update8<kF32, NT>(t, c, h, s, scale);
+    else if (dt == kBF16) update8<kBF16, NT>(t, c, h, s, scale);
+    else update8<kF16, NT>(t, c, h, s, scale);
 }
 
 // The moments that 8-bit states stand for: t.p and t.g receive m and v in float32.
+template <bool NT>
 __global__ __launch_bounds__(256) void k_adamw8_moments(const AdamwTable t) {
-    constexpr int U = 4;
-    const Chunk c = chunk_at(t, blockIdx.x);
+    constexpr int U = kUpdateVectors;
+    const Chunk c = chunk_at(t, blockIdx.x, kUpdateChunk);
     const uint8_t *ms = static_cast<const uint8_t*>(t.m[c.tensor]), *vs = static_cast<const uint8_t*>(t.v[c.tensor]);
     const Bases* bs = reinterpret_cast<const Bases*>(t.bases[c.tensor]);
     void *mo = t.p[c.tensor], *vo = const_cast<void*>(t.g[c.tensor]);
-    for (int64_t b = c.begin + threadIdx.x * 4; b < c.end; b += U * 1024) {
-        uint32_t cm[U], cv[U], base[U];
+    const int64_t b = c.begin + threadIdx.x * 4;
+    uint32_t cm[U], cv[U], base[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t e = b + u * 1024;
-            cm[u] = load_codes(ms, e, c.end);
-            cv[u] = load_codes(vs, e, c.end);
-            base[u] = e < c.end ? bs[e / kBlock] : 0;
+    for (int u = 0; u < U; ++u) {
+        const int64_t e = b + u * 1024;
+        cm[u] = load_codes(ms, e, c.end);
+        cv[u] = load_codes(vs, e, c.end);
+        base[u] = e < c.end ? bs[e / kBlock] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float m[4], v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            m[k] = decode_m(cm[u] >> 8 * k & 255, int16_t(base[u]));
+            v[k] = decode_v(cv[u] >> 8 * k & 255, int16_t(base[u] >> 16));
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float m[4], v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                m[k] = decode_m(cm[u] >> 8 * k & 255, int16_t(base[u]));
-                v[k] = decode_v(cv[u] >> 8 * k & 255, int16_t(base[u] >> 16));
-            }
-            store4<kF32>(mo, b + u * 1024, c.end, m);
-            store4<kF32>(vo, b + u * 1024, c.end, v);
-        }
+        store4<kF32, NT>(mo, b + u * 1024, c.end, m);
+        store4<kF32, NT>(vo, b + u * 1024, c.end, v);
     }
 }
 
-static int chunk_size(const int64_t* numel, int64_t count) {
+static int64_t total_of(const int64_t* numel, int64_t count) {
     int64_t total = 0;
     for (int64_t i = 0; i < count; ++i) total += std::max<int64_t>(numel[i], 0);
-    return chunk_of(total);
+    return total;
 }
-static int64_t chunks_of(const int64_t* numel, int64_t count, int chunk) {
+// Partial sums of the norm.
+static int64_t norm_chunks(const int64_t* numel, int64_t count) {
+    const int chunk = norm_chunk(total_of(numel, count));
     int64_t chunks = 0;
     for (int64_t i = 0; i < count; ++i) chunks += ceil_div(std::max<int64_t>(numel[i], 0), chunk);
     return chunks;
+}
+
+// The first tensor of the launch whose last one is hi - 1: as many as a table holds and a grid takes.
+static int64_t table_start(const int64_t* numel, int64_t hi) {
+    int64_t lo = hi, chunks = 0;
+    while (lo > 0 && hi - lo < kTensors) {
+        chunks += ceil_div(numel[lo - 1], kUpdateChunk);
+        if (lo < hi && chunks > kMostChunks) break;
+        --lo;
+    }
+    return lo;
 }
 
 static int check_tensors(const char* what, int64_t count, const int64_t* numel, const int32_t* dtype) {
@@ -473,12 +511,12 @@ static int check_tensors(const char* what, int64_t count, const int64_t* numel, 
     return MNX_OK;
 }
 
-// Sums of squares of every chunk; `partial` has chunks_of() places.
+// Sums of squares of every chunk; `partial` has norm_chunks() places.
 static int launch_sumsq(const void* const* grads, const int64_t* numel, const int32_t* dtype, int64_t count,
                         double* partial, mnx_stream_t stream) {
     NormTable t;
     t.count = 0;
-    t.chunk = chunk_size(numel, count);
+    t.chunk = norm_chunk(total_of(numel, count));
     t.out = 0;
     uint32_t chunks = 0;
     auto flush = [&]() -> int {
@@ -495,7 +533,7 @@ static int launch_sumsq(const void* const* grads, const int64_t* numel, const in
         if (!numel[i]) continue;
         MNX_REQUIRE(grads[i], "gradient norm: tensor %lld is null", (long long)i);
         const int64_t c = ceil_div(numel[i], t.chunk);
-        if (t.count == kNormTensors || chunks + c > (1u << 23))
+        if (t.count == kNormTensors || chunks + c > kMostChunks)
             if (int rc = flush()) return rc;
         t.g[t.count] = grads[i];
         t.n[t.count] = numel[i];
@@ -513,7 +551,7 @@ using namespace mnx;
 extern "C" {
 
 size_t mnx_grad_norm_workspace_bytes(const int64_t* numel, int64_t count) {
-    return size_t(std::max<int64_t>(count > 0 && numel ? chunks_of(numel, count, chunk_size(numel, count)) : 0, 1)) * sizeof(double);
+    return size_t(std::max<int64_t>(count > 0 && numel ? norm_chunks(numel, count) : 0, 1)) * sizeof(double);
 }
 
 int mnx_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtype, int64_t count, float* norm,
@@ -525,7 +563,7 @@ int mnx_grad_norm(const void* const* grads, const int64_t* numel, const int32_t*
         return set_error(MNX_ERR_WORKSPACE, "gradient norm: workspace too small");
     double* partial = static_cast<double*>(workspace);
     if (int rc = launch_sumsq(grads, numel, dtype, count, partial, stream)) return rc;
-    k_norm<<<1, 1024, 0, stream>>>(partial, chunks_of(numel, count, chunk_size(numel, count)), norm);
+    k_norm<<<1, 1024, 0, stream>>>(partial, norm_chunks(numel, count), norm);
     MNX_CHECK_LAUNCH();
     return MNX_OK;
 }
@@ -557,8 +595,7 @@ int mnx_adamw_step(const mnx_adamw_args* args, mnx_stream_t stream) {
     Workspace ws{static_cast<char*>(a.workspace), a.workspace_bytes};
     CallScalars* call = ws.take<CallScalars>(1);
     TensorScalars* scalars = ws.take<TensorScalars>(size_t(std::max<int64_t>(a.count, 1)));
-    const int chunk = chunk_size(a.numel, a.count);
-    const int64_t chunks = chunks_of(a.numel, a.count, chunk);
+    const int64_t chunks = norm_chunks(a.numel, a.count);
     double* partial = ws.take<double>(size_t(std::max<int64_t>(chunks, 1)));
     if (!a.workspace || !ws.fits()) return set_error(MNX_ERR_WORKSPACE, "adamw: workspace too small");
 
@@ -576,27 +613,30 @@ int mnx_adamw_step(const mnx_adamw_args* args, mnx_stream_t stream) {
         MNX_CHECK_LAUNCH();
     }
     const Hyper h{float(a.beta1), float(1 - a.beta1), float(a.beta2), float(1 - a.beta2), float(a.eps)};
-    AdamwTable t;
-    t.chunk = chunk;
-    for (int64_t at = (a.count - 1) / kTensors * kTensors; at >= 0 && a.count; at -= kTensors) {  // the last ones first
-        t.first = int(at);
-        t.count = int(std::min<int64_t>(kTensors, a.count - at));
-        int64_t c = 0;
+    int64_t bytes = 0;
+    for (int64_t i = 0; i < a.count; ++i) bytes += a.numel[i] * (3 * elem_bytes(a.dtype[i]) + (eight ? 4 : 16));
+    const auto kernel = bytes > kCacheBytes ? (eight ? k_adamw8<true> : k_adamw<true>)
+                                            : (eight ? k_adamw8<false> : k_adamw<false>);
+    for (int64_t hi = a.count, lo; hi > 0; hi = lo) {  // the last tensors first
+        AdamwTable t;
+        lo = table_start(a.numel, hi);
+        t.first = int(lo);
+        t.count = int(hi - lo);
+        uint32_t c = 0;
         for (int i = 0; i < t.count; ++i) {
-            t.p[i] = a.params[at + i];
-            t.g[i] = a.grads[at + i];
-            t.m[i] = a.exp_avgs[at + i];
-            t.v[i] = a.exp_avg_sqs[at + i];
-            t.bases[i] = eight ? a.bases[at + i] : nullptr;
-            t.n[i] = a.numel[at + i];
-            t.dtype[i] = uint8_t(a.dtype[at + i]);
-            t.start[i] = uint32_t(c);
-            c += ceil_div(t.n[i], t.chunk);
+            t.p[i] = a.params[lo + i];
+            t.g[i] = a.grads[lo + i];
+            t.m[i] = a.exp_avgs[lo + i];
+            t.v[i] = a.exp_avg_sqs[lo + i];
+            t.bases[i] = eight ? a.bases[lo + i] : nullptr;
+            t.n[i] = a.numel[lo + i];
+            t.dtype[i] = uint8_t(a.dtype[lo + i]);
+            t.start[i] = c;
+            c += uint32_t(ceil_div(t.n[i], kUpdateChunk));
         }
-        t.start[t.count] = uint32_t(c);
+        t.start[t.count] = c;
         if (!c) continue;
-        if (eight) k_adamw8<<<uint32_t(c), 256, 0, stream>>>(t, h, call, scalars);
-        else k_adamw<<<uint32_t(c), 256, 0, stream>>>(t, h, call, scalars);
+        kernel<<<c, 256, 0, stream>>>(t, h, call, scalars);
         MNX_CHECK_LAUNCH();
     }
     return MNX_OK;
@@ -609,14 +649,15 @@ int mnx_adamw8_moments(const void* const* exp_avgs, const void* const* exp_avg_s
     if (int rc = check_tensors("adamw8 moments", count, numel, nullptr)) return rc;
     MNX_REQUIRE(count == 0 || (exp_avgs && exp_avg_sqs && bases && out_avgs && out_avg_sqs),
                 "adamw8 moments: null pointer");
-    AdamwTable t;
-    t.chunk = chunk_size(numel, count);
-    for (int64_t at = 0; at < count; at += kTensors) {
-        t.first = int(at);
-        t.count = int(std::min<int64_t>(kTensors, count - at));
-        int64_t c = 0;
+    const auto kernel = total_of(numel, count) * 10 > kCacheBytes ? k_adamw8_moments<true> : k_adamw8_moments<false>;
+    for (int64_t hi = count, lo; hi > 0; hi = lo) {
+        AdamwTable t;
+        lo = table_start(numel, hi);
+        t.first = int(lo);
+        t.count = int(hi - lo);
+        uint32_t c = 0;
         for (int i = 0; i < t.count; ++i) {
-            const int64_t k = at + i;
+            const int64_t k = lo + i;
             MNX_REQUIRE(!numel[k] || (exp_avgs[k] && exp_avg_sqs[k] && bases[k] && out_avgs[k] && out_avg_sqs[k]),
                         "adamw8 moments: tensor %lld has a null pointer", (long long)k);
             t.p[i] = out_avgs[k];
@@ -626,12 +667,12 @@ int mnx_adamw8_moments(const void* const* exp_avgs, const void* const* exp_avg_s
             t.bases[i] = bases[k];
             t.n[i] = numel[k];
             t.dtype[i] = kF32;
-            t.start[i] = uint32_t(c);
-            c += ceil_div(t.n[i], t.chunk);
+            t.start[i] = c;
+            c += uint32_t(ceil_div(t.n[i], kUpdateChunk));
         }
-        t.start[t.count] = uint32_t(c);
+        t.start[t.count] = c;
         if (!c) continue;
-        k_adamw8_moments<<<uint32_t(c), 256, 0, stream>>>(t);
+        kernel<<<c, 256, 0, stream>>>(t);
         MNX_CHECK_LAUNCH();
     }
     return MNX_OK;

@@ -5,7 +5,7 @@
 // and backward took 179 us, most of it the autograd engine's thread and the caller passing the interpreter's lock to
 // and fro, and a step over 60 tensors 119 us, the time to ask each tensor its type, layout and address.  The library
 // is a Python module too, whose functions take the lists of tensors straight to the ops: through torch.ops, each of
-// 300 tensors is boxed first (BOXED_MEASURE).
+// 300 tensors is boxed first (a step over 60 tensors of 3.2 M elements took 40 us so, 26 us now).
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
