@@ -8,8 +8,9 @@
 //     dx = J(p g) - r (alpha J u + ups J a) - r h mean(u J a)
 // Every sum is in float32; the variance is the mean square about the mean, not a difference of moments.
 //
-// Each array is read or written once, and the bytes bound every kernel here (8 to 40 operations a value).  A row is
-// held in the registers of TPR threads, VPL vectors of 16 bytes each: its sums, and then its results, come from
+// Each array is read or written once, and the bytes bound every kernel here (8 to 40 operations a value): 50,000 x 2048
+// fp32 forward 138 us (6.0 TB/s), backward 208 us (5.9), second order 375 us (5.5), where a copy reaches 4.8 TB/s.  A row is
+// held in the registers of TPR threads, VPL vectors of four values each: its sums, and then its results, come from
 // there.  A workgroup has several such groups of threads, takes rows in turn, and keeps the weights in registers.  The
 // backward kernels sum over the rows they take in registers too and leave one partial row of sums a workgroup, which a
 // second launch joins, so nothing is read again and the order of the sums is fixed.
@@ -18,66 +19,71 @@
 
 namespace mnx {
 
-template <int DT>
-constexpr int kVec = DT == kF32 ? 4 : 8;  // values of a vector of 16 bytes
+constexpr int kVec = 4;  // values of a vector
 
 // Vectors are read at the alignment of a value (rows of an odd width start anywhere).
 template <int DT>
 struct Vec {
     typedef typename Elem<DT>::T T;
-    typedef T Packed __attribute__((ext_vector_type(kVec<DT>), aligned(sizeof(T))));
+    typedef T Packed __attribute__((ext_vector_type(kVec), aligned(sizeof(T))));
 };
 
-// Columns c .. c + kVec - 1 of a row of `width` values; 0 past its end.
-template <int DT>
-__device__ __forceinline__ void load_vec(const typename Elem<DT>::T* p, int c, int width, float (&v)[kVec<DT>]) {
-    if (c + kVec<DT> <= width) {
-        const auto t = *reinterpret_cast<const typename Vec<DT>::Packed*>(p + c);
-#pragma unroll
-        for (int e = 0; e < kVec<DT>; ++e) v[e] = float(t[e]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < kVec<DT>; ++e) v[e] = c + e < width ? float(p[c + e]) : 0.0f;
+// Columns c .. c + kVec - 1 of a row of `width` values; 0 past its end.  NT: past the caches.
+template <int DT, bool NT = false>
+__device__ __forceinline__ typename Vec<DT>::Packed load_raw(const typename Elem<DT>::T* p, int c, int width) {
+    typename Vec<DT>::Packed t;
+    if (c + kVec <= width) {
+        const auto* q = reinterpret_cast<const typename Vec<DT>::Packed*>(p + c);
+        if constexpr (NT) t = __builtin_nontemporal_load(q);
+        else t = *q;
+        return t;
     }
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) t[e] = c + e < width ? p[c + e] : typename Elem<DT>::T(0.0f);
+    return t;
 }
 template <int DT>
-__device__ __forceinline__ void store_vec(typename Elem<DT>::T* p, int c, int width, const float (&v)[kVec<DT>]) {
+__device__ __forceinline__ void unpack(const typename Vec<DT>::Packed& t, float (&v)[kVec]) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) v[e] = float(t[e]);
+}
+template <int DT, bool NT = false>
+__device__ __forceinline__ void load_vec(const typename Elem<DT>::T* p, int c, int width, float (&v)[kVec]) {
+    unpack<DT>(load_raw<DT, NT>(p, c, width), v);
+}
+template <int DT>
+__device__ __forceinline__ void store_vec(typename Elem<DT>::T* p, int c, int width, const float (&v)[kVec]) {
     using T = typename Elem<DT>::T;
-    if (c + kVec<DT> <= width) {
+    if (c + kVec <= width) {
         typename Vec<DT>::Packed t;
 #pragma unroll
-        for (int e = 0; e < kVec<DT>; ++e) t[e] = T(v[e]);
-        *reinterpret_cast<typename Vec<DT>::Packed*>(p + c) = t;
+        for (int e = 0; e < kVec; ++e) t[e] = T(v[e]);
+        // past the caches: 50,000 x 1152 fp32 forward 73 against 92 us, 20,001 x 576 bf16 11.4 against 14.9 us
+        __builtin_nontemporal_store(t, reinterpret_cast<typename Vec<DT>::Packed*>(p + c));
     } else {
 #pragma unroll
-        for (int e = 0; e < kVec<DT>; ++e)
+        for (int e = 0; e < kVec; ++e)
             if (c + e < width) p[c + e] = T(v[e]);
     }
 }
 // Values of a vector of weights, of the rows' type or float32; `none` where there is no vector, 0 past the end.
 template <int DT>
 __device__ __forceinline__ void load_weights(const void* p, int c, int width, int dtype, float none,
-                                             float (&v)[kVec<DT>]) {
-    constexpr int V = kVec<DT>;
+                                             float (&v)[kVec]) {
+    constexpr int V = kVec;
     if (!p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = c + e < width ? none : 0.0f;
     } else if (DT == kF32 || dtype == DT) {
         load_vec<DT>(static_cast<const typename Elem<DT>::T*>(p), c, width, v);
     } else {
-#pragma unroll
-        for (int k = 0; k < V; k += 4) {
-            float f[4];
-            load_vec<kF32>(static_cast<const float*>(p), c + k, width, f);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[k + e] = f[e];
-        }
+        load_vec<kF32>(static_cast<const float*>(p), c, width, v);
     }
 }
 
 // K sums over the TPR threads of a group, on all of them.  More than a wavefront joins through `lds` (K floats a
-// wavefront, two sets used in turn so that one barrier a call suffices).
-template <int TPR, int K>
+// wavefront, two sets used in turn so that one barrier a call suffices; every thread of the workgroup calls it).
+template <int TPR, int THREADS, int K>
 __device__ __forceinline__ void group_sum(float (&s)[K], float* lds, int& turn) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -96,12 +102,13 @@ __device__ __forceinline__ void group_sum(float (&s)[K], float* lds, int& turn) 
     }
     if constexpr (TPR > 64) {
         constexpr int W = TPR / 64;
-        float* set = lds + turn * W * K;
+        float* set = lds + turn * (THREADS / 64) * K;
         turn ^= 1;
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
             for (int k = 0; k < K; ++k) set[(threadIdx.x >> 6) * K + k] = s[k];
         __syncthreads();
+        set += threadIdx.x / TPR * W * K;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             s[k] = set[k];
@@ -115,7 +122,7 @@ template <int DT, int TPR, int VPL, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_ln_fwd(const typename Elem<DT>::T* x, int64_t rows, int width,
                                                     int64_t ldx, const void* w, const void* b, int wdt, float eps,
                                                     typename Elem<DT>::T* y, float* stats) {
-    constexpr int V = kVec<DT>, G = THREADS / TPR;
+    constexpr int V = kVec, G = THREADS / TPR;
     __shared__ float lds[2 * THREADS / 64];
     int turn = 0;
     const int t = threadIdx.x % TPR;
@@ -126,15 +133,17 @@ __global__ __launch_bounds__(THREADS) void k_ln_fwd(const typename Elem<DT>::T* 
         load_weights<DT>(b, (j * TPR + t) * V, width, wdt, 0.0f, bv[j]);
     }
     const float inv = 1.0f / width;
-    for (int64_t row = int64_t(blockIdx.x) * G + threadIdx.x / TPR; row < rows; row += int64_t(gridDim.x) * G) {
+    for (int64_t first = int64_t(blockIdx.x) * G; first < rows; first += int64_t(gridDim.x) * G) {
+        const int64_t row = first + threadIdx.x / TPR;
+        const int here = row < rows ? width : 0;  // a group past the last row reads and stores nothing
         float v[VPL][V], s[1] = {0};
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) load_vec<DT>(x + row * ldx, (j * TPR + t) * V, width, v[j]);
+        for (int j = 0; j < VPL; ++j) load_vec<DT>(x + row * ldx, (j * TPR + t) * V, here, v[j]);
 #pragma unroll
         for (int j = 0; j < VPL; ++j)
 #pragma unroll
             for (int e = 0; e < V; ++e) s[0] += v[j][e];
-        group_sum<TPR>(s, lds, turn);
+        group_sum<TPR, THREADS>(s, lds, turn);
         const float mu = s[0] * inv;
         s[0] = 0;
 #pragma unroll
@@ -144,15 +153,15 @@ __global__ __launch_bounds__(THREADS) void k_ln_fwd(const typename Elem<DT>::T* 
                 v[j][e] = (j * TPR + t) * V + e < width ? v[j][e] - mu : 0.0f;
                 s[0] += v[j][e] * v[j][e];
             }
-        group_sum<TPR>(s, lds, turn);
+        group_sum<TPR, THREADS>(s, lds, turn);
         const float r = 1.0f / sqrtf(s[0] * inv + eps);
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
 #pragma unroll
             for (int e = 0; e < V; ++e) v[j][e] = v[j][e] * r * wv[j][e] + bv[j][e];
-            store_vec<DT>(y + row * width, (j * TPR + t) * V, width, v[j]);
+            store_vec<DT>(y + row * width, (j * TPR + t) * V, here, v[j]);
         }
-        if (t == 0) {
+        if (t == 0 && here) {
             stats[row] = mu;
             stats[rows + row] = r;
         }
@@ -162,9 +171,9 @@ __global__ __launch_bounds__(THREADS) void k_ln_fwd(const typename Elem<DT>::T* 
 // Sums over the rows that the groups of a workgroup took: `acc` of each thread's columns, joined over the groups into
 // row blockIdx.x of partial (.., N, width), or as the results where there is one workgroup.
 template <int DT, int TPR, int VPL, int N, int THREADS>
-__device__ __forceinline__ void join_groups(const float (&acc)[N][VPL][kVec<DT>], float* lds, int width,
+__device__ __forceinline__ void join_groups(const float (&acc)[N][VPL][kVec], float* lds, int width,
                                             float* partial, void* const (&result)[N], int wdt) {
-    constexpr int V = kVec<DT>, G = THREADS / TPR, C = TPR * V;  // columns of a vector index
+    constexpr int V = kVec, G = THREADS / TPR, C = TPR * V;  // columns of a vector index
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
         __syncthreads();
@@ -184,28 +193,50 @@ __device__ __forceinline__ void join_groups(const float (&acc)[N][VPL][kVec<DT>]
     }
 }
 
-template <int DT, int TPR, int VPL, int THREADS>
+// In 16 bits the next row is on its way, as it lies in memory, while one is worked on: such a row is too short for the
+// wavefronts of a compute unit to cover the latency by their number (20,001 x 576 bf16: 25.8 against 31.3 us); in 32
+// bits the registers cost more wavefronts than that gains (50,000 x 1152: 172 against 129 us).
+template <int DT, int TPR, int VPL, bool NT, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_ln_bwd(const typename Elem<DT>::T* g, int64_t ldg,
                                                     const typename Elem<DT>::T* x, int64_t ldx, int64_t rows,
                                                     int width, const void* w, int wdt, const float* stats,
                                                     typename Elem<DT>::T* gx, float* partial, void* gw, void* gb,
                                                     int sums) {
-    constexpr int V = kVec<DT>, G = THREADS / TPR;
+    constexpr int V = kVec, G = THREADS / TPR;
+    constexpr bool kAhead = DT != kF32;
     extern __shared__ float lds[];
     int turn = 0;
     const int t = threadIdx.x % TPR;
+    typename Vec<DT>::Packed nx[VPL], ng[VPL];
+    float nmu, nr;
+    const auto fetch = [&](int64_t row) {
+        const int here = row < rows ? width : 0;  // a group past the last row reads and stores nothing
+        nmu = here ? stats[row] : 0.0f;
+        nr = here ? stats[rows + row] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            nx[j] = load_raw<DT, NT>(x + row * ldx, (j * TPR + t) * V, here);
+            ng[j] = load_raw<DT, NT>(g + row * ldg, (j * TPR + t) * V, here);
+        }
+    };
+    int64_t first = int64_t(blockIdx.x) * G;
+    if constexpr (kAhead) fetch(first + threadIdx.x / TPR);
     float wv[VPL][V], acc[2][VPL][V] = {};
 #pragma unroll
     for (int j = 0; j < VPL; ++j) load_weights<DT>(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
     const float inv = 1.0f / width;
-    for (int64_t row = int64_t(blockIdx.x) * G + threadIdx.x / TPR; row < rows; row += int64_t(gridDim.x) * G) {
+    for (; first < rows; first += int64_t(gridDim.x) * G) {
+        const int64_t row = first + threadIdx.x / TPR;
+        const int here = row < rows ? width : 0;
         float h[VPL][V], a[VPL][V], s[2] = {0, 0};
-        const float mu = stats[row], r = stats[rows + row];
+        if constexpr (!kAhead) fetch(row);
+        const float mu = nmu, r = nr;
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
-            load_vec<DT>(x + row * ldx, (j * TPR + t) * V, width, h[j]);
-            load_vec<DT>(g + row * ldg, (j * TPR + t) * V, width, a[j]);
+            unpack<DT>(nx[j], h[j]);
+            unpack<DT>(ng[j], a[j]);
         }
+        if constexpr (kAhead) fetch(row + int64_t(gridDim.x) * G);
 #pragma unroll
         for (int j = 0; j < VPL; ++j)
 #pragma unroll
@@ -218,26 +249,28 @@ __global__ __launch_bounds__(THREADS) void k_ln_bwd(const typename Elem<DT>::T* 
                 s[1] += a[j][e] * h[j][e];
             }
         if (!gx) continue;
-        group_sum<TPR>(s, lds, turn);
+        group_sum<TPR, THREADS>(s, lds, turn);
         const float sa = s[0] * inv, sah = s[1] * inv;
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
 #pragma unroll
             for (int e = 0; e < V; ++e) a[j][e] = r * (a[j][e] - sa - h[j][e] * sah);
-            store_vec<DT>(gx + row * width, (j * TPR + t) * V, width, a[j]);
+            store_vec<DT>(gx + row * width, (j * TPR + t) * V, here, a[j]);
         }
     }
     if (sums) join_groups<DT, TPR, VPL, 2, THREADS>(acc, lds, width, partial, {gw, gb}, wdt);
 }
 
-template <int DT, int TPR, int VPL, int THREADS>
+// SEEDS: whether there are p and q.  Force matching has neither, and their registers would cost it a third of the
+// wavefronts.
+template <int DT, int TPR, int VPL, bool SEEDS, bool NT, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_ln_bwd2(const typename Elem<DT>::T* g, int64_t ldg,
                                                      const typename Elem<DT>::T* x, int64_t ldx,
                                                      const typename Elem<DT>::T* u, int64_t ldu, int64_t rows,
                                                      int width, const void* w, const void* p, const void* q, int wdt,
                                                      const float* stats, typename Elem<DT>::T* dg,
                                                      typename Elem<DT>::T* dx, float* partial, void* dw, int sums) {
-    constexpr int V = kVec<DT>, G = THREADS / TPR;
+    constexpr int V = kVec, G = THREADS / TPR;
     extern __shared__ float lds[];
     int turn = 0;
     const int t = threadIdx.x % TPR;
@@ -245,36 +278,41 @@ __global__ __launch_bounds__(THREADS) void k_ln_bwd2(const typename Elem<DT>::T*
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
         load_weights<DT>(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
-        load_weights<DT>(p, (j * TPR + t) * V, width, wdt, 0.0f, pv[j]);
-        load_weights<DT>(q, (j * TPR + t) * V, width, wdt, 0.0f, qv[j]);
+        if constexpr (SEEDS) {
+            load_weights<DT>(p, (j * TPR + t) * V, width, wdt, 0.0f, pv[j]);
+            load_weights<DT>(q, (j * TPR + t) * V, width, wdt, 0.0f, qv[j]);
+        }
     }
     const float inv = 1.0f / width;
-    for (int64_t row = int64_t(blockIdx.x) * G + threadIdx.x / TPR; row < rows; row += int64_t(gridDim.x) * G) {
-        float h[VPL][V], gv[VPL][V], uv[VPL][V], s[7] = {};
-        const float mu = stats[row], r = stats[rows + row];
+    for (int64_t first = int64_t(blockIdx.x) * G; first < rows; first += int64_t(gridDim.x) * G) {
+        const int64_t row = first + threadIdx.x / TPR;
+        const int here = row < rows ? width : 0;  // a group past the last row reads and stores nothing
+        float h[VPL][V], gv[VPL][V], uv[VPL][V], s[SEEDS ? 7 : 5] = {};
+        const float mu = here ? stats[row] : 0.0f, r = here ? stats[rows + row] : 0.0f;
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
-            load_vec<DT>(x + row * ldx, (j * TPR + t) * V, width, h[j]);
-            load_vec<DT>(g + row * ldg, (j * TPR + t) * V, width, gv[j]);
-            load_vec<DT>(u + row * ldu, (j * TPR + t) * V, width, uv[j]);
+            load_vec<DT, NT>(x + row * ldx, (j * TPR + t) * V, here, h[j]);
+            load_vec<DT, NT>(g + row * ldg, (j * TPR + t) * V, here, gv[j]);
+            load_vec<DT, NT>(u + row * ldu, (j * TPR + t) * V, here, uv[j]);
         }
 #pragma unroll
         for (int j = 0; j < VPL; ++j)
 #pragma unroll
             for (int e = 0; e < V; ++e) {  // past the end gv, uv and the weights are 0
                 h[j][e] = (h[j][e] - mu) * r;
-                const float a = gv[j][e] * wv[j][e], b = gv[j][e] * pv[j][e];
+                const float a = gv[j][e] * wv[j][e];
                 s[0] += a;
                 s[1] += a * h[j][e];
                 s[2] += uv[j][e];
                 s[3] += uv[j][e] * h[j][e];
                 s[4] += uv[j][e] * a;
-                s[5] += b;
-                s[6] += b * h[j][e];
+                if constexpr (SEEDS) {
+                    s[5] += gv[j][e] * pv[j][e];
+                    s[6] += gv[j][e] * pv[j][e] * h[j][e];
+                }
             }
-        group_sum<TPR>(s, lds, turn);
+        group_sum<TPR, THREADS>(s, lds, turn);
         const float sa = s[0] * inv, sah = s[1] * inv, su = s[2] * inv, suh = s[3] * inv, sua = s[4] * inv;
-        const float sb = s[5] * inv, sbh = s[6] * inv;
         const float phi = r * (sua - su * sa - suh * sah);  // mean(u J a)
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
@@ -282,13 +320,16 @@ __global__ __launch_bounds__(THREADS) void k_ln_bwd2(const typename Elem<DT>::T*
             for (int e = 0; e < V; ++e) {
                 const float hv = h[j][e], gg = gv[j][e];
                 const float ju = r * (uv[j][e] - su - hv * suh), ja = r * (gg * wv[j][e] - sa - hv * sah);
-                const float jb = r * (gg * pv[j][e] - sb - hv * sbh);
                 acc[0][j][e] += gg * ju;
-                gv[j][e] = wv[j][e] * ju + pv[j][e] * hv + qv[j][e];
-                uv[j][e] = jb - r * (sah * ju + suh * ja) - r * hv * phi;
+                gv[j][e] = wv[j][e] * ju;
+                uv[j][e] = -r * (sah * ju + suh * ja + hv * phi);
+                if constexpr (SEEDS) {
+                    gv[j][e] += pv[j][e] * hv + qv[j][e];
+                    uv[j][e] += r * (gg * pv[j][e] - s[5] * inv - hv * (s[6] * inv));
+                }
             }
-            store_vec<DT>(dg + row * width, (j * TPR + t) * V, width, gv[j]);
-            store_vec<DT>(dx + row * width, (j * TPR + t) * V, width, uv[j]);
+            store_vec<DT>(dg + row * width, (j * TPR + t) * V, here, gv[j]);
+            store_vec<DT>(dx + row * width, (j * TPR + t) * V, here, uv[j]);
         }
     }
     if (sums) join_groups<DT, TPR, VPL, 1, THREADS>(acc, lds, width, partial, {dw}, wdt);
@@ -328,14 +369,14 @@ __global__ __launch_bounds__(256) void k_ln_fwd_wide(const typename Elem<DT>::T*
         const float inv = 1.0f / width;
         float s[1] = {0};
         for (int c = threadIdx.x; c < width; c += 256) s[0] += float(xr[c]);
-        group_sum<256>(s, lds, turn);
+        group_sum<256, 256>(s, lds, turn);
         const float mu = s[0] * inv;
         s[0] = 0;
         for (int c = threadIdx.x; c < width; c += 256) {
             const float d = float(xr[c]) - mu;
             s[0] += d * d;
         }
-        group_sum<256>(s, lds, turn);
+        group_sum<256, 256>(s, lds, turn);
         const float r = 1.0f / sqrtf(s[0] * inv + eps);
         for (int c = threadIdx.x; c < width; c += 256) {
             const float h = (float(xr[c]) - mu) * r;
@@ -365,7 +406,7 @@ __global__ __launch_bounds__(256) void k_ln_bwd_wide(const typename Elem<DT>::T*
             s[0] += a;
             s[1] += a * ((float(xr[c]) - mu) * r);
         }
-        group_sum<256>(s, lds, turn);
+        group_sum<256, 256>(s, lds, turn);
         const float sa = s[0] * inv, sah = s[1] * inv;
         for (int c = threadIdx.x; c < width; c += 256) {
             const float a = float(gr[c]) * (w ? load_elem(w, c, wdt) : 1.0f), h = (float(xr[c]) - mu) * r;
@@ -400,7 +441,7 @@ __global__ __launch_bounds__(256) void k_ln_bwd2_wide(const typename Elem<DT>::T
             s[5] += b;
             s[6] += b * h;
         }
-        group_sum<256>(s, lds, turn);
+        group_sum<256, 256>(s, lds, turn);
         const float sa = s[0] * inv, sah = s[1] * inv, su = s[2] * inv, suh = s[3] * inv, sua = s[4] * inv;
         const float sb = s[5] * inv, sbh = s[6] * inv;
         const float phi = r * (sua - su * sa - suh * sah);  // mean(u J a)
@@ -443,9 +484,11 @@ __global__ __launch_bounds__(256) void k_ln_cols(const typename Elem<DT>::T* g, 
     }
 }
 
-// A variant by the vectors of a row: as few threads a row as hold it in up to `Most` values each, a wavefront at most
-// where that is enough, so that its sums need no barrier (8192 x 1024 fp32: MEASURE).  Calls f(TPR, VPL) with
-// the two as integral constants; false where no variant holds the row.
+// A variant by the vectors of a row: threads and vectors a thread that leave few lanes without a value.  A wavefront or
+// less a row needs no barrier for its sums, but beyond four vectors a thread its registers leave too few rows on the way
+// (50,000 x 2048 fp32 backward: eight vectors 251 us, 256 threads of two 228 us).  Vectors of four values in 16 bits,
+// too: eight a thread cost 20,001 x 576 bf16 63 us for its second order, four 35 us, with the same loads otherwise.
+// Calls f(TPR, VPL) with the two as integral constants; false where no variant holds the row.
 template <int N>
 using Int = std::integral_constant<int, N>;
 
@@ -456,40 +499,43 @@ static void with_type(int dtype, F&& f) {
     else f(Int<kF16>());
 }
 
-template <int DT, int Most, typename F>
+template <typename F>
 static bool ln_variant(int64_t width, F&& f) {
-    constexpr int M = Most / kVec<DT>;
-    const int64_t nv = ceil_div(width, kVec<DT>);
+    const int64_t nv = ceil_div(width, kVec);
     if (nv <= 8) return f(Int<8>(), Int<1>()), true;
     if (nv <= 16) return f(Int<16>(), Int<1>()), true;
     if (nv <= 32) return f(Int<32>(), Int<1>()), true;
-    if constexpr (M >= 3)
-        if (nv <= 48) return f(Int<16>(), Int<3>()), true;
+    if (nv <= 48) return f(Int<16>(), Int<3>()), true;
     if (nv <= 64) return f(Int<64>(), Int<1>()), true;
-    if constexpr (M >= 3)
-        if (nv <= 96) return f(Int<32>(), Int<3>()), true;
+    if (nv <= 96) return f(Int<32>(), Int<3>()), true;
     if (nv <= 128) return f(Int<64>(), Int<2>()), true;
-    if constexpr (M >= 3)
-        if (nv <= 192) return f(Int<64>(), Int<3>()), true;
-    if constexpr (M >= 4)
-        if (nv <= 256) return f(Int<64>(), Int<4>()), true;
-    if constexpr (M >= 8)
-        if (nv <= 512) return f(Int<64>(), Int<8>()), true;
-    if (nv <= 256) return f(Int<256>(), Int<1>()), true;
+    if (nv <= 192) return f(Int<64>(), Int<3>()), true;
+    if (nv <= 256) return f(Int<64>(), Int<4>()), true;
+    if (nv <= 384) return f(Int<128>(), Int<3>()), true;
     if (nv <= 512) return f(Int<256>(), Int<2>()), true;
-    if constexpr (M >= 4)
-        if (nv <= 1024) return f(Int<256>(), Int<4>()), true;
-    if (nv <= 1024) return f(Int<512>(), Int<2>()), true;
-    if constexpr (M >= 4)
-        if (nv <= 2048) return f(Int<512>(), Int<4>()), true;
+    if (nv <= 768) return f(Int<256>(), Int<3>()), true;
+    if (nv <= 1024) return f(Int<256>(), Int<4>()), true;
+    if (nv <= 2048) return f(Int<512>(), Int<4>()), true;
     return false;
 }
 
-// Values of a row a thread holds at most: forward (three arrays of them in registers), backward (five), second order
-// (seven).
-constexpr int kLnMost = 32, kLnMost1 = 32, kLnMost2 = 16;
 constexpr int kLnParts = 512;  // workgroups of the backward kernels at most, so rows of partial sums
-constexpr int ln_threads(int tpr) { return tpr > 64 ? tpr : 512; }  // of their workgroups
+constexpr int kLnThreads = 512;  // of their workgroups
+
+// Workgroups of the forward kernel for `need` turns of its groups: what the device holds at once, so that the weights
+// are read once a group; but where each would take more than four turns, workgroups of two, whose rows come closer to
+// the order of memory (50,000 x 2048 fp32: 138 against 154 us; 20,001 x 576 bf16, 2.4 turns: 13.1 against 12.4).
+static int64_t ln_forward_grid(const void* kernel, int threads, int64_t need) {
+    const int64_t fill = device_fill_grid(kernel, threads, need);
+    return fill > 0 && need > 4 * fill && need <= (int64_t(1) << 24) ? ceil_div(need, 2) : fill;
+}
+
+// Whether a backward pass over `arrays` arrays reads past the 256 MB cache: 50,000 x 2048 takes 208 against 226 us so,
+// its second order 375 against 390; in 16 bits a lane's loads are narrower and lose by it.
+template <int DT>
+static bool ln_past_cache(int64_t rows, int64_t width, int arrays) {
+    return DT == kF32 && rows * width * arrays * 4 > int64_t(256) << 20;
+}
 
 // Strips of rows of the wide form's column sums.
 static int ln_strips(int64_t rows) { return int(std::max<int64_t>(1, std::min<int64_t>(256, rows / 64))); }
@@ -531,10 +577,10 @@ int mnx_layer_norm_fwd(const void* x, int64_t ldx, int64_t rows, int64_t width, 
         using T = typename Elem<DT>::T;
         const T* xs = static_cast<const T*>(x);
         T* ys = static_cast<T*>(y);
-        const bool held = ln_variant<DT, kLnMost>(width, [&](auto tpr, auto vpl) {
+        const bool held = ln_variant(width, [&](auto tpr, auto vpl) {
             constexpr int TPR = decltype(tpr)::value, VPL = decltype(vpl)::value, THREADS = TPR > 256 ? TPR : 256;
             const auto kernel = k_ln_fwd<DT, TPR, VPL, THREADS>;
-            grid = device_fill_grid(reinterpret_cast<const void*>(kernel), THREADS, ceil_div(rows, THREADS / TPR));
+            grid = ln_forward_grid(reinterpret_cast<const void*>(kernel), THREADS, ceil_div(rows, THREADS / TPR));
             if (grid > 0)
                 kernel<<<grid, THREADS, 0, stream>>>(xs, rows, int(width), ldx, weight, bias, wdtype, float(eps), ys,
                                                      stats);
@@ -586,10 +632,11 @@ int mnx_layer_norm_bwd(const void* grad, int64_t ldg, const void* x, int64_t ldx
         using T = typename Elem<DT>::T;
         const T *gs = static_cast<const T*>(grad), *xs = static_cast<const T*>(x);
         T* gx = static_cast<T*>(grad_x);
-        held = ln_variant<DT, DT == kF32 ? kLnMost1 : kLnMost1 / 2>(width, [&](auto tpr, auto vpl) {
-            constexpr int TPR = decltype(tpr)::value, VPL = decltype(vpl)::value, THREADS = ln_threads(TPR);
-            const auto kernel = k_ln_bwd<DT, TPR, VPL, THREADS>;
-            const size_t lds = size_t(2) * THREADS * kVec<DT> * sizeof(float);
+        held = ln_variant(width, [&](auto tpr, auto vpl) {
+            constexpr int TPR = decltype(tpr)::value, VPL = decltype(vpl)::value, THREADS = kLnThreads;
+            const auto kernel = ln_past_cache<DT>(rows, width, 3) ? k_ln_bwd<DT, TPR, VPL, DT == kF32, THREADS>
+                                                                  : k_ln_bwd<DT, TPR, VPL, false, THREADS>;
+            const size_t lds = size_t(2) * THREADS * kVec * sizeof(float);
             parts = ln_parts(reinterpret_cast<const void*>(kernel), THREADS, rows, THREADS / TPR);
             if (parts > 0)
                 kernel<<<parts, THREADS, lds, stream>>>(gs, ldg, xs, ldx, rows, int(width), weight, wdtype, stats, gx,
@@ -632,10 +679,13 @@ int mnx_layer_norm_bwd2(const void* grad, int64_t ldg, const void* x, int64_t ld
         using T = typename Elem<DT>::T;
         const T *gs = static_cast<const T*>(grad), *xs = static_cast<const T*>(x), *us = static_cast<const T*>(seed_x);
         T *dg = static_cast<T*>(dgrad), *dxs = static_cast<T*>(dx);
-        held = ln_variant<DT, kLnMost2>(width, [&](auto tpr, auto vpl) {
-            constexpr int TPR = decltype(tpr)::value, VPL = decltype(vpl)::value, THREADS = ln_threads(TPR);
-            const auto kernel = k_ln_bwd2<DT, TPR, VPL, THREADS>;
-            const size_t lds = size_t(THREADS) * kVec<DT> * sizeof(float);
+        held = ln_variant(width, [&](auto tpr, auto vpl) {
+            constexpr int TPR = decltype(tpr)::value, VPL = decltype(vpl)::value, THREADS = kLnThreads;
+            const bool seeds = seed_w || seed_b;
+            const auto kernel = seeds                               ? k_ln_bwd2<DT, TPR, VPL, true, false, THREADS>
+                                : ln_past_cache<DT>(rows, width, 5) ? k_ln_bwd2<DT, TPR, VPL, false, DT == kF32, THREADS>
+                                                                    : k_ln_bwd2<DT, TPR, VPL, false, false, THREADS>;
+            const size_t lds = size_t(THREADS) * kVec * sizeof(float);
             parts = ln_parts(reinterpret_cast<const void*>(kernel), THREADS, rows, THREADS / TPR);
             if (parts > 0)
                 kernel<<<parts, THREADS, lds, stream>>>(gs, ldg, xs, ldx, us, ldu, rows, int(width), weight, seed_w,
