@@ -75,6 +75,9 @@ struct StepTable {
     int count, first;
 };
 
+// The arguments of a launch, with a few pointers and numbers beside the table.
+static_assert(sizeof(AdamwTable) <= 3840 && sizeof(NormTable) <= 3840 && sizeof(StepTable) <= 3856, "4 KB of arguments");
+
 struct Hyper {
     float b1, w1, b2, w2, eps;  // w = 1 - b
 };
@@ -502,7 +505,7 @@ static int64_t table_start(const int64_t* numel, int64_t hi) {
 }
 
 static int check_tensors(const char* what, int64_t count, const int64_t* numel, const int32_t* dtype) {
-    MNX_REQUIRE(count >= 0 && (count == 0 || numel), "%s: no tensors' sizes", what);
+    MNX_REQUIRE(count >= 0 && count <= (1 << 30) && (count == 0 || numel), "%s: 0 to 2^30 tensors with their sizes", what);
     for (int64_t i = 0; i < count; ++i) {
         MNX_REQUIRE(numel[i] >= 0 && numel[i] <= MNX_OPTIM_MAX_ELEMENTS, "%s: tensor %lld has %lld elements", what,
                     (long long)i, (long long)numel[i]);

@@ -364,6 +364,16 @@ Tensor grad_norm(at::TensorList grads) {
     return norm;
 }
 
+Tensor grad_norm_autograd(at::TensorList grads) {
+    if (at::GradMode::is_enabled())
+        for (const Tensor& g : grads)
+            TORCH_CHECK(!g.requires_grad(), "molix::grad_norm is not differentiable: detach its tensors, or call it "
+                                            "under no_grad");
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto o = op<decltype(grad_norm)>("molix::grad_norm");
+    return o.call(grads);
+}
+
 struct Options {
     double lr, beta1, beta2, eps, weight_decay;
     bool maximize;
@@ -595,8 +605,9 @@ TORCH_LIBRARY_IMPL(molix, Autograd, m) {
     m.impl("layer_norm", layer_norm_autograd);
     m.impl("layer_norm_backward", layer_norm_backward_autograd);
     m.impl("layer_norm_backward2", layer_norm_backward2_autograd);
-    // no gradients: they write into leaves (their versions rise) or read gradients
-    for (const char* name : {"grad_norm", "adamw_step", "adamw8_step", "adamw8_moments"})
+    m.impl("grad_norm", grad_norm_autograd);
+    // no gradients: they write into leaves, whose versions rise
+    for (const char* name : {"adamw_step", "adamw8_step", "adamw8_moments"})
         m.impl(name, torch::CppFunction::makeFallthrough());
 }
 

@@ -44,6 +44,14 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: state_bits 8 or 32, got {bits}")
         super().add_param_group(param_group)
 
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        for group in self.param_groups:  # a group that torch.optim.AdamW saved lacks these
+            if group.get("amsgrad"):
+                raise ValueError("AdamW: amsgrad is not supported")
+            for key, value in (("maximize", False), ("state_bits", 32), ("min_8bit_size", 4096)):
+                group.setdefault(key, value)
+
     def _new_state(self, p: Tensor, group) -> dict:
         eight = group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"]
         kind = torch.uint8 if eight else torch.float32
@@ -91,8 +99,8 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict) -> None:
-        """Also takes ``torch.optim.AdamW``'s state.  The moments keep the type they were saved in (the base class
-        would give them the parameters'), and the step counts go to the device."""
+        """Also takes ``torch.optim.AdamW``'s state.  Each tensor's moments keep the form they were saved in, 8 or 32
+        bits (the base class would give them the parameters' type), and the step counts go to the device."""
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):

@@ -512,6 +512,53 @@ def test_optimizer_loads_torch_state():
         assert float((p - q).abs().max()) <= 1e-7
 
 
+def test_optimizer_group_saved_by_torch():
+    """Groups that torch.optim.AdamW saved lack this class's options; amsgrad is refused."""
+    a, b = _model(5), _model(5)
+    ob = torch.optim.AdamW(b[0].parameters())
+    _grads(b, 0)
+    ob.step()
+    oa = AdamW(a[0].parameters())
+    oa.load_state_dict(ob.state_dict())
+    oa.add_param_group({"params": a[2].parameters(), "state_bits": 8, "min_8bit_size": 1})
+    _grads(a, 1)
+    oa.step()
+    assert oa.state[a[2].weight]["exp_avg"].dtype == torch.uint8 and float(oa.state[a[0].weight]["step"]) == 2
+    with pytest.raises(ValueError, match="amsgrad"):
+        AdamW(a[0].parameters()).load_state_dict(torch.optim.AdamW(a[0].parameters(), amsgrad=True).state_dict())
+
+
+def test_opcheck_and_compile():
+    from torch.library import opcheck
+
+    p, g, m, v, s = make([300, 5])
+    num = (1e-3, 0.9, 0.999, 1e-8, 0.01, False, 1.0, None, False, None)
+    opcheck(torch.ops.molix.adamw_step.default, (p, g, m, v, s, *num))
+    p8, g8, m8, v8, b8, s8 = make([300, 5], bits=8)
+    opcheck(torch.ops.molix.adamw8_step.default, (p8, g8, m8, v8, b8, s8, *num, 3))
+    out = [torch.zeros(300, device=DEV), torch.zeros(5, device=DEV)]
+    opcheck(torch.ops.molix.adamw8_moments.default, (m8, v8, b8, out, [t.clone() for t in out]))
+    opcheck(torch.ops.molix.grad_norm.default, (g,))
+
+    def step(p, g, m, v, s):
+        return F.adamw_step(p, [t * 2 for t in g], m, v, s, max_norm=0.5, **H)
+
+    data = make([700, 33])
+    a, b = ([[t.clone() for t in ts] for ts in data] for _ in range(2))
+    na, nb = step(*a), torch.compile(step, backend="aot_eager", fullgraph=True)(*b)
+    assert torch.equal(na, nb)
+    for x, y in zip(a, b):
+        assert all(torch.equal(t, u) for t, u in zip(x, y))
+
+
+def test_norm_is_not_differentiable():
+    g = torch.ones(5, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        F.grad_norm([g * 2])
+    with torch.no_grad():
+        assert abs(float(F.grad_norm([g * 2])) - 20 ** 0.5) <= 1e-6
+
+
 def test_optimizer_closure_missing_gradients_and_versions():
     model = _model(4)
     opt = AdamW(model.parameters(), state_bits=8, min_8bit_size=1000, max_norm=1.0)

@@ -407,6 +407,17 @@ def test_opcheck():
     opcheck(torch.ops.molix.layer_norm_backward2.default, (g, x, w, stats, 1e-5, u, None, None, True))
 
 
+def test_compile_and_export():
+    mod = LayerNorm(48).to(DEV)
+    x = torch.randn(20, 48, device=DEV, requires_grad=True)
+    ref = torch.autograd.grad(mod(x).square().sum(), (x, mod.weight, mod.bias))
+    compiled = torch.compile(lambda t: mod(t).square().sum(), backend="aot_eager", fullgraph=True)
+    for a, r in zip(torch.autograd.grad(compiled(x), (x, mod.weight, mod.bias)), ref):
+        assert torch.equal(a, r)
+    program = torch.export.export(mod, (x.detach(),), strict=False)
+    assert torch.equal(program.module()(x.detach()), mod(x.detach()))
+
+
 def test_mace_layer_norms():
     """MACE's norms between interactions are the kernels', with nn.LayerNorm's parameters; its features and forces
     stay those of torch's norm to rounding."""
