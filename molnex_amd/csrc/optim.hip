@@ -26,7 +26,7 @@ namespace mnx {
 
 constexpr int kTensors = 64;       // tensors of one update launch: the table stays below 4 KB of arguments
 constexpr int kNormTensors = 160;  // tensors of one norm launch
-constexpr int kStepTensors = 480;  // tensors of one launch of the step counts
+constexpr int kStepTensors = 480;  // tensors of one launch of the step counts, a thread each
 constexpr int kBlock = 256;        // elements of a block of 8-bit states
 
 // Elements that a workgroup takes.  The update reads all that its chunk has, two vectors of each array a thread, and is
@@ -248,6 +248,18 @@ __global__ __launch_bounds__(1024) void k_adamw_prepare(const StepTable t, const
                                                        int skip_nonfinite, int maximize, double lr, const float* lr_dev,
                                                        double b1, double b2, double wd, uint32_t seed,
                                                        CallScalars* call, TensorScalars* tensors) {
+    // what does not need the norm first, so that its loads and the sum's are on the way together
+    const int i = threadIdx.x;
+    float step = 0;
+    TensorScalars s;
+    if (i < t.count) {
+        step = *t.step[i] + 1.0f;
+        if (lr_dev) lr = *lr_dev;
+        s.size = float(lr / (1 - power(b1, uint32_t(step))));
+        s.inv_root = float(1 / sqrt(1 - power(b2, uint32_t(step))));
+        s.decay = float(1 - lr * wd);
+        s.key = mix(mix(seed * 0x3C6EF373u + uint32_t(t.first + i) * 0xA54FF53Bu) + uint32_t(step) * 0x510E527Fu);
+    }
     double norm = 0;
     if (partial) norm = float(sqrt(sum_partial(partial, chunks)));
     else if (norm_in) norm = *norm_in;
@@ -262,18 +274,9 @@ __global__ __launch_bounds__(1024) void k_adamw_prepare(const StepTable t, const
         call->skip = skip;
         if (norm_out) *norm_out = float(norm);
     }
-    if (skip) return;
-    if (lr_dev) lr = *lr_dev;
-    for (int i = threadIdx.x; i < t.count; i += 1024) {
-        const float step = *t.step[i] + 1.0f;
-        *t.step[i] = step;
-        TensorScalars s;
-        s.size = float(lr / (1 - power(b1, uint32_t(step))));
-        s.inv_root = float(1 / sqrt(1 - power(b2, uint32_t(step))));
-        s.decay = float(1 - lr * wd);
-        s.key = mix(mix(seed * 0x3C6EF373u + uint32_t(t.first + i) * 0xA54FF53Bu) + uint32_t(step) * 0x510E527Fu);
-        tensors[t.first + i] = s;
-    }
+    if (skip || i >= t.count) return;
+    *t.step[i] = step;
+    tensors[t.first + i] = s;
 }
 
 struct Moments {
