@@ -13,6 +13,6 @@ class LayerNorm(nn.LayerNorm):
     the HIP kernels on GPU tensors of up to 32 bits, and as torch's own otherwise."""
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
-        if input.device.type != "cuda":
+        if not input.is_cuda:
             return super().forward(input)
         return layer_norm(input, self.normalized_shape, self.weight, self.bias, self.eps)
