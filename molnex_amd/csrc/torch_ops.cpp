@@ -218,6 +218,7 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
         ctx->save_for_backward({x, or_undefined(weight), or_undefined(bias), stats});
         ctx->saved_data["eps"] = eps;
         ctx->mark_non_differentiable({stats});
+        ctx->set_materialize_grads(false);  // of stats: a fill a call
         return {y, stats};
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
