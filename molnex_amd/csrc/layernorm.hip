@@ -8,9 +8,9 @@
 //     dx = J(p g) - r (alpha J u + ups J a) - r h mean(u J a)
 // Every sum is in float32; the variance is the mean square about the mean, not a difference of moments.
 //
-// Each array is read or written once, and the bytes bound every kernel here (8 to 40 operations a value): 50,000 x 2048
-// fp32 forward 138 us (6.0 TB/s), backward 208 us (5.9), second order 375 us (5.5), where a copy reaches 4.8 TB/s.  A row is
-// held in the registers of TPR threads, VPL vectors of four values each: its sums, and then its results, come from
+// Each array is read or written once, and the bytes bound every kernel here (8 to 40 operations a value): 50,000 x
+// 2048 fp32 forward 138 us (6.0 TB/s), backward 208 us (5.9), second order 375 us (5.5); a copy reaches 4.8 TB/s.  A row
+// is held in the registers of TPR threads, VPL vectors of four values each: its sums, and then its results, come from
 // there.  A workgroup has several such groups of threads, takes rows in turn, and keeps the weights in registers.  The
 // backward kernels sum over the rows they take in registers too and leave one partial row of sums a workgroup, which a
 // second launch joins, so nothing is read again and the order of the sums is fixed.
@@ -261,8 +261,8 @@ __global__ __launch_bounds__(THREADS) void k_ln_bwd(const typename Elem<DT>::T* 
     if (sums) join_groups<DT, TPR, VPL, 2, THREADS>(acc, lds, width, partial, {gw, gb}, wdt);
 }
 
-// SEEDS: whether there are p and q.  Force matching has neither, and their registers would cost it a third of the
-// wavefronts.
+// SEEDS: whether there are p and q.  Force matching has neither, and their registers would cost it a wavefront in four
+// (20,001 x 576 bf16: 71 against 45 us; 50,000 x 1152 fp32: 275 against 214 us).
 template <int DT, int TPR, int VPL, bool SEEDS, bool NT, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_ln_bwd2(const typename Elem<DT>::T* g, int64_t ldg,
                                                      const typename Elem<DT>::T* x, int64_t ldx,
@@ -358,9 +358,10 @@ __global__ __launch_bounds__(1024) void k_ln_join(const float* partial, int part
 // Rows too wide for a workgroup's registers: a workgroup takes a row and reads it again for each sum (from L2: a row is
 // at most a few hundred KB where many are in flight), and the column sums are a launch of their own.
 template <int DT>
-__global__ __launch_bounds__(256) void k_ln_fwd_wide(const typename Elem<DT>::T* x, int64_t rows, int width, int64_t ldx,
-                                                const void* w, const void* b, int wdt, float eps,
-                                                typename Elem<DT>::T* y, float* stats) {
+__global__ __launch_bounds__(256) void k_ln_fwd_wide(const typename Elem<DT>::T* x, int64_t rows, int width,
+                                                     int64_t ldx,
+                                                     const void* w, const void* b, int wdt, float eps,
+                                                     typename Elem<DT>::T* y, float* stats) {
     using T = typename Elem<DT>::T;
     __shared__ float lds[2 * 4 * 7];
     int turn = 0;
@@ -391,9 +392,9 @@ __global__ __launch_bounds__(256) void k_ln_fwd_wide(const typename Elem<DT>::T*
 
 template <int DT>
 __global__ __launch_bounds__(256) void k_ln_bwd_wide(const typename Elem<DT>::T* g, int64_t ldg,
-                                                const typename Elem<DT>::T* x, int64_t ldx, int64_t rows, int width,
-                                                const void* w, int wdt, const float* stats,
-                                                typename Elem<DT>::T* gx) {
+                                                     const typename Elem<DT>::T* x, int64_t ldx, int64_t rows,
+                                                     int width, const void* w, int wdt, const float* stats,
+                                                     typename Elem<DT>::T* gx) {
     using T = typename Elem<DT>::T;
     __shared__ float lds[2 * 4 * 7];
     int turn = 0;
@@ -418,11 +419,12 @@ __global__ __launch_bounds__(256) void k_ln_bwd_wide(const typename Elem<DT>::T*
 // Second order, row part; mean(u) and mean(u h) go to the column sums.
 template <int DT>
 __global__ __launch_bounds__(256) void k_ln_bwd2_wide(const typename Elem<DT>::T* g, int64_t ldg,
-                                                 const typename Elem<DT>::T* x, int64_t ldx,
-                                                 const typename Elem<DT>::T* u, int64_t ldu, int64_t rows, int width,
-                                                 const void* w, const void* p, const void* q, int wdt,
-                                                 const float* stats, typename Elem<DT>::T* dg,
-                                                 typename Elem<DT>::T* dx, float* usums) {
+                                                      const typename Elem<DT>::T* x, int64_t ldx,
+                                                      const typename Elem<DT>::T* u, int64_t ldu, int64_t rows,
+                                                      int width,
+                                                      const void* w, const void* p, const void* q, int wdt,
+                                                      const float* stats, typename Elem<DT>::T* dg,
+                                                      typename Elem<DT>::T* dx, float* usums) {
     using T = typename Elem<DT>::T;
     __shared__ float lds[2 * 4 * 7];
     int turn = 0;
@@ -484,11 +486,6 @@ __global__ __launch_bounds__(256) void k_ln_cols(const typename Elem<DT>::T* g, 
     }
 }
 
-// A variant by the vectors of a row: threads and vectors a thread that leave few lanes without a value.  A wavefront or
-// less a row needs no barrier for its sums, but beyond four vectors a thread its registers leave too few rows on the way
-// (50,000 x 2048 fp32 backward: eight vectors 251 us, 256 threads of two 228 us).  Vectors of four values in 16 bits,
-// too: eight a thread cost 20,001 x 576 bf16 63 us for its second order, four 35 us, with the same loads otherwise.
-// Calls f(TPR, VPL) with the two as integral constants; false where no variant holds the row.
 template <int N>
 using Int = std::integral_constant<int, N>;
 
@@ -499,6 +496,11 @@ static void with_type(int dtype, F&& f) {
     else f(Int<kF16>());
 }
 
+// A variant by the vectors of a row: threads and vectors a thread that leave few lanes without a value.  A wavefront
+// or less a row needs no barrier for its sums, but beyond four vectors a thread its registers leave too few rows on the
+// way (50,000 x 2048 fp32 backward: eight vectors 251 us, 256 threads of two 228 us).  Vectors of four values in 16 bits,
+// too (12,345 x 333 f16 forward: 7.6 us, 8.5 with eight).  Calls f(TPR, VPL) with the two as integral constants; false
+// where no variant holds the row.
 template <typename F>
 static bool ln_variant(int64_t width, F&& f) {
     const int64_t nv = ceil_div(width, kVec);
@@ -681,10 +683,9 @@ int mnx_layer_norm_bwd2(const void* grad, int64_t ldg, const void* x, int64_t ld
         T *dg = static_cast<T*>(dgrad), *dxs = static_cast<T*>(dx);
         held = ln_variant(width, [&](auto tpr, auto vpl) {
             constexpr int TPR = decltype(tpr)::value, VPL = decltype(vpl)::value, THREADS = kLnThreads;
-            const bool seeds = seed_w || seed_b;
-            const auto kernel = seeds                               ? k_ln_bwd2<DT, TPR, VPL, true, false, THREADS>
-                                : ln_past_cache<DT>(rows, width, 5) ? k_ln_bwd2<DT, TPR, VPL, false, DT == kF32, THREADS>
-                                                                    : k_ln_bwd2<DT, TPR, VPL, false, false, THREADS>;
+            auto kernel = k_ln_bwd2<DT, TPR, VPL, false, false, THREADS>;
+            if (seed_w || seed_b) kernel = k_ln_bwd2<DT, TPR, VPL, true, false, THREADS>;
+            else if (ln_past_cache<DT>(rows, width, 5)) kernel = k_ln_bwd2<DT, TPR, VPL, false, DT == kF32, THREADS>;
             const size_t lds = size_t(THREADS) * kVec * sizeof(float);
             parts = ln_parts(reinterpret_cast<const void*>(kernel), THREADS, rows, THREADS / TPR);
             if (parts > 0)

@@ -455,12 +455,14 @@ Tensor step(const char* name, int bits, at::TensorList params, at::TensorList gr
         numel[i] = p.numel();
         dtype[i] = dtype_of(p.scalar_type());
     }
-    std::vector<void*> order;
-    for (void* p : p_ptr)
-        if (p) order.push_back(p);
-    std::sort(order.begin(), order.end());
-    TORCH_CHECK_VALUE(std::adjacent_find(order.begin(), order.end()) == order.end(), "molix::", name,
-                      ": a parameter is given twice");
+    const auto twice = [](auto ptrs) {
+        std::sort(ptrs.begin(), ptrs.end());
+        typename decltype(ptrs)::value_type none{};  // of tensors without elements
+        const auto first = std::upper_bound(ptrs.begin(), ptrs.end(), none);
+        return std::adjacent_find(first, ptrs.end()) != ptrs.end();
+    };
+    TORCH_CHECK_VALUE(!twice(p_ptr), "molix::", name, ": a parameter is given twice");
+    TORCH_CHECK_VALUE(!twice(s_ptr), "molix::", name, ": a step count is given twice");
 
     mnx_adamw_args a{};
     a.count = int64_t(count);

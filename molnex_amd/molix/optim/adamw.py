@@ -44,6 +44,10 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: state_bits 8 or 32, got {bits}")
         super().add_param_group(param_group)
 
+    def __getstate__(self) -> dict:
+        return super().__getstate__() | {"max_norm": self.max_norm, "skip_nonfinite": self.skip_nonfinite,
+                                         "seed": self.seed, "grad_norm": None}
+
     def __setstate__(self, state) -> None:
         super().__setstate__(state)
         for group in self.param_groups:  # a group that torch.optim.AdamW saved lacks these
@@ -80,7 +84,7 @@ class AdamW(torch.optim.Optimizer):
                 lists = calls.setdefault((p.device, k, bases is not None), ([], [], [], [], [], []))
                 for l, t in zip(lists, (p, p.grad, state["exp_avg"], state["exp_avg_sq"], state["step"], bases)):
                     l.append(t)
-        norm = None
+        norm = self.grad_norm = None
         if self.max_norm is not None or self.skip_nonfinite:
             if len({device for device, _, _ in calls}) > 1:
                 raise RuntimeError("AdamW: clipping and skip_nonfinite take parameters of one device")

@@ -163,6 +163,7 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, lr, betas
 
 def adamw8_moments(exp_avgs, exp_avg_sqs, bases, out=None) -> tuple[list[Tensor], list[Tensor]]:
     """The moments that 8-bit states stand for, in float32 (into ``out``, two lists of tensors, if given)."""
+    exp_avgs, exp_avg_sqs = list(exp_avgs), list(exp_avg_sqs)
     if out is None:
         out = tuple([torch.empty_like(t, dtype=torch.float32) for t in ts] for ts in (exp_avgs, exp_avg_sqs))
     if exp_avgs or exp_avg_sqs:

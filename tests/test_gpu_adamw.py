@@ -495,6 +495,23 @@ def test_optimizer_state_dict(bits, dtype):
         assert s["step"].device.type == "cuda" and float(s["step"]) == 6
 
 
+def test_optimizer_copy():
+    """A copied optimizer with its copied model steps as the original does."""
+    import copy
+
+    a = _model(6)
+    oa = AdamW(a.parameters(), max_norm=0.1, state_bits=8, min_8bit_size=100, seed=3)
+    _grads(a, 0)
+    oa.step()
+    both = {"model": a, "opt": oa}
+    twin = copy.deepcopy(both)
+    for m, o in ((a, oa), (twin["model"], twin["opt"])):
+        _grads(m, 1)
+        o.step()
+    assert all(torch.equal(p, q) for p, q in zip(a.parameters(), twin["model"].parameters()))
+    assert float(oa.grad_norm) == float(twin["opt"].grad_norm)
+
+
 def test_optimizer_loads_torch_state():
     a, b = _model(3), _model(3)
     ob = torch.optim.AdamW(b.parameters())
@@ -594,6 +611,9 @@ def test_refusals():
         F.adamw_step(p, g, m, v, [s[0].double()], **H)
     with pytest.raises(ValueError):
         F.adamw_step(p * 2, g * 2, m * 2, v * 2, s * 2, **H)
+    two = make([300, 300])
+    with pytest.raises(ValueError, match="step count"):
+        F.adamw_step(*two[:4], [two[4][0]] * 2, **H)
     with pytest.raises(ValueError):
         F.adamw_step(p, g, m, v, s, **{**H, "betas": (1.0, 0.9)})
     with pytest.raises(ValueError):

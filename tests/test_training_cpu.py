@@ -44,6 +44,15 @@ def test_nothing_to_do():
     assert opt.step() is None and opt.step(lambda: 2.5) == 2.5 and torch.equal(p, torch.ones(3))
 
 
+def test_copies_of_an_optimizer_keep_its_options():
+    p = torch.nn.Parameter(torch.ones(3))
+    opt = AdamW([p], lr=0.5, max_norm=2.0, skip_nonfinite=True, seed=11, state_bits=8)
+    for again in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert (again.max_norm, again.skip_nonfinite, again.seed) == (2.0, True, 11)
+        assert again.param_groups[0]["state_bits"] == 8 and again.param_groups[0]["lr"] == 0.5
+        assert again.step() is None and again.grad_norm is None
+
+
 def test_arguments():
     p = [torch.nn.Parameter(torch.ones(3))]
     for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(betas=(0.9,)), dict(eps=-1e-8), dict(weight_decay=-1.0),
