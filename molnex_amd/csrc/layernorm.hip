@@ -9,9 +9,9 @@
 // Every sum is in float32; the variance is the mean square about the mean, not a difference of moments.
 //
 // Each array is read or written once, and the bytes bound every kernel here (8 to 40 operations a value): 50,000 x
-// 2048 fp32 forward 138 us (6.0 TB/s), backward 208 us (5.9), second order 375 us (5.5); a copy reaches 4.8 TB/s.  A row
-// is held in the registers of TPR threads, VPL vectors of four values each: its sums, and then its results, come from
-// there.  A workgroup has several such groups of threads, takes rows in turn, and keeps the weights in registers.  The
+// 2048 fp32 forward 138 us (6.0 TB/s), backward 208 us (5.9), second order 375 us (5.5); a copy reaches 4.8 TB/s.  A
+// row is held in the registers of TPR threads, VPL vectors of four values each: its sums, and then its results, come
+// from there.  A workgroup has several such groups of threads, takes rows in turn, and keeps the weights in registers.  The
 // backward kernels sum over the rows they take in registers too and leave one partial row of sums a workgroup, which a
 // second launch joins, so nothing is read again and the order of the sums is fixed.
 #include "elem.h"
@@ -498,8 +498,8 @@ static void with_type(int dtype, F&& f) {
 
 // A variant by the vectors of a row: threads and vectors a thread that leave few lanes without a value.  A wavefront
 // or less a row needs no barrier for its sums, but beyond four vectors a thread its registers leave too few rows on the
-// way (50,000 x 2048 fp32 backward: eight vectors 251 us, 256 threads of two 228 us).  Vectors of four values in 16 bits,
-// too (12,345 x 333 f16 forward: 7.6 us, 8.5 with eight).  Calls f(TPR, VPL) with the two as integral constants; false
+// way (50,000 x 2048 fp32 backward: eight vectors 251 us, 256 threads of two 228 us).  Vectors of four values in 16
+// bits, too (12,345 x 333 f16 forward: 7.6 us, 8.5 with eight).  Calls f(TPR, VPL) with the two as integral constants; false
 // where no variant holds the row.
 template <typename F>
 static bool ln_variant(int64_t width, F&& f) {

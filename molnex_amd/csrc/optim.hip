@@ -32,8 +32,8 @@ constexpr int kBlock = 256;        // elements of a block of 8-bit states
 // Elements that a workgroup takes.  The update reads all that its chunk has, two vectors of each array a thread, and is
 // done: 128 M fp32 parameters take 645 us so, 656 us with four vectors, and 721 us in chunks of 8192 looped over; 24 M
 // bf16 ones 95, 99 and 117 us, 64 M with 8-bit states 261, 269 and 282 us.
-// The norm's workgroups leave a partial sum each, for one workgroup to add up, and take more; small calls are cut finer,
-// so that they reach every compute unit.
+// The norm's workgroups leave a partial sum each, for one workgroup to add up, and take more; small calls are cut
+// finer, so that they reach every compute unit.
 constexpr int kUpdateVectors = 2, kUpdateChunk = kUpdateVectors * 1024;
 inline int norm_chunk(int64_t total) {
     int chunk = 1024;
@@ -45,8 +45,8 @@ inline int norm_chunk(int64_t total) {
 constexpr int64_t kMostChunks = int64_t(1) << 23;
 static_assert(MNX_OPTIM_MAX_ELEMENTS / kUpdateChunk <= kMostChunks, "a tensor fits a launch");
 
-// Calls that move more than the 256 MB cache holds pass it by: 128 M fp32 parameters take 645 us so against 788 us, 64 M
-// with 8-bit states and their read-back 261 against 307 us; 3.2 M, which fit, 31.9 against 29.9 us.
+// Calls that move more than the 256 MB cache holds pass it by: 128 M fp32 parameters take 645 us so against 788 us,
+// 64 M with 8-bit states and their read-back 261 against 307 us; 3.2 M, which fit, 31.9 against 29.9 us.
 constexpr int64_t kCacheBytes = int64_t(256) << 20;
 
 struct AdamwTable {
@@ -76,7 +76,8 @@ struct StepTable {
 };
 
 // The arguments of a launch, with a few pointers and numbers beside the table.
-static_assert(sizeof(AdamwTable) <= 3840 && sizeof(NormTable) <= 3840 && sizeof(StepTable) <= 3856, "4 KB of arguments");
+static_assert(sizeof(AdamwTable) <= 3840 && sizeof(NormTable) <= 3840 && sizeof(StepTable) <= 3856,
+              "4 KB of arguments");
 
 struct Hyper {
     float b1, w1, b2, w2, eps;  // w = 1 - b
@@ -234,7 +235,7 @@ __device__ __forceinline__ uint32_t mix(uint32_t x) {
     return x ^ (x >> 16);
 }
 
-// b^t of a whole number t by squaring: 24 multiplications deep at most, where the library's pow takes microseconds.
+// b^t of a whole number t by squaring, 24 multiplications deep at most.
 __device__ __forceinline__ double power(double b, uint32_t t) {
     double r = 1;
     for (; t; t >>= 1, b *= b)
@@ -287,8 +288,8 @@ __device__ __forceinline__ Moments moments(const Hyper& h, float m, float v, flo
     return {m * h.b1 + g * h.w1, v * h.b2 + (g * g) * h.w2};
 }
 // The square root and the reciprocal by the hardware's instructions, a unit of the last place each: the update is lr
-// times a number of the order of one, added to p, and the exact forms are a third of k_adamw8's instructions (then 230
-// against 223 us for 64 M elements, before other steps brought that to 166 us, 6.2 TB/s).
+// times a number of the order of one, added to p.  (k_adamw8 took 223 us for 64 M elements with them and 230 with the
+// exact forms, before other steps brought it to 166 us, 6.2 TB/s.)
 // The root's instruction takes no subnormals: a v below 2^-96 is scaled (its root is far below any eps but 0).
 __device__ __forceinline__ float updated(const Hyper& h, const TensorScalars& s, float p, const Moments& a) {
     const bool tiny = a.v < 0x1p-96f;
@@ -508,7 +509,8 @@ static int64_t table_start(const int64_t* numel, int64_t hi) {
 }
 
 static int check_tensors(const char* what, int64_t count, const int64_t* numel, const int32_t* dtype) {
-    MNX_REQUIRE(count >= 0 && count <= (1 << 30) && (count == 0 || numel), "%s: 0 to 2^30 tensors with their sizes", what);
+    MNX_REQUIRE(count >= 0 && count <= (1 << 30) && (count == 0 || numel), "%s: 0 to 2^30 tensors with their sizes",
+                what);
     for (int64_t i = 0; i < count; ++i) {
         MNX_REQUIRE(numel[i] >= 0 && numel[i] <= MNX_OPTIM_MAX_ELEMENTS, "%s: tensor %lld has %lld elements", what,
                     (long long)i, (long long)numel[i]);
@@ -593,7 +595,8 @@ int mnx_adamw_step(const mnx_adamw_args* args, mnx_stream_t stream) {
     MNX_REQUIRE(a.count == 0 || (a.params && a.grads && a.exp_avgs && a.exp_avg_sqs && a.steps && a.dtype &&
                                  (!eight || a.bases)),
                 "adamw: null pointer");
-    MNX_REQUIRE(a.beta1 >= 0 && a.beta1 < 1 && a.beta2 >= 0 && a.beta2 < 1 && a.eps >= 0, "adamw: 0 <= beta < 1, eps >= 0");
+    MNX_REQUIRE(a.beta1 >= 0 && a.beta1 < 1 && a.beta2 >= 0 && a.beta2 < 1 && a.eps >= 0,
+                "adamw: 0 <= beta < 1, eps >= 0");
     for (int64_t i = 0; i < a.count; ++i)
         MNX_REQUIRE(a.steps[i] && (!a.numel[i] || (a.params[i] && a.grads[i] && a.exp_avgs[i] && a.exp_avg_sqs[i] &&
                                                    (!eight || a.bases[i]))),

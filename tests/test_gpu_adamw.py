@@ -23,7 +23,7 @@ from molnex_amd.molix.optim import AdamW
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 U = 2.0 ** -24
-HALF = {torch.float32: 0.0, torch.bfloat16: torch.finfo(torch.bfloat16).eps / 2, torch.float16: torch.finfo(torch.float16).eps / 2}
+HALF = {torch.float32: 0.0, **{d: torch.finfo(d).eps / 2 for d in (torch.bfloat16, torch.float16)}}
 H = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.05)
 B = 256
 

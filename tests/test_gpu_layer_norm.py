@@ -4,7 +4,8 @@ Tolerances, with u = 2^-24, per row of D values.  A sum over the row is at most 
 (D / 64 + 8) u of the sum of magnitudes; x - mean is off by u max|x|, which in units of the row's deviation is u k with
 k = max|x| rstd; a handful of further roundings follows.  With c = D / 64 + 32:
     y           c u (|y| + |b| + k |w|), value by value
-    grad_x      (c + 8 k) u rstd |a|_2, a = g w, in the row's 2-norm (h has norm sqrt(D), mean(a h) is below |a| / sqrt(D))
+    grad_x      (c + 8 k) u rstd |a|_2, a = g w, in the row's 2-norm (h has norm sqrt(D), mean(a h) is below
+                |a| / sqrt(D))
     dgrad       (c + 8 k) u (max|w| rstd |u|_2 + max|p| |h|_2 + |q|_2)
     dx          (c + 16 k) u (rstd |p g|_2 + 4 rstd^2 |a|_2 |u|_2 / sqrt(D))
 Sums over R rows are at most 320 + R / 512 additions deep: that many u more, of the sum of the magnitudes.
@@ -336,8 +337,11 @@ def test_weight_gradients_are_reproducible():
 
 def test_side_stream_and_graph():
     x, w, b, g, _ = _inputs(900, 192)
-    stats_of = lambda: torch.ops.molix.layer_norm(x, w, b, 1e-5)  # noqa: E731
-    both = lambda: (lambda ys: (ys[0], *torch.ops.molix.layer_norm_backward(g, x, w, b, ys[1], 1e-5, True, True, True)))(stats_of())  # noqa: E731
+
+    def both():
+        y, stats = torch.ops.molix.layer_norm(x, w, b, 1e-5)
+        return (y, *torch.ops.molix.layer_norm_backward(g, x, w, b, stats, 1e-5, True, True, True))
+
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
