@@ -869,7 +869,8 @@ int mnx_channel_outer_stack_bwd_f32(const float* grad, const float* y, const flo
 /* Layer norm over the last axis of rows x width values, rows ldx (ldg, ldu)  */
 /* elements apart, unit stride within a row; outputs are contiguous.  dtype   */
 /* is the type of every rows x width array, wdtype that of the vectors of     */
-/* width values; sums are in float32.  weight and bias may be NULL (1 and 0). */
+/* width values, any of the three whatever dtype; sums are in float32.        */
+/* weight and bias may be NULL (1 and 0).                                      */
 /*   y = (x - mean) rstd weight + bias,  rstd = 1 / sqrt(var + eps)            */
 /* stats [2][rows] float32: mean, rstd, as the backward reads them.           */
 /* bwd: NULL outputs are skipped.  bwd2: the derivatives of                    */

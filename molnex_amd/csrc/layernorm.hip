@@ -66,18 +66,19 @@ __device__ __forceinline__ void store_vec(typename Elem<DT>::T* p, int c, int wi
             if (c + e < width) p[c + e] = T(v[e]);
     }
 }
-// Values of a vector of weights, of the rows' type or float32; `none` where there is no vector, 0 past the end.
-template <int DT>
+// Values of a vector of weights, of any type whatever the rows'; `none` where there is no vector, 0 past the end.
 __device__ __forceinline__ void load_weights(const void* p, int c, int width, int dtype, float none,
                                              float (&v)[kVec]) {
     constexpr int V = kVec;
     if (!p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = c + e < width ? none : 0.0f;
-    } else if (DT == kF32 || dtype == DT) {
-        load_vec<DT>(static_cast<const typename Elem<DT>::T*>(p), c, width, v);
-    } else {
+    } else if (dtype == kF32) {
         load_vec<kF32>(static_cast<const float*>(p), c, width, v);
+    } else if (dtype == kBF16) {
+        load_vec<kBF16>(static_cast<const __bf16*>(p), c, width, v);
+    } else {
+        load_vec<kF16>(static_cast<const _Float16*>(p), c, width, v);
     }
 }
 
@@ -129,8 +130,8 @@ __global__ __launch_bounds__(THREADS) void k_ln_fwd(const typename Elem<DT>::T* 
     float wv[VPL][V], bv[VPL][V];
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-        load_weights<DT>(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
-        load_weights<DT>(b, (j * TPR + t) * V, width, wdt, 0.0f, bv[j]);
+        load_weights(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
+        load_weights(b, (j * TPR + t) * V, width, wdt, 0.0f, bv[j]);
     }
     const float inv = 1.0f / width;
     for (int64_t first = int64_t(blockIdx.x) * G; first < rows; first += int64_t(gridDim.x) * G) {
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(THREADS) void k_ln_bwd(const typename Elem<DT>::T* 
     if constexpr (kAhead) fetch(first + threadIdx.x / TPR);
     float wv[VPL][V], acc[2][VPL][V] = {};
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) load_weights<DT>(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
+    for (int j = 0; j < VPL; ++j) load_weights(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
     const float inv = 1.0f / width;
     for (; first < rows; first += int64_t(gridDim.x) * G) {
         const int64_t row = first + threadIdx.x / TPR;
@@ -277,10 +278,10 @@ __global__ __launch_bounds__(THREADS) void k_ln_bwd2(const typename Elem<DT>::T*
     float wv[VPL][V], pv[VPL][V], qv[VPL][V], acc[1][VPL][V] = {};
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-        load_weights<DT>(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
+        load_weights(w, (j * TPR + t) * V, width, wdt, 1.0f, wv[j]);
         if constexpr (SEEDS) {
-            load_weights<DT>(p, (j * TPR + t) * V, width, wdt, 0.0f, pv[j]);
-            load_weights<DT>(q, (j * TPR + t) * V, width, wdt, 0.0f, qv[j]);
+            load_weights(p, (j * TPR + t) * V, width, wdt, 0.0f, pv[j]);
+            load_weights(q, (j * TPR + t) * V, width, wdt, 0.0f, qv[j]);
         }
     }
     const float inv = 1.0f / width;
