@@ -63,8 +63,8 @@ struct Shape {
     int dtype, wdtype;
 };
 
+// Checks the arguments, but for x's device.
 Shape norm_shape(const char* name, const Tensor& x, const OptTensor& weight, const OptTensor& bias) {
-    TORCH_CHECK(x.is_cuda(), "molix::", name, " runs on the GPU only (got a ", x.device(), " tensor)");
     Shape s{0, 0, dtype_of(x.scalar_type()), -1};
     TORCH_CHECK_TYPE(s.dtype >= 0, "molix::", name, ": float32, bfloat16 or float16, got ", x.scalar_type());
     TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= MNX_LAYER_NORM_MAX_WIDTH, "molix::", name,
@@ -84,6 +84,11 @@ Shape norm_shape(const char* name, const Tensor& x, const OptTensor& weight, con
     }
     if (s.wdtype < 0) s.wdtype = s.dtype;
     return s;
+}
+
+Shape gpu_shape(const char* name, const Tensor& x, const OptTensor& weight, const OptTensor& bias) {
+    TORCH_CHECK(x.is_cuda(), "molix::", name, " runs on the GPU only (got a ", x.device(), " tensor)");
+    return norm_shape(name, x, weight, bias);
 }
 
 // A tensor's rows in place where they are evenly spaced (a column block of a wider matrix), else a contiguous copy.
@@ -111,7 +116,7 @@ void check_like(const char* name, const char* what, const Tensor& t, const Tenso
 }
 
 std::tuple<Tensor, Tensor> layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
-    const Shape s = norm_shape("layer_norm", x, weight, bias);
+    const Shape s = gpu_shape("layer_norm", x, weight, bias);
     const c10::DeviceGuard guard(x.device());
     const Rows xs(x, s.width);
     const OptTensor w = contiguous(weight), b = contiguous(bias);
@@ -131,7 +136,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& grad, const
                                                        bool need_x, bool need_w, bool need_b) {
     (void)eps;  // higher orders read it
     const char* name = "layer_norm_backward";
-    const Shape s = norm_shape(name, x, weight, bias);
+    const Shape s = gpu_shape(name, x, weight, bias);
     check_like(name, "grad", grad, x);
     check_stats(name, stats, x, s.rows);
     TORCH_CHECK_VALUE((!need_w || given(weight)) && (!need_b || given(bias)), "molix::", name,
@@ -161,7 +166,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward2(const Tensor& grad, cons
                                                         bool need_w) {
     (void)eps;
     const char* name = "layer_norm_backward2";
-    Shape s = norm_shape(name, x, weight, std::nullopt);
+    Shape s = gpu_shape(name, x, weight, std::nullopt);
     check_like(name, "grad", grad, x);
     check_stats(name, stats, x, s.rows);
     if (given(seed_x)) check_like(name, "seed_x", *seed_x, x);
@@ -209,6 +214,68 @@ bool wants_grad(const OptTensor& t) { return given(t) && t->requires_grad(); }
 OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 Tensor or_undefined(const OptTensor& t) { return given(t) ? *t : Tensor(); }
 
+// Whether t carries a tangent (forward-mode differentiation).  The autograd Functions below know backward mode only.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+
+// The three ops as torch operations in float32, rounded once at the end: differentiable in every mode and to any order.
+// Tensors that carry tangents take them, and the third order in backward mode.
+std::tuple<Tensor, Tensor> layer_norm_formula(const Tensor& x, const OptTensor& weight, const OptTensor& bias,
+                                              double eps) {
+    norm_shape("layer_norm", x, weight, bias);
+    const auto f32 = [](const OptTensor& t) { return given(t) ? OptTensor(t->to(at::kFloat)) : std::nullopt; };
+    const auto [y, mu, r] = at::native_layer_norm(x.to(at::kFloat), {x.size(-1)}, f32(weight), f32(bias), eps);
+    return {y.to(x.scalar_type()), at::stack({mu.detach().reshape(-1), r.detach().reshape(-1)})};
+}
+
+// A row h of float32 values without mean and of variance one, and its derivative J.
+struct Normed {
+    Tensor h, r;
+    Normed(const Tensor& x, double eps) {
+        const Tensor xc = x - x.mean(1, true);
+        r = (xc.square().mean(1, true) + eps).rsqrt();
+        h = xc * r;
+    }
+    Tensor J(const Tensor& a) const { return r * (a - a.mean(1, true) - h * (a * h).mean(1, true)); }
+};
+Tensor rows_f32(const Tensor& t) { return t.reshape({-1, t.size(-1)}).to(at::kFloat); }
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_formula(const Tensor& grad, const Tensor& x,
+                                                               const OptTensor& weight, const OptTensor& bias,
+                                                               double eps, bool need_x, bool need_w, bool need_b) {
+    norm_shape("layer_norm_backward", x, weight, bias);
+    check_like("layer_norm_backward", "grad", grad, x);
+    const Normed n(rows_f32(x), eps);
+    const Tensor g = rows_f32(grad);
+    Tensor gx = at::empty({0}, x.options()), gw = vector_like(x, weight, false), gb = vector_like(x, bias, false);
+    if (need_x) gx = n.J(given(weight) ? g * weight->to(at::kFloat) : g).to(x.scalar_type()).reshape(x.sizes());
+    if (need_w) gw = (g * n.h).sum(0).to(gw.scalar_type());
+    if (need_b) gb = g.sum(0).to(gb.scalar_type());
+    return {gx, gw, gb};
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward2_formula(const Tensor& grad, const Tensor& x,
+                                                                const OptTensor& weight, double eps,
+                                                                const OptTensor& seed_x, const OptTensor& seed_w,
+                                                                const OptTensor& seed_b, bool need_w) {
+    const Tensor g = rows_f32(grad), x2 = rows_f32(x);
+    const Normed n(x2, eps);
+    const Tensor& h = n.h;
+    const Tensor u = given(seed_x) ? rows_f32(*seed_x) : at::zeros_like(x2);
+    const Tensor w = given(weight) ? weight->to(at::kFloat) : at::ones({x.size(-1)}, x2.options());
+    const Tensor a = g * w, ju = n.J(u);
+    Tensor dg = w * ju;
+    Tensor dx = -n.r * ((a * h).mean(1, true) * ju + (u * h).mean(1, true) * n.J(a)) - n.r * h * (ju * a).mean(1, true);
+    if (given(seed_w)) {
+        const Tensor p = seed_w->to(at::kFloat);
+        dg = dg + p * h;
+        dx = dx + n.J(g * p);
+    }
+    if (given(seed_b)) dg = dg + seed_b->to(at::kFloat);
+    Tensor dw = need_w ? (g * ju).sum(0).to(weight->scalar_type()) : vector_like(x, weight, false);
+    return {dg.to(x.scalar_type()).reshape(x.sizes()), dx.to(x.scalar_type()).reshape(x.sizes()), dw};
+}
+
 class LayerNorm : public torch::autograd::Function<LayerNorm> {
   public:
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias,
@@ -236,6 +303,7 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
 
 std::tuple<Tensor, Tensor> layer_norm_autograd(const Tensor& x, const OptTensor& weight, const OptTensor& bias,
                                                double eps) {
+    if (has_tangent(x) || has_tangent(weight) || has_tangent(bias)) return layer_norm_formula(x, weight, bias, eps);
     if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias))) {
         auto r = LayerNorm::apply(x, weight, bias, eps);
         return {r[0], r[1]};
@@ -285,6 +353,8 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_autograd(const Tensor& gr
                                                                 const OptTensor& weight, const OptTensor& bias,
                                                                 const Tensor& stats, double eps, bool need_x,
                                                                 bool need_w, bool need_b) {
+    if (has_tangent(grad) || has_tangent(x) || has_tangent(weight))
+        return layer_norm_backward_formula(grad, x, weight, bias, eps, need_x, need_w, need_b);
     if (at::GradMode::is_enabled() && (grad.requires_grad() || x.requires_grad() || wants_grad(weight))) {
         auto r = LayerNormBackward::apply(grad, x, weight, bias, stats, eps, need_x, need_w, need_b);
         return {r[0], r[1], r[2]};
@@ -293,35 +363,18 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_autograd(const Tensor& gr
     return layer_norm_backward_op().call(grad, x, weight, bias, stats, eps, need_x, need_w, need_b);
 }
 
-// Third and higher orders: the second order as differentiable torch operations in float32.
 std::tuple<Tensor, Tensor, Tensor> layer_norm_backward2_autograd(const Tensor& grad, const Tensor& x,
                                                                  const OptTensor& weight, const Tensor& stats,
                                                                  double eps, const OptTensor& seed_x,
                                                                  const OptTensor& seed_w, const OptTensor& seed_b,
                                                                  bool need_w) {
-    bool tracked = grad.requires_grad() || x.requires_grad();
-    for (const auto* t : {&weight, &seed_x, &seed_w, &seed_b}) tracked |= wants_grad(*t);
-    if (!at::GradMode::is_enabled() || !tracked) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        return layer_norm_backward2_op().call(grad, x, weight, stats, eps, seed_x, seed_w, seed_b, need_w);
-    }
-    const int64_t D = x.size(-1);
-    const Tensor g2 = grad.reshape({-1, D}).to(at::kFloat), x2 = x.reshape({-1, D}).to(at::kFloat);
-    const Tensor u = given(seed_x) ? seed_x->reshape({-1, D}).to(at::kFloat) : at::zeros_like(x2);
-    const Tensor w = given(weight) ? weight->to(at::kFloat) : at::ones({D}, x2.options());
-    const Tensor xc = x2 - x2.mean(1, true), r = (xc.square().mean(1, true) + eps).rsqrt(), h = xc * r;
-    const auto J = [&](const Tensor& a) { return r * (a - a.mean(1, true) - h * (a * h).mean(1, true)); };
-    const Tensor a = g2 * w, ju = J(u);
-    Tensor dg = w * ju;
-    Tensor dx = -r * ((a * h).mean(1, true) * ju + (u * h).mean(1, true) * J(a)) - r * h * (ju * a).mean(1, true);
-    if (given(seed_w)) {
-        const Tensor p = seed_w->to(at::kFloat);
-        dg = dg + p * h;
-        dx = dx + J(g2 * p);
-    }
-    if (given(seed_b)) dg = dg + seed_b->to(at::kFloat);
-    Tensor dw = need_w ? (g2 * ju).sum(0).to(weight->scalar_type()) : at::empty({0}, x.options());
-    return {dg.to(x.scalar_type()).reshape(x.sizes()), dx.to(x.scalar_type()).reshape(x.sizes()), dw};
+    bool tracked = false, tangent = false;
+    for (const OptTensor& t : {OptTensor(grad), OptTensor(x), weight, seed_x, seed_w, seed_b})
+        tracked |= wants_grad(t), tangent |= has_tangent(t);
+    if ((at::GradMode::is_enabled() && tracked) || tangent)
+        return layer_norm_backward2_formula(grad, x, weight, eps, seed_x, seed_w, seed_b, need_w);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return layer_norm_backward2_op().call(grad, x, weight, stats, eps, seed_x, seed_w, seed_b, need_w);
 }
 
 // ---------------------------------------------------------------------------

@@ -1,0 +1,52 @@
+"""Derivatives of molix::layer_norm other than backward mode's, on the kernels, against torch's norm in float64.
+
+Rows of 24 values within 5 deviations: each result, a few sums of float32 terms, is within 1e-5 of its norm."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+
+from molnex_amd.molix import F
+from molnex_amd.molix.nn import LayerNorm
+
+pytestmark = pytest.mark.gpu
+DEV, D = "cuda", 24
+
+
+def _data(dtype, rows=(6,)):
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device=DEV)  # noqa: E731
+    x, w, b, t, tw, tb = rnd(*rows, D) * 2 + 1, 1 + 0.3 * rnd(D), rnd(D), rnd(*rows, D), rnd(D), rnd(D)
+    return [v.to(dtype).requires_grad_() for v in (x, w, b)], [v.to(dtype) for v in (t, tw, tb)]
+
+
+def norm(x, w, b):
+    return (F.layer_norm if x.dtype == torch.float32 else torch.nn.functional.layer_norm)(x, (D,), w, b)
+
+
+def close(got, ref):
+    assert got.shape == ref.shape
+    assert float((got.detach().double() - ref.detach()).norm()) <= 1e-5 * float(ref.detach().norm())
+
+
+def test_forward_mode_and_forward_over_reverse():
+    def run(dtype):
+        primals, tangents = _data(dtype)
+        with fw.dual_level():
+            args = [fw.make_dual(p, t) for p, t in zip(primals, tangents)]
+            y = norm(*args)
+            grads = torch.autograd.grad(y.pow(3).sum(), args)
+            return [p for v in (y, *grads) for p in fw.unpack_dual(v)]
+
+    for a, r in zip(run(torch.float32), run(torch.float64)):
+        close(a, r)
+
+
+def test_module_without_gradients():
+    mod, ref = LayerNorm(D).to(DEV), torch.nn.LayerNorm(D).to(DEV).double()
+    (x, _, _), (t, _, _) = _data(torch.float32)
+    with torch.no_grad(), fw.dual_level():
+        got = fw.unpack_dual(mod(fw.make_dual(x, t)))
+        want = fw.unpack_dual(ref(fw.make_dual(x.double(), t.double())))
+        close(got.primal, want.primal)
+        close(got.tangent, want.tangent)
