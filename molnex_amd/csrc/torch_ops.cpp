@@ -214,12 +214,15 @@ bool wants_grad(const OptTensor& t) { return given(t) && t->requires_grad(); }
 OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 Tensor or_undefined(const OptTensor& t) { return given(t) ? *t : Tensor(); }
 
-// Whether t carries a tangent (forward-mode differentiation).  The autograd Functions below know backward mode only.
+// Whether t carries a tangent (forward-mode differentiation).  The autograd Functions below know backward mode only,
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+// ... outside torch.func's transforms: whether this call is inside one (the key is in force while one is).
+bool transformed() { return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerBackMode); }
 
 // The three ops as torch operations in float32, rounded once at the end: differentiable in every mode and to any order.
-// Tensors that carry tangents take them, and the third order in backward mode.
+// Tensors that carry tangents, calls that torch.func's transforms differentiate or batch, and the third order in
+// backward mode take them.
 std::tuple<Tensor, Tensor> layer_norm_formula(const Tensor& x, const OptTensor& weight, const OptTensor& bias,
                                               double eps) {
     norm_shape("layer_norm", x, weight, bias);
@@ -242,7 +245,8 @@ Tensor rows_f32(const Tensor& t) { return t.reshape({-1, t.size(-1)}).to(at::kFl
 
 std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_formula(const Tensor& grad, const Tensor& x,
                                                                const OptTensor& weight, const OptTensor& bias,
-                                                               double eps, bool need_x, bool need_w, bool need_b) {
+                                                               const Tensor& /*stats*/, double eps, bool need_x,
+                                                               bool need_w, bool need_b) {
     norm_shape("layer_norm_backward", x, weight, bias);
     check_like("layer_norm_backward", "grad", grad, x);
     const Normed n(rows_f32(x), eps);
@@ -255,9 +259,10 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_formula(const Tensor& gra
 }
 
 std::tuple<Tensor, Tensor, Tensor> layer_norm_backward2_formula(const Tensor& grad, const Tensor& x,
-                                                                const OptTensor& weight, double eps,
-                                                                const OptTensor& seed_x, const OptTensor& seed_w,
-                                                                const OptTensor& seed_b, bool need_w) {
+                                                                const OptTensor& weight, const Tensor& /*stats*/,
+                                                                double eps, const OptTensor& seed_x,
+                                                                const OptTensor& seed_w, const OptTensor& seed_b,
+                                                                bool need_w) {
     const Tensor g = rows_f32(grad), x2 = rows_f32(x);
     const Normed n(x2, eps);
     const Tensor& h = n.h;
@@ -305,6 +310,7 @@ std::tuple<Tensor, Tensor> layer_norm_autograd(const Tensor& x, const OptTensor&
                                                double eps) {
     if (has_tangent(x) || has_tangent(weight) || has_tangent(bias)) return layer_norm_formula(x, weight, bias, eps);
     if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias))) {
+        if (transformed()) return layer_norm_formula(x, weight, bias, eps);
         auto r = LayerNorm::apply(x, weight, bias, eps);
         return {r[0], r[1]};
     }
@@ -354,8 +360,10 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_autograd(const Tensor& gr
                                                                 const Tensor& stats, double eps, bool need_x,
                                                                 bool need_w, bool need_b) {
     if (has_tangent(grad) || has_tangent(x) || has_tangent(weight))
-        return layer_norm_backward_formula(grad, x, weight, bias, eps, need_x, need_w, need_b);
+        return layer_norm_backward_formula(grad, x, weight, bias, stats, eps, need_x, need_w, need_b);
     if (at::GradMode::is_enabled() && (grad.requires_grad() || x.requires_grad() || wants_grad(weight))) {
+        if (transformed())
+            return layer_norm_backward_formula(grad, x, weight, bias, stats, eps, need_x, need_w, need_b);
         auto r = LayerNormBackward::apply(grad, x, weight, bias, stats, eps, need_x, need_w, need_b);
         return {r[0], r[1], r[2]};
     }
@@ -372,7 +380,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward2_autograd(const Tensor& g
     for (const OptTensor& t : {OptTensor(grad), OptTensor(x), weight, seed_x, seed_w, seed_b})
         tracked |= wants_grad(t), tangent |= has_tangent(t);
     if ((at::GradMode::is_enabled() && tracked) || tangent)
-        return layer_norm_backward2_formula(grad, x, weight, eps, seed_x, seed_w, seed_b, need_w);
+        return layer_norm_backward2_formula(grad, x, weight, stats, eps, seed_x, seed_w, seed_b, need_w);
     at::AutoDispatchBelowADInplaceOrView below;
     return layer_norm_backward2_op().call(grad, x, weight, stats, eps, seed_x, seed_w, seed_b, need_w);
 }
@@ -657,6 +665,12 @@ TORCH_LIBRARY_IMPL(molix, CUDA, m) {
     m.impl("adamw_step", adamw_step);
     m.impl("adamw8_step", adamw8_step);
     m.impl("adamw8_moments", adamw8_moments);
+}
+
+TORCH_LIBRARY_IMPL(molix, FuncTorchBatched, m) {  // torch.vmap
+    m.impl("layer_norm", layer_norm_formula);
+    m.impl("layer_norm_backward", layer_norm_backward_formula);
+    m.impl("layer_norm_backward2", layer_norm_backward2_formula);
 }
 
 TORCH_LIBRARY_IMPL(molix, Autograd, m) {

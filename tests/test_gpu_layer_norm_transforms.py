@@ -50,3 +50,17 @@ def test_module_without_gradients():
         want = fw.unpack_dual(ref(fw.make_dual(x.double(), t.double())))
         close(got.primal, want.primal)
         close(got.tangent, want.tangent)
+
+
+def test_func_transforms():
+    def run(dtype):
+        (x, w, b), (t, _, _) = _data(dtype, (2, 3))
+        x, w, b = x.detach(), w.detach(), b.detach()
+        loss = lambda x, w, b: norm(x, w, b).pow(3).sum()  # noqa: E731
+        grad = torch.func.grad(loss, argnums=(0, 1, 2))
+        return [*grad(x, w, b), *torch.vmap(grad, (0, None, None))(x, w, b), torch.vmap(norm, (1, None, None))(x, w, b),
+                *torch.func.jvp(lambda x: norm(x, w, b), (x,), (t,)),
+                torch.func.hessian(lambda v: loss(v, w, b))(x[0, 0])]
+
+    for a, r in zip(run(torch.float32), run(torch.float64)):
+        close(a, r)

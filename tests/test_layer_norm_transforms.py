@@ -150,3 +150,72 @@ def test_sixteen_bits_keep_their_type():
     assert got.primal.dtype == got.tangent.dtype == torch.bfloat16
     for a, r in zip(got, ref):  # rounded once: half a unit of the last place
         assert bool(((a.double() - r).abs() <= 2.0 ** -8 * r.abs() + 1e-4).all())
+
+
+def close_all(got, ref):
+    got, ref = (torch.utils._pytree.tree_leaves(t) for t in (got, ref))
+    assert len(got) == len(ref)
+    for a, r in zip(got, ref):
+        close(a, r)
+
+
+def both(transform, *args):
+    """transform(the norm's function) at float32 and at float64."""
+    close_all(transform(norm)(*args), transform(plain)(*(a.double() for a in args)))
+
+
+def loss(fn):
+    return lambda x, w, b: (fn(x, w, b).pow(3) * torch.linspace(0, 1, D, dtype=x.dtype)).sum()
+
+
+def test_func_grad_and_its_nesting():
+    args, _ = _data()
+    both(lambda fn: torch.func.grad(loss(fn), argnums=(0, 1, 2)), *args)
+    both(lambda fn: torch.func.grad(lambda *a: torch.func.grad(loss(fn))(*a).square().sum(), argnums=(0, 1)), *args)
+    both(lambda fn: torch.func.grad(lambda x: loss(fn)(x, None, None)), args[0])
+
+
+def test_func_jvp_and_vjp():
+    args, tangents = _data()
+    both(lambda fn: lambda *a: torch.func.jvp(fn, a, tuple(t.to(a[0].dtype) for t in tangents)), *args)
+    both(lambda fn: lambda *a: torch.func.vjp(fn, *a)[1](tangents[0].to(a[0].dtype)), *args)
+
+
+def test_func_hessian_and_jacobians():
+    (x, w, b), _ = _data((1,))
+    both(lambda fn: torch.func.hessian(loss(fn), argnums=(0, 1)), x, w, b)
+    both(lambda fn: torch.func.jacrev(fn, argnums=(0, 1, 2)), x, w, b)
+    both(lambda fn: torch.func.jacfwd(fn, argnums=(0, 1, 2)), x, w, b)
+
+
+@pytest.mark.parametrize("in_dims", [(0, None, None), (1, None, None), (0, 0, 0), (None, 0, None)])
+def test_vmap(in_dims):
+    gen = torch.Generator().manual_seed(3)
+    args = [torch.randn(*((5,) if d is not None else ()), *shape, generator=gen) for d, shape in
+            zip(in_dims, ((4, D), (D,), (D,)))]
+    if in_dims[0] == 1:
+        args[0] = args[0].transpose(0, 1).contiguous()
+    both(lambda fn: torch.vmap(fn, in_dims), *args)
+    both(lambda fn: torch.vmap(torch.func.grad(loss(fn), argnums=(0, 1)), in_dims), *args)  # per sample
+
+
+def test_batched_gradients_of_a_recorded_graph():
+    """Vectorised Jacobians run a graph's backward inside vmap, with a second order through it where it is recorded."""
+
+    def run(fn, dtype):
+        (x, w, b), _ = _data((2,))
+        x, w, b = (v.to(dtype).requires_grad_() for v in (x, w, b))
+        seeds = torch.eye(2 * D, dtype=dtype).reshape(2 * D, 2, D)
+        out = torch.autograd.grad(fn(x, w, b), (x, w, b), seeds, is_grads_batched=True, create_graph=True)
+        more = torch.autograd.grad(out[0], (x, w), torch.stack([out[0].detach()] * 3), is_grads_batched=True)
+        return [*out, *more]
+
+    for a, r in zip(run(norm, torch.float32), run(plain, torch.float64)):
+        close(a, r)
+
+
+def test_calls_after_a_transform_take_the_ops():
+    """What a transform did leaves later calls as they were: the node of the registered op."""
+    args, _ = _data()
+    torch.func.grad(loss(norm))(*args)
+    assert "LayerNorm" in norm(args[0].requires_grad_(), *args[1:]).grad_fn.name() and "Native" not in norm(*args).grad_fn.name()
