@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from ...training import STATE_BLOCK, adamw8_step, adamw_step, dense, grad_norm
+from ...training import STATE_BLOCK, adamw8_relayout, adamw8_step, adamw_step, dense, grad_norm, same_order
 
 
 class AdamW(torch.optim.Optimizer):
@@ -102,22 +102,36 @@ class AdamW(torch.optim.Optimizer):
             self.grad_norm = got
         return loss
 
+    @staticmethod
+    def _fitted(p: Tensor, saved: dict) -> dict:
+        """A saved state in the form that ``p``'s steps take: on its device, in its memory order."""
+        like = p if dense(p) else p.detach().contiguous()
+        state = {}
+        if "step" in saved:
+            state["step"] = torch.as_tensor(saved["step"], dtype=torch.float32, device=p.device).reshape(()).clone()
+        moments = {k: saved[k] for k in ("exp_avg", "exp_avg_sq") if k in saved}
+        for key, value in moments.items():
+            if value.shape != p.shape:
+                raise ValueError(f"AdamW: saved {key} of shape {tuple(value.shape)} for a parameter of {tuple(p.shape)}")
+        if any(t.dtype == torch.uint8 for t in moments.values()):
+            codes = [t.to(p.device, copy=True) for t in (*moments.values(), saved.get("bases", p.new_empty(0)))]
+            blocks = -(-p.numel() // STATE_BLOCK)
+            if codes[-1].shape != (blocks, 2) or len(codes) != 3 or not all(dense(t) for t in codes):
+                raise ValueError(f"AdamW: 8-bit moments must be dense, with ({blocks}, 2) bases")
+            if not (same_order(codes[0], like) and same_order(codes[1], like)):
+                codes = adamw8_relayout(*codes, like)
+            return state | {"exp_avg": codes[0].as_strided(like.shape, like.stride()),
+                            "exp_avg_sq": codes[1].as_strided(like.shape, like.stride()), "bases": codes[2]}
+        return state | {k: torch.empty_like(like, dtype=torch.float32).copy_(v) for k, v in moments.items()}
+
     def load_state_dict(self, state_dict) -> None:
         """Also takes ``torch.optim.AdamW``'s state.  Each tensor's moments keep the form they were saved in, 8 or 32
-        bits (the base class would give them the parameters' type), and the step counts go to the device."""
-        super().load_state_dict(state_dict)
+        bits (the base class would give them the parameters' type), and the step counts go to the device.  Moments
+        saved from a parameter of another memory order are brought into this one's."""
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
-            if i not in state_dict["state"]:
-                continue
-            for key, value in state_dict["state"][i].items():
-                if key == "step":
-                    value = torch.as_tensor(value, dtype=torch.float32, device=p.device).reshape(()).clone()
-                elif key in ("exp_avg", "exp_avg_sq", "bases"):
-                    kind = value.dtype if value.dtype in (torch.uint8, torch.int16) else torch.float32
-                    new = torch.empty_like(p if dense(p) else p.detach().contiguous(), dtype=kind)
-                    value = (value.to(p.device, copy=True) if key == "bases"
-                             else new.copy_(value))
-                else:
-                    continue
-                self.state[p][key] = value
+        params = [p for g in self.param_groups for p in g["params"]]
+        fitted = {p: self._fitted(p, state_dict["state"][i]) for i, p in zip(saved, params)
+                  if i in state_dict["state"] and len(saved) == len(params)}
+        super().load_state_dict(state_dict)
+        for p, state in fitted.items():
+            self.state[p].update(state)

@@ -100,6 +100,11 @@ def dense(t: Tensor) -> bool:
     return True
 
 
+def same_order(a: Tensor, b: Tensor) -> bool:
+    """Whether a and b, of one shape, step through memory alike (an axis of one element may have any stride)."""
+    return all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride())) or a.numel() == 0
+
+
 def grad_norm(grads) -> Tensor:
     """The 2-norm of all of ``grads`` together (float32, 0-dim, on their device; no synchronisation): squares are
     summed in float64 in a fixed order."""
@@ -170,3 +175,43 @@ def adamw8_moments(exp_avgs, exp_avg_sqs, bases, out=None) -> tuple[list[Tensor]
         call = torch.ops.molix.adamw8_moments if torch.compiler.is_compiling() else _host.moments
         call(exp_avgs, exp_avg_sqs, bases, *out)
     return out
+
+
+def adamw8_relayout(exp_avg: Tensor, exp_avg_sq: Tensor, bases: Tensor, like: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    """8-bit moments in the memory order of ``like``, a dense tensor of their shape: blocks are 256 elements in memory,
+    so their bases are formed again.  Values within a new block's range keep their bits; below it a first moment goes to
+    the nearer of zero and the smallest code, a second one to the smallest code."""
+    n, blocks = like.numel(), bases.shape[0]
+
+    def memory(t):
+        return t.as_strided((n,), (1,))
+
+    def reordered(values, source):  # values in source's memory order, in like's
+        t = torch.empty_like(source, dtype=values.dtype)
+        memory(t).copy_(values)
+        return memory(torch.empty_like(like, dtype=values.dtype).copy_(t))
+
+    def keys(sizes, column):  # a value's bits >> 20
+        sizes = sizes.int()
+        return torch.where(sizes > 0, sizes + bases[:, column].int().repeat_interleave(STATE_BLOCK)[:n], 0)
+
+    def coded(key, nan, top):  # sizes of the codes, and the bases
+        padded = torch.nn.functional.pad(torch.where(nan, 0, key), (0, blocks * STATE_BLOCK - n)).view(blocks, STATE_BLOCK)
+        base = (padded.amax(1) + 1 - top).clamp_(min=0)
+        return key - base.repeat_interleave(STATE_BLOCK)[:n], base
+
+    codes = memory(exp_avg)
+    nan = reordered(codes == 128, exp_avg)
+    sign = reordered(codes & 128, exp_avg)
+    key = reordered(keys(codes & 127, 0), exp_avg)
+    size, base_m = coded(key, nan, 127)
+    half = ((key - size + 1) << 20).view(torch.float32) / 2  # of the smallest code
+    size = torch.where(size > 0, size, ((key << 20).view(torch.float32) > half).int())
+    m = torch.where(nan, 128, torch.where(size > 0, size | sign, 0))
+    key = reordered(keys(memory(exp_avg_sq), 1), exp_avg_sq)
+    size, base_v = coded(key, nan, 255)
+    v = torch.where(nan, 255, torch.where(key > 0, size.clamp(min=1), 0))
+    out = [torch.empty_like(like, dtype=torch.uint8) for _ in range(2)]
+    for t, values in zip(out, (m, v)):
+        memory(t).copy_(values)
+    return *out, torch.stack([base_m, base_v], 1).short()
