@@ -19,7 +19,6 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
-#include <algorithm>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -403,6 +402,34 @@ void check_values(const char* name, const char* what, const Tensor& t, at::Devic
                      " float32, bfloat16 or float16, got ", t.scalar_type());
 }
 
+// Addresses that one call writes: its workgroups run at once, so none may be given twice.  Up to `count` of them; null
+// (tensors without elements) any number of times.
+class Written {
+  public:
+    explicit Written(size_t count) {
+        size_t size = 16;
+        for (; size < 2 * count; size *= 2) --shift_;
+        places_.resize(size);
+    }
+    template <typename Pointers>
+    bool add(const Pointers& pointers) {  // whether all are new
+        for (const void* p : pointers)
+            if (p && !add_one(p)) return false;
+        return true;
+    }
+
+  private:
+    bool add_one(const void* p) {
+        for (size_t at = reinterpret_cast<uintptr_t>(p) * 0x9E3779B97F4A7C15u >> shift_;; ++at) {
+            const void*& place = places_[at & (places_.size() - 1)];
+            if (place == p) return false;
+            if (!place) return place = p, true;
+        }
+    }
+    int shift_ = 60;
+    std::vector<const void*> places_;
+};
+
 Tensor grad_norm(at::TensorList grads) {
     if (grads.empty()) return at::zeros({});
     const at::Device device = gpu_of("grad_norm", grads);
@@ -471,7 +498,7 @@ Tensor step(const char* name, int bits, at::TensorList params, at::TensorList gr
     std::vector<int64_t> numel(count);
     std::vector<int32_t> dtype(count);
     std::vector<Tensor> kept;                          // gradients laid out like their parameters
-    std::vector<std::pair<const Tensor*, Tensor>> gaps;  // parameters with gaps and their copies
+    std::vector<std::pair<size_t, Tensor>> gaps;  // parameters with gaps and their copies
     for (size_t i = 0; i < count; ++i) {
         const Tensor &p = params[i], &g = grads[i], &m = exp_avgs[i], &v = exp_avg_sqs[i], &s = steps[i];
         check_values(name, "parameters", p, device);
@@ -497,7 +524,7 @@ Tensor step(const char* name, int bits, at::TensorList params, at::TensorList gr
         const Tensor *pp = &p, *gg = &g;
         if (!(p.is_contiguous() && g.is_contiguous() && m.is_contiguous() && v.is_contiguous())) {
             if (!p.is_non_overlapping_and_dense()) {
-                gaps.emplace_back(&p, p.detach().contiguous());
+                gaps.emplace_back(i, p.detach().contiguous());
                 pp = &gaps.back().second;
             }
             TORCH_CHECK_VALUE(m.strides() == pp->strides() && v.strides() == pp->strides(), "molix::", name,
@@ -508,7 +535,7 @@ Tensor step(const char* name, int bits, at::TensorList params, at::TensorList gr
                 gg = &kept.back();
             }
         }
-        p_ptr[i] = out(*pp);
+        p_ptr[i] = out(p);
         g_ptr[i] = gg->numel() ? gg->const_data_ptr() : nullptr;
         m_ptr[i] = out(m);
         v_ptr[i] = out(v);
@@ -516,14 +543,12 @@ Tensor step(const char* name, int bits, at::TensorList params, at::TensorList gr
         numel[i] = p.numel();
         dtype[i] = dtype_of(p.scalar_type());
     }
-    const auto twice = [](auto ptrs) {
-        std::sort(ptrs.begin(), ptrs.end());
-        typename decltype(ptrs)::value_type none{};  // of tensors without elements
-        const auto first = std::upper_bound(ptrs.begin(), ptrs.end(), none);
-        return std::adjacent_find(first, ptrs.end()) != ptrs.end();
-    };
-    TORCH_CHECK_VALUE(!twice(p_ptr), "molix::", name, ": a parameter is given twice");
-    TORCH_CHECK_VALUE(!twice(s_ptr), "molix::", name, ": a step count is given twice");
+    Written written((bits == 8 ? 5 : 4) * count);
+    TORCH_CHECK_VALUE(written.add(p_ptr), "molix::", name, ": a parameter is given twice");
+    TORCH_CHECK_VALUE(written.add(m_ptr) && written.add(v_ptr) && written.add(b_ptr), "molix::", name,
+                      ": a moment or its bases are given twice");
+    TORCH_CHECK_VALUE(written.add(s_ptr), "molix::", name, ": a step count is given twice");
+    for (const auto& [i, copy] : gaps) p_ptr[i] = out(copy);
 
     mnx_adamw_args a{};
     a.count = int64_t(count);
@@ -566,7 +591,7 @@ Tensor step(const char* name, int bits, at::TensorList params, at::TensorList gr
     Tensor ws = at::empty({int64_t(a.workspace_bytes)}, f32.dtype(at::kByte));
     a.workspace = out(ws);
     check(mnx_adamw_step(&a, stream_of(ws)), name);
-    for (auto& [p, copy] : gaps) p->detach().copy_(copy);
+    for (const auto& [i, copy] : gaps) params[i].detach().copy_(copy);
     for (const at::TensorList& l : {params, exp_avgs, exp_avg_sqs, steps, bases})
         for (const Tensor& t : l) t.unsafeGetTensorImpl()->bump_version();
     return norm.defined() ? norm : at::empty({0}, f32);
@@ -624,6 +649,8 @@ void adamw8_moments(at::TensorList exp_avgs, at::TensorList exp_avg_sqs, at::Ten
         ov_ptr[i] = static_cast<float*>(out(out_avg_sqs[i]));
         numel[i] = m.numel();
     }
+    Written written(2 * count);
+    TORCH_CHECK_VALUE(written.add(om_ptr) && written.add(ov_ptr), "molix::", name, ": an out is given twice");
     check(mnx_adamw8_moments(m_ptr.data(), v_ptr.data(), b_ptr.data(), numel.data(), int64_t(count), om_ptr.data(),
                              ov_ptr.data(), stream_of(exp_avgs[0])),
           name);
