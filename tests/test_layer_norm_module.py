@@ -1,0 +1,53 @@
+"""molix.nn.LayerNorm as a module that other tools take apart: TorchScript, torch.fx, tracing (no GPU needed)."""
+
+import copy
+import io
+import pickle
+
+import pytest
+import torch
+
+from molnex_amd.molix.nn import LayerNorm
+
+pytestmark = pytest.mark.filterwarnings("ignore::DeprecationWarning")
+MODULES = [lambda c: c(8), lambda c: c((3, 4), eps=1e-3), lambda c: c(8, elementwise_affine=False), lambda c: c(8, bias=False)]
+
+
+def pair(make):
+    mod, ref = make(LayerNorm), make(torch.nn.LayerNorm)
+    with torch.no_grad():
+        for p in ref.parameters():
+            p.normal_()
+    mod.load_state_dict(ref.state_dict())
+    return mod, ref, torch.randn(5, *ref.normalized_shape)
+
+
+@pytest.mark.parametrize("make", MODULES)
+def test_script(make):
+    mod, ref, x = pair(make)
+    scripted = torch.jit.script(mod)
+    assert torch.equal(scripted(x), ref(x))
+    file = io.BytesIO()
+    torch.jit.save(torch.jit.script(torch.nn.Sequential(mod)), file)
+    file.seek(0)
+    assert torch.equal(torch.jit.load(file)(x), ref(x))
+
+
+@pytest.mark.parametrize("make", MODULES)
+def test_symbolic_trace(make):
+    mod, ref, x = pair(make)
+    traced = torch.fx.symbolic_trace(mod)
+    assert torch.equal(traced(x), ref(x))
+    inside = torch.fx.symbolic_trace(torch.nn.Sequential(mod, torch.nn.SiLU()))
+    for again in (inside, copy.deepcopy(inside), pickle.loads(pickle.dumps(inside))):
+        assert torch.equal(again(x), torch.nn.functional.silu(ref(x)))
+    x.requires_grad_()
+    a, r = (torch.autograd.grad(f(x).square().sum(), x)[0] for f in (traced, ref))
+    assert torch.equal(a, r)
+
+
+@pytest.mark.parametrize("make", MODULES)
+def test_trace_and_export(make):
+    mod, ref, x = pair(make)
+    assert torch.equal(torch.jit.trace(mod, x)(x), ref(x))
+    assert torch.equal(torch.export.export(mod, (x,)).module()(x), ref(x))
