@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/autocast_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -711,12 +712,39 @@ TORCH_LIBRARY_IMPL(molix, Autograd, m) {
 }
 
 // ---------------------------------------------------------------------------
-// The Python module: the ops called through the dispatcher without boxing
+// The Python module: the ops called through the dispatcher without boxing.  A function that finds a tensor (or a mode)
+// with __torch_function__ among its arguments calls nothing and returns NotImplemented: the caller hands the call over.
 // ---------------------------------------------------------------------------
 
 namespace {
 
-std::vector<Tensor> tensors(PyObject* o, const char* what) {
+// Tensor and Parameter themselves, which have no __torch_function__.
+bool plain_tensor(PyObject* o) {
+    const auto* type = reinterpret_cast<const PyObject*>(Py_TYPE(o));
+    return type == THPVariableClass || type == ParameterClass;
+}
+
+// Whether o's class has one in force (or a mode is on, too).
+bool has_torch_function(PyObject* o) {
+    if (plain_tensor(o)) return false;
+    static PyObject* const ask = [] {
+        PyObject* module = PyImport_ImportModule("torch._C");
+        PyObject* f = module ? PyObject_GetAttrString(module, "_has_torch_function_unary") : nullptr;
+        Py_XDECREF(module);
+        return f;
+    }();
+    if (!ask) throw python_error();
+    PyObject* r = PyObject_CallOneArg(ask, o);
+    if (!r) throw python_error();
+    const bool yes = r == Py_True;
+    Py_DECREF(r);
+    return yes;
+}
+
+bool mode_on() { return at::impl::torch_function_mode_enabled(); }
+
+// The tensors of a list; `overridden` where one of them has __torch_function__.
+std::vector<Tensor> tensors(PyObject* o, const char* what, bool& overridden) {
     PyObject* seq = PySequence_Fast(o, "");
     if (!seq) {
         PyErr_Clear();
@@ -727,16 +755,23 @@ std::vector<Tensor> tensors(PyObject* o, const char* what) {
     std::vector<Tensor> got;
     got.reserve(n);
     Py_ssize_t i = 0;
-    for (; i < n && THPVariable_Check(items[i]); ++i) got.push_back(THPVariable_Unpack(items[i]));
+    for (; i < n; ++i) {
+        if (!plain_tensor(items[i])) {
+            if (!THPVariable_Check(items[i])) break;
+            overridden |= has_torch_function(items[i]);
+        }
+        got.push_back(THPVariable_Unpack(items[i]));
+    }
     const char* other = i < n ? Py_TYPE(items[i])->tp_name : nullptr;
     Py_DECREF(seq);
     TORCH_CHECK_TYPE(!other, what, ": tensors, got ", other ? other : "");
     return got;
 }
 
-OptTensor tensor_or_none(PyObject* o, const char* what) {
+OptTensor tensor_or_none(PyObject* o, const char* what, bool& overridden) {
     if (o == Py_None) return std::nullopt;
     TORCH_CHECK_TYPE(THPVariable_Check(o), what, ": a tensor or None, got ", Py_TYPE(o)->tp_name);
+    overridden |= has_torch_function(o);
     return THPVariable_Unpack(o);
 }
 
@@ -763,16 +798,18 @@ PyObject* py_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == 18, "step: 18 arguments, got ", n);
     const bool eight = number(a[0]) == 8;
-    const auto params = tensors(a[1], "parameters"), grads = tensors(a[2], "gradients");
-    const auto avgs = tensors(a[3], "first moments"), sqs = tensors(a[4], "second moments");
-    const auto bases = eight ? tensors(a[5], "bases") : std::vector<Tensor>();
-    const auto steps = tensors(a[6], "steps");
+    bool overridden = mode_on();
+    const auto params = tensors(a[1], "parameters", overridden), grads = tensors(a[2], "gradients", overridden);
+    const auto avgs = tensors(a[3], "first moments", overridden), sqs = tensors(a[4], "second moments", overridden);
+    const auto bases = eight ? tensors(a[5], "bases", overridden) : std::vector<Tensor>();
+    const auto steps = tensors(a[6], "steps", overridden);
     const double lr = number(a[7]), b1 = number(a[8]), b2 = number(a[9]), eps = number(a[10]), wd = number(a[11]);
     const bool maximize = truth(a[12]), skip = truth(a[15]);
     const std::optional<double> max_norm = a[13] == Py_None ? std::nullopt : std::optional<double>(number(a[13]));
-    const OptTensor norm_in = tensor_or_none(a[14], "grad_norm"), rate = tensor_or_none(a[16], "lr");
+    const OptTensor norm_in = tensor_or_none(a[14], "grad_norm", overridden), rate = tensor_or_none(a[16], "lr", overridden);
     const int64_t seed = eight ? PyLong_AsLongLong(a[17]) : 0;
     if (PyErr_Occurred()) throw python_error();
+    if (overridden) Py_RETURN_NOTIMPLEMENTED;
     Tensor norm;
     {
         Released r;
@@ -793,6 +830,9 @@ PyObject* py_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == 5, "layer_norm: 5 arguments, got ", n);
+    if (mode_on()) Py_RETURN_NOTIMPLEMENTED;
+    for (int k : {0, 2, 3})
+        if (a[k] != Py_None && has_torch_function(a[k])) Py_RETURN_NOTIMPLEMENTED;
     if (!THPVariable_Check(a[0])) Py_RETURN_NONE;
     for (int k : {2, 3})
         if (a[k] != Py_None && !THPVariable_Check(a[k])) Py_RETURN_NONE;
@@ -805,7 +845,8 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (w == -1 && PyErr_Occurred()) throw python_error();
     const int dt = dtype_of(x.scalar_type());
     if (dt < 0 || w != x.size(-1) || w < 1 || w > MNX_LAYER_NORM_MAX_WIDTH) Py_RETURN_NONE;
-    const OptTensor weight = tensor_or_none(a[2], "weight"), bias = tensor_or_none(a[3], "bias");
+    const auto argument = [](PyObject* o) { return o == Py_None ? OptTensor() : OptTensor(THPVariable_Unpack(o)); };
+    const OptTensor weight = argument(a[2]), bias = argument(a[3]);
     int wd = -1;
     for (const auto* t : {&weight, &bias}) {
         if (!given(*t)) continue;
@@ -827,7 +868,9 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyObject* py_grad_norm(PyObject*, PyObject* list) {
     HANDLE_TH_ERRORS
-    const auto grads = tensors(list, "gradients");
+    bool overridden = mode_on();
+    const auto grads = tensors(list, "gradients", overridden);
+    if (overridden) Py_RETURN_NOTIMPLEMENTED;
     Tensor norm;
     {
         Released r;
@@ -841,8 +884,10 @@ PyObject* py_grad_norm(PyObject*, PyObject* list) {
 PyObject* py_moments(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == 5, "moments: 5 lists, got ", n);
-    const auto avgs = tensors(a[0], "first moments"), sqs = tensors(a[1], "second moments");
-    const auto bases = tensors(a[2], "bases"), om = tensors(a[3], "out"), ov = tensors(a[4], "out");
+    bool overridden = mode_on();
+    const auto avgs = tensors(a[0], "first moments", overridden), sqs = tensors(a[1], "second moments", overridden);
+    const auto bases = tensors(a[2], "bases", overridden), om = tensors(a[3], "out", overridden), ov = tensors(a[4], "out", overridden);
+    if (overridden) Py_RETURN_NOTIMPLEMENTED;
     {
         Released r;
         static auto o = op<decltype(adamw8_moments)>("molix::adamw8_moments");

@@ -6,6 +6,7 @@ import math
 
 import torch
 from torch import Tensor
+from torch.overrides import handle_torch_function
 
 from ...training import DTYPES, LAYER_NORM_MAX_WIDTH, _host
 
@@ -20,6 +21,9 @@ def layer_norm(input: Tensor, normalized_shape, weight: Tensor | None = None, bi
     models) go to torch.  Under autocast it computes and returns float32, as torch's does.  GPU tensors only."""
     if not torch.compiler.is_compiling():
         y = _host.layer_norm(input, normalized_shape, weight, bias, eps)  # None for what needs more than the kernels
+        if y is NotImplemented:
+            return handle_torch_function(layer_norm, (input, weight, bias), input, normalized_shape, weight=weight,
+                                         bias=bias, eps=eps)
         if y is not None:
             return y
     if input.device.type != "cuda":

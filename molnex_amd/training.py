@@ -14,6 +14,7 @@ import sys
 
 import torch
 from torch import Tensor
+from torch.overrides import handle_torch_function
 
 from . import _lib
 
@@ -111,7 +112,10 @@ def grad_norm(grads) -> Tensor:
     grads = list(grads)
     if not grads:
         return torch.zeros(())
-    return torch.ops.molix.grad_norm(grads) if torch.compiler.is_compiling() else _host.grad_norm(grads)
+    if torch.compiler.is_compiling():
+        return torch.ops.molix.grad_norm(grads)
+    norm = _host.grad_norm(grads)
+    return handle_torch_function(grad_norm, grads, grads) if norm is NotImplemented else norm
 
 
 def _rate(lr) -> tuple[float, Tensor | None]:
@@ -140,6 +144,11 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
         return grad_norm if norm.dim() else norm
     norm = _host.step(32, params, grads, exp_avgs, exp_avg_sqs, None, steps, rate, betas[0], betas[1], eps,
                       weight_decay, maximize, max_norm, grad_norm, skip_nonfinite, lr_tensor, 0)
+    if norm is NotImplemented:
+        return handle_torch_function(adamw_step, (*params, *grads, *exp_avgs, *exp_avg_sqs, *steps, grad_norm, lr_tensor),
+                                     params, grads, exp_avgs, exp_avg_sqs, steps, lr=lr, betas=betas, eps=eps,
+                                     weight_decay=weight_decay, maximize=maximize, max_norm=max_norm,
+                                     grad_norm=grad_norm, skip_nonfinite=skip_nonfinite)
     return grad_norm if norm is None else norm
 
 
@@ -163,6 +172,12 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, lr, betas
         return grad_norm if norm.dim() else norm
     norm = _host.step(8, params, grads, exp_avgs, exp_avg_sqs, bases, steps, rate, betas[0], betas[1], eps,
                       weight_decay, maximize, max_norm, grad_norm, skip_nonfinite, lr_tensor, seed & 0xFFFFFFFF)
+    if norm is NotImplemented:
+        return handle_torch_function(adamw8_step, (*params, *grads, *exp_avgs, *exp_avg_sqs, *bases, *steps, grad_norm,
+                                                   lr_tensor),
+                                     params, grads, exp_avgs, exp_avg_sqs, bases, steps, lr=lr, betas=betas, eps=eps,
+                                     weight_decay=weight_decay, maximize=maximize, max_norm=max_norm,
+                                     grad_norm=grad_norm, skip_nonfinite=skip_nonfinite, seed=seed)
     return grad_norm if norm is None else norm
 
 
@@ -172,8 +187,11 @@ def adamw8_moments(exp_avgs, exp_avg_sqs, bases, out=None) -> tuple[list[Tensor]
     if out is None:
         out = tuple([torch.empty_like(t, dtype=torch.float32) for t in ts] for ts in (exp_avgs, exp_avg_sqs))
     if exp_avgs or exp_avg_sqs:
-        call = torch.ops.molix.adamw8_moments if torch.compiler.is_compiling() else _host.moments
-        call(exp_avgs, exp_avg_sqs, bases, *out)
+        if torch.compiler.is_compiling():
+            torch.ops.molix.adamw8_moments(exp_avgs, exp_avg_sqs, bases, *out)
+        elif _host.moments(exp_avgs, exp_avg_sqs, bases, *out) is NotImplemented:
+            return handle_torch_function(adamw8_moments, (*exp_avgs, *exp_avg_sqs, *bases, *out[0], *out[1]), exp_avgs,
+                                         exp_avg_sqs, bases, out=out)
     return out
 
 

@@ -64,3 +64,27 @@ def test_func_transforms():
 
     for a, r in zip(run(torch.float32), run(torch.float64)):
         close(a, r)
+
+
+class Wrapped(torch.Tensor):
+    """A subclass with the default handlers."""
+
+
+def test_tensor_subclasses_and_tracers():
+    (x, w, b), _ = _data(torch.float32)
+    ref = norm(x, w, b)
+    y = F.layer_norm(x.detach().as_subclass(Wrapped), D, w, b)
+    assert type(y) is Wrapped and torch.equal(y.as_subclass(torch.Tensor), ref)
+    with torch.device("cuda"):  # a mode
+        assert torch.equal(norm(x, w, b), ref)
+    mod = LayerNorm(D).to(DEV)
+    mod.load_state_dict({"weight": w, "bias": b})
+    assert torch.equal(torch.fx.symbolic_trace(mod)(x), ref) and torch.equal(torch.jit.trace(mod, (x,))(x), ref)
+    close(torch.jit.script(mod)(x), ref)
+
+
+def test_optimizer_functions_on_subclasses():
+    s = [[torch.ones(300, device=DEV).as_subclass(Wrapped)] for _ in range(4)] + [[torch.zeros((), device=DEV)]]
+    norm = F.adamw_step(*s, lr=1e-2, max_norm=1.0)
+    assert abs(float(norm) - 300 ** 0.5) < 1e-4 and float(s[0][0].max()) < 1 and float(s[4][0]) == 1
+    assert abs(float(F.grad_norm(s[1])) - 300 ** 0.5) < 1e-4
