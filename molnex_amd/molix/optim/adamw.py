@@ -9,7 +9,9 @@ from ...training import STATE_BLOCK, adamw8_relayout, adamw8_step, adamw_step, d
 
 
 class AdamW(torch.optim.Optimizer):
-    """AdamW (decoupled weight decay) for parameters on the GPU, with the arguments of ``torch.optim.AdamW`` and
+    """AdamW (decoupled weight decay) for parameters on the GPU, with the arguments of ``torch.optim.AdamW`` and those
+    below.  ``foreach``, ``fused`` and ``capturable`` choose between torch's implementations and change nothing here
+    (a step is always a few launches over all tensors and can be captured); ``amsgrad`` and ``differentiable`` are refused.
 
     ``state_bits``     32, or 8: the moments of tensors of at least ``min_8bit_size`` elements take 2 bytes an element
                        instead of 8 (``molix.F.adamw8_step``); a group's option
@@ -23,8 +25,11 @@ class AdamW(torch.optim.Optimizer):
     states exist (after a first step)."""
 
     def __init__(self, params, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
-                 weight_decay: float = 1e-2, *, maximize: bool = False, state_bits: int = 32,
-                 min_8bit_size: int = 4096, max_norm: float | None = None, skip_nonfinite: bool = False, seed: int = 0):
+                 weight_decay: float = 1e-2, amsgrad: bool = False, *, maximize: bool = False,
+                 foreach: bool | None = None, capturable: bool = False, differentiable: bool = False,
+                 fused: bool | None = None, state_bits: int = 32, min_8bit_size: int = 4096,
+                 max_norm: float | None = None, skip_nonfinite: bool = False, seed: int = 0):
+        self._refuse({"amsgrad": amsgrad, "differentiable": differentiable})
         if not isinstance(lr, Tensor) and not lr >= 0:
             raise ValueError(f"AdamW: lr {lr}")
         if not (len(betas) == 2 and all(0 <= b < 1 for b in betas)):
@@ -38,7 +43,14 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, maximize=maximize,
                                       state_bits=state_bits, min_8bit_size=min_8bit_size))
 
+    @staticmethod
+    def _refuse(group: dict) -> None:
+        for name in ("amsgrad", "differentiable"):
+            if group.get(name):
+                raise ValueError(f"AdamW: {name} is not supported")
+
     def add_param_group(self, param_group) -> None:
+        self._refuse(param_group)
         bits = param_group.get("state_bits", self.defaults["state_bits"])
         if bits not in (8, 32):
             raise ValueError(f"AdamW: state_bits 8 or 32, got {bits}")
@@ -51,8 +63,7 @@ class AdamW(torch.optim.Optimizer):
     def __setstate__(self, state) -> None:
         super().__setstate__(state)
         for group in self.param_groups:  # a group that torch.optim.AdamW saved lacks these
-            if group.get("amsgrad"):
-                raise ValueError("AdamW: amsgrad is not supported")
+            self._refuse(group)
             for key, value in (("maximize", False), ("state_bits", 32), ("min_8bit_size", 4096)):
                 group.setdefault(key, value)
 

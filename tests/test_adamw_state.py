@@ -130,3 +130,22 @@ def test_moments_of_another_shape_are_refused(kind):
     del bad["bases"]
     with pytest.raises(ValueError, match="bases"):
         loaded(bad, row(80, 64), target)
+
+
+def test_torch_constructor_arguments():
+    """What torch.optim.AdamW's constructor takes, in its order and by its names."""
+    p = [torch.nn.Parameter(torch.ones(3))]
+    a = AdamW(p, 1e-2, (0.8, 0.9), 1e-7, 0.1, False)
+    assert [a.defaults[k] for k in ("lr", "betas", "eps", "weight_decay")] == [1e-2, (0.8, 0.9), 1e-7, 0.1]
+    for value in (None, True, False):
+        AdamW(p, foreach=value, fused=value, capturable=bool(value), amsgrad=False, differentiable=False)
+    AdamW([{"params": p, "amsgrad": False, "foreach": None, "fused": None, "capturable": True, "differentiable": False}])
+    a.load_state_dict(torch.optim.AdamW(p, foreach=True).state_dict())
+    torch.optim.AdamW(p).load_state_dict(a.state_dict())
+    for name in ("amsgrad", "differentiable"):
+        with pytest.raises(ValueError, match=name):
+            AdamW(p, **{name: True})
+        with pytest.raises(ValueError, match=name):
+            AdamW([{"params": p, name: True}])
+        with pytest.raises(ValueError, match=name):
+            a.load_state_dict(torch.optim.AdamW(p, **{name: True}).state_dict())
