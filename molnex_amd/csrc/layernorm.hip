@@ -550,9 +550,18 @@ static int64_t ln_parts(const void* kernel, int threads, int64_t rows, int group
 }
 
 constexpr int64_t kLnWideGrid = 1 << 16;
-static size_t ln_partial_floats(int64_t rows, int64_t width) {
-    return size_t(std::min<int64_t>(std::max<int64_t>(rows, 1), kLnParts)) * 2 * size_t(width);
-}
+
+// The backward passes' workspace: the rows of partial sums that the form of this width leaves, and for the wide form's
+// column sums two numbers a row.
+struct LnWorkspace : Workspace {
+    float *partial, *usums;
+    LnWorkspace(void* p, size_t bytes, int64_t rows, int64_t width) : Workspace{static_cast<char*>(p), bytes} {
+        const bool held = ln_variant(width, [](auto, auto) {});
+        const int64_t parts = held ? std::min<int64_t>(std::max<int64_t>(rows, 1), kLnParts) : ln_strips(rows);
+        partial = take<float>(size_t(parts) * 2 * size_t(width));
+        usums = take<float>(held ? 0 : size_t(rows) * 2);
+    }
+};
 
 static int ln_check(const char* what, int64_t rows, int64_t width, int dtype, int wdtype) {
     MNX_REQUIRE(elem_valid(dtype) && elem_valid(wdtype), "%s: unknown element type", what);
@@ -600,11 +609,7 @@ int mnx_layer_norm_fwd(const void* x, int64_t ldx, int64_t rows, int64_t width, 
 }
 
 size_t mnx_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width) {
-    Workspace ws{nullptr, 0};
-    rows = std::max<int64_t>(rows, 0);
-    ws.take<float>(ln_partial_floats(rows, std::max<int64_t>(width, 1)));
-    ws.take<float>(size_t(rows) * 2);
-    return ws.used;
+    return LnWorkspace(nullptr, 0, std::max<int64_t>(rows, 0), std::max<int64_t>(width, 1)).used;
 }
 
 // `parts` rows of sums in `partial`, joined into the results.
@@ -625,8 +630,9 @@ int mnx_layer_norm_bwd(const void* grad, int64_t ldg, const void* x, int64_t ldx
                 "layer norm backward: null pointer or a row stride below the width");
     const bool sums = grad_weight || grad_bias;
     if (!sums && (!rows || !grad_x)) return MNX_OK;
-    float* partial = static_cast<float*>(workspace);
-    if (sums && (!workspace || workspace_bytes < mnx_layer_norm_bwd_workspace_bytes(rows, width)))
+    const LnWorkspace ws(workspace, workspace_bytes, rows, width);
+    float* partial = ws.partial;
+    if (sums && (!workspace || !ws.fits()))
         return set_error(MNX_ERR_WORKSPACE, "layer norm backward: workspace too small");
     int64_t parts = 0;
     bool held = true;
@@ -671,9 +677,8 @@ int mnx_layer_norm_bwd2(const void* grad, int64_t ldg, const void* x, int64_t ld
                               ldu >= width),
                 "layer norm second order: null pointer or a row stride below the width");
     if (!rows && !dweight) return MNX_OK;
-    Workspace ws{static_cast<char*>(workspace), workspace_bytes};
-    float* partial = ws.take<float>(ln_partial_floats(rows, width));
-    float* usums = ws.take<float>(size_t(rows) * 2);
+    const LnWorkspace ws(workspace, workspace_bytes, rows, width);
+    float *partial = ws.partial, *usums = ws.usums;
     if (!workspace || !ws.fits()) return set_error(MNX_ERR_WORKSPACE, "layer norm second order: workspace too small");
     int64_t parts = 0;
     bool held = true;
