@@ -621,7 +621,10 @@ int mnx_adamw_step(const mnx_adamw_args* args, mnx_stream_t stream) {
                                                a.beta2, a.weight_decay, a.seed, call, scalars);
         MNX_CHECK_LAUNCH();
     }
-    const Hyper h{float(a.beta1), float(1 - a.beta1), float(a.beta2), float(1 - a.beta2), float(a.eps)};
+    // An eps below the smallest normal number counts as that one: its only use is beside a second moment of zero, and the
+    // reciprocal's instruction takes no subnormals.
+    const float eps = a.eps > 0 ? std::max(float(a.eps), 0x1p-126f) : 0.0f;
+    const Hyper h{float(a.beta1), float(1 - a.beta1), float(a.beta2), float(1 - a.beta2), eps};
     int64_t bytes = 0;
     for (int64_t i = 0; i < a.count; ++i) bytes += a.numel[i] * (3 * elem_bytes(a.dtype[i]) + (eight ? 4 : 16));
     const auto kernel = bytes > kCacheBytes ? (eight ? k_adamw8<true> : k_adamw<true>)
