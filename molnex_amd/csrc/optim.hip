@@ -287,11 +287,16 @@ struct Moments {
 __device__ __forceinline__ Moments moments(const Hyper& h, float m, float v, float g) {
     return {m * h.b1 + g * h.w1, v * h.b2 + (g * g) * h.w2};
 }
-// The square root and the reciprocal by the hardware's instructions, a unit of the last place each: the update is lr
-// times a number of the order of one, added to p.  (k_adamw8 took 223 us for 64 M elements with them and 230 with the
-// exact forms, before other steps brought it to 166 us, 6.2 TB/s.)
-// The root's instruction takes no subnormals: a v below 2^-96 is scaled (its root is far below any eps but 0).
+// The formula's float32 operations, a unit of half a place each.  They are free beside 32-bit moments, whose bytes
+// bound the kernel (k_adamw: 3.2 M elements 16.4 us with them and 16.3 with those below, 128 M 186 a launch with both).
 __device__ __forceinline__ float updated(const Hyper& h, const TensorScalars& s, float p, const Moments& a) {
+    return p * s.decay - s.size * a.m / (sqrtf(a.v) * s.inv_root + h.eps);
+}
+// Beside 8-bit moments, which know m to one part in 16 at best, the square root and the reciprocal are the hardware's
+// instructions, a unit of the last place each: instructions bound that kernel (3.2 M elements 16.5 us with them and 18.0
+// with the exact forms, 64 M 94 against 103 a launch).
+// The root's instruction takes no subnormals: a v below 2^-96 is scaled (its root is far below any eps but 0).
+__device__ __forceinline__ float updated_fast(const Hyper& h, const TensorScalars& s, float p, const Moments& a) {
     const bool tiny = a.v < 0x1p-96f;
     const float root = __builtin_amdgcn_sqrtf(tiny ? a.v * 0x1p96f : a.v) * (tiny ? 0x1p-48f : 1.0f);
     return p * s.decay - s.size * a.m * __builtin_amdgcn_rcpf(root * s.inv_root + h.eps);
@@ -420,7 +425,7 @@ __device__ __forceinline__ void update8(const AdamwTable& t, const Chunk& c, con
         for (int k = 0; k < 4; ++k) {  // past the end the codes and the gradient are 0, and so are the moments
             a[k] = moments(h, decode_m(cm[u] >> 8 * k & 255, bm), decode_v(cv[u] >> 8 * k & 255, bv),
                            g[u][k] * scale);
-            p[u][k] = updated(h, s, p[u][k], a[k]);
+            p[u][k] = updated_fast(h, s, p[u][k], a[k]);
             const uint32_t um = __float_as_uint(a[k].m) & 0x7FFFFFFFu, uv = __float_as_uint(a[k].v);
             finite[k] = finite_bits(um) && finite_bits(uv);
             top_m = max(top_m, finite[k] ? um : 0);
