@@ -348,6 +348,7 @@ __global__ __launch_bounds__(256) void k_adamw(const AdamwTable t, const Hyper h
 }
 
 constexpr int kTopM = 127, kTopV = 255, kNanM = 0x80;
+constexpr int kFinite = 0x7F7;  // bits >> 20 of the largest finite number
 
 __device__ __forceinline__ float decode_m(uint32_t code, int base) {
     if (code == kNanM) return __uint_as_float(0x7FC00000u);
@@ -369,10 +370,11 @@ __device__ __forceinline__ uint32_t encode_m(float m, int base, uint32_t dither)
     }
     return c ? c | (bits >> 24 & 128) : 0;
 }
-__device__ __forceinline__ uint32_t encode_v(float v, int base, uint32_t dither) {
+// `top`: the largest code of a finite number.
+__device__ __forceinline__ uint32_t encode_v(float v, int base, int top, uint32_t dither) {
     const uint32_t bits = __float_as_uint(v);
     const int c = int((bits + (dither << 4) + 8) >> 20) - base;
-    return bits == 0 ? 0 : uint32_t(min(max(c, 1), kTopV));
+    return bits == 0 ? 0 : uint32_t(min(max(c, 1), top));
 }
 __device__ __forceinline__ int base_of(uint32_t largest, int top) { return max(int(largest >> 20) + 1 - top, 0); }
 
@@ -433,12 +435,13 @@ __device__ __forceinline__ void update8(const AdamwTable& t, const Chunk& c, con
         }
         store4<DT, NT>(ps, e, c.end, p[u]);
         const int nm = base_of(wave_max(top_m), kTopM), nv = base_of(wave_max(top_v), kTopV);
+        const int most_v = min(kTopV, kFinite - nv);  // (a finite v has an m far below the largest number)
         uint32_t om = 0, ov = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const uint32_t r = mix(s.key + uint32_t(e + k) * 0x9E3779B1u);
             om |= (finite[k] ? encode_m(a[k].m, nm, r & 0xFFFF) : kNanM) << 8 * k;
-            ov |= (finite[k] ? encode_v(a[k].v, nv, r >> 16) : kTopV) << 8 * k;
+            ov |= (finite[k] ? encode_v(a[k].v, nv, most_v, r >> 16) : kTopV) << 8 * k;
         }
         store_codes(ms, e, c.end, om);
         store_codes(vs, e, c.end, ov);

@@ -58,3 +58,16 @@ def test_bits_of_the_update(dtype):
     F.adamw_step(*new, lr=lr, betas=betas, eps=eps, weight_decay=wd)
     for got, ref in ((new[2][0], rm), (new[3][0], rv), (new[0][0], want.to(dtype))):
         assert torch.equal(got.cpu(), ref)
+
+
+def test_8bit_second_moments_next_to_the_largest_number():
+    """A finite second moment keeps a finite code: the largest is 15/16 of 2^128 and its neighbour below 14/16, so the
+    codes here are within 1/8 of their values."""
+    n = 1024
+    g = torch.linspace(1.0e19, 1.8446e19, n, device=DEV)  # squares up to 3.4026e38, the largest number 3.4028e38
+    m, v, bases, steps = states(8, n)
+    p = torch.zeros(n, device=DEV)
+    F.adamw8_step([p], [g], m, v, bases, steps, lr=1e-3, betas=(0.9, 0.0), weight_decay=0.0)
+    (m,), (v,) = F.adamw8_moments(m, v, bases)
+    assert bool(m.isfinite().all()) and bool(v.isfinite().all())
+    assert float((v.double() / g.double() ** 2 - 1).abs().max()) <= 0.125 + 1e-6
