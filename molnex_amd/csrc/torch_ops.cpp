@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/autocast_mode.h>
 #include <c10/core/DeviceGuard.h>
@@ -525,6 +526,8 @@ Tensor step(const char* name, int bits, at::TensorList params, at::TensorList gr
         const Tensor *pp = &p, *gg = &g;
         if (!(p.is_contiguous() && g.is_contiguous() && m.is_contiguous() && v.is_contiguous())) {
             if (!p.is_non_overlapping_and_dense()) {
+                TORCH_CHECK_VALUE(at::has_internal_overlap(p) != at::MemOverlap::Yes, "molix::", name, ": parameter ",
+                                  i, " has elements that share memory");
                 gaps.emplace_back(i, p.detach().contiguous());
                 pp = &gaps.back().second;
             }

@@ -79,3 +79,10 @@ def test_many_tensors_pass():
     s = state(32, 700, 3)
     F.adamw_step(*s, **H)
     assert all(float(t) == 1.0 for t in s[-1])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_parameter_whose_elements_share_memory(bits):
+    s = state(bits, 1)
+    s[0] = [torch.ones(1, device=DEV).expand(512)]
+    refused(bits, s, "share memory")
