@@ -139,10 +139,21 @@ class AdamW(torch.optim.Optimizer):
         """Also takes ``torch.optim.AdamW``'s state.  Each tensor's moments keep the form they were saved in, 8 or 32
         bits (the base class would give them the parameters' type), and the step counts go to the device.  Moments
         saved from a parameter of another memory order are brought into this one's."""
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        fitted = {p: self._fitted(p, state_dict["state"][i]) for i, p in zip(saved, params)
-                  if i in state_dict["state"] and len(saved) == len(params)}
-        super().load_state_dict(state_dict)
-        for p, state in fitted.items():
-            self.state[p].update(state)
+        fitted: dict = {}
+
+        def fit(_, final):  # after the other hooks that may replace it
+            saved = [i for g in final["param_groups"] for i in g["params"]]
+            params = [p for g in self.param_groups for p in g["params"]]
+            fitted.update({p: self._fitted(p, final["state"][i]) for i, p in zip(saved, params)
+                           if i in final["state"] and len(saved) == len(params)})
+
+        def put(_):  # before the other hooks that look at the outcome
+            for p, state in fitted.items():
+                self.state[p].update(state)
+
+        hooks = [self.register_load_state_dict_pre_hook(fit), self.register_load_state_dict_post_hook(put, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()

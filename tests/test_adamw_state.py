@@ -149,3 +149,25 @@ def test_torch_constructor_arguments():
             AdamW([{"params": p, name: True}])
         with pytest.raises(ValueError, match=name):
             a.load_state_dict(torch.optim.AdamW(p, **{name: True}).state_dict())
+
+
+@pytest.mark.parametrize("kind", [8, 32])
+def test_load_state_dict_hooks(kind):
+    """A hook that replaces the state before loading is heard, and one that runs afterwards sees the loaded states."""
+    p = torch.nn.Parameter(row(80, 64))
+    fresh = random_state(p) if kind == 8 else {"step": torch.tensor(1.0), "exp_avg": torch.randn(80, 64),
+                                               "exp_avg_sq": torch.rand(80, 64)}
+    a, b = AdamW([p], state_bits=kind), AdamW([p], state_bits=kind)
+    a.state[p] = fresh
+
+    def renamed(opt, state_dict):  # as from a file with other names
+        return {"state": {0: {k[4:]: v for k, v in state_dict["old"].items()}}, "param_groups": state_dict["param_groups"]}
+
+    seen = []
+    b.register_load_state_dict_pre_hook(renamed)
+    b.register_load_state_dict_post_hook(lambda opt: seen.append({k: v.clone() for k, v in opt.state[p].items()}))
+    saved = a.state_dict()
+    b.load_state_dict({"old": {"old_" + k: v for k, v in fresh.items()}, "param_groups": saved["param_groups"]})
+    for state in (b.state[p], *seen):
+        assert all(state[k].dtype == fresh[k].dtype and torch.equal(state[k], fresh[k]) for k in fresh)
+    assert len(seen) == 1
