@@ -6,6 +6,7 @@ weights' gradients are rounded once more, to the weights' type."""
 import pytest
 import torch
 
+import molnex_amd.kernels  # noqa: F401  (registers the ops)
 from molnex_amd import _lib
 
 pytestmark = pytest.mark.gpu
