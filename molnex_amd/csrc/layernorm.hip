@@ -66,9 +66,7 @@ __device__ __forceinline__ void store_vec(typename Elem<DT>::T* p, int c, int wi
             if (c + e < width) p[c + e] = T(v[e]);
     }
 }
-// Values of a vector of weights, of any type whatever the rows'; `none` where there is no vector, 0 past the end.  Types
-// other than the rows' and float32 are rare, so their code is short and out of the way: a small call's time is partly
-// that of fetching code (700 x 128 fp32 forward 2.96 us, 3.14 with that loop unrolled).
+// Values of a vector of weights, of the rows' type or float32 (ln_reads); `none` where there is no vector, 0 past the end.
 template <int DT>
 __device__ __forceinline__ void load_weights(const void* p, int c, int width, int dtype, float none,
                                              float (&v)[kVec]) {
@@ -76,13 +74,6 @@ __device__ __forceinline__ void load_weights(const void* p, int c, int width, in
     if (!p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = c + e < width ? none : 0.0f;
-    } else if (__builtin_expect(dtype != DT && dtype != kF32, 0)) {
-#pragma nounroll
-        for (int e = 0; e < V; ++e) {
-            const float x = c + e < width ? load_elem(p, c + e, dtype) : 0.0f;
-#pragma unroll
-            for (int k = 0; k < V; ++k) v[k] = k == e ? x : v[k];
-        }
     } else if (DT == kF32 || dtype == DT) {
         load_vec<DT>(static_cast<const typename Elem<DT>::T*>(p), c, width, v);
     } else {
@@ -364,8 +355,9 @@ __global__ __launch_bounds__(1024) void k_ln_join(const float* partial, int part
     if (r) store_elem(r, col < width ? col : col - width, wdt, s);
 }
 
-// Rows too wide for a workgroup's registers: a workgroup takes a row and reads it again for each sum (from L2: a row is
-// at most a few hundred KB where many are in flight), and the column sums are a launch of their own.
+// Rows too wide for a workgroup's registers, and weights of a type that load_weights does not read (these kernels read
+// any): a workgroup takes a row and reads it again for each sum (from L2: a row is at most a few hundred KB where many are
+// in flight), and the column sums are a launch of their own.
 template <int DT>
 __global__ __launch_bounds__(256) void k_ln_fwd_wide(const typename Elem<DT>::T* x, int64_t rows, int width,
                                                      int64_t ldx,
@@ -530,6 +522,11 @@ static bool ln_variant(int64_t width, F&& f) {
     return false;
 }
 
+// Whether load_weights reads the weights.  Other types go to the wide form at any width: asking each vector for its type
+// cost the calls that have none of them (700 x 128 fp32 forward 2.92 -> 3.17 us; as a rare branch 2.96, but the fp16
+// backward of 166,666 x 120 31.2 -> 33.4).
+static bool ln_reads(int dtype, int wdtype) { return wdtype == dtype || wdtype == kF32; }
+
 constexpr int kLnParts = 512;  // workgroups of the backward kernels at most, so rows of partial sums
 constexpr int kLnThreads = 512;  // of their workgroups
 
@@ -560,14 +557,14 @@ static int64_t ln_parts(const void* kernel, int threads, int64_t rows, int group
 constexpr int64_t kLnWideGrid = 1 << 16;
 
 // The backward passes' workspace: the rows of partial sums that the form of this width leaves, and for the wide form's
-// column sums two numbers a row.
+// column sums two numbers a row.  Rows that fit registers may take either (ln_reads); the wide form's strips are fewer.
 struct LnWorkspace : Workspace {
     float *partial, *usums;
     LnWorkspace(void* p, size_t bytes, int64_t rows, int64_t width) : Workspace{static_cast<char*>(p), bytes} {
         const bool held = ln_variant(width, [](auto, auto) {});
         const int64_t parts = held ? std::min<int64_t>(std::max<int64_t>(rows, 1), kLnParts) : ln_strips(rows);
         partial = take<float>(size_t(parts) * 2 * size_t(width));
-        usums = take<float>(held ? 0 : size_t(rows) * 2);
+        usums = take<float>(size_t(rows) * 2);
     }
 };
 
@@ -597,7 +594,7 @@ int mnx_layer_norm_fwd(const void* x, int64_t ldx, int64_t rows, int64_t width, 
         using T = typename Elem<DT>::T;
         const T* xs = static_cast<const T*>(x);
         T* ys = static_cast<T*>(y);
-        const bool held = ln_variant(width, [&](auto tpr, auto vpl) {
+        const bool held = ln_reads(dtype, wdtype) && ln_variant(width, [&](auto tpr, auto vpl) {
             constexpr int TPR = decltype(tpr)::value, VPL = decltype(vpl)::value, THREADS = TPR > 256 ? TPR : 256;
             const auto kernel = k_ln_fwd<DT, TPR, VPL, THREADS>;
             grid = ln_forward_grid(reinterpret_cast<const void*>(kernel), THREADS, ceil_div(rows, THREADS / TPR));
@@ -649,7 +646,7 @@ int mnx_layer_norm_bwd(const void* grad, int64_t ldg, const void* x, int64_t ldx
         using T = typename Elem<DT>::T;
         const T *gs = static_cast<const T*>(grad), *xs = static_cast<const T*>(x);
         T* gx = static_cast<T*>(grad_x);
-        held = ln_variant(width, [&](auto tpr, auto vpl) {
+        held = ln_reads(dtype, wdtype) && ln_variant(width, [&](auto tpr, auto vpl) {
             constexpr int TPR = decltype(tpr)::value, VPL = decltype(vpl)::value, THREADS = kLnThreads;
             const auto kernel = ln_past_cache<DT>(rows, width, 3) ? k_ln_bwd<DT, TPR, VPL, DT == kF32, THREADS>
                                                                   : k_ln_bwd<DT, TPR, VPL, false, THREADS>;
@@ -695,7 +692,7 @@ int mnx_layer_norm_bwd2(const void* grad, int64_t ldg, const void* x, int64_t ld
         using T = typename Elem<DT>::T;
         const T *gs = static_cast<const T*>(grad), *xs = static_cast<const T*>(x), *us = static_cast<const T*>(seed_x);
         T *dg = static_cast<T*>(dgrad), *dxs = static_cast<T*>(dx);
-        held = ln_variant(width, [&](auto tpr, auto vpl) {
+        held = ln_reads(dtype, wdtype) && ln_variant(width, [&](auto tpr, auto vpl) {
             constexpr int TPR = decltype(tpr)::value, VPL = decltype(vpl)::value, THREADS = kLnThreads;
             auto kernel = k_ln_bwd2<DT, TPR, VPL, false, false, THREADS>;
             if (seed_w || seed_b) kernel = k_ln_bwd2<DT, TPR, VPL, true, false, THREADS>;

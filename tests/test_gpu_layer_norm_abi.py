@@ -1,13 +1,15 @@
 """The layer norm's C ABI: weights of any element type, whatever the rows'.
 
-16-bit weights are float32 numbers, so every output has the bits of the call with the same weights in float32; the
-weights' gradients are rounded once more, to the weights' type."""
+The formulas and bounds are test_gpu_layer_norm's.  Where the same kernels run, every output has the bits of the call
+with the same weights in float32; the weights' gradients are rounded once more, to the weights' type."""
 
 import pytest
 import torch
 
 import molnex_amd.kernels  # noqa: F401  (registers the ops)
 from molnex_amd import _lib
+from tests.test_gpu_layer_norm import _second as _second_formula
+from tests.test_gpu_layer_norm import check_backward, check_forward, check_rows, check_sum
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -55,7 +57,7 @@ def _second(g, x, u, p, q, w, stats):
 
 @pytest.mark.parametrize("wdtype", list(TYPES))
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("rows,width", [(3, 1), (9, 30), (50, 333), (20, 1024), (3, 8190), (2, 9001)])
+@pytest.mark.parametrize("rows,width", [(3, 1), (9, 30), (50, 333), (200, 1024), (3, 8190), (2, 9001)])
 def test_weights_of_any_type(rows, width, dtype, wdtype):
     gen = torch.Generator(device=DEV).manual_seed(rows + width)
     x, g, u = (torch.randn(rows, width, generator=gen, device=DEV).to(dtype) for _ in range(3))
@@ -65,14 +67,23 @@ def test_weights_of_any_type(rows, width, dtype, wdtype):
         ww, bb, pp, qq = (cast(t) for t in (w, b, p, q))
         y, stats = _forward(x, ww, bb)
         outs.append((y, stats, *_backward(g, x, ww, stats), *_second(g, x, u, pp, qq, ww, stats)))
-    for got, ref in zip(*outs):
-        assert torch.equal(got, ref.to(got.dtype))
+    y, stats, gx, gw, gb, dg, dx, dw = outs[0]
+    check_forward(y, x, w, b)
+    check_backward(gx, gw, gb, g, x, w)
+    (rg, bg), (rx, bx), (tw, sw) = _second_formula(g, x, w, u, p, q)
+    check_rows(dg, rg, bg)
+    check_rows(dx, rx, bx)
+    check_sum(dw, tw, sw)
+    if wdtype in (dtype, torch.float32) or width > 8192:  # the same kernels: the same bits
+        for got, ref in zip(*outs):
+            assert torch.equal(got, ref.to(got.dtype))
 
 
 def test_seeds_of_sixteen_bits_without_a_weight():
     x, g, u = (torch.randn(40, 100, device=DEV) for _ in range(3))
     p, q = (torch.randn(100, device=DEV).half() for _ in range(2))
     _, stats = torch.ops.molix.layer_norm(x, None, None, EPS)
-    got, ref = (torch.ops.molix.layer_norm_backward2(g, x, None, stats, EPS, u, s, t, False)
-                for s, t in ((p, q), (p.float(), q.float())))
-    assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+    dg, dx, _ = torch.ops.molix.layer_norm_backward2(g, x, None, stats, EPS, u, p, q, False)
+    (rg, bg), (rx, bx), _ = _second_formula(g, x, None, u, p, q)
+    check_rows(dg, rg, bg)
+    check_rows(dx, rx, bx)
