@@ -282,17 +282,19 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward2_formula(const Tensor& gr
     return {dg.to(x.scalar_type()).reshape(x.sizes()), dx.to(x.scalar_type()).reshape(x.sizes()), dw};
 }
 
+// The statistics are not differentiable: they leave through `out`, not as an output that is marked so, which compiled
+// autograd does not take.
 class LayerNorm : public torch::autograd::Function<LayerNorm> {
   public:
-    static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias,
-                                 double eps) {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias,
+                          double eps, Tensor* out) {
         at::AutoDispatchBelowADInplaceOrView below;
         auto [y, stats] = layer_norm_op().call(x, weight, bias, eps);
         ctx->save_for_backward({x, or_undefined(weight), or_undefined(bias), stats});
         ctx->saved_data["eps"] = eps;
-        ctx->mark_non_differentiable({stats});
-        ctx->set_materialize_grads(false);  // of stats: a fill a call
-        return {y, stats};
+        ctx->set_materialize_grads(false);
+        *out = stats;
+        return y;
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         const auto saved = ctx->get_saved_variables();
@@ -300,10 +302,10 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
         // edges are numbered over the tensors that were there
         const bool nx = ctx->needs_input_grad(0), nw = w.defined() && ctx->needs_input_grad(1);
         const bool nb = b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1);
-        if (!grads[0].defined() || !(nx || nw || nb)) return {Tensor(), Tensor(), Tensor(), Tensor()};
+        if (!grads[0].defined() || !(nx || nw || nb)) return variable_list(5);
         auto [gx, gw, gb] = layer_norm_backward_op().call(grads[0], x, optional(w), optional(b), saved[3],
                                                           ctx->saved_data["eps"].toDouble(), nx, nw, nb);
-        return {nx ? gx : Tensor(), nw ? gw : Tensor(), nb ? gb : Tensor(), Tensor()};
+        return {nx ? gx : Tensor(), nw ? gw : Tensor(), nb ? gb : Tensor(), Tensor(), Tensor()};
     }
 };
 
@@ -312,8 +314,9 @@ std::tuple<Tensor, Tensor> layer_norm_autograd(const Tensor& x, const OptTensor&
     if (has_tangent(x) || has_tangent(weight) || has_tangent(bias)) return layer_norm_formula(x, weight, bias, eps);
     if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias))) {
         if (transformed()) return layer_norm_formula(x, weight, bias, eps);
-        auto r = LayerNorm::apply(x, weight, bias, eps);
-        return {r[0], r[1]};
+        Tensor stats;
+        Tensor y = LayerNorm::apply(x, weight, bias, eps, &stats);
+        return {y, stats};
     }
     at::AutoDispatchBelowADInplaceOrView below;
     return layer_norm_op().call(x, weight, bias, eps);

@@ -219,3 +219,28 @@ def test_calls_after_a_transform_take_the_ops():
     args, _ = _data()
     torch.func.grad(loss(norm))(*args)
     assert "LayerNorm" in norm(args[0].requires_grad_(), *args[1:]).grad_fn.name() and "Native" not in norm(*args).grad_fn.name()
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_compiled_autograd():
+    """A backward pass that the compiler records and runs."""
+    import torch._dynamo.compiled_autograd as compiled
+
+    (x, w, b), _ = _data()
+    grads = []
+    for fn, enabled in ((norm, True), (norm, False)):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        loss = fn(*leaves).pow(3).sum()
+        if enabled:
+            with compiled._enable(torch.compile(backend="eager")):
+                loss.backward()
+        else:
+            loss.backward()
+        grads.append([t.grad for t in leaves])
+    assert all(torch.equal(a, r) for a, r in zip(*grads))
+
+
+def test_the_statistics_carry_no_gradient():
+    (x, w, b), _ = _data()
+    y, stats = OPS.layer_norm(x.requires_grad_(), w, b, 1e-5)
+    assert y.requires_grad and not stats.requires_grad and stats.grad_fn is None
