@@ -892,7 +892,8 @@ PyObject* py_moments(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK_TYPE(n == 5, "moments: 5 lists, got ", n);
     bool overridden = mode_on();
     const auto avgs = tensors(a[0], "first moments", overridden), sqs = tensors(a[1], "second moments", overridden);
-    const auto bases = tensors(a[2], "bases", overridden), om = tensors(a[3], "out", overridden), ov = tensors(a[4], "out", overridden);
+    const auto bases = tensors(a[2], "bases", overridden);
+    const auto om = tensors(a[3], "out", overridden), ov = tensors(a[4], "out", overridden);
     if (overridden) Py_RETURN_NOTIMPLEMENTED;
     {
         Released r;

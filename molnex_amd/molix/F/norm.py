@@ -15,7 +15,8 @@ _layer_norm = torch.ops.molix.layer_norm.default
 
 def layer_norm(input: Tensor, normalized_shape, weight: Tensor | None = None, bias: Tensor | None = None,
                eps: float = 1e-5) -> Tensor:
-    """Norm over the trailing axes ``normalized_shape``, in float32 whatever the type, with derivatives of any order.
+    """Norm over the trailing axes ``normalized_shape``, in float32 whatever the type, with derivatives of any order and
+    mode.  The kernels know backward mode up to the second order; the rest are torch operations.
 
     The kernels take float32, bfloat16 and float16 with weights of that type or float32; other types (float64
     models) go to torch.  Under autocast it computes and returns float32, as torch's does.  GPU tensors only."""
