@@ -66,16 +66,17 @@ __device__ __forceinline__ void store_vec(typename Elem<DT>::T* p, int c, int wi
             if (c + e < width) p[c + e] = T(v[e]);
     }
 }
-// The backward kernels' h past the row's end has to be 0, not (0 - mu) r, which may overflow and make a NaN of the sums'
-// zeros.  The vectors of a thread that need no test for it: in float16 all, since mu r stays finite; in float32 those
-// inside the row at every width of the variant, all but the last, or the last two of the widest; in bfloat16 none, which
-// takes fewer registers (6896 x 2900: 36.6 us, 39.7 with neither test nor mend; elsewhere within 1 % of that).
+// The backward kernels' h past the row's end has to be 0, not (0 - mu) r, which may overflow and make a NaN of the
+// sums' zeros.  The vectors of a thread that need no test for it: in float16 all, since mu r stays finite; in float32
+// those inside the row at every width of the variant, all but the last, or the last two of the widest; in bfloat16
+// none, which takes fewer registers (6896 x 2900: 36.6 us, 39.7 without any test; elsewhere within 1 % of that).
 template <int DT, int TPR, int VPL>
 constexpr int inner_vectors() {
     return DT == kF16 ? VPL : DT == kBF16 ? 0 : TPR == 512 ? VPL / 2 : VPL - 1;
 }
 
-// Values of a vector of weights, of the rows' type or float32 (ln_reads); `none` where there is no vector, 0 past the end.
+// Values of a vector of weights, of the rows' type or float32 (ln_reads); `none` where there is no vector, 0 past the
+// end.
 template <int DT>
 __device__ __forceinline__ void load_weights(const void* p, int c, int width, int dtype, float none,
                                              float (&v)[kVec]) {
@@ -375,11 +376,12 @@ __device__ __forceinline__ void load_any(const void* p, int c, int width, int dt
 }
 
 // Rows too wide for a workgroup's registers, and weights of a type that load_weights does not read (these kernels read
-// any): a workgroup takes a row and reads it again for each sum (from L2: a row is at most a few hundred KB where many are
-// in flight), and the column sums are a launch of their own.
-// Threads of a row: many, so that few rows still have many loads on the way, of a vector each.  2000 x 20,000 fp32: forward
-// 75 us (4.3 TB/s), forward with all gradients 252; with 256 threads reading value by value 118 and 366, and 4 x 70,001
-// 131 where it takes 18 now.
+// any): a workgroup takes a row and reads it again for each sum (from L2: a row is at most a few hundred KB where many
+// are in flight), and the column sums are a launch of their own.
+//
+// Threads of a row: many, so that few rows still have many loads on the way, of a vector each.  2000 x 20,000 fp32:
+// forward 75 us (4.3 TB/s), forward with all gradients 252; with 256 threads reading value by value 118 and 366.
+// 4 x 70,001: forward 18 us, with those 131.
 constexpr int kLnWide = 1024;
 
 template <int DT>
@@ -589,9 +591,9 @@ static bool ln_variant(int64_t width, F&& f) {
     return false;
 }
 
-// Whether load_weights reads the weights.  Other types go to the wide form at any width: asking each vector for its type
-// cost the calls that have none of them (700 x 128 fp32 forward 2.92 -> 3.17 us; as a rare branch 2.96, but the fp16
-// backward of 166,666 x 120 31.2 -> 33.4).
+// Whether load_weights reads the weights.  Other types go to the wide form at any width: asking each vector for its
+// type cost the calls that have none of them (700 x 128 fp32 forward 2.92 -> 3.17 us; as a rare branch 2.96, but the
+// fp16 backward of 166,666 x 120 31.2 -> 33.4).
 static bool ln_reads(int dtype, int wdtype) { return wdtype == dtype || wdtype == kF32; }
 
 constexpr int kLnParts = 512;  // workgroups of the backward kernels at most, so rows of partial sums
@@ -671,8 +673,8 @@ int mnx_layer_norm_fwd(const void* x, int64_t ldx, int64_t rows, int64_t width, 
         });
         if (!held) {
             grid = std::min<int64_t>(rows, kLnWideGrid);
-            k_ln_fwd_wide<DT><<<grid, kLnWide, 0, stream>>>(xs, rows, int(width), ldx, weight, bias, wdtype, float(eps), ys,
-                                                        stats);
+            k_ln_fwd_wide<DT><<<grid, kLnWide, 0, stream>>>(xs, rows, int(width), ldx, weight, bias, wdtype, float(eps),
+                                                            ys, stats);
         }
     });
     MNX_REQUIRE(grid > 0, "layer norm: device query failed");

@@ -293,8 +293,8 @@ __device__ __forceinline__ float updated(const Hyper& h, const TensorScalars& s,
     return p * s.decay - s.size * a.m / (sqrtf(a.v) * s.inv_root + h.eps);
 }
 // Beside 8-bit moments, which know m to one part in 16 at best, the square root and the reciprocal are the hardware's
-// instructions, a unit of the last place each: instructions bound that kernel (3.2 M elements 16.5 us with them and 18.0
-// with the exact forms, 64 M 94 against 103 a launch).
+// instructions, a unit of the last place each: instructions bound that kernel (3.2 M elements 16.5 us with them and
+// 18.0 with the exact forms, 64 M 94 against 103 a launch).
 // The root's instruction takes no subnormals: a v below 2^-96 is scaled (its root is far below any eps but 0).
 __device__ __forceinline__ float updated_fast(const Hyper& h, const TensorScalars& s, float p, const Moments& a) {
     const bool tiny = a.v < 0x1p-96f;
@@ -629,8 +629,8 @@ int mnx_adamw_step(const mnx_adamw_args* args, mnx_stream_t stream) {
                                                a.beta2, a.weight_decay, a.seed, call, scalars);
         MNX_CHECK_LAUNCH();
     }
-    // An eps below the smallest normal number counts as that one: its only use is beside a second moment of zero, and the
-    // reciprocal's instruction takes no subnormals.
+    // An eps below the smallest normal number counts as that one: its only use is beside a second moment of zero, and
+    // the reciprocal's instruction takes no subnormals.
     const float eps = a.eps > 0 ? std::max(float(a.eps), 0x1p-126f) : 0.0f;
     const Hyper h{float(a.beta1), float(1 - a.beta1), float(a.beta2), float(1 - a.beta2), eps};
     int64_t bytes = 0;

@@ -215,10 +215,10 @@ bool wants_grad(const OptTensor& t) { return given(t) && t->requires_grad(); }
 OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 Tensor or_undefined(const OptTensor& t) { return given(t) ? *t : Tensor(); }
 
-// Whether t carries a tangent (forward-mode differentiation).  The autograd Functions below know backward mode only,
+// The autograd Functions below know backward mode, outside torch.func's transforms.  Whether t carries a tangent
+// (forward mode), and whether this call is inside a transform (the key is in force while one is):
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
-// ... outside torch.func's transforms: whether this call is inside one (the key is in force while one is).
 bool transformed() { return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerBackMode); }
 
 // The three ops as torch operations in float32, rounded once at the end: differentiable in every mode and to any order.
@@ -812,7 +812,8 @@ PyObject* py_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const double lr = number(a[7]), b1 = number(a[8]), b2 = number(a[9]), eps = number(a[10]), wd = number(a[11]);
     const bool maximize = truth(a[12]), skip = truth(a[15]);
     const std::optional<double> max_norm = a[13] == Py_None ? std::nullopt : std::optional<double>(number(a[13]));
-    const OptTensor norm_in = tensor_or_none(a[14], "grad_norm", overridden), rate = tensor_or_none(a[16], "lr", overridden);
+    const OptTensor norm_in = tensor_or_none(a[14], "grad_norm", overridden);
+    const OptTensor rate = tensor_or_none(a[16], "lr", overridden);
     const int64_t seed = eight ? PyLong_AsLongLong(a[17]) : 0;
     if (PyErr_Occurred()) throw python_error();
     if (overridden) Py_RETURN_NOTIMPLEMENTED;

@@ -11,7 +11,8 @@ from ...training import STATE_BLOCK, adamw8_relayout, adamw8_step, adamw_step, d
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) for parameters on the GPU, with the arguments of ``torch.optim.AdamW`` and those
     below.  ``foreach``, ``fused`` and ``capturable`` choose between torch's implementations and change nothing here
-    (a step is always a few launches over all tensors and can be captured); ``amsgrad`` and ``differentiable`` are refused.
+    (a step is always a few launches over all tensors and can be captured); ``amsgrad`` and ``differentiable`` are
+    refused.
 
     ``state_bits``     32, or 8: the moments of tensors of at least ``min_8bit_size`` elements take 2 bytes an element
                        instead of 8 (``molix.F.adamw8_step``); a group's option
@@ -123,7 +124,7 @@ class AdamW(torch.optim.Optimizer):
         moments = {k: saved[k] for k in ("exp_avg", "exp_avg_sq") if k in saved}
         for key, value in moments.items():
             if value.shape != p.shape:
-                raise ValueError(f"AdamW: saved {key} of shape {tuple(value.shape)} for a parameter of {tuple(p.shape)}")
+                raise ValueError(f"AdamW: saved {key} of shape {tuple(value.shape)}, its parameter {tuple(p.shape)}")
         if any(t.dtype == torch.uint8 for t in moments.values()):
             codes = [t.to(p.device, copy=True) for t in (*moments.values(), saved.get("bases", p.new_empty(0)))]
             blocks = -(-p.numel() // STATE_BLOCK)
@@ -151,7 +152,8 @@ class AdamW(torch.optim.Optimizer):
             for p, state in fitted.items():
                 self.state[p].update(state)
 
-        hooks = [self.register_load_state_dict_pre_hook(fit), self.register_load_state_dict_post_hook(put, prepend=True)]
+        hooks = [self.register_load_state_dict_pre_hook(fit),
+                 self.register_load_state_dict_post_hook(put, prepend=True)]
         try:
             super().load_state_dict(state_dict)
         finally:

@@ -145,7 +145,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     norm = _host.step(32, params, grads, exp_avgs, exp_avg_sqs, None, steps, rate, betas[0], betas[1], eps,
                       weight_decay, maximize, max_norm, grad_norm, skip_nonfinite, lr_tensor, 0)
     if norm is NotImplemented:
-        return handle_torch_function(adamw_step, (*params, *grads, *exp_avgs, *exp_avg_sqs, *steps, grad_norm, lr_tensor),
+        return handle_torch_function(adamw_step, (*params, *grads, *exp_avgs, *exp_avg_sqs, *steps, grad_norm,
+                                                  lr_tensor),
                                      params, grads, exp_avgs, exp_avg_sqs, steps, lr=lr, betas=betas, eps=eps,
                                      weight_decay=weight_decay, maximize=maximize, max_norm=max_norm,
                                      grad_norm=grad_norm, skip_nonfinite=skip_nonfinite)
@@ -214,8 +215,8 @@ def adamw8_relayout(exp_avg: Tensor, exp_avg_sq: Tensor, bases: Tensor, like: Te
         return torch.where(sizes > 0, sizes + bases[:, column].int().repeat_interleave(STATE_BLOCK)[:n], 0)
 
     def coded(key, nan, top):  # sizes of the codes, and the bases
-        padded = torch.nn.functional.pad(torch.where(nan, 0, key), (0, blocks * STATE_BLOCK - n)).view(blocks, STATE_BLOCK)
-        base = (padded.amax(1) + 1 - top).clamp_(min=0)
+        padded = torch.nn.functional.pad(torch.where(nan, 0, key), (0, blocks * STATE_BLOCK - n))
+        base = (padded.view(blocks, STATE_BLOCK).amax(1) + 1 - top).clamp_(min=0)
         return key - base.repeat_interleave(STATE_BLOCK)[:n], base
 
     codes = memory(exp_avg)

@@ -67,7 +67,8 @@ def channels_last(*shape):
 
 
 @pytest.mark.parametrize("source,target", [(column(80, 64), row(80, 64)), (row(80, 64), column(80, 64)),
-                                           (channels_last(9, 7, 5, 3), row(9, 7, 5, 3)), (row(9, 7, 5, 3), channels_last(9, 7, 5, 3)),
+                                           (channels_last(9, 7, 5, 3), row(9, 7, 5, 3)),
+                                           (row(9, 7, 5, 3), channels_last(9, 7, 5, 3)),
                                            (column(80, 64), torch.zeros(80, 128)[:, ::2])])
 def test_eight_bit_moments_keep_their_values(source, target):
     state = random_state(source)
@@ -77,14 +78,12 @@ def test_eight_bit_moments_keep_their_values(source, target):
     (m, v), (nm, nv) = decode(state), decode(new)
     assert torch.equal(m.isnan(), nm.isnan()) and bool(m.isnan().any())
     live = ~m.isnan()
-    flat = new["exp_avg"].as_strided((source.numel(),), (1,))
-    least = torch.empty_like(new["exp_avg"], dtype=torch.float32)
-    least.as_strided((source.numel(),), (1,)).copy_(bits(new["bases"][:, 0].int() + 1).repeat_interleave(B)[:flat.numel()])
+    least, floor = (torch.empty_like(new["exp_avg"], dtype=torch.float32) for _ in range(2))
+    for t, base in zip((least, floor), new["bases"].int().unbind(1)):  # the smallest codes' values
+        t.as_strided((t.numel(),), (1,)).copy_(bits(base + 1).repeat_interleave(B)[:t.numel()])
     small = live & (m.abs() < least)
     assert torch.equal(m[live & ~small], nm[live & ~small])
     assert bool(((m - nm)[small].abs() <= least[small] / 2).all()) and float(small.float().mean()) < 0.2
-    floor = torch.empty_like(least)
-    floor.as_strided((source.numel(),), (1,)).copy_(bits(new["bases"][:, 1].int() + 1).repeat_interleave(B)[:flat.numel()])
     assert torch.equal(torch.where(v > 0, torch.maximum(v, floor), v)[live], nv[live])
 
 
@@ -120,7 +119,8 @@ def test_float_moments_move_as_they_are():
 @pytest.mark.parametrize("kind", [8, 32])
 def test_moments_of_another_shape_are_refused(kind):
     source, target = row(1, 64), row(80, 64)  # copying would broadcast
-    state = random_state(source) if kind == 8 else {"step": torch.tensor(1.0), "exp_avg": row(1, 64), "exp_avg_sq": row(1, 64)}
+    state = {"step": torch.tensor(1.0), "exp_avg": row(1, 64), "exp_avg_sq": row(1, 64)}
+    state = random_state(source) if kind == 8 else state
     with pytest.raises(ValueError, match="shape"):
         loaded(state, source, target)
     bad = random_state(row(80, 64))
@@ -139,7 +139,8 @@ def test_torch_constructor_arguments():
     assert [a.defaults[k] for k in ("lr", "betas", "eps", "weight_decay")] == [1e-2, (0.8, 0.9), 1e-7, 0.1]
     for value in (None, True, False):
         AdamW(p, foreach=value, fused=value, capturable=bool(value), amsgrad=False, differentiable=False)
-    AdamW([{"params": p, "amsgrad": False, "foreach": None, "fused": None, "capturable": True, "differentiable": False}])
+    AdamW([{"params": p, "amsgrad": False, "foreach": None, "fused": None, "capturable": True,
+            "differentiable": False}])
     a.load_state_dict(torch.optim.AdamW(p, foreach=True).state_dict())
     torch.optim.AdamW(p).load_state_dict(a.state_dict())
     for name in ("amsgrad", "differentiable"):
@@ -161,7 +162,8 @@ def test_load_state_dict_hooks(kind):
     a.state[p] = fresh
 
     def renamed(opt, state_dict):  # as from a file with other names
-        return {"state": {0: {k[4:]: v for k, v in state_dict["old"].items()}}, "param_groups": state_dict["param_groups"]}
+        return {"state": {0: {k[4:]: v for k, v in state_dict["old"].items()}},
+                "param_groups": state_dict["param_groups"]}
 
     seen = []
     b.register_load_state_dict_pre_hook(renamed)

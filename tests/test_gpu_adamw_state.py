@@ -18,7 +18,8 @@ def test_a_state_of_another_memory_order():
     gen = torch.Generator(device=DEV).manual_seed(0)
     w = torch.randn(70, 60, generator=gen, device=DEV)
     # m of a first step is g / 10: magnitudes from 1/4 to 4 are 4 octaves, of 15
-    g = torch.randn(70, 60, generator=gen, device=DEV).sign() * (4.0 ** (2 * torch.rand(70, 60, generator=gen, device=DEV) - 1))
+    g = torch.randn(70, 60, generator=gen, device=DEV).sign()
+    g = g * 4.0 ** (2 * torch.rand(70, 60, generator=gen, device=DEV) - 1)
     a = torch.nn.Parameter(w.t().contiguous().t())  # column by column
     b = torch.nn.Parameter(w.clone())
     oa, ob = (AdamW([p], lr=1e-2, state_bits=8, min_8bit_size=1) for p in (a, b))

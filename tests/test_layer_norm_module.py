@@ -10,7 +10,8 @@ import torch
 from molnex_amd.molix.nn import LayerNorm
 
 pytestmark = pytest.mark.filterwarnings("ignore::DeprecationWarning")
-MODULES = [lambda c: c(8), lambda c: c((3, 4), eps=1e-3), lambda c: c(8, elementwise_affine=False), lambda c: c(8, bias=False)]
+MODULES = [lambda c: c(8), lambda c: c((3, 4), eps=1e-3), lambda c: c(8, elementwise_affine=False),
+           lambda c: c(8, bias=False)]
 
 
 def pair(make):

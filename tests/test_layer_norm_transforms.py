@@ -36,7 +36,8 @@ def _bwd(g, x, w, b, stats, eps, nx, nw, nb):
 def _bwd2(g, x, w, stats, eps, u, p, q, nw):
     h, r, J = _parts(x, eps)
     one, zero = torch.ones(x.shape[-1]), torch.zeros(x.shape[-1])
-    u, w, p, q = (torch.zeros_like(x) if u is None else u), *(d if t is None else t for t, d in ((w, one), (p, zero), (q, zero)))
+    u = torch.zeros_like(x) if u is None else u
+    w, p, q = (d if t is None else t for t, d in ((w, one), (p, zero), (q, zero)))
     a, ju = g * w, J(u)
     mean = lambda t: t.mean(-1, keepdim=True)  # noqa: E731
     dx = J(p * g) - r * (mean(a * h) * ju + mean(u * h) * J(a)) - r * h * mean(u * J(a))
@@ -103,7 +104,8 @@ def test_forward_over_reverse(which):
     def grads(fn):
         def run(x, w, b):
             y = fn(x, w, b)
-            g = torch.autograd.grad((y.square() * torch.linspace(0, 1, D, dtype=y.dtype)).sum(), (x, w, b), create_graph=True)
+            total = (y.square() * torch.linspace(0, 1, D, dtype=y.dtype)).sum()
+            g = torch.autograd.grad(total, (x, w, b), create_graph=True)
             return torch.cat([t.reshape(-1) for t in g])
         return run
 
@@ -214,11 +216,26 @@ def test_batched_gradients_of_a_recorded_graph():
         close(a, r)
 
 
+def test_transforms_of_one_argument_beside_trained_ones():
+    """torch.func.grad over x where the weights are in an outer, ordinary graph, which is differentiated afterwards."""
+
+    def run(fn, dtype):
+        (x, w, b), _ = _data()
+        x, w, b = x.to(dtype), w.to(dtype).requires_grad_(), b.to(dtype).requires_grad_()
+        gx = torch.func.grad(lambda x: loss(fn)(x, w, b))(x)
+        per_row = torch.vmap(torch.func.grad(lambda r: loss(fn)(r, w, b)))(x)
+        return [gx, per_row, *torch.autograd.grad(gx.square().sum() + per_row.pow(3).sum(), (w, b))]
+
+    for a, r in zip(run(norm, torch.float32), run(plain, torch.float64)):
+        close(a, r)
+
+
 def test_calls_after_a_transform_take_the_ops():
     """What a transform did leaves later calls as they were: the node of the registered op."""
     args, _ = _data()
     torch.func.grad(loss(norm))(*args)
-    assert "LayerNorm" in norm(args[0].requires_grad_(), *args[1:]).grad_fn.name() and "Native" not in norm(*args).grad_fn.name()
+    name = norm(args[0].requires_grad_(), *args[1:]).grad_fn.name()
+    assert "LayerNorm" in name and "Native" not in name
 
 
 @pytest.mark.filterwarnings("ignore")
