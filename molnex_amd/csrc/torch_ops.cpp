@@ -804,7 +804,8 @@ PyObject* py_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == 18, "step: 18 arguments, got ", n);
     const bool eight = number(a[0]) == 8;
-    bool overridden = mode_on();
+    if (mode_on()) Py_RETURN_NOTIMPLEMENTED;
+    bool overridden = false;
     const auto params = tensors(a[1], "parameters", overridden), grads = tensors(a[2], "gradients", overridden);
     const auto avgs = tensors(a[3], "first moments", overridden), sqs = tensors(a[4], "second moments", overridden);
     const auto bases = eight ? tensors(a[5], "bases", overridden) : std::vector<Tensor>();
@@ -875,7 +876,8 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyObject* py_grad_norm(PyObject*, PyObject* list) {
     HANDLE_TH_ERRORS
-    bool overridden = mode_on();
+    if (mode_on()) Py_RETURN_NOTIMPLEMENTED;
+    bool overridden = false;
     const auto grads = tensors(list, "gradients", overridden);
     if (overridden) Py_RETURN_NOTIMPLEMENTED;
     Tensor norm;
@@ -891,7 +893,8 @@ PyObject* py_grad_norm(PyObject*, PyObject* list) {
 PyObject* py_moments(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == 5, "moments: 5 lists, got ", n);
-    bool overridden = mode_on();
+    if (mode_on()) Py_RETURN_NOTIMPLEMENTED;
+    bool overridden = false;
     const auto avgs = tensors(a[0], "first moments", overridden), sqs = tensors(a[1], "second moments", overridden);
     const auto bases = tensors(a[2], "bases", overridden);
     const auto om = tensors(a[3], "out", overridden), ov = tensors(a[4], "out", overridden);

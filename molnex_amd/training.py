@@ -106,6 +106,16 @@ def same_order(a: Tensor, b: Tensor) -> bool:
     return all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride())) or a.numel() == 0
 
 
+_PLAIN = {Tensor, torch.nn.Parameter, type(None)}
+
+
+def _handed_over(func, lists, *args, **kwargs):
+    """The call by torch's protocol for subclasses and modes.  Tensors of no subclass have no say in it and are left out:
+    a default device is a mode, too, and lists can be long."""
+    relevant = [t for ts in lists if not _PLAIN.issuperset(map(type, ts)) for t in ts]
+    return handle_torch_function(func, relevant, *args, **kwargs)
+
+
 def grad_norm(grads) -> Tensor:
     """The 2-norm of all of ``grads`` together (float32, 0-dim, on their device; no synchronisation): squares are
     summed in float64 in a fixed order."""
@@ -115,7 +125,7 @@ def grad_norm(grads) -> Tensor:
     if torch.compiler.is_compiling():
         return torch.ops.molix.grad_norm(grads)
     norm = _host.grad_norm(grads)
-    return handle_torch_function(grad_norm, grads, grads) if norm is NotImplemented else norm
+    return _handed_over(grad_norm, (grads,), grads) if norm is NotImplemented else norm
 
 
 def _rate(lr) -> tuple[float, Tensor | None]:
@@ -145,11 +155,10 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     norm = _host.step(32, params, grads, exp_avgs, exp_avg_sqs, None, steps, rate, betas[0], betas[1], eps,
                       weight_decay, maximize, max_norm, grad_norm, skip_nonfinite, lr_tensor, 0)
     if norm is NotImplemented:
-        return handle_torch_function(adamw_step, (*params, *grads, *exp_avgs, *exp_avg_sqs, *steps, grad_norm,
-                                                  lr_tensor),
-                                     params, grads, exp_avgs, exp_avg_sqs, steps, lr=lr, betas=betas, eps=eps,
-                                     weight_decay=weight_decay, maximize=maximize, max_norm=max_norm,
-                                     grad_norm=grad_norm, skip_nonfinite=skip_nonfinite)
+        return _handed_over(adamw_step, (params, grads, exp_avgs, exp_avg_sqs, steps, (grad_norm, lr_tensor)), params,
+                            grads, exp_avgs, exp_avg_sqs, steps, lr=lr, betas=betas, eps=eps,
+                            weight_decay=weight_decay, maximize=maximize, max_norm=max_norm, grad_norm=grad_norm,
+                            skip_nonfinite=skip_nonfinite)
     return grad_norm if norm is None else norm
 
 
@@ -174,11 +183,10 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, lr, betas
     norm = _host.step(8, params, grads, exp_avgs, exp_avg_sqs, bases, steps, rate, betas[0], betas[1], eps,
                       weight_decay, maximize, max_norm, grad_norm, skip_nonfinite, lr_tensor, seed & 0xFFFFFFFF)
     if norm is NotImplemented:
-        return handle_torch_function(adamw8_step, (*params, *grads, *exp_avgs, *exp_avg_sqs, *bases, *steps, grad_norm,
-                                                   lr_tensor),
-                                     params, grads, exp_avgs, exp_avg_sqs, bases, steps, lr=lr, betas=betas, eps=eps,
-                                     weight_decay=weight_decay, maximize=maximize, max_norm=max_norm,
-                                     grad_norm=grad_norm, skip_nonfinite=skip_nonfinite, seed=seed)
+        return _handed_over(adamw8_step, (params, grads, exp_avgs, exp_avg_sqs, bases, steps, (grad_norm, lr_tensor)),
+                            params, grads, exp_avgs, exp_avg_sqs, bases, steps, lr=lr, betas=betas, eps=eps,
+                            weight_decay=weight_decay, maximize=maximize, max_norm=max_norm, grad_norm=grad_norm,
+                            skip_nonfinite=skip_nonfinite, seed=seed)
     return grad_norm if norm is None else norm
 
 
@@ -191,8 +199,8 @@ def adamw8_moments(exp_avgs, exp_avg_sqs, bases, out=None) -> tuple[list[Tensor]
         if torch.compiler.is_compiling():
             torch.ops.molix.adamw8_moments(exp_avgs, exp_avg_sqs, bases, *out)
         elif _host.moments(exp_avgs, exp_avg_sqs, bases, *out) is NotImplemented:
-            return handle_torch_function(adamw8_moments, (*exp_avgs, *exp_avg_sqs, *bases, *out[0], *out[1]), exp_avgs,
-                                         exp_avg_sqs, bases, out=out)
+            return _handed_over(adamw8_moments, (exp_avgs, exp_avg_sqs, bases, *out), exp_avgs, exp_avg_sqs, bases,
+                                out=out)
     return out
 
 
