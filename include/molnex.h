@@ -947,6 +947,44 @@ int mnx_adamw8_moments(const void* const* exp_avgs, const void* const* exp_avg_s
                        const int64_t* numel, int64_t count, float* const* out_avgs, float* const* out_avg_sqs,
                        mnx_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Orthogonalised updates (Muon) of `count` tensors, each `batch` matrices of  */
+/* rows x cols (contiguous); a matrix of no elements is left out.              */
+/*   m = momentum m + (1 - momentum) g  (g = -grad to maximise)                */
+/*   u = (1 - momentum) g + momentum m with nesterov, m without                */
+/*   X = u / max(|u|, eps) (Frobenius norm), transposed if rows > cols         */
+/*   steps times: A = X X^T, X = a X + (b A + c A A) X                         */
+/*   p = (1 - lr weight_decay) p - lr s X                                      */
+/* s = sqrt(max(1, rows / cols)) with adjust 0, 0.2 sqrt(max(rows, cols)) with */
+/* 1.  Parameters and gradients of one tensor share its dtype, momenta are     */
+/* float32.  bfloat16 matrices are iterated in float16 (scaled, float32 sums),  */
+/* others in pairs of it.  momenta NULL: u = grad, and X itself is        */
+/* written to params.  lr_device (or NULL) holds the learning rate in place of  */
+/* lr.  Coefficients under which singular values of [0, 1] grow past 64 are    */
+/* refused.  A matrix with an infinite or NaN entry becomes NaN.               */
+/* ------------------------------------------------------------------------ */
+#define MNX_MUON_MAX_SIDE 65536
+#define MNX_MUON_MAX_STEPS 100
+typedef struct mnx_muon_args {
+    int64_t count;
+    void* const* params;
+    const void* const* grads;
+    float* const* momenta;
+    const int64_t* batch;
+    const int64_t* rows;
+    const int64_t* cols;
+    const int32_t* dtype;
+    int32_t nesterov, maximize, adjust, steps;
+    double coefficients[3];
+    double lr, momentum, weight_decay, eps;
+    const float* lr_device;
+    void* workspace;
+    size_t workspace_bytes;
+} mnx_muon_args;
+/* 0 for arguments that the step refuses. */
+size_t mnx_muon_workspace_bytes(const mnx_muon_args* args);
+int mnx_muon_step(const mnx_muon_args* args, mnx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

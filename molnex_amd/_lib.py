@@ -163,6 +163,8 @@ SIGNATURES = {
     "mnx_adamw_workspace_bytes": (c_sz, [vp, c_i64]),
     "mnx_adamw_step": (C.c_int, [vp, vp]),
     "mnx_adamw8_moments": (C.c_int, [vp, vp, vp, vp, c_i64, vp, vp, vp]),
+    "mnx_muon_workspace_bytes": (c_sz, [vp]),
+    "mnx_muon_step": (C.c_int, [vp, vp]),
 }
 
 

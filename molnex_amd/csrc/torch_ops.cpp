@@ -21,6 +21,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <cmath>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -665,6 +667,212 @@ void adamw8_moments(at::TensorList exp_avgs, at::TensorList exp_avg_sqs, at::Ten
         for (const Tensor& t : l) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// ---------------------------------------------------------------------------
+// Orthogonalised updates
+// ---------------------------------------------------------------------------
+
+// A list's workspace is at most this, or one tensor's: longer lists take several calls.
+constexpr size_t kMuonWorkspace = size_t(4) << 30;
+
+// Whether memory that is written overlaps other memory of the call.  Tensors with gaps may interleave: of those only
+// the first address counts.
+class Overlap {
+  public:
+    void add(const Tensor& t, bool written) {
+        if (!t.numel()) return;
+        const auto lo = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+        const size_t length = t.is_non_overlapping_and_dense() ? t.numel() * t.element_size() : 1;
+        spans_.push_back({lo, lo + length, written});
+    }
+    bool found() {
+        std::sort(spans_.begin(), spans_.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+        uintptr_t any = 0, written = 0;
+        for (const Span& s : spans_) {
+            if (s.lo < (s.written ? any : written)) return true;
+            any = std::max(any, s.hi);
+            if (s.written) written = std::max(written, s.hi);
+        }
+        return false;
+    }
+
+  private:
+    struct Span {
+        uintptr_t lo, hi;
+        bool written;
+    };
+    std::vector<Span> spans_;
+};
+
+struct Iteration {
+    int64_t steps;
+    double a, b, c, eps;
+};
+
+void check_iteration(const char* name, const Iteration& it) {
+    TORCH_CHECK_VALUE(it.steps >= 1 && it.steps <= MNX_MUON_MAX_STEPS, "molix::", name, ": 1 to ", MNX_MUON_MAX_STEPS,
+                      " steps, got ", it.steps);
+    TORCH_CHECK_VALUE(it.eps >= 0 && std::isfinite(it.eps) && std::isfinite(it.a) && std::isfinite(it.b) &&
+                          std::isfinite(it.c),
+                      "molix::", name, ": coefficients (", it.a, ", ", it.b, ", ", it.c, "), eps ", it.eps);
+}
+
+void check_matrices(const char* name, const char* what, const Tensor& t) {
+    TORCH_CHECK_VALUE(t.dim() >= 2 && t.size(-1) <= MNX_MUON_MAX_SIDE && t.size(-2) <= MNX_MUON_MAX_SIDE, "molix::",
+                      name, ": ", what, " must be matrices (or stacks of them) with sides of at most ",
+                      MNX_MUON_MAX_SIDE, ", got ", t.sizes());
+}
+
+// The lists of one call, the tensors contiguous.
+struct MuonLists {
+    std::vector<void*> p;
+    std::vector<const void*> g;
+    std::vector<float*> m;
+    std::vector<int64_t> batch, rows, cols;
+    std::vector<int32_t> dtype;
+    void add(const Tensor& to, const Tensor& from, float* momentum) {
+        p.push_back(out(to));
+        g.push_back(from.numel() ? from.const_data_ptr() : nullptr);
+        m.push_back(momentum);
+        rows.push_back(from.size(-2));
+        cols.push_back(from.size(-1));
+        batch.push_back(from.numel() ? from.numel() / (from.size(-2) * from.size(-1)) : 0);
+        dtype.push_back(dtype_of(from.scalar_type()));
+    }
+};
+
+void muon_call(const char* name, const MuonLists& l, bool momenta, mnx_muon_args a, const Tensor& like) {
+    const auto part = [&](size_t at, size_t count) {
+        a.count = int64_t(count);
+        a.params = l.p.data() + at;
+        a.grads = l.g.data() + at;
+        a.momenta = momenta ? l.m.data() + at : nullptr;
+        a.batch = l.batch.data() + at;
+        a.rows = l.rows.data() + at;
+        a.cols = l.cols.data() + at;
+        a.dtype = l.dtype.data() + at;
+        const size_t bytes = mnx_muon_workspace_bytes(&a);
+        TORCH_CHECK(bytes, "molix::", name, ": ", mnx_last_error());
+        return bytes;
+    };
+    const auto step = [&](size_t at, size_t count) {
+        a.workspace_bytes = part(at, count);
+        Tensor ws = at::empty({int64_t(a.workspace_bytes)}, like.options().dtype(at::kByte).requires_grad(false));
+        a.workspace = out(ws);
+        check(mnx_muon_step(&a, stream_of(like)), name);
+    };
+    const size_t count = l.p.size();
+    if (!count) return;
+    if (part(0, count) <= kMuonWorkspace) return step(0, count);
+    for (size_t at = 0; at < count;) {
+        size_t n = 1, bytes = part(at, 1);
+        while (at + n < count && (bytes += part(at + n, 1)) <= kMuonWorkspace) ++n;
+        step(at, n);
+        at += n;
+    }
+}
+
+mnx_muon_args muon_args(const Iteration& it) {
+    mnx_muon_args a{};
+    a.steps = int32_t(it.steps);
+    a.coefficients[0] = it.a;
+    a.coefficients[1] = it.b;
+    a.coefficients[2] = it.c;
+    a.eps = it.eps;
+    return a;
+}
+
+Tensor orthogonalize(const Tensor& x, int64_t steps, double a, double b, double c, double eps) {
+    const char* name = "orthogonalize";
+    TORCH_CHECK(x.is_cuda(), "molix::", name, " runs on the GPU only (got a ", x.device(), " tensor)");
+    check_values(name, "matrices", x, x.device());
+    check_matrices(name, "x", x);
+    const Iteration it{steps, a, b, c, eps};
+    check_iteration(name, it);
+    const c10::DeviceGuard guard(x.device());
+    const Tensor from = x.contiguous();
+    Tensor y = at::empty(x.sizes(), x.options());
+    MuonLists l;
+    l.add(y, from, nullptr);
+    muon_call(name, l, false, muon_args(it), from);
+    return y;
+}
+
+Tensor orthogonalize_autograd(const Tensor& x, int64_t steps, double a, double b, double c, double eps) {
+    TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()) && !has_tangent(x),
+                "molix::orthogonalize is not differentiable: detach its tensor, or call it under no_grad");
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto o = op<decltype(orthogonalize)>("molix::orthogonalize");
+    return o.call(x, steps, a, b, c, eps);
+}
+
+void muon_step(at::TensorList params, at::TensorList grads, at::TensorList momenta, double lr, double momentum,
+               bool nesterov, double weight_decay, int64_t steps, double ca, double cb, double cc, double eps,
+               bool match_rms, bool maximize, const OptTensor& lr_tensor) {
+    const char* name = "muon_step";
+    const size_t count = params.size();
+    TORCH_CHECK_VALUE(grads.size() == count && momenta.size() == count, "molix::", name, ": lists of ", count, ", ",
+                      grads.size(), " and ", momenta.size(), " tensors");
+    const Iteration it{steps, ca, cb, cc, eps};
+    check_iteration(name, it);
+    TORCH_CHECK_VALUE(momentum >= 0 && momentum < 1, "molix::", name, ": momentum ", momentum);
+    if (!count) return;
+    const at::Device device = gpu_of(name, params);
+    const c10::DeviceGuard guard(device);
+    MuonLists l;
+    Overlap memory;
+    std::vector<Tensor> kept;
+    std::vector<std::pair<size_t, Tensor>> copies;  // of parameters that are not contiguous
+    for (size_t i = 0; i < count; ++i) {
+        const Tensor &p = params[i], &g = grads[i], &m = momenta[i];
+        check_values(name, "parameters", p, device);
+        check_matrices(name, "parameters", p);
+        TORCH_CHECK(g.layout() == at::kStrided, "molix::", name, ": sparse gradients are not supported");
+        TORCH_CHECK_VALUE(g.scalar_type() == p.scalar_type() && g.sizes() == p.sizes() && g.device() == device,
+                          "molix::", name, ": gradient ", i, " is ", g.scalar_type(), " ", g.sizes(), " on ",
+                          g.device(), ", its parameter ", p.scalar_type(), " ", p.sizes(), " on ", device);
+        TORCH_CHECK_VALUE(m.scalar_type() == at::kFloat && m.sizes() == p.sizes() && m.device() == device &&
+                              m.is_contiguous(),
+                          "molix::", name, ": momentum ", i, " must be contiguous float32 of its parameter's shape on ",
+                          device);
+        TORCH_CHECK_VALUE(at::has_internal_overlap(p) != at::MemOverlap::Yes, "molix::", name, ": parameter ", i,
+                          " has elements that share memory");
+        memory.add(p, true);
+        memory.add(m, true);
+        memory.add(g, false);
+        const Tensor *to = &p, *from = &g;
+        if (!p.is_contiguous()) {
+            copies.emplace_back(i, p.detach().contiguous());
+            kept.push_back(copies.back().second);
+            to = &copies.back().second;
+        }
+        if (!g.is_contiguous()) {
+            kept.push_back(g.detach().contiguous());
+            from = &kept.back();
+        }
+        l.add(*to, *from, static_cast<float*>(out(m)));
+    }
+    TORCH_CHECK_VALUE(!memory.found(), "molix::", name, ": parameters and momenta must not share memory with each "
+                                                        "other, nor with a gradient");
+    mnx_muon_args a = muon_args(it);
+    a.nesterov = nesterov;
+    a.maximize = maximize;
+    a.adjust = match_rms;
+    a.lr = lr;
+    a.momentum = momentum;
+    a.weight_decay = weight_decay;
+    Tensor rate;
+    if (given(lr_tensor)) {
+        TORCH_CHECK_VALUE(lr_tensor->numel() == 1 && lr_tensor->device() == device, "molix::", name,
+                          ": lr must be a number or one value on ", device);
+        rate = lr_tensor->detach().to(at::kFloat);
+        a.lr_device = rate.const_data_ptr<float>();
+    }
+    muon_call(name, l, true, a, params[0]);
+    for (const auto& [i, copy] : copies) params[i].detach().copy_(copy);
+    for (const at::TensorList& ts : {params, momenta})
+        for (const Tensor& t : ts) t.unsafeGetTensorImpl()->bump_version();
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(molix, m) {
@@ -689,6 +897,11 @@ TORCH_LIBRARY_FRAGMENT(molix, m) {
     m.def("adamw8_moments(Tensor[] exp_avgs, Tensor[] exp_avg_sqs, Tensor[] bases, Tensor(a!)[] out_avgs, "
           "Tensor(b!)[] out_avg_sqs) -> ()",
           tags);
+    m.def("orthogonalize(Tensor x, int steps, float a, float b, float c, float eps) -> Tensor", tags);
+    m.def("muon_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] momenta, float lr, float momentum, "
+          "bool nesterov, float weight_decay, int steps, float a, float b, float c, float eps, bool match_rms, "
+          "bool maximize, Tensor? lr_tensor) -> ()",
+          tags);
 }
 
 TORCH_LIBRARY_IMPL(molix, CUDA, m) {
@@ -699,6 +912,13 @@ TORCH_LIBRARY_IMPL(molix, CUDA, m) {
     m.impl("adamw_step", adamw_step);
     m.impl("adamw8_step", adamw8_step);
     m.impl("adamw8_moments", adamw8_moments);
+    m.impl("orthogonalize", orthogonalize);
+    m.impl("muon_step", muon_step);
+}
+
+TORCH_LIBRARY_IMPL(molix, CPU, m) {  // these say that they run on the GPU only
+    m.impl("orthogonalize", orthogonalize);
+    m.impl("muon_step", muon_step);
 }
 
 TORCH_LIBRARY_IMPL(molix, FuncTorchBatched, m) {  // torch.vmap
@@ -712,8 +932,9 @@ TORCH_LIBRARY_IMPL(molix, Autograd, m) {
     m.impl("layer_norm_backward", layer_norm_backward_autograd);
     m.impl("layer_norm_backward2", layer_norm_backward2_autograd);
     m.impl("grad_norm", grad_norm_autograd);
+    m.impl("orthogonalize", orthogonalize_autograd);
     // no gradients: they write into leaves, whose versions rise
-    for (const char* name : {"adamw_step", "adamw8_step", "adamw8_moments"})
+    for (const char* name : {"adamw_step", "adamw8_step", "adamw8_moments", "muon_step"})
         m.impl(name, torch::CppFunction::makeFallthrough());
 }
 
@@ -784,6 +1005,12 @@ OptTensor tensor_or_none(PyObject* o, const char* what, bool& overridden) {
 double number(PyObject* o) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) throw python_error();
+    return v;
+}
+
+int64_t integer(PyObject* o) {
+    const long long v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw python_error();
     return v;
 }
 
@@ -908,6 +1135,48 @@ PyObject* py_moments(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// (x, steps, a, b, c, eps)
+PyObject* py_orthogonalize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 6, "orthogonalize: 6 arguments, got ", n);
+    if (mode_on() || has_torch_function(a[0])) Py_RETURN_NOTIMPLEMENTED;
+    TORCH_CHECK_TYPE(THPVariable_Check(a[0]), "orthogonalize: a tensor, got ", Py_TYPE(a[0])->tp_name);
+    const Tensor& x = THPVariable_Unpack(a[0]);
+    const int64_t steps = integer(a[1]);
+    const double c0 = number(a[2]), c1 = number(a[3]), c2 = number(a[4]), eps = number(a[5]);
+    Tensor y;
+    {
+        Released r;
+        static auto o = op<decltype(orthogonalize)>("molix::orthogonalize");
+        y = o.call(x, steps, c0, c1, c2, eps);
+    }
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// (params, grads, momenta, lr, momentum, nesterov, weight_decay, steps, a, b, c, eps, match_rms, maximize, lr_tensor)
+PyObject* py_muon(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 15, "muon: 15 arguments, got ", n);
+    if (mode_on()) Py_RETURN_NOTIMPLEMENTED;
+    bool overridden = false;
+    const auto params = tensors(a[0], "parameters", overridden), grads = tensors(a[1], "gradients", overridden);
+    const auto momenta = tensors(a[2], "momenta", overridden);
+    const double lr = number(a[3]), mu = number(a[4]), wd = number(a[6]);
+    const bool nesterov = truth(a[5]), match = truth(a[12]), maximize = truth(a[13]);
+    const int64_t steps = integer(a[7]);
+    const double c0 = number(a[8]), c1 = number(a[9]), c2 = number(a[10]), eps = number(a[11]);
+    const OptTensor rate = tensor_or_none(a[14], "lr", overridden);
+    if (overridden) Py_RETURN_NOTIMPLEMENTED;
+    {
+        Released r;
+        static auto o = op<decltype(muon_step)>("molix::muon_step");
+        o.call(params, grads, momenta, lr, mu, nesterov, wd, steps, c0, c1, c2, eps, match, maximize, rate);
+    }
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
     {"step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_step)), METH_FASTCALL,
      "molix::adamw_step or adamw8_step; the norm, or None"},
@@ -916,6 +1185,9 @@ PyMethodDef kMethods[] = {
     {"grad_norm", py_grad_norm, METH_O, "molix::grad_norm"},
     {"moments", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_moments)), METH_FASTCALL,
      "molix::adamw8_moments"},
+    {"orthogonalize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_orthogonalize)), METH_FASTCALL,
+     "molix::orthogonalize"},
+    {"muon", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_muon)), METH_FASTCALL, "molix::muon_step"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "libmolnex_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr,

@@ -1,3 +1,4 @@
 from .adamw import AdamW
+from .muon import Muon
 
-__all__ = ["AdamW"]
+__all__ = ["AdamW", "Muon"]

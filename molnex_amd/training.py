@@ -88,6 +88,17 @@ def _(exp_avgs, exp_avg_sqs, bases, out_avgs, out_avg_sqs):
     return None
 
 
+@_fake("orthogonalize")
+def _(x, steps, a, b, c, eps):
+    return x.new_empty(x.shape)
+
+
+@_fake("muon_step")
+def _(params, grads, momenta, lr, momentum, nesterov, weight_decay, steps, a, b, c, eps, match_rms, maximize,
+      lr_tensor):
+    return None
+
+
 def dense(t: Tensor) -> bool:
     """Whether t's elements fill its part of memory, in any order of the axes (then it is stepped through as it
     lies)."""
@@ -242,3 +253,53 @@ def adamw8_relayout(exp_avg: Tensor, exp_avg_sq: Tensor, bases: Tensor, like: Te
     for t, values in zip(out, (m, v)):
         memory(t).copy_(values)
     return *out, torch.stack([base_m, base_v], 1).short()
+
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(x: Tensor, *, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7) -> Tensor:
+    """Newton-Schulz orthogonalisation of a matrix, or of each of a stack of them (..., m, n): with X = x / max(|x|, eps)
+    (Frobenius norm), transposed if m > n, and (a, b, c) the ``coefficients``, ``steps`` times
+    X <- a X + (b A + c A A) X, A = X X^T.  The singular values of the result lie near 1 (the usual coefficients: 0.7 to
+    1.2, those that began below 0.002 excepted).  A matrix of zeros stays so; one with an infinite or NaN entry becomes
+    NaN; coefficients under which the iteration grows past 64 are refused.
+
+    float32, bfloat16 or float16; bfloat16 matrices are iterated in scaled float16, others in pairs of it, with float32
+    sums.  Not differentiable.  GPU tensors only."""
+    a, b, c = coefficients
+    if torch.compiler.is_compiling():
+        return torch.ops.molix.orthogonalize(x, steps, a, b, c, eps)
+    y = _host.orthogonalize(x, steps, a, b, c, eps)
+    if y is NotImplemented:
+        return handle_torch_function(orthogonalize, (x,), x, steps=steps, coefficients=coefficients, eps=eps)
+    return y
+
+
+_ADJUST = {"original": False, "match_rms_adamw": True}
+
+
+def muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weight_decay=0.1, steps=5,
+              coefficients=NEWTON_SCHULZ, eps=1e-7, adjust="original", maximize=False) -> None:
+    """One Muon step over lists of matrices (or stacks of them, whose leading axes count matrices), in place: parameters
+    (float32, bfloat16 or float16) with gradients of their type and contiguous float32 ``momenta`` of their shape.
+
+    m = momentum m + (1 - momentum) grad; u = (1 - momentum) grad + momentum m, or m without ``nesterov``;
+    p = (1 - lr weight_decay) p - lr s ``orthogonalize(u)``, with s = sqrt(max(1, rows / columns)) ("original") or
+    0.2 sqrt(max(rows, columns)) ("match_rms_adamw").  ``lr`` may be a tensor on the device.  Nothing synchronises, and
+    the call can be captured in a graph.  Memory that is written may not be given twice."""
+    if adjust not in _ADJUST:
+        raise ValueError(f"molix.muon_step: adjust {adjust!r}, one of {', '.join(_ADJUST)}")
+    if not params:
+        if grads or momenta:
+            raise ValueError("molix.muon_step: no parameters, but other tensors")
+        return
+    rate, lr_tensor = _rate(lr)
+    a, b, c = coefficients
+    args = (rate, momentum, nesterov, weight_decay, steps, a, b, c, eps, _ADJUST[adjust], maximize, lr_tensor)
+    if torch.compiler.is_compiling():
+        torch.ops.molix.muon_step(params, grads, momenta, *args)
+    elif _host.muon(params, grads, momenta, *args) is NotImplemented:
+        _handed_over(muon_step, (params, grads, momenta, (lr_tensor,)), params, grads, momenta, lr=lr,
+                     momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                     coefficients=coefficients, eps=eps, adjust=adjust, maximize=maximize)
