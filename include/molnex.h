@@ -985,6 +985,27 @@ typedef struct mnx_muon_args {
 size_t mnx_muon_workspace_bytes(const mnx_muon_args* args);
 int mnx_muon_step(const mnx_muon_args* args, mnx_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Indexed linear map: rows times the weights of their class (per-element      */
+/* weights, src/molrep/interaction/element_update.py:101-109, of any width and  */
+/* of 16-bit types).  order and class_start: mnx_class_groups of the rows'      */
+/* classes.  weight [classes][in][out] contiguous; a has `rows` rows lda apart. */
+/*   result[i] = a[i] weight[class of i]          (rows x out), or              */
+/*   result[i] = a[i] weight[class of i]^T        (rows x in) if transposed     */
+/* rows of no class become zero.  wgrad: grad_weight[s] = sum over the rows of  */
+/* class s of x[i]^T grad[i], in a fixed order.  All arrays are of type dtype,  */
+/* sums float32.                                                                */
+/* ------------------------------------------------------------------------ */
+#define MNX_INDEXED_MAX_WIDTH 65536
+int mnx_indexed_linear(const void* a, int64_t lda, int64_t rows, const int32_t* order, const int32_t* class_start,
+                       int32_t classes, const void* weight, int64_t in, int64_t out, int32_t dtype, int32_t transposed,
+                       void* result, mnx_stream_t stream);
+size_t mnx_indexed_linear_wgrad_workspace_bytes(int64_t rows, int32_t classes, int64_t in, int64_t out);
+int mnx_indexed_linear_wgrad(const void* x, int64_t ldx, const void* grad, int64_t ldg, int64_t rows,
+                             const int32_t* order, const int32_t* class_start, int32_t classes, int64_t in,
+                             int64_t out, int32_t dtype, void* grad_weight, void* workspace, size_t workspace_bytes,
+                             mnx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,532 @@
+// The indexed linear map: rows multiplied with the weights of their class, ragged groups in one launch.
+//
+//   y[i] = x[i] W[z[i]]            W (S, K, N): one K x N matrix a class; a row out of range gets zeros
+//   gx[i] = g[i] W[z[i]]^T
+//   gw[s] = sum over the rows i of class s of x[i]^T g[i]
+//
+// The rows of a class are found through `order` (row numbers by class, those out of range last) and `class_start`
+// (mnx_class_groups): they are read and written in place, with no sorted copy.  The grid is sized for the worst case
+// (a partial tile per class) and surplus workgroups leave at once, so nothing synchronises.
+//
+// A workgroup forms a 128 x BN tile.  Both operands pass through registers into LDS, the next chunk's loads in flight
+// under this one's products; vectors of 16 bytes at the alignment of one element, so any width and row distance will
+// do.  An operand whose sum index is contiguous in memory lies in LDS by rows and is read 16 bytes a lane; one whose
+// rows are the sum index (W in the forward, x and g in the weights' gradient) lies as it is in memory too and is read
+// with the transposing LDS load.  16-bit types go to the matrix cores as they are; float32 is split into three bfloat16
+// parts on the way into LDS, of whose nine products the six above 2^-24 are formed, smallest first, so that products
+// are as exact as float32's whatever the values' range.  Sums are float32.
+//
+// The weights' gradient sums a class's rows in slices of `slice` rows; a class of several leaves partial sums in the
+// workspace, which a second kernel adds in order: the same bits every time.
+#include "bf16_split.h"
+#include "elem.h"
+
+namespace mnx {
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr int kBM = 128;
+
+enum { kForward = 0, kGradX = 1 };
+
+template <int DT>
+struct Kind {
+    static constexpr int planes = DT == kF32 ? 3 : 1;
+    static constexpr int kc = DT == kF32 ? 32 : 64;  // sum indices of a chunk
+    static constexpr int vec = DT == kF32 ? 4 : 8;   // elements of 16 bytes
+    typedef typename Elem<DT>::T T;
+    typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+};
+
+template <int DT>
+__device__ __forceinline__ f32x16 mfma(const short8v& a, const short8v& b, const f32x16& c) {
+    if constexpr (DT == kF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+// `left` elements of a vector at p; zeros behind them.
+template <int DT>
+__device__ __forceinline__ f32x4 load_vec(const typename Kind<DT>::T* p, int left) {
+    constexpr int V = Kind<DT>::vec;
+    typename Kind<DT>::Vec v;
+    if (left >= V) {
+        v = *reinterpret_cast<const typename Kind<DT>::Vec*>(p);
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = e < left ? p[e] : typename Kind<DT>::T(0);
+    }
+    return __builtin_bit_cast(f32x4, v);
+}
+
+// A vector into LDS at element `at` of every plane.
+template <int DT>
+__device__ __forceinline__ void store_vec(short* lds, int plane, int at, const f32x4& v) {
+    if constexpr (DT == kF32) {
+        uint32_t p[3][2];
+        bf16_split2(v[0], v[1], p[0][0], p[1][0], p[2][0]);
+        bf16_split2(v[2], v[3], p[0][1], p[1][1], p[2][1]);
+        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<u2*>(lds + k * plane + at) = u2{p[k][0], p[k][1]};
+    } else {
+        *reinterpret_cast<f32x4*>(lds + at) = v;
+    }
+}
+
+// Where element (row, k) of an operand by rows lies in LDS, KC a row: 16-byte pieces permuted so that 16 rows' pieces
+// of one k meet every bank once.
+template <int KC>
+__device__ __forceinline__ int by_rows(int row, int k) {
+    const int turn = KC == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+    return row * KC + ((((k >> 3) ^ turn) << 3) | (k & 7));
+}
+// ... and element (k, col) of one whose rows are the sum index, W columns a row: 4 rows' 64 bytes meet every bank once.
+template <int W>
+__device__ __forceinline__ int by_sums(int k, int col) {
+    const int turn = W == 128 ? (k & 3) << 2 : ((k >> 1) & 1) << 2;
+    return k * W + ((((col >> 3) ^ turn) << 3) | (col & 7));
+}
+
+// The matrix cores' operand of 32 rows from row0, sum indices k0 to k0 + 15.
+template <int KC>
+__device__ __forceinline__ short8v read_rows(const short* lds, int row0, int k0) {
+    const int lane = threadIdx.x & 63;
+    return *reinterpret_cast<const short8v*>(lds + by_rows<KC>(row0 + (lane & 31), k0 + 8 * (lane >> 5)));
+}
+// ... of 32 columns from col0: the load hands lane l of 16 the four k of column l from four rows of 16 columns.
+template <int W>
+__device__ __forceinline__ short8v read_sums(const short* lds, int col0, int k0) {
+    const int lane = threadIdx.x & 63;
+    const int k = k0 + 8 * (lane >> 5) + ((lane & 15) >> 2), col = col0 + (lane & 16) + (lane & 3) * 4;
+    typedef __attribute__((address_space(3))) short4v* P;
+    const short* q = lds + by_sums<W>(k, col);
+    const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)q);
+    const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(q + 4 * W));  // k + 4 turns alike
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Which class workgroup `unit` serves, when a class of n rows has units(n) of them: the class, the unit's number in it,
+// and the sum of extra(n) over the classes before.  cls = classes if it is surplus.  Every lane of a wavefront takes part.
+struct Found {
+    int cls, unit, extra;
+};
+// (Positions and row numbers are kept in [0, rows], whatever the caller's plan holds.)
+struct Plan {
+    const int32_t* order;
+    const int32_t* class_start;
+    int32_t rows, classes;
+    __device__ __forceinline__ int start(int c) const { return min(max(class_start[c], 0), rows); }
+    __device__ __forceinline__ int count(int c) const { return max(start(c + 1) - start(c), 0); }
+    __device__ __forceinline__ int row(int at) const { return min(max(order[at], 0), rows - 1); }
+};
+template <typename U, typename E>
+__device__ __forceinline__ Found find_class(const Plan& plan, int classes, int unit, U units, E extra) {
+    const int lane = threadIdx.x & 63;
+    int before = 0, more = 0;
+    for (int base = 0; base < classes; base += 64) {
+        const int c = base + lane;
+        const int n = c < classes ? plan.count(c) : 0;
+        const int mine = c < classes ? units(n) : 0, own = c < classes ? extra(n) : 0;
+        int sum = mine, esum = own;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int s = __shfl_up(sum, d), t = __shfl_up(esum, d);
+            if (lane >= d) {
+                sum += s;
+                esum += t;
+            }
+        }
+        const uint64_t past = __ballot(before + sum > unit);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            return {__builtin_amdgcn_readfirstlane(base + at),
+                    __builtin_amdgcn_readfirstlane(unit - before - __shfl(sum - mine, at)),
+                    __builtin_amdgcn_readfirstlane(more + __shfl(esum - own, at))};
+        }
+        before += __shfl(sum, 63);
+        more += __shfl(esum, 63);
+    }
+    return {classes, 0, 0};
+}
+
+template <int DT, int MT, int NT>
+__device__ __forceinline__ void clear(f32x16 (&acc)[MT][NT]) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) acc[m][n][q] = 0.f;
+}
+
+// The products of one chunk's 16 sum indices, fragments of every plane read.
+template <int DT, int MT, int NT>
+__device__ __forceinline__ void multiply(const short8v (&a)[Kind<DT>::planes][MT], const short8v (&b)[Kind<DT>::planes][NT],
+                                         f32x16 (&acc)[MT][NT]) {
+    constexpr int PA[6] = {2, 1, 0, 1, 0, 0}, PB[6] = {0, 1, 2, 0, 1, 0};
+    constexpr int Z = Kind<DT>::planes == 3 ? 6 : 1;
+#pragma unroll
+    for (int z = 0; z < Z; ++z)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                acc[m][n] = mfma<DT>(a[Z == 6 ? PA[z] : 0][m], b[Z == 6 ? PB[z] : 0][n], acc[m][n]);
+}
+
+struct RowsArgs {
+    const void* a;  // x or g: rows of `sums` values, lda apart
+    const void* w;
+    void* out;      // rows of `cols` values
+    int64_t lda;
+    Plan plan;
+    int32_t sums, cols, col_tiles;
+    uint32_t units;
+};
+
+// y or gx: 128 rows of one class against BN columns.
+template <int DT, int DIR, int BN>
+__global__ void __launch_bounds__(kThreads) k_indexed_rows(RowsArgs p) {
+    using T = typename Kind<DT>::T;
+    constexpr int KC = Kind<DT>::kc, V = Kind<DT>::vec, PL = Kind<DT>::planes;
+    constexpr int NA = kBM * KC / V / kThreads, NB = BN * KC / V / kThreads;  // vectors a thread
+    constexpr int VR = KC / V;       // vectors of a row's chunk
+    constexpr int VC = BN / V;       // vectors of a sum index's columns
+    constexpr int WN = BN / 2, MT = 2, NT = WN / 32;
+    __shared__ short sA[PL * kBM * KC], sB[PL * BN * KC];
+    __shared__ int32_t rows[kBM];
+    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // Column tiles of the same rows, and then rows of the same class, side by side on one XCD
+    const uint32_t per = (p.units + 7) / 8, u = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (u >= p.units) return;
+    const int row_tile = int(u / uint32_t(p.col_tiles)), col0 = int(u % uint32_t(p.col_tiles)) * BN;
+    const int classes = p.plan.classes;
+    const Found f = find_class(p.plan, classes + 1, row_tile, [](int n) { return (n + kBM - 1) / kBM; },
+                               [](int) { return 0; });
+    if (f.cls > classes) return;
+    const int first = p.plan.start(f.cls) + f.unit * kBM;
+    const int count = min(kBM, p.plan.start(f.cls + 1) - first);  // at least 1
+    for (int i = tid; i < kBM; i += kThreads) rows[i] = p.plan.row(first + min(i, count - 1));
+    __syncthreads();
+    const int K = f.cls == classes ? 0 : p.sums;  // zeros for rows out of range
+    const T* W = static_cast<const T*>(p.w) + (f.cls == classes ? 0 : int64_t(f.cls) * p.sums * p.cols);
+    const T* A = static_cast<const T*>(p.a);
+
+    const T* arow[NA];
+#pragma unroll
+    for (int i = 0; i < NA; ++i) arow[i] = A + int64_t(rows[(tid + i * kThreads) / VR]) * p.lda;
+    f32x4 va[NA], vb[NB];
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int k = k0 + (tid % VR) * V;
+            va[i] = load_vec<DT>(arow[i] + k, K - k);
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int it = tid + i * kThreads;
+            if constexpr (DIR == kForward) {
+                const int k = k0 + it / VC, c = col0 + (it % VC) * V;
+                vb[i] = load_vec<DT>(W + int64_t(k) * p.cols + c, k < K ? p.cols - c : 0);
+            } else {
+                const int c = col0 + it / VR, k = k0 + (it % VR) * V;
+                vb[i] = load_vec<DT>(W + int64_t(c) * p.sums + k, c < p.cols ? K - k : 0);
+            }
+        }
+    };
+    auto put = [&]() {
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            store_vec<DT>(sA, kBM * KC, by_rows<KC>((tid + i * kThreads) / VR, (tid % VR) * V), va[i]);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int it = tid + i * kThreads;
+            if constexpr (DIR == kForward) store_vec<DT>(sB, BN * KC, by_sums<BN>(it / VC, (it % VC) * V), vb[i]);
+            else store_vec<DT>(sB, BN * KC, by_rows<KC>(it / VR, (it % VR) * V), vb[i]);
+        }
+    };
+    f32x16 acc[MT][NT];
+    clear<DT>(acc);
+    const int wm = wave & 1, wn = wave >> 1;
+    if (K > 0) load(0);
+    for (int k0 = 0; k0 < K; k0 += KC) {
+        __syncthreads();
+        put();
+        __syncthreads();
+        if (k0 + KC < K) load(k0 + KC);
+#pragma unroll
+        for (int ks = 0; ks < KC; ks += 16) {
+            short8v a[PL][MT], b[PL][NT];
+#pragma unroll
+            for (int pl = 0; pl < PL; ++pl) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m) a[pl][m] = read_rows<KC>(sA + pl * kBM * KC, wm * 64 + m * 32, ks);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    b[pl][n] = DIR == kForward ? read_sums<BN>(sB + pl * BN * KC, wn * WN + n * 32, ks)
+                                               : read_rows<KC>(sB + pl * BN * KC, wn * WN + n * 32, ks);
+            }
+            multiply<DT, MT, NT>(a, b, acc);
+        }
+    }
+    // acc[m][n][q]: row 32 m + 8 (q / 4) + 4 half + q % 4, column 32 n + l32 of the wave's tile
+    T* out = static_cast<T*>(p.out);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            const int r = wm * 64 + m * 32 + 8 * (q / 4) + 4 * half + q % 4;
+            if (r >= count) continue;
+            T* to = out + int64_t(rows[r]) * p.cols;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int c = col0 + wn * WN + n * 32 + l32;
+                if (c < p.cols) to[c] = T(acc[m][n][q]);
+            }
+        }
+}
+
+struct WeightArgs {
+    const void* x;
+    const void* g;
+    void* gw;
+    float* part;
+    int64_t ldx, ldg;
+    Plan plan;
+    int32_t K, N, kt, nt, slice;
+    uint32_t units;
+};
+
+__device__ __forceinline__ int slices(int n, int slice) { return n > slice ? (n + slice - 1) / slice : 1; }
+__device__ __forceinline__ int slots(int n, int slice) { return n > slice ? (n + slice - 1) / slice : 0; }
+
+// A 128 x 128 tile of one class's gradient over one slice of its rows.
+template <int DT>
+__global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
+    using T = typename Kind<DT>::T;
+    constexpr int KC = Kind<DT>::kc, V = Kind<DT>::vec, PL = Kind<DT>::planes;
+    constexpr int VC = kBM / V, NV = kBM * KC / V / kThreads, STEP = kThreads / VC;
+    __shared__ short sA[PL * kBM * KC], sB[PL * kBM * KC];
+    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t per = (p.units + 7) / 8, u = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (u >= p.units) return;
+    const uint32_t tiles = uint32_t(p.kt) * uint32_t(p.nt);
+    const int slice_at = int(u / tiles), tile = int(u % tiles);
+    const int k0 = tile / p.nt * kBM, n0 = tile % p.nt * kBM;
+    const int slice = p.slice;
+    const Found f = find_class(p.plan, p.plan.classes, slice_at, [=](int n) { return slices(n, slice); },
+                               [=](int n) { return slots(n, slice); });
+    if (f.cls >= p.plan.classes) return;
+    const int lo = p.plan.start(f.cls), n_class = p.plan.count(f.cls);
+    const int begin = lo + f.unit * slice, end = lo + min(n_class, (f.unit + 1) * slice);
+    const T *X = static_cast<const T*>(p.x), *G = static_cast<const T*>(p.g);
+    const int col = (tid % VC) * V, krow = tid / VC;
+
+    f32x4 va[NV], vb[NV];
+    int row[NV];
+    auto find_rows = [&](int r0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int at = r0 + krow + i * STEP;
+            row[i] = at < end ? p.plan.row(at) : -1;
+        }
+    };
+    auto load = [&]() {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t r = max(row[i], 0);
+            va[i] = load_vec<DT>(X + r * p.ldx + k0 + col, row[i] >= 0 ? p.K - k0 - col : 0);
+            vb[i] = load_vec<DT>(G + r * p.ldg + n0 + col, row[i] >= 0 ? p.N - n0 - col : 0);
+        }
+    };
+    f32x16 acc[2][2];
+    clear<DT>(acc);
+    const int wm = wave & 1, wn = wave >> 1;
+    if (begin < end) {
+        find_rows(begin);
+        load();
+        find_rows(begin + KC);
+    }
+    for (int r0 = begin; r0 < end; r0 += KC) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            store_vec<DT>(sA, kBM * KC, by_sums<kBM>(krow + i * STEP, col), va[i]);
+            store_vec<DT>(sB, kBM * KC, by_sums<kBM>(krow + i * STEP, col), vb[i]);
+        }
+        __syncthreads();
+        if (r0 + KC < end) {
+            load();
+            find_rows(r0 + 2 * KC);
+        }
+#pragma unroll
+        for (int ks = 0; ks < KC; ks += 16) {
+            short8v a[PL][2], b[PL][2];
+#pragma unroll
+            for (int pl = 0; pl < PL; ++pl)
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    a[pl][m] = read_sums<kBM>(sA + pl * kBM * KC, wm * 64 + m * 32, ks);
+                    b[pl][m] = read_sums<kBM>(sB + pl * kBM * KC, wn * 64 + m * 32, ks);
+                }
+            multiply<DT, 2, 2>(a, b, acc);
+        }
+    }
+    const bool whole = n_class <= slice;
+    T* out = static_cast<T*>(p.gw) + int64_t(f.cls) * p.K * p.N;
+    float* part = p.part + (whole ? 0 : int64_t(f.extra + f.unit) * p.K * p.N);
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            const int k = k0 + wm * 64 + m * 32 + 8 * (q / 4) + 4 * half + q % 4;
+            if (k >= p.K) continue;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int c = n0 + wn * 64 + n * 32 + l32;
+                if (c >= p.N) continue;
+                if (whole) out[int64_t(k) * p.N + c] = T(acc[m][n][q]);
+                else part[int64_t(k) * p.N + c] = acc[m][n][q];
+            }
+        }
+}
+
+// The partial sums of the classes with several slices, added in order.
+template <int DT>
+__global__ void __launch_bounds__(kThreads) k_indexed_join(WeightArgs p) {
+    using T = typename Kind<DT>::T;
+    const int cls = blockIdx.y, slice = p.slice;
+    const int n = p.plan.count(cls);
+    if (n <= slice) return;
+    // the class's own first unit: the scan's answer for it
+    int before = 0;
+    for (int c = int(threadIdx.x & 63); c < cls; c += 64) before += slots(p.plan.count(c), slice);
+    for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d);
+    const int count = slots(n, slice);
+    const int64_t size = int64_t(p.K) * p.N;
+    const float* part = p.part + before * size;
+    T* out = static_cast<T*>(p.gw) + cls * size;
+    for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < size; e += int64_t(gridDim.x) * kThreads) {
+        float sum = part[e];
+        for (int s = 1; s < count; ++s) sum += part[s * size + e];
+        out[e] = T(sum);
+    }
+}
+
+int check_shape(const char* what, int64_t rows, int32_t classes, int64_t in, int64_t out, int32_t dtype) {
+    MNX_REQUIRE(elem_valid(dtype), "%s: unknown type %d", what, dtype);
+    MNX_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) - 65536, "%s: %lld rows", what, (long long)rows);
+    MNX_REQUIRE(classes >= 1 && classes <= MNX_CLASS_GROUPS_MAX_CLASSES, "%s: 1 to %d classes, got %d", what,
+                MNX_CLASS_GROUPS_MAX_CLASSES, classes);
+    MNX_REQUIRE(in >= 1 && out >= 1 && in <= MNX_INDEXED_MAX_WIDTH && out <= MNX_INDEXED_MAX_WIDTH,
+                "%s: widths of 1 to %d, got %lld and %lld", what, MNX_INDEXED_MAX_WIDTH, (long long)in, (long long)out);
+    return MNX_OK;
+}
+
+template <int DT>
+int rows_product(int dir, RowsArgs p, int64_t rows, mnx_stream_t stream) {
+    const int BN = p.cols <= 64 ? 64 : 128;
+    p.col_tiles = int32_t(ceil_div(p.cols, BN));
+    const int64_t row_tiles = rows / kBM + std::min<int64_t>(rows, p.plan.classes + 1);
+    const int64_t units = row_tiles * p.col_tiles;
+    MNX_REQUIRE(units < (int64_t(1) << 23), "indexed linear: too many rows and columns for one call");
+    p.units = uint32_t(units);
+    const uint32_t grid = uint32_t(ceil_div(units, 8) * 8);
+    if (dir == kForward) {
+        if (BN == 64) k_indexed_rows<DT, kForward, 64><<<grid, kThreads, 0, stream>>>(p);
+        else k_indexed_rows<DT, kForward, 128><<<grid, kThreads, 0, stream>>>(p);
+    } else {
+        if (BN == 64) k_indexed_rows<DT, kGradX, 64><<<grid, kThreads, 0, stream>>>(p);
+        else k_indexed_rows<DT, kGradX, 128><<<grid, kThreads, 0, stream>>>(p);
+    }
+    MNX_CHECK_LAUNCH();
+    return MNX_OK;
+}
+
+// Rows of a slice: enough slices for the card where the tiles of one gradient are few.
+int64_t slice_rows(int64_t rows, int64_t K, int64_t N) {
+    const int64_t tiles = ceil_div(K, kBM) * ceil_div(N, kBM);
+    const int64_t want = std::max<int64_t>(1, 1024 / tiles);
+    return std::max<int64_t>(256, ceil_div(ceil_div(std::max<int64_t>(rows, 1), want), 64) * 64);
+}
+
+template <int DT>
+int weights_product(WeightArgs p, int64_t rows, mnx_stream_t stream) {
+    p.kt = int32_t(ceil_div(p.K, kBM));
+    p.nt = int32_t(ceil_div(p.N, kBM));
+    const int64_t units = (rows / p.slice + p.plan.classes) * p.kt * p.nt;
+    MNX_REQUIRE(units < (int64_t(1) << 23), "indexed linear: too many classes and columns for one call");
+    p.units = uint32_t(units);
+    k_indexed_weights<DT><<<uint32_t(ceil_div(units, 8) * 8), kThreads, 0, stream>>>(p);
+    MNX_CHECK_LAUNCH();
+    if (rows > p.slice) {
+        const uint32_t blocks = uint32_t(std::min<int64_t>(ceil_div(int64_t(p.K) * p.N, kThreads), 2048));
+        k_indexed_join<DT><<<dim3(blocks, uint32_t(p.plan.classes)), kThreads, 0, stream>>>(p);
+        MNX_CHECK_LAUNCH();
+    }
+    return MNX_OK;
+}
+
+}  // namespace
+}  // namespace mnx
+
+using namespace mnx;
+
+extern "C" {
+
+int mnx_indexed_linear(const void* a, int64_t lda, int64_t rows, const int32_t* order, const int32_t* class_start,
+                       int32_t classes, const void* weight, int64_t in, int64_t out, int32_t dtype, int32_t transposed,
+                       void* result, mnx_stream_t stream) {
+    clear_error();
+    if (int rc = check_shape("indexed linear", rows, classes, in, out, dtype)) return rc;
+    MNX_REQUIRE(lda >= (transposed ? out : in), "indexed linear: rows of %lld values %lld apart",
+                (long long)(transposed ? out : in), (long long)lda);
+    if (rows == 0) return MNX_OK;
+    MNX_REQUIRE(a && order && class_start && weight && result, "indexed linear: null pointer");
+    RowsArgs p{a, weight, result, lda, Plan{order, class_start, int32_t(rows), classes},
+               int32_t(transposed ? out : in), int32_t(transposed ? in : out), 0, 0};
+    const int dir = transposed ? kGradX : kForward;
+    if (dtype == kF32) return rows_product<kF32>(dir, p, rows, stream);
+    if (dtype == kBF16) return rows_product<kBF16>(dir, p, rows, stream);
+    return rows_product<kF16>(dir, p, rows, stream);
+}
+
+size_t mnx_indexed_linear_wgrad_workspace_bytes(int64_t rows, int32_t classes, int64_t in, int64_t out) {
+    if (check_shape("indexed linear", rows, classes, in, out, kF32)) return 0;
+    // a class of several slices has at most twice its share of them
+    const int64_t slice = slice_rows(rows, in, out);
+    if (rows <= slice) return 0;
+    return size_t(std::min(2 * (rows / slice), rows / slice + classes)) * size_t(in) * size_t(out) * sizeof(float);
+}
+
+int mnx_indexed_linear_wgrad(const void* x, int64_t ldx, const void* grad, int64_t ldg, int64_t rows,
+                             const int32_t* order, const int32_t* class_start, int32_t classes, int64_t in, int64_t out,
+                             int32_t dtype, void* grad_weight, void* workspace, size_t workspace_bytes,
+                             mnx_stream_t stream) {
+    clear_error();
+    if (int rc = check_shape("indexed linear", rows, classes, in, out, dtype)) return rc;
+    MNX_REQUIRE(ldx >= in && ldg >= out, "indexed linear: rows of %lld and %lld values %lld and %lld apart",
+                (long long)in, (long long)out, (long long)ldx, (long long)ldg);
+    MNX_REQUIRE(class_start && grad_weight && (rows == 0 || (x && grad && order)), "indexed linear: null pointer");
+    const size_t need = mnx_indexed_linear_wgrad_workspace_bytes(rows, classes, in, out);
+    if (need && (!workspace || workspace_bytes < need))
+        return set_error(MNX_ERR_WORKSPACE, "indexed linear: workspace too small");
+    WeightArgs p{x, grad, grad_weight, static_cast<float*>(workspace), ldx, ldg,
+                 Plan{order, class_start, int32_t(rows), classes}, int32_t(in), int32_t(out), 0, 0,
+                 int32_t(std::min<int64_t>(slice_rows(rows, in, out), INT32_MAX / 2)), 0};
+    if (dtype == kF32) return weights_product<kF32>(p, rows, stream);
+    if (dtype == kBF16) return weights_product<kBF16>(p, rows, stream);
+    return weights_product<kF16>(p, rows, stream);
+}
+
+}  // extern "C"

@@ -873,6 +873,175 @@ void muon_step(at::TensorList params, at::TensorList grads, at::TensorList momen
         for (const Tensor& t : ts) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// ---------------------------------------------------------------------------
+// Indexed linear map
+// ---------------------------------------------------------------------------
+
+struct Grouped {
+    int64_t rows;
+    int32_t classes;
+};
+
+// Checks the rows' plan (class_groups: order, starts) against `rows`.
+Grouped check_groups(const char* name, const Tensor& order, const Tensor& starts, const Tensor& x) {
+    for (const Tensor* t : {&order, &starts})
+        TORCH_CHECK_VALUE(t->scalar_type() == at::kInt && t->dim() == 1 && t->is_contiguous() &&
+                              t->device() == x.device(),
+                          "molix::", name, ": groups are two contiguous int32 vectors on x's device (class_groups)");
+    TORCH_CHECK_VALUE(order.size(0) == x.size(0), "molix::", name, ": groups of ", order.size(0), " rows for ",
+                      x.size(0));
+    const int64_t classes = starts.size(0) - 2;
+    TORCH_CHECK_VALUE(classes >= 1 && classes <= MNX_CLASS_GROUPS_MAX_CLASSES, "molix::", name, ": 1 to ",
+                      MNX_CLASS_GROUPS_MAX_CLASSES, " classes, got ", classes);
+    return {x.size(0), int32_t(classes)};
+}
+
+void check_rows(const char* name, const char* what, const Tensor& x) {
+    TORCH_CHECK(x.is_cuda(), "molix::", name, " runs on the GPU only (got a ", x.device(), " tensor)");
+    TORCH_CHECK(x.layout() == at::kStrided, "molix::", name, ": ", what, " must be dense, got ", x.layout());
+    TORCH_CHECK_TYPE(dtype_of(x.scalar_type()) >= 0, "molix::", name, ": ", what,
+                     " float32, bfloat16 or float16, got ", x.scalar_type());
+    TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) >= 1 && x.size(1) <= MNX_INDEXED_MAX_WIDTH, "molix::", name, ": ", what,
+                      " must be (rows, width) of at most ", MNX_INDEXED_MAX_WIDTH, " columns, got ", x.sizes());
+}
+
+Tensor indexed_linear(const Tensor& x, const Tensor& weight, const Tensor& order, const Tensor& starts,
+                      bool transposed) {
+    const char* name = "indexed_linear";
+    check_rows(name, "x", x);
+    const Grouped n = check_groups(name, order, starts, x);
+    TORCH_CHECK_VALUE(weight.dim() == 3 && weight.size(0) == n.classes && weight.size(transposed ? 2 : 1) == x.size(1) &&
+                          weight.size(transposed ? 1 : 2) >= 1 &&
+                          weight.size(transposed ? 1 : 2) <= MNX_INDEXED_MAX_WIDTH,
+                      "molix::", name, ": weight must be (", n.classes, ", in, out) for x ", x.sizes(), ", got ",
+                      weight.sizes());
+    TORCH_CHECK_TYPE(weight.scalar_type() == x.scalar_type() && weight.device() == x.device(), "molix::", name,
+                     ": weight is ", weight.scalar_type(), " on ", weight.device(), ", x ", x.scalar_type(), " on ",
+                     x.device());
+    const c10::DeviceGuard guard(x.device());
+    const Rows a(x, x.size(1));
+    const Tensor w = weight.contiguous();
+    const int64_t in = w.size(1), cols = w.size(2);
+    Tensor y = at::empty({n.rows, transposed ? in : cols}, x.options().requires_grad(false));
+    check(mnx_indexed_linear(a.ptr(), a.ld, n.rows, order.const_data_ptr<int32_t>(), starts.const_data_ptr<int32_t>(),
+                             n.classes, w.const_data_ptr(), in, cols, dtype_of(x.scalar_type()), transposed, out(y),
+                             stream_of(x)),
+          name);
+    return y;
+}
+
+Tensor indexed_linear_wgrad(const Tensor& x, const Tensor& grad, const Tensor& order, const Tensor& starts) {
+    const char* name = "indexed_linear_wgrad";
+    check_rows(name, "x", x);
+    check_rows(name, "grad", grad);
+    const Grouped n = check_groups(name, order, starts, x);
+    TORCH_CHECK_VALUE(grad.size(0) == n.rows && grad.scalar_type() == x.scalar_type() && grad.device() == x.device(),
+                      "molix::", name, ": grad ", grad.scalar_type(), " ", grad.sizes(), " for x ", x.scalar_type(),
+                      " ", x.sizes());
+    const c10::DeviceGuard guard(x.device());
+    const int64_t in = x.size(1), cols = grad.size(1);
+    const Rows a(x, in), g(grad, cols);
+    Tensor gw = at::empty({n.classes, in, cols}, x.options().requires_grad(false)), ws;
+    const size_t bytes = mnx_indexed_linear_wgrad_workspace_bytes(n.rows, n.classes, in, cols);
+    if (bytes) ws = at::empty({int64_t(bytes)}, x.options().dtype(at::kByte).requires_grad(false));
+    check(mnx_indexed_linear_wgrad(a.ptr(), a.ld, g.ptr(), g.ld, n.rows, order.const_data_ptr<int32_t>(),
+                                   starts.const_data_ptr<int32_t>(), n.classes, in, cols, dtype_of(x.scalar_type()),
+                                   out(gw), bytes ? out(ws) : nullptr, bytes, stream_of(x)),
+          name);
+    return gw;
+}
+
+auto indexed_linear_op() {
+    static auto o = op<decltype(indexed_linear)>("molix::indexed_linear");
+    return o;
+}
+auto indexed_linear_wgrad_op() {
+    static auto o = op<decltype(indexed_linear_wgrad)>("molix::indexed_linear_wgrad");
+    return o;
+}
+
+// Both ops are bilinear, and their gradients are the same ops again: differentiable to any order in backward mode.
+class IndexedLinear : public torch::autograd::Function<IndexedLinear> {
+  public:
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& order,
+                          const Tensor& starts, bool transposed) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({x, weight, order, starts});
+        ctx->saved_data["transposed"] = transposed;
+        return indexed_linear_op().call(x, weight, order, starts, transposed);
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        variable_list none(5);
+        if (!grads[0].defined()) return none;
+        const auto saved = ctx->get_saved_variables();
+        const bool t = ctx->saved_data["transposed"].toBool();
+        const Tensor &g = grads[0], &x = saved[0], &order = saved[2], &starts = saved[3];
+        if (ctx->needs_input_grad(0)) none[0] = indexed_linear_op().call(g, saved[1], order, starts, !t);
+        if (ctx->needs_input_grad(1)) none[1] = indexed_linear_wgrad_op().call(t ? g : x, t ? x : g, order, starts);
+        return none;
+    }
+};
+
+class IndexedLinearWgrad : public torch::autograd::Function<IndexedLinearWgrad> {
+  public:
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& grad, const Tensor& order,
+                          const Tensor& starts) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({x, grad, order, starts});
+        return indexed_linear_wgrad_op().call(x, grad, order, starts);
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        variable_list none(4);
+        if (!grads[0].defined()) return none;
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &s = grads[0], &order = saved[2], &starts = saved[3];
+        if (ctx->needs_input_grad(0)) none[0] = indexed_linear_op().call(saved[1], s, order, starts, true);
+        if (ctx->needs_input_grad(1)) none[1] = indexed_linear_op().call(saved[0], s, order, starts, false);
+        return none;
+    }
+};
+
+void backward_mode_only(const char* name, const Tensor& a, const Tensor& b) {
+    TORCH_CHECK(!has_tangent(a) && !has_tangent(b), "molix::", name, " has no forward-mode derivative");
+    TORCH_CHECK(!transformed(), "molix::", name, " does not run inside torch.func's transforms");
+}
+
+Tensor indexed_linear_autograd(const Tensor& x, const Tensor& weight, const Tensor& order, const Tensor& starts,
+                               bool transposed) {
+    if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad())) {
+        backward_mode_only("indexed_linear", x, weight);
+        return IndexedLinear::apply(x, weight, order, starts, transposed);
+    }
+    TORCH_CHECK(!has_tangent(x) && !has_tangent(weight), "molix::indexed_linear has no forward-mode derivative");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return indexed_linear_op().call(x, weight, order, starts, transposed);
+}
+
+Tensor indexed_linear_wgrad_autograd(const Tensor& x, const Tensor& grad, const Tensor& order, const Tensor& starts) {
+    if (at::GradMode::is_enabled() && (x.requires_grad() || grad.requires_grad())) {
+        backward_mode_only("indexed_linear_wgrad", x, grad);
+        return IndexedLinearWgrad::apply(x, grad, order, starts);
+    }
+    TORCH_CHECK(!has_tangent(x) && !has_tangent(grad), "molix::indexed_linear_wgrad has no forward-mode derivative");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return indexed_linear_wgrad_op().call(x, grad, order, starts);
+}
+
+// (order, starts) of molix::class_groups.
+std::tuple<Tensor, Tensor> grouped(const Tensor& index, int64_t classes) {
+    const Tensor z = index.to(at::kLong).contiguous();
+    const c10::DeviceGuard guard(z.device());
+    const auto i32 = z.options().dtype(at::kInt);
+    Tensor order = at::empty({z.size(0)}, i32), starts = at::empty({classes + 2}, i32);
+    const size_t bytes = mnx_class_groups_workspace_bytes(z.size(0), int32_t(classes));
+    Tensor ws = at::empty({int64_t(bytes)}, z.options().dtype(at::kByte));
+    check(mnx_class_groups(z.numel() ? z.const_data_ptr<int64_t>() : nullptr, z.size(0), int32_t(classes),
+                           static_cast<int32_t*>(out(order)), static_cast<int32_t*>(out(starts)), out(ws), bytes,
+                           stream_of(z)),
+          "class_groups");
+    return {order, starts};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(molix, m) {
@@ -897,6 +1066,8 @@ TORCH_LIBRARY_FRAGMENT(molix, m) {
     m.def("adamw8_moments(Tensor[] exp_avgs, Tensor[] exp_avg_sqs, Tensor[] bases, Tensor(a!)[] out_avgs, "
           "Tensor(b!)[] out_avg_sqs) -> ()",
           tags);
+    m.def("indexed_linear(Tensor x, Tensor weight, Tensor order, Tensor starts, bool transposed) -> Tensor", tags);
+    m.def("indexed_linear_wgrad(Tensor x, Tensor grad, Tensor order, Tensor starts) -> Tensor", tags);
     m.def("orthogonalize(Tensor x, int steps, float a, float b, float c, float eps) -> Tensor", tags);
     m.def("muon_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] momenta, float lr, float momentum, "
           "bool nesterov, float weight_decay, int steps, float a, float b, float c, float eps, bool match_rms, "
@@ -912,11 +1083,17 @@ TORCH_LIBRARY_IMPL(molix, CUDA, m) {
     m.impl("adamw_step", adamw_step);
     m.impl("adamw8_step", adamw8_step);
     m.impl("adamw8_moments", adamw8_moments);
+    m.impl("indexed_linear", indexed_linear);
+    m.impl("indexed_linear_wgrad", indexed_linear_wgrad);
     m.impl("orthogonalize", orthogonalize);
     m.impl("muon_step", muon_step);
 }
 
 TORCH_LIBRARY_IMPL(molix, CPU, m) {  // these say that they run on the GPU only
+    m.impl("indexed_linear", indexed_linear);
+    m.impl("indexed_linear_wgrad", indexed_linear_wgrad);
+    m.impl("indexed_linear", indexed_linear);
+    m.impl("indexed_linear_wgrad", indexed_linear_wgrad);
     m.impl("orthogonalize", orthogonalize);
     m.impl("muon_step", muon_step);
 }
@@ -932,6 +1109,8 @@ TORCH_LIBRARY_IMPL(molix, Autograd, m) {
     m.impl("layer_norm_backward", layer_norm_backward_autograd);
     m.impl("layer_norm_backward2", layer_norm_backward2_autograd);
     m.impl("grad_norm", grad_norm_autograd);
+    m.impl("indexed_linear", indexed_linear_autograd);
+    m.impl("indexed_linear_wgrad", indexed_linear_wgrad_autograd);
     m.impl("orthogonalize", orthogonalize_autograd);
     // no gradients: they write into leaves, whose versions rise
     for (const char* name : {"adamw_step", "adamw8_step", "adamw8_moments", "muon_step"})
@@ -1135,6 +1314,42 @@ PyObject* py_moments(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// (x, weight, index, order, starts): molix.F.indexed_linear of rows; index or the plan (order, starts) may be None
+PyObject* py_indexed_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 5, "indexed_linear: 5 arguments, got ", n);
+    if (mode_on()) Py_RETURN_NOTIMPLEMENTED;
+    bool overridden = false;
+    const OptTensor x = tensor_or_none(a[0], "x", overridden), w = tensor_or_none(a[1], "weight", overridden);
+    const OptTensor z = tensor_or_none(a[2], "index", overridden);
+    const OptTensor order = tensor_or_none(a[3], "groups", overridden);
+    const OptTensor starts = tensor_or_none(a[4], "groups", overridden);
+    if (overridden) Py_RETURN_NOTIMPLEMENTED;
+    TORCH_CHECK_TYPE(given(x) && given(w) && (given(z) || (given(order) && given(starts))),
+                     "indexed_linear: x, weight and an index or groups");
+    TORCH_CHECK(!transformed(), "molix::indexed_linear does not run inside torch.func's transforms");
+    Tensor y;
+    {
+        Released r;
+        if (given(order) && given(starts)) {
+            y = indexed_linear_op().call(*x, *w, *order, *starts, false);
+        } else {
+            check_rows("indexed_linear", "x", *x);
+            TORCH_CHECK_VALUE(z->dim() == 1 && z->size(0) == x->size(0) && z->device() == x->device() &&
+                                  at::isIntegralType(z->scalar_type(), false),
+                              "indexed_linear: index of integers, one a row, on x's device; got ", z->scalar_type(),
+                              " ", z->sizes(), " on ", z->device(), " for x ", x->sizes());
+            TORCH_CHECK_VALUE(w->dim() == 3 && w->size(0) >= 1 && w->size(0) <= MNX_CLASS_GROUPS_MAX_CLASSES,
+                              "indexed_linear: weight (classes, in, out) of 1 to ", MNX_CLASS_GROUPS_MAX_CLASSES,
+                              " classes, got ", w->sizes());
+            const auto [o, s] = grouped(*z, w->size(0));
+            y = indexed_linear_op().call(*x, *w, o, s, false);
+        }
+    }
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
 // (x, steps, a, b, c, eps)
 PyObject* py_orthogonalize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -1185,6 +1400,8 @@ PyMethodDef kMethods[] = {
     {"grad_norm", py_grad_norm, METH_O, "molix::grad_norm"},
     {"moments", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_moments)), METH_FASTCALL,
      "molix::adamw8_moments"},
+    {"indexed_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_indexed_linear)), METH_FASTCALL,
+     "molix::indexed_linear of rows"},
     {"orthogonalize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_orthogonalize)), METH_FASTCALL,
      "molix::orthogonalize"},
     {"muon", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_muon)), METH_FASTCALL, "molix::muon_step"},

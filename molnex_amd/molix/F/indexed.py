@@ -1,0 +1,44 @@
+"""The linear map whose weights each row's class selects, by the ``molix::indexed_linear`` kernels."""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+from torch.overrides import handle_torch_function
+
+from ...kernels import class_groups
+from ...training import DTYPES, _host
+
+__all__ = ["class_groups", "indexed_linear"]
+
+
+def indexed_linear(x: Tensor, weight: Tensor, index: Tensor | None = None,
+                   groups: tuple[Tensor, Tensor] | None = None) -> Tensor:
+    """``y[i] = x[i] @ weight[index[i]]`` for rows ``x`` (..., in), ``weight`` (classes, in, out) and the rows' classes
+    ``index`` (..., of integers); a row whose class lies outside [0, classes) gives zeros.
+
+    ``groups``: ``class_groups(index, classes)``, kept where the same rows are mapped again (layers, steps); ``index`` is
+    not read then and may be left out.  float32, bfloat16 or float16, the same for both; products of float32 values are
+    exact to float32, sums are float32.  Differentiable in backward mode to any order; the weights' gradient is summed
+    in a fixed order.  Nothing synchronises.  Under autocast both go to its type, as for a matrix product."""
+    order, starts = (None, None) if groups is None else groups
+    if torch.is_autocast_enabled("cuda"):
+        to = torch.get_autocast_dtype("cuda")
+        x, weight = (t.to(to) if t.is_cuda and t.dtype in DTYPES else t for t in (x, weight))
+    lead = None
+    if x.dim() != 2:
+        if x.dim() < 1 or (index is not None and index.shape != x.shape[:-1]):
+            raise ValueError(f"indexed_linear: x of shape {tuple(x.shape)} and index of shape "
+                             f"{None if index is None else tuple(index.shape)}")
+        lead, x = x.shape[:-1], x.reshape(-1, x.shape[-1])
+        index = None if index is None else index.reshape(-1)
+    if torch.compiler.is_compiling():
+        if order is None:
+            order, starts = class_groups(index, weight.shape[0])
+        y = torch.ops.molix.indexed_linear(x, weight, order, starts, False)
+    else:
+        y = _host.indexed_linear(x, weight, index, order, starts)
+        if y is NotImplemented:
+            return handle_torch_function(indexed_linear, (x, weight, index, order, starts), x, weight, index=index,
+                                         groups=groups)
+    return y if lead is None else y.reshape(*lead, y.shape[-1])

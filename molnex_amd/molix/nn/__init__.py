@@ -1,4 +1,5 @@
+from .indexed import IndexedLinear
 from .locality import NeighborList
 from .norm import LayerNorm
 
-__all__ = ["NeighborList", "LayerNorm"]
+__all__ = ["NeighborList", "LayerNorm", "IndexedLinear"]

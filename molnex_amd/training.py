@@ -88,6 +88,16 @@ def _(exp_avgs, exp_avg_sqs, bases, out_avgs, out_avg_sqs):
     return None
 
 
+@_fake("indexed_linear")
+def _(x, weight, order, starts, transposed):
+    return x.new_empty((x.shape[0], weight.shape[1 if transposed else 2]))
+
+
+@_fake("indexed_linear_wgrad")
+def _(x, grad, order, starts):
+    return x.new_empty((starts.shape[0] - 2, x.shape[1], grad.shape[1]))
+
+
 @_fake("orthogonalize")
 def _(x, steps, a, b, c, eps):
     return x.new_empty(x.shape)
