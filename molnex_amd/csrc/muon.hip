@@ -22,6 +22,7 @@
 #include "elem.h"
 
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 namespace mnx {
@@ -32,7 +33,7 @@ typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kPad = 128;
+constexpr int kPad = 128;  // sides of the padded matrices are multiples of it
 constexpr int kChunk = 4096;  // elements of a matrix that a workgroup of the momentum kernel takes
 constexpr int kCast = 64;     // side of the cast kernel's tiles
 constexpr int kTableArgs = 24;
@@ -215,10 +216,15 @@ __device__ __forceinline__ f32x16 mfma(const half8& a, const half8& b, const f32
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ void load_lds(const _Float16* from, _Float16* to) {
-    __builtin_amdgcn_global_load_lds(
-        const_cast<__attribute__((address_space(1))) void*>((const __attribute__((address_space(1))) void*)from),
-        (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+// 16 bytes a lane from base + offset (bytes) to LDS, lane by lane from `to` on (M0).  In assembly, because for the builtin
+// the compiler waits for every such load before the next read of LDS, also of other memory there.  The caller waits
+// (vmcnt) and has a barrier before anyone reads what has come, and before it ends.
+__device__ __forceinline__ void load_lds(const _Float16* base, uint32_t offset, _Float16* to) {
+    const uint32_t m0 = uint32_t(uintptr_t((__attribute__((address_space(3))) _Float16*)to));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(m0), "v"(offset), "s"(base)
+                 : "memory", "m0");
 }
 
 // Four columns (k, k + 4) of the transposed 16-bit read: see read_tr.
@@ -229,32 +235,65 @@ __device__ __forceinline__ half8 read_tr(const _Float16* lo, const _Float16* hi)
     return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// Four values of the last X, at columns j of row i, go into the parameters (or are the result); `count` of them exist.
+template <typename T, bool TALL>
+__device__ __forceinline__ void apply(T* p, int cols, int i, int j, int count, float decay, float rate,
+                                      const float (&v)[4]) {
+    typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    const int64_t at = TALL ? int64_t(j) * cols + i : int64_t(i) * cols + j, step = TALL ? cols : 1;
+    if (!TALL && count >= 4) {
+        Four* q = reinterpret_cast<Four*>(p + at);
+        Four o = {};
+        if (decay != 0) o = *q;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = T(decay * float(o[e]) - rate * v[e]);
+        *q = o;
+        return;
+    }
+    float old[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) old[e] = decay != 0 && e < count ? float(p[at + e * step]) : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e < count) p[at + e * step] = T(decay * old[e] - rate * v[e]);
+}
+
 constexpr int kKC = 64;  // k of a chunk
 
-// A tile of I rows against J columns of one product, sum over k of I[i][k] J[j][k] (rows of both in memory), or with TR
-// of I[i][k] J[k][j].  Tiles go from memory straight to LDS, 16 bytes a lane, one chunk ahead.  Within a row of LDS the
-// 16-byte pieces are permuted (by the lanes' source addresses: LDS itself is filled in lane order) so that the reads,
-// 16 bytes of 32 rows or 64 bytes of 4 rows, meet every bank once.
-template <int MODE, int PL, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) k_muon_product(const Mat* __restrict__ table, int count,
-                                                                           uint32_t units, Step s,
-                                                                           const Stat* __restrict__ stats, Apply ap) {
+// A BT x BT tile of one product, the sum over k of I[i][k] J[j][k] (rows of both in memory), or with TR of I[i][k] J[k][j].
+// Four wavefronts share it, a quarter each.  Chunks go from memory straight to LDS, 16 bytes a lane, into two buffers.
+// Within a row of LDS the 16-byte pieces are permuted (by the lanes' source addresses: LDS itself is filled in lane order)
+// so that the reads, 16 bytes of 16 rows or 64 bytes of 4 rows, meet every bank once.
+//
+// Operands of the next 16 k are read from LDS between the products of these.  The one barrier of a chunk stands before its
+// last 16 k: by then every read of this buffer has come back and the next chunk has arrived, so behind it half the loads
+// of the chunk after next and the first reads of the next run between those products, the other half of the loads between
+// the next chunk's first ones.
+//
+// The last tile of a row or column may reach past the padded matrix: it reads what lies behind it in the workspace (rows
+// and columns of the result that are not stored) and stores none of that.
+template <int MODE, int PL, int BT>
+__global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const Mat* __restrict__ table, int count,
+                                                                        uint32_t units, Step s,
+                                                                        const Stat* __restrict__ stats, Apply ap) {
     constexpr bool SYM = MODE == kGram || MODE == kPoly, TR = !SYM;
-    constexpr int WAVES = (BM / WM) * (BN / WN), MT = WM / 32, NT = WN / 32;
+    constexpr int W = BT / 2, MT = W / 32;  // a wavefront's part
     constexpr int SEG = PL == 1 ? 1 : 3;
-    __shared__ _Float16 sI[2][BM * kKC], sJ[2][BN * kKC];
+    constexpr int FETCH = BT / 32;  // loads a lane of either operand's chunk
+    constexpr int PIECES = BT / 8;  // of a sum's columns
+    __shared__ _Float16 sI0[BT * kKC], sI1[BT * kKC], sJ0[BT * kKC], sJ1[BT * kKC];
     const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wi = wave % (BM / WM), wj = wave / (BM / WM);
+    const int wi = wave & 1, wj = wave >> 1;
     const uint32_t per = (units + 7) / 8;
     uint32_t u = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if (u >= units) return;
     const int at = find_mat(table, count, SYM ? &Mat::sym0 : &Mat::upd0, u);
     const Mat& t = table[at];
     u -= SYM ? t.sym0 : t.upd0;
-    const int ni = t.rp / BM, nj = t.cp / BN;
+    const int ni = (t.rp + BT - 1) / BT, nj = (t.cp + BT - 1) / BT;
     const uint32_t tiles = SYM ? uint32_t(ni * (ni + 1) / 2) : uint32_t(ni * nj);
-    const uint32_t which = u / tiles;
+    const uint32_t which = __builtin_amdgcn_readfirstlane(u / tiles);
     u -= which * tiles;
     int ti, tj;
     if (SYM) {
@@ -262,9 +301,10 @@ __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) k_muon_product(con
         while (uint32_t(ti * (ti + 1) / 2) > u) --ti;
         while (uint32_t((ti + 1) * (ti + 2) / 2) <= u) ++ti;
         tj = int(u) - ti * (ti + 1) / 2;
-    } else {
-        tj = int(u) / ni;
-        ti = int(u) - tj * ni;
+    } else {  // bands of four tiles' rows: what an XCD works on at a time is nearly square
+        const int band = int(u) / (4 * nj), in = int(u) - band * 4 * nj, high = min(4, ni - 4 * band);
+        tj = in / high;
+        ti = 4 * band + in - tj * high;
     }
     ti = __builtin_amdgcn_readfirstlane(ti);
     tj = __builtin_amdgcn_readfirstlane(tj);
@@ -272,83 +312,140 @@ __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) k_muon_product(con
     const _Float16* X = t.x[s.from] + int64_t(which) * t.rp * t.cp;
     const _Float16* A = t.a + int64_t(which) * t.rp * t.rp;
     const _Float16* B = t.b + int64_t(which) * t.rp * t.rp;
-    const _Float16* I = (MODE == kGram ? X : MODE == kPoly ? A : B) + int64_t(ti) * BM * K;
+    const _Float16* I = (MODE == kGram ? X : MODE == kPoly ? A : B) + int64_t(ti) * BT * K;
     const int64_t iplane = MODE == kGram ? t.xplane : t.aplane;
-    const _Float16* J = TR ? X + tj * BN : (MODE == kGram ? X : A) + int64_t(tj) * BN * K;
+    const _Float16* J = TR ? X + tj * BT : (MODE == kGram ? X : A) + int64_t(tj) * BT * K;
     const int64_t jplane = MODE == kPoly ? t.aplane : t.xplane;
 
-    f32x16 acc[MT][NT];
+    f32x16 acc[MT][MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < MT; ++n)
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[m][n][q] = 0.f;
 
     const int per_seg = K / kKC, chunks = SEG * per_seg;
-    auto fetch = [&](int chunk, int buf) {
-        int k0 = chunk;
-        const _Float16 *i = I, *j = J;
-        if constexpr (PL == 2) {
-            const int seg = chunk >= 2 * per_seg ? 2 : chunk >= per_seg ? 1 : 0;
-            k0 -= seg * per_seg;
-            if (seg == 0) i += iplane;
-            if (seg == 1) j += jplane;
-        }
-        k0 *= kKC;
+    // a wavefront fills 1 KB of LDS at a time, every fourth: 8 rows of 64 k, or sums' columns piece after piece
+    const int frow = wave * 8 + (lane >> 3);
+    const uint32_t irow = 2 * (uint32_t(frow) * K + (((lane & 7) ^ ((frow >> 1) & 7)) << 3));  // bytes
+    const int64_t istep = int64_t(32) * K;
+    uint32_t jrow[TR ? FETCH : 1];
+    if constexpr (TR) {
 #pragma unroll
-        for (int n = wave; n < BM / 8; n += WAVES) {
-            const int row = n * 8 + (lane >> 3);
-            load_lds(i + int64_t(row) * K + k0 + (((lane & 7) ^ ((row >> 1) & 7)) << 3), &sI[buf][n * 512]);
-        }
-        if constexpr (!TR) {
-#pragma unroll
-            for (int n = wave; n < BN / 8; n += WAVES) {
-                const int row = n * 8 + (lane >> 3);
-                load_lds(j + int64_t(row) * K + k0 + (((lane & 7) ^ ((row >> 1) & 7)) << 3), &sJ[buf][n * 512]);
-            }
-        } else {
-            constexpr int LPR = BN / 8;  // lanes of a row
-#pragma unroll
-            for (int n = wave; n < BN / 8; n += WAVES) {
-                const int k = n * (64 / LPR) + lane / LPR;
-                load_lds(j + int64_t(k0 + k) * t.cp + (((lane % LPR) ^ ((k & 3) << 2)) << 3), &sJ[buf][n * 512]);
-            }
-        }
-    };
-    fetch(0, 0);
-    for (int chunk = 0; chunk < chunks; ++chunk) {
-        __syncthreads();  // this chunk has arrived, and the other buffer is read
-        if (chunk + 1 < chunks) fetch(chunk + 1, (chunk + 1) & 1);
-        const _Float16 *pi = sI[chunk & 1], *pj = sJ[chunk & 1];
-#pragma unroll
-        for (int ks = 0; ks < kKC / 16; ++ks) {
-            half8 fi[MT], fj[NT];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const int row = wi * WM + m * 32 + l32;
-                fi[m] = *reinterpret_cast<const half8*>(pi + row * kKC + (((2 * ks + half) ^ ((row >> 1) & 7)) << 3));
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if constexpr (!TR) {
-                    const int row = wj * WN + n * 32 + l32;
-                    fj[n] = *reinterpret_cast<const half8*>(pj + row * kKC + (((2 * ks + half) ^ ((row >> 1) & 7)) << 3));
-                } else {
-                    const int k = 16 * ks + 8 * half + ((lane & 15) >> 2);
-                    const int col = wj * WN + n * 32 + (l32 & 16) + (lane & 3) * 4;
-                    const _Float16* q = pj + k * BN + (((col >> 3) ^ ((k & 3) << 2)) << 3) + (col & 4);
-                    fj[n] = read_tr(q, q + 4 * BN);
-                }
-            }
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) acc[m][n] = mfma(fj[n], fi[m], acc[m][n]);
+        for (int n = 0; n < FETCH; ++n) {
+            const int piece = (n * 4 + wave) * 64 + lane, k = piece / PIECES, c = piece % PIECES;
+            const int turn = BT == 192 ? ((k >> 1) & 1) << 2 : (k & 3) << 2;
+            jrow[n] = 2 * (uint32_t(k) * t.cp + ((c ^ turn) << 3));
         }
     }
+    struct Source {
+        const _Float16 *i, *j;
+    };
+    auto source = [&](int chunk) {
+        Source f{I, J};
+        if constexpr (PL == 2) {
+            const int seg = chunk >= 2 * per_seg ? 2 : chunk >= per_seg ? 1 : 0;
+            chunk -= seg * per_seg;
+            if (seg == 0) f.i += iplane;
+            if (seg == 1) f.j += jplane;
+        }
+        f.i += chunk * kKC;
+        f.j += TR ? int64_t(chunk * kKC) * t.cp : chunk * kKC;
+        return f;
+    };
+    // the n-th of a chunk's 2 FETCH loads
+    auto fetch = [&](const Source& f, int n, _Float16* bi, _Float16* bj) {
+        if (n < FETCH) load_lds(f.i + n * istep, irow, bi + (n * 4 + wave) * 512);
+        else if constexpr (TR) load_lds(f.j, jrow[n - FETCH], bj + ((n - FETCH) * 4 + wave) * 512);
+        else load_lds(f.j + (n - FETCH) * istep, irow, bj + ((n - FETCH) * 4 + wave) * 512);
+    };
+    struct Frags {
+        half8 i[MT], j[MT];
+    };
+    const int ki = (wi * W + l32) * kKC, kj = (wj * W + l32) * kKC, turn = (l32 >> 1) & 7;  // 32 rows on turn alike
+    const int trow = 8 * half + ((lane & 15) >> 2), tcol = wj * W + (l32 & 16) + (lane & 3) * 4;
+    const int tturn = BT == 192 ? ((trow >> 1) & 1) << 2 : (trow & 3) << 2;
+    auto read_i = [&](int m, int ks, const _Float16* bi) {
+        return *reinterpret_cast<const half8*>(bi + ki + m * 32 * kKC + (((2 * ks + half) ^ turn) << 3));
+    };
+    auto read_j = [&](int n, int ks, const _Float16* bj) {
+        if constexpr (!TR) {
+            return *reinterpret_cast<const half8*>(bj + kj + n * 32 * kKC + (((2 * ks + half) ^ turn) << 3));
+        } else {
+            const int col = tcol + n * 32;
+            const _Float16* q = bj + (16 * ks + trow) * BT + (((col >> 3) ^ tturn) << 3) + (col & 4);
+            return read_tr(q, q + 4 * BT);  // four sums on turn alike
+        }
+    };
+    // The products of `now`, with the reads of `next` and `loads` between them.
+    auto multiply = [&](const Frags& now, Frags& next, int ks, const _Float16* bi, const _Float16* bj, auto loads) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            next.j[m] = read_j(m, ks, bj);
+            next.i[m] = read_i(m, ks, bi);
+            loads(m);
+#pragma unroll
+            for (int n = 0; n < MT; ++n) acc[m][n] = mfma(now.j[n], now.i[m], acc[m][n]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto arrived = [] {  // everyone's loads and reads
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    Frags f0, f1;
+    // Chunk c in (bi, bj), its first operands in f0; (oi, oj) takes or holds the next.  REST: the second half of the next
+    // chunk's loads is still to come; MORE: a chunk after next begins.
+    auto body = [&](int c, _Float16* bi, _Float16* bj, _Float16* oi, _Float16* oj, auto rest, auto more) {
+        const auto nothing = [](int) {};
+        if constexpr (rest) {
+            const Source f = source(c + 1);
+            multiply(f0, f1, 1, bi, bj, [&](int m) {
+#pragma unroll
+                for (int n = 0; n < FETCH / MT; ++n) fetch(f, FETCH + m * (FETCH / MT) + n, oi, oj);
+            });
+        } else {
+            multiply(f0, f1, 1, bi, bj, nothing);
+        }
+        multiply(f1, f0, 2, bi, bj, nothing);
+        multiply(f0, f1, 3, bi, bj, nothing);
+        arrived();
+        if constexpr (more) {
+            const Source f = source(c + 2);
+            multiply(f1, f0, 0, oi, oj, [&](int m) {
+#pragma unroll
+                for (int n = 0; n < FETCH / MT; ++n) fetch(f, m * (FETCH / MT) + n, bi, bj);
+            });
+        } else {
+            multiply(f1, f0, 0, oi, oj, nothing);  // after the last chunk, reads of the one before that nobody uses
+        }
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    {
+        const Source f = source(0), g = source(1);
+#pragma unroll
+        for (int n = 0; n < 2 * FETCH; ++n) fetch(f, n, sI0, sJ0);
+        arrived();
+#pragma unroll
+        for (int n = 0; n < FETCH; ++n) fetch(g, n, sI1, sJ1);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            f0.i[m] = read_i(m, 0, sI0);
+            f0.j[m] = read_j(m, 0, sJ0);
+        }
+    }
+    int c = 0;  // chunks are an even number: K is a multiple of 128
+    for (; c + 2 < chunks; c += 2) {
+        body(c, sI0, sJ0, sI1, sJ1, yes, yes);
+        body(c + 1, sI1, sJ1, sI0, sJ0, yes, yes);
+    }
+    body(c, sI0, sJ0, sI1, sJ1, yes, no);
+    body(c + 1, sI1, sJ1, sI0, sJ0, no, no);
 
-    // acc[m][n][q] belongs to row i = 32 m + l32 and column j = 32 n + 8 (q / 4) + 4 half + q % 4 of the wave's tile
+    // acc[m][n][q] belongs to row i = 32 m + l32 and column j = 32 n + 8 (q / 4) + 4 half + q % 4 of the wave's part
     float own = s.own, prod = s.prod;
     if (s.first) {
         const float rho = stats[t.stat0 + which].rho;
@@ -362,62 +459,75 @@ __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) k_muon_product(con
     const int64_t oplane = SYM ? t.aplane : t.xplane;
     const _Float16* E = MODE == kPoly ? A : X;
     _Float16* out = (MODE == kGram ? t.a : MODE == kPoly ? t.b : t.x[s.from ^ 1]) + int64_t(which) * t.rp * ld;
-    float decay = 1, rate = -ap.inv;  // rate: of p's change, or of the result itself
+    const int i0 = ti * BT + wi * W + l32, j0 = tj * BT + wj * W + 4 * half;
+    const int rows = MODE == kFinal ? t.r : t.rp, cols = MODE == kFinal ? t.c : SYM ? t.rp : t.cp;
+    float decay = 0, rate = -ap.inv;  // of p and of its change; the result itself has no p
     if (MODE == kFinal && t.m) {
         const float lr = ap.lr_device ? *ap.lr_device : ap.lr;
         decay = 1 - lr * ap.wd;
         rate = lr * t.adjust * ap.inv;
     }
+    // every four consecutive columns of a row
+    auto each = [&](auto store) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int i = ti * BM + wi * WM + m * 32 + l32;
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < MT; ++n)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int j = tj * BN + wj * WN + n * 32 + 8 * q + 4 * half;
-                float v[4];
+                for (int q = 0; q < 4; ++q) {
+                    const int i = i0 + m * 32, j = j0 + n * 32 + 8 * q;
+                    if (i >= rows || j >= cols) continue;
+                    float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = prod * acc[m][n][4 * q + e];
-                const int64_t place = int64_t(i) * ld + j;
-                if constexpr (MODE != kGram) {
+                    for (int e = 0; e < 4; ++e) v[e] = prod * acc[m][n][4 * q + e];
+                    if constexpr (MODE != kGram) {
 #pragma unroll
-                    for (int pl = PL - 1; pl >= 0; --pl) {
-                        const half4 old = *reinterpret_cast<const half4*>(E + pl * oplane + place);
+                        for (int pl = PL - 1; pl >= 0; --pl) {
+                            const half4 old = *reinterpret_cast<const half4*>(E + pl * oplane + int64_t(i) * ld + j);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] += own * float(old[e]);
-                    }
-                }
-                if constexpr (MODE == kFinal) {
-                    if (i >= t.r) continue;
-                    const bool tall = t.rows > t.cols;
-                    const int64_t off = int64_t(which) * t.rows * t.cols;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (j + e >= t.c) continue;
-                        const int64_t at = off + (tall ? int64_t(j + e) * t.cols + i : int64_t(i) * t.cols + j + e);
-                        const float old = t.m ? decay * load_any(t.p, at, t.dtype) : 0.f;
-                        store_elem(t.p, at, t.dtype, old - rate * v[e]);
-                    }
-                } else {
-                    half4 hi, lo;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        hi[e] = _Float16(v[e]);
-                        lo[e] = _Float16(v[e] - float(hi[e]));
-                    }
-                    *reinterpret_cast<half4*>(out + place) = hi;
-                    if constexpr (PL == 2) *reinterpret_cast<half4*>(out + oplane + place) = lo;
-                    if (SYM && ti != tj) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int64_t mirror = int64_t(j + e) * ld + i;
-                            out[mirror] = hi[e];
-                            if constexpr (PL == 2) out[oplane + mirror] = lo[e];
+                            for (int e = 0; e < 4; ++e) v[e] += own * float(old[e]);
                         }
                     }
+                    store(i, j, v);
+                }
+    };
+    if constexpr (MODE == kFinal) {
+        auto as = [&](auto type, auto tall) {
+            auto* p = static_cast<decltype(type)*>(t.p) + int64_t(which) * t.rows * t.cols;
+            each([&](int i, int j, const float (&v)[4]) {
+                apply<decltype(type), decltype(tall)::value>(p, t.cols, i, j, cols - j, decay, rate, v);
+            });
+        };
+        const bool tall = t.rows > t.cols;
+        if constexpr (PL == 1) {
+            if (tall) as(__bf16{}, yes);
+            else as(__bf16{}, no);
+        } else if (t.dtype == kF32) {
+            if (tall) as(float{}, yes);
+            else as(float{}, no);
+        } else {
+            if (tall) as(_Float16{}, yes);
+            else as(_Float16{}, no);
+        }
+    } else {
+        each([&](int i, int j, const float (&v)[4]) {
+            half4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                hi[e] = _Float16(v[e]);
+                lo[e] = _Float16(v[e] - float(hi[e]));
+            }
+            *reinterpret_cast<half4*>(out + int64_t(i) * ld + j) = hi;
+            if constexpr (PL == 2) *reinterpret_cast<half4*>(out + oplane + int64_t(i) * ld + j) = lo;
+            if (SYM && ti != tj) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int64_t mirror = int64_t(j + e) * ld + i;
+                    out[mirror] = hi[e];
+                    if constexpr (PL == 2) out[oplane + mirror] = lo[e];
                 }
             }
+        });
     }
 }
 
@@ -466,6 +576,7 @@ struct Plan {
     Prefix total{};
     uint32_t stats = 0;
     size_t bytes = 0;
+    int sym_tile = 128, upd_tile = 128;
     double* partial = nullptr;
     Stat* stat = nullptr;
     Mat* table = nullptr;
@@ -488,13 +599,30 @@ int check_args(const mnx_muon_args& a) {
     return MNX_OK;
 }
 
+// Tiles of a tensor's symmetric products, or of its updates.
+inline int64_t tiles_of(const Mat& t, bool sym, int tile) {
+    const int64_t ni = ceil_div(t.rp, tile), nj = ceil_div(t.cp, tile);
+    return t.batch * (sym ? ni * (ni + 1) / 2 : ni * nj);
+}
+
+constexpr int kTile[] = {256, 192, 128}, kTiles = 3;
+
+// The time of a launch, about: rounds of the tiles that the card holds at once (256 CUs; two tiles of 128 a CU), by what a
+// tile takes.
+double cost(const std::vector<Mat>& mats, bool sym, int tile) {
+    double tiles = 0;
+    for (const Mat& t : mats) tiles += double(tiles_of(t, sym, tile));
+    const double slots = tile == 128 ? 512 : 256, each = tile == 256 ? 4.0 : tile == 192 ? 2.4 : 2.2;
+    return std::ceil(tiles / slots) * each;
+}
+
 // float16 numbers that stand for one of X, A and B
 inline int planes_of(int dtype) { return dtype == kBF16 ? 1 : 2; }
 
 // Lays the tensors of `planes` planes out over the workspace (from `base`, which may be null for its size alone).
 int lay_out(const mnx_muon_args& a, int planes, char* base, Plan& plan) {
     Workspace ws{base, 0};
-    uint64_t chunk = 0, cast = 0, sym = 0, upd = 0, stat = 0;
+    uint64_t chunk = 0, cast = 0, stat = 0;
     for (int64_t i = 0; i < a.count; ++i) {
         if (planes_of(a.dtype[i]) != planes || !a.batch[i] || !a.rows[i] || !a.cols[i]) continue;
         Mat t{};
@@ -516,27 +644,53 @@ int lay_out(const mnx_muon_args& a, int planes, char* base, Plan& plan) {
         t.stat0 = uint32_t(stat);
         t.chunk0 = uint32_t(chunk);
         t.cast0 = uint32_t(cast);
-        t.sym0 = uint32_t(sym);
-        t.upd0 = uint32_t(upd);
-        const uint64_t b = uint64_t(a.batch[i]), ni = t.rp / kPad, nj = t.cp / kPad;
+        const uint64_t b = uint64_t(a.batch[i]);
         stat += b;
         chunk += b * uint64_t(ceil_div(int64_t(t.rows) * t.cols, kChunk));
         cast += b * uint64_t(t.rp / kCast) * (t.cp / kCast);
-        sym += b * (ni * (ni + 1) / 2);
-        upd += b * ni * nj;
         for (_Float16*& x : t.x) x = ws.take<_Float16>(size_t(planes * t.xplane));
         t.a = ws.take<_Float16>(size_t(planes * t.aplane));
         t.b = ws.take<_Float16>(size_t(planes * t.aplane));
         // a grid has fewer than 2^32 threads
-        MNX_REQUIRE(std::max({chunk, cast, sym, upd, stat}) < (1u << 23), "muon: too many matrices in one call");
+        MNX_REQUIRE(std::max({chunk, cast, stat}) < (1u << 23), "muon: too many matrices in one call");
         plan.mat.push_back(t);
     }
+    for (int kind = 0; kind < 2; ++kind) {
+        int best = 0;
+        for (int k = 1; k < kTiles; ++k)
+            if (cost(plan.mat, kind == 0, kTile[k]) < cost(plan.mat, kind == 0, kTile[best])) best = k;
+        (kind == 0 ? plan.sym_tile : plan.upd_tile) = kTile[best];
+    }
+    uint64_t sym = 0, upd = 0;
+    for (Mat& t : plan.mat) {
+        t.sym0 = uint32_t(sym);
+        t.upd0 = uint32_t(upd);
+        sym += tiles_of(t, true, plan.sym_tile);
+        upd += tiles_of(t, false, plan.upd_tile);
+    }
     plan.total = {uint32_t(chunk), uint32_t(cast), uint32_t(sym), uint32_t(upd)};
+    // the last tiles read past the last matrix
+    int64_t past = 0;
+    for (const Mat& t : plan.mat) past = std::max<int64_t>(past, int64_t(256) * t.cp);
+    if (past) ws.take<_Float16>(size_t(past));
     plan.stats = uint32_t(stat);
     plan.partial = ws.take<double>(size_t(chunk));
     plan.stat = ws.take<Stat>(size_t(stat));
     plan.table = ws.take<Mat>(plan.mat.size());
     plan.bytes = ws.used;
+    return MNX_OK;
+}
+
+template <int MODE, int PL>
+int product(const Plan& plan, const Step& s, const Apply& ap, mnx_stream_t stream) {
+    constexpr bool SYM = MODE == kGram || MODE == kPoly;
+    const int tile = SYM ? plan.sym_tile : plan.upd_tile;
+    const uint32_t units = SYM ? plan.total.sym : plan.total.upd, grid = uint32_t(up(units, 8));
+    const int count = int(plan.mat.size());
+    const auto kernel = tile == 256 ? k_muon_product<MODE, PL, 256>
+                                    : tile == 192 ? k_muon_product<MODE, PL, 192> : k_muon_product<MODE, PL, 128>;
+    kernel<<<grid, 256, 0, stream>>>(plan.table, count, units, s, plan.stat, ap);
+    MNX_CHECK_LAUNCH();
     return MNX_OK;
 }
 
@@ -560,31 +714,20 @@ int run(const mnx_muon_args& a, const Plan& plan, const Scales& sc, mnx_stream_t
     k_muon_cast<PL><<<plan.total.cast, 256, 0, stream>>>(plan.table, count, h, plan.stat);
     MNX_CHECK_LAUNCH();
     const double ca = a.coefficients[0], cb = a.coefficients[1], cc = a.coefficients[2];
-    const uint32_t gs = uint32_t(up(plan.total.sym, 8)), gu = uint32_t(up(plan.total.upd, 8));
     const Apply none{};
     for (int k = 0; k < a.steps; ++k) {
-        const double x = sc.x[k], A = sc.a[k], B = sc.b[k];
-        const int from = k & 1, first = k == 0;
-        // the first X is stored at 2^12 whatever the bounds say
-        const double xs = first ? 4096.0 : x;
-        k_muon_product<kGram, PL, 128, 128, 64, 64><<<gs, 256, 0, stream>>>(
-            plan.table, count, plan.total.sym, Step{0.f, float(A / (xs * xs)), from, first}, plan.stat, none);
-        MNX_CHECK_LAUNCH();
-        k_muon_product<kPoly, PL, 128, 128, 64, 64><<<gs, 256, 0, stream>>>(
-            plan.table, count, plan.total.sym, Step{float(B * cb / A), float(B * cc / (A * A)), from, first}, plan.stat,
-            none);
-        MNX_CHECK_LAUNCH();
-        const double to = k + 1 == a.steps ? 1.0 : sc.x[k + 1];
-        const Step s{float(to * ca / xs), float(to / (B * xs)), from, first};
-        if (k + 1 < a.steps) {
-            k_muon_product<kUpdate, PL, 128, 128, 64, 64><<<gu, 256, 0, stream>>>(plan.table, count, plan.total.upd, s,
-                                                                                plan.stat, none);
-        } else {
-            const Apply ap{float(a.lr), a.lr_device, float(a.weight_decay), 1.0f};
-            k_muon_product<kFinal, PL, 128, 128, 64, 64><<<gu, 256, 0, stream>>>(plan.table, count, plan.total.upd, s,
-                                                                               plan.stat, ap);
-        }
-        MNX_CHECK_LAUNCH();
+        const double A = sc.a[k], B = sc.b[k];
+        const int from = k & 1, first = k == 0, last = k + 1 == a.steps;
+        const double xs = first ? 4096.0 : sc.x[k];  // the first X is stored at 2^12 whatever the bounds say
+        const Step gram{0.f, float(A / (xs * xs)), from, first};
+        const Step poly{float(B * cb / A), float(B * cc / (A * A)), from, first};
+        const double to = last ? 1.0 : sc.x[k + 1];
+        const Step update{float(to * ca / xs), float(to / (B * xs)), from, first};
+        if (int rc = product<kGram, PL>(plan, gram, none, stream)) return rc;
+        if (int rc = product<kPoly, PL>(plan, poly, none, stream)) return rc;
+        const Apply ap{float(a.lr), a.lr_device, float(a.weight_decay), 1.0f};
+        if (int rc = last ? product<kFinal, PL>(plan, update, ap, stream) : product<kUpdate, PL>(plan, update, none, stream))
+            return rc;
     }
     return MNX_OK;
 }

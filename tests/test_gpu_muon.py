@@ -383,3 +383,37 @@ def test_compiled():
     q, n, x = p.clone(), m.clone(), normal(20, 30, seed=9)
     y = torch.compile(both, fullgraph=True, backend="aot_eager")(p, g, m, x)
     assert torch.equal(y, both(q, g, n, x)) and torch.equal(p, q) and torch.equal(m, n)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,rows,cols", [(64, 200, 300), (128, 250, 200), (40, 300, 700), (16, 900, 700), (9, 1100, 1300)])
+def test_large_calls_are_as_each_matrix_alone(batch, rows, cols, dtype):
+    """Tiles are sized by what a call holds; every element's sum runs in the same order in all of them."""
+    x = normal(batch, rows, cols, seed=batch, dtype=dtype)
+    y = F.orthogonalize(x)
+    for k in (0, batch // 2, batch - 1):
+        assert torch.equal(y[k], F.orthogonalize(x[k]))
+    assert y.isfinite().all()
+
+
+def test_large_matrix():
+    """Of singular values that are known: Q1 diag(s) Q2^T has the result Q1 diag(p(p(...s))) Q2^T."""
+    n, m = 1500, 2300
+    q1, _ = torch.linalg.qr(normal(n, n, seed=1).double())
+    q2, _ = torch.linalg.qr(normal(m, n, seed=2).double())
+    s = torch.logspace(0, -2, n, device=DEV, dtype=torch.float64)
+    x = (q1 * s) @ q2.t().contiguous()
+    for dtype in DTYPES:
+        given = x.to(dtype)
+        a, b, c = COEFF
+        t = s / s.norm()
+        for _ in range(5):
+            t = a * t + b * t ** 3 + c * t ** 5
+        want = (q1 * t) @ q2.t().contiguous()
+        # the input's rounding, which grows 3.5 times a step at most where it lies beside small singular values,
+        # and as much again for the iteration's own roundings (u of it in each of A, B and X, see the top)
+        half = torch.finfo(dtype).eps / 2
+        grown = float((given.double() - x).norm() / s.norm()) * 3.5 ** 5
+        allowed = 2 * grown + half * float(want.norm()) + 25 * U[dtype] * 3.5 ** 5
+        off = float((F.orthogonalize(given).double() - want).norm())
+        assert off <= allowed, (dtype, off, allowed, float(want.norm()))
