@@ -22,6 +22,7 @@
 #include "elem.h"
 
 #include <cmath>
+#include <numeric>
 #include <type_traits>
 #include <vector>
 
@@ -32,6 +33,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kPad = 128;  // sides of the padded matrices are multiples of it
 constexpr int kChunk = 4096;  // elements of a matrix that a workgroup of the momentum kernel takes
@@ -90,11 +92,43 @@ struct Stat {
     float rho;     // X = (u 2^exponent) 2^-12 rho; the first step's sums take rho
 };
 
-__device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) { return load_elem(p, i, dtype); }
-
-// The gradient, and the momentum after this step.
+// u, from the gradient and the momentum after this step.
 __device__ __forceinline__ float direction(float g, float m, const Momentum& h) {
     return h.nesterov ? h.w * g + h.mu * m : m;
+}
+
+// Four consecutive elements, at the alignment of one; `left` of them exist, the others are 0 and not stored.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, int64_t left, float (&v)[4]) {
+    typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (left >= 4) {
+        const Four t = *reinterpret_cast<const Four*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = float(t[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = e < left ? float(p[e]) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int64_t left, const float (&v)[4]) {
+    typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (left >= 4) {
+        Four t;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = T(v[e]);
+        *reinterpret_cast<Four*>(p) = t;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < left) p[e] = T(v[e]);
+    }
+}
+template <typename F>
+__device__ __forceinline__ void by_type(int dtype, F f) {
+    if (dtype == kF32) f(float{});
+    else if (dtype == kBF16) f(__bf16{});
+    else f(_Float16{});
 }
 
 // Momenta, and a partial sum of squares for each chunk of a matrix (float64: squares of any float32).
@@ -106,18 +140,33 @@ __global__ void __launch_bounds__(256) k_muon_momentum(const Mat* __restrict__ t
     const int64_t n = int64_t(t.rows) * t.cols;
     const uint32_t per = uint32_t((n + kChunk - 1) / kChunk), u = unit - t.chunk0;
     const uint32_t which = u / per;
-    const int64_t lo = int64_t(u - which * per) * kChunk, hi = min(lo + kChunk, n), off = which * n;
+    const int64_t lo = int64_t(u - which * per) * kChunk, off = which * n;
     double sum = 0;
-    for (int64_t i = lo + threadIdx.x; i < hi; i += 256) {
-        float v = load_any(t.g, off + i, t.dtype);
-        if (t.m) {
-            if (h.maximize) v = -v;
-            const float m = t.m[off + i] * h.mu + h.w * v;
-            t.m[off + i] = m;
-            v = direction(v, m, h);
+    by_type(t.dtype, [&](auto type) {
+        const auto* g = static_cast<const decltype(type)*>(t.g) + off;
+        float v[kChunk / 1024][4], m[kChunk / 1024][4];
+#pragma unroll
+        for (int k = 0; k < kChunk / 1024; ++k) {
+            const int64_t i = lo + k * 1024 + threadIdx.x * 4;
+            load4(g + i, n - i, v[k]);
+            if (t.m) load4(t.m + off + i, n - i, m[k]);
         }
-        sum += double(v) * double(v);
-    }
+#pragma unroll
+        for (int k = 0; k < kChunk / 1024; ++k) {
+            const int64_t i = lo + k * 1024 + threadIdx.x * 4;
+            if (t.m) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (h.maximize) v[k][e] = -v[k][e];
+                    m[k][e] = m[k][e] * h.mu + h.w * v[k][e];
+                    v[k][e] = direction(v[k][e], m[k][e], h);
+                }
+                store4(t.m + off + i, n - i, m[k]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum += double(v[k][e]) * double(v[k][e]);
+        }
+    });
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     __shared__ double part[4];
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
@@ -125,20 +174,9 @@ __global__ void __launch_bounds__(256) k_muon_momentum(const Mat* __restrict__ t
     if (threadIdx.x == 0) partial[unit] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// The norm of each matrix: a wavefront a matrix.
-__global__ void __launch_bounds__(64) k_muon_norm(const Mat* __restrict__ table, int count,
-                                                  const double* __restrict__ partial, double eps,
-                                                  Stat* __restrict__ stats) {
-    const int at = find_mat(table, count, &Mat::stat0, blockIdx.x);
-    const Mat& t = table[at];
-    const uint32_t per = uint32_t((int64_t(t.rows) * t.cols + kChunk - 1) / kChunk);
-    const double* mine = partial + t.chunk0 + uint64_t(blockIdx.x - t.stat0) * per;
-    double sum = 0;
-    for (uint32_t i = threadIdx.x; i < per; i += 64) sum += mine[i];
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    if (threadIdx.x) return;
+// X = (u 2^exponent) 2^-12 rho for a matrix of this norm.
+__device__ __forceinline__ Stat stat_of(double norm, double eps) {
     Stat s{0, 1.0f};
-    const double norm = sqrt(sum);
     if (!(norm < HUGE_VAL)) s.rho = __builtin_nanf("");  // infinite or NaN somewhere: so is every result
     else if (norm > 0) {
         int e;
@@ -146,14 +184,36 @@ __global__ void __launch_bounds__(64) k_muon_norm(const Mat* __restrict__ table,
         s.exponent = 12 - e;
         s.rho = float(ldexp(1.0, 12 - s.exponent) / fmax(norm, eps));  // 1 to 2 for a norm of eps or more
     }
-    stats[blockIdx.x] = s;
+    return s;
+}
+
+// The norm of each matrix: a workgroup a matrix.
+__global__ void __launch_bounds__(256) k_muon_norm(const Mat* __restrict__ table, int count,
+                                                   const double* __restrict__ partial, double eps,
+                                                   Stat* __restrict__ stats) {
+    const int at = find_mat(table, count, &Mat::stat0, blockIdx.x);
+    const Mat& t = table[at];
+    const uint32_t per = uint32_t((int64_t(t.rows) * t.cols + kChunk - 1) / kChunk);
+    const double* mine = partial + t.chunk0 + uint64_t(blockIdx.x - t.stat0) * per;
+    double sum = 0;
+    for (uint32_t i = threadIdx.x; i < per; i += 256) sum += mine[i];
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    __shared__ double part[4];
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) stats[blockIdx.x] = stat_of(sqrt((part[0] + part[1]) + (part[2] + part[3])), eps);
 }
 
 template <int PL>
-__device__ __forceinline__ void put(_Float16* to, int64_t plane, float v) {
-    const _Float16 hi = _Float16(v);
-    to[0] = hi;
-    if constexpr (PL == 2) to[plane] = _Float16(v - float(hi));
+__device__ __forceinline__ void put4(_Float16* to, int64_t plane, const float (&v)[4]) {
+    half4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        hi[e] = _Float16(v[e]);
+        lo[e] = _Float16(v[e] - float(hi[e]));
+    }
+    *reinterpret_cast<half4*>(to) = hi;
+    if constexpr (PL == 2) *reinterpret_cast<half4*>(to + plane) = lo;
 }
 
 // u in the products' layout, zeros around it.
@@ -172,25 +232,36 @@ __global__ void __launch_bounds__(256) k_muon_cast(const Mat* __restrict__ table
     const Stat s = stats[t.stat0 + which];
     const bool tall = t.rows > t.cols;
     const int i0 = tall ? c0 : r0, j0 = tall ? r0 : c0;  // of the tensor's own rows and columns
-    for (int k = threadIdx.x; k < kCast * kCast; k += 256) {
-        const int i = i0 + k / kCast, j = j0 + k % kCast;
-        float v = 0;
-        if (i < t.rows && j < t.cols) {
-            const int64_t e = off + int64_t(i) * t.cols + j;
-            v = load_any(t.g, e, t.dtype);
-            if (t.m) {
-                if (h.maximize) v = -v;
-                v = direction(v, t.m[e], h);
-            }
-            v = ldexpf(v, s.exponent);
+    const int row = threadIdx.x / 16, col = threadIdx.x % 16 * 4;
+    _Float16* x = t.x[0] + int64_t(which) * t.rp * t.cp + int64_t(r0) * t.cp + c0;
+    float v[4][4], m[4][4];
+    by_type(t.dtype, [&](auto type) {
+        const auto* g = static_cast<const decltype(type)*>(t.g) + off;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = i0 + row + 16 * k, left = i < t.rows ? t.cols - j0 - col : 0;
+            const int64_t e = int64_t(i) * t.cols + j0 + col;
+            load4(g + e, left, v[k]);
+            if (t.m) load4(t.m + off + e, left, m[k]);
         }
-        tile[k / kCast][k % kCast] = v;
+    });
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (t.m) v[k][e] = direction(h.maximize ? -v[k][e] : v[k][e], m[k][e], h);
+            v[k][e] = ldexpf(v[k][e], s.exponent);
+            if (tall) tile[row + 16 * k][col + e] = v[k][e];
+        }
+        if (!tall) put4<PL>(x + int64_t(row + 16 * k) * t.cp + col, t.xplane, v[k]);
     }
+    if (!tall) return;
     __syncthreads();
-    _Float16* x = t.x[0] + int64_t(which) * t.rp * t.cp;
-    for (int k = threadIdx.x; k < kCast * kCast; k += 256) {
-        const int i = k / kCast, j = k % kCast;
-        put<PL>(x + int64_t(r0 + i) * t.cp + c0 + j, t.xplane, tall ? tile[j][i] : tile[i][j]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[k][e] = tile[col + e][row + 16 * k];
+        put4<PL>(x + int64_t(row + 16 * k) * t.cp + col, t.xplane, v[k]);
     }
 }
 
@@ -235,27 +306,40 @@ __device__ __forceinline__ half8 read_tr(const _Float16* lo, const _Float16* hi)
     return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// Four values of the last X, at columns j of row i, go into the parameters (or are the result); `count` of them exist.
-template <typename T, bool TALL>
-__device__ __forceinline__ void apply(T* p, int cols, int i, int j, int count, float decay, float rate,
-                                      const float (&v)[4]) {
-    typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    const int64_t at = TALL ? int64_t(j) * cols + i : int64_t(i) * cols + j, step = TALL ? cols : 1;
-    if (!TALL && count >= 4) {
-        Four* q = reinterpret_cast<Four*>(p + at);
-        Four o = {};
-        if (decay != 0) o = *q;
+// Eight consecutive parameters (or results) from p on, of which `count` exist.
+template <typename T>
+__device__ __forceinline__ void apply(T* p, int count, float decay, float rate, const float (&v)[8]) {
+    typedef T Eight __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    if (count >= 8) {
+        Eight o = {};
+        if (decay != 0) o = *reinterpret_cast<const Eight*>(p);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = T(decay * float(o[e]) - rate * v[e]);
-        *q = o;
-        return;
+        for (int e = 0; e < 8; ++e) o[e] = T(decay * float(o[e]) - rate * v[e]);
+        *reinterpret_cast<Eight*>(p) = o;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < count) p[e] = T((decay != 0 ? decay * float(p[e]) : 0.f) - rate * v[e]);
     }
-    float old[4];
+}
+
+template <int PL>
+__device__ __forceinline__ void put8(_Float16* to, int64_t plane, const float (&v)[8]) {
+    half8 hi, lo;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) old[e] = decay != 0 && e < count ? float(p[at + e * step]) : 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (e < count) p[at + e * step] = T(decay * old[e] - rate * v[e]);
+    for (int e = 0; e < 8; ++e) {
+        hi[e] = _Float16(v[e]);
+        lo[e] = _Float16(v[e] - float(hi[e]));
+    }
+    *reinterpret_cast<half8*>(to) = hi;
+    if constexpr (PL == 2) *reinterpret_cast<half8*>(to + plane) = lo;
+}
+
+// LDS that one lane wrote is read by others of the wavefront.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 constexpr int kKC = 64;  // k of a chunk
@@ -281,12 +365,14 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
     constexpr int SEG = PL == 1 ? 1 : 3;
     constexpr int FETCH = BT / 32;  // loads a lane of either operand's chunk
     constexpr int PIECES = BT / 8;  // of a sum's columns
-    __shared__ _Float16 sI0[BT * kKC], sI1[BT * kKC], sJ0[BT * kKC], sJ1[BT * kKC];
+    constexpr int BUFS = BT == 64 ? 6 : 2;
+    __shared__ _Float16 lds[2 * BUFS * BT * kKC];
+    _Float16 *const sI0 = lds, *const sI1 = sI0 + BT * kKC, *const sJ0 = sI1 + BT * kKC, *const sJ1 = sJ0 + BT * kKC;
     const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave & 1, wj = wave >> 1;
-    const uint32_t per = (units + 7) / 8;
-    uint32_t u = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    // 16 tiles next to each other run on one XCD (workgroups are dealt to the eight in turn)
+    uint32_t u = (((blockIdx.x >> 7) << 3 | (blockIdx.x & 7)) << 4) | (blockIdx.x >> 3 & 15);
     if (u >= units) return;
     const int at = find_mat(table, count, SYM ? &Mat::sym0 : &Mat::upd0, u);
     const Mat& t = table[at];
@@ -335,7 +421,7 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
 #pragma unroll
         for (int n = 0; n < FETCH; ++n) {
             const int piece = (n * 4 + wave) * 64 + lane, k = piece / PIECES, c = piece % PIECES;
-            const int turn = BT == 192 ? ((k >> 1) & 1) << 2 : (k & 3) << 2;
+            const int turn = BT % 128 ? ((k >> 1) & 1) << 2 : (k & 3) << 2;
             jrow[n] = 2 * (uint32_t(k) * t.cp + ((c ^ turn) << 3));
         }
     }
@@ -365,7 +451,7 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
     };
     const int ki = (wi * W + l32) * kKC, kj = (wj * W + l32) * kKC, turn = (l32 >> 1) & 7;  // 32 rows on turn alike
     const int trow = 8 * half + ((lane & 15) >> 2), tcol = wj * W + (l32 & 16) + (lane & 3) * 4;
-    const int tturn = BT == 192 ? ((trow >> 1) & 1) << 2 : (trow & 3) << 2;
+    const int tturn = BT % 128 ? ((trow >> 1) & 1) << 2 : (trow & 3) << 2;
     auto read_i = [&](int m, int ks, const _Float16* bi) {
         return *reinterpret_cast<const half8*>(bi + ki + m * 32 * kKC + (((2 * ks + half) ^ turn) << 3));
     };
@@ -424,28 +510,58 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
     };
     const std::true_type yes;
     const std::false_type no;
-    {
-        const Source f = source(0), g = source(1);
+    if constexpr (BT == 64) {
+        // Few tiles: the latency of a chunk counts, not the products.  Six buffers, and five chunks on their way.
+        auto buf = [&](int c) { return lds + c % BUFS * 2 * BT * kKC; };
+        auto load = [&](int c) {
+            const Source f = source(c);
 #pragma unroll
-        for (int n = 0; n < 2 * FETCH; ++n) fetch(f, n, sI0, sJ0);
-        arrived();
+            for (int n = 0; n < 2 * FETCH; ++n) fetch(f, n, buf(c), buf(c) + BT * kKC);
+        };
+        for (int c = 0; c < min(BUFS - 1, chunks); ++c) load(c);
+        for (int c = 0; c < chunks; ++c) {
+            // this chunk has come when no more than the later ones' loads are out
+            if (c + BUFS - 1 <= chunks) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(2 * FETCH * (BUFS - 2)) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (c + BUFS - 1 < chunks) load(c + BUFS - 1);  // into the buffer of the chunk before, which everyone has read
+            const _Float16 *bi = buf(c), *bj = bi + BT * kKC;
+            Frags f[4];
 #pragma unroll
-        for (int n = 0; n < FETCH; ++n) fetch(g, n, sI1, sJ1);
+            for (int ks = 0; ks < 4; ++ks) {
+                f[ks].i[0] = read_i(0, ks, bi);
+                f[ks].j[0] = read_j(0, ks, bj);
+            }
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            f0.i[m] = read_i(m, 0, sI0);
-            f0.j[m] = read_j(m, 0, sJ0);
+            for (int ks = 0; ks < 4; ++ks) acc[0][0] = mfma(f[ks].j[0], f[ks].i[0], acc[0][0]);
         }
+    } else {
+        {
+            const Source f = source(0), g = source(1);
+    #pragma unroll
+            for (int n = 0; n < 2 * FETCH; ++n) fetch(f, n, sI0, sJ0);
+            arrived();
+    #pragma unroll
+            for (int n = 0; n < FETCH; ++n) fetch(g, n, sI1, sJ1);
+    #pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                f0.i[m] = read_i(m, 0, sI0);
+                f0.j[m] = read_j(m, 0, sJ0);
+            }
+        }
+        int c = 0;  // chunks are an even number: K is a multiple of 128
+        for (; c + 2 < chunks; c += 2) {
+            body(c, sI0, sJ0, sI1, sJ1, yes, yes);
+            body(c + 1, sI1, sJ1, sI0, sJ0, yes, yes);
+        }
+        body(c, sI0, sJ0, sI1, sJ1, yes, no);
+        body(c + 1, sI1, sJ1, sI0, sJ0, no, no);
     }
-    int c = 0;  // chunks are an even number: K is a multiple of 128
-    for (; c + 2 < chunks; c += 2) {
-        body(c, sI0, sJ0, sI1, sJ1, yes, yes);
-        body(c + 1, sI1, sJ1, sI0, sJ0, yes, yes);
-    }
-    body(c, sI0, sJ0, sI1, sJ1, yes, no);
-    body(c + 1, sI1, sJ1, sI0, sJ0, no, no);
 
-    // acc[m][n][q] belongs to row i = 32 m + l32 and column j = 32 n + 8 (q / 4) + 4 half + q % 4 of the wave's part
+    // The result, 32 rows of a wavefront's part at a time by way of LDS (its own part of it), from where rows and, for the
+    // second place of a symmetric one and for tall matrices' parameters, columns leave 8 values a lane.  acc[m][n][q] is
+    // of row 32 m + l32 and column 32 n + 8 (q / 4) + 4 half + q % 4.
     float own = s.own, prod = s.prod;
     if (s.first) {
         const float rho = stats[t.stat0 + which].rho;
@@ -459,75 +575,365 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
     const int64_t oplane = SYM ? t.aplane : t.xplane;
     const _Float16* E = MODE == kPoly ? A : X;
     _Float16* out = (MODE == kGram ? t.a : MODE == kPoly ? t.b : t.x[s.from ^ 1]) + int64_t(which) * t.rp * ld;
-    const int i0 = ti * BT + wi * W + l32, j0 = tj * BT + wj * W + 4 * half;
-    const int rows = MODE == kFinal ? t.r : t.rp, cols = MODE == kFinal ? t.c : SYM ? t.rp : t.cp;
     float decay = 0, rate = -ap.inv;  // of p and of its change; the result itself has no p
     if (MODE == kFinal && t.m) {
         const float lr = ap.lr_device ? *ap.lr_device : ap.lr;
         decay = 1 - lr * ap.wd;
         rate = lr * t.adjust * ap.inv;
     }
-    // every four consecutive columns of a row
-    auto each = [&](auto store) {
+    const bool tall = t.rows > t.cols;
+    const int64_t off = int64_t(which) * t.rows * t.cols;
+    // Symmetric results are stored from the diagonal downwards and from there above it, on the diagonal's own 32 x 32 blocks
+    // too: the two halves' sums run in different orders with pairs, and results would differ with the size of tiles.
+    const bool columns = SYM || (MODE == kFinal && tall), corner = SYM && ti == tj && wi == wj;
+    constexpr int LD = W + 4, ITEMS = W / 16;  // items of 8 values a lane
+    float* part = reinterpret_cast<float*>(lds + wave * BT * kKC);
+    const int j0 = tj * BT + wj * W;
+    __syncthreads();
+    if (SYM && ti == tj && wi < wj) return;  // above the diagonal
+    auto strip = [&](auto type, auto at_m) {
+        constexpr int m = decltype(at_m)::value;
+        auto* p = static_cast<decltype(type)*>(t.p) + off;
+        const int i0 = ti * BT + wi * W + 32 * m;
+        half8 old[MODE == kGram ? 1 : PL][ITEMS];
+        if constexpr (MODE != kGram) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+            for (int it = 0; it < ITEMS; ++it) {
+                const int item = it * 64 + lane, i = i0 + item / (W / 8), j = j0 + item % (W / 8) * 8;
 #pragma unroll
-            for (int n = 0; n < MT; ++n)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int i = i0 + m * 32, j = j0 + n * 32 + 8 * q;
-                    if (i >= rows || j >= cols) continue;
-                    float v[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = prod * acc[m][n][4 * q + e];
-                    if constexpr (MODE != kGram) {
-#pragma unroll
-                        for (int pl = PL - 1; pl >= 0; --pl) {
-                            const half4 old = *reinterpret_cast<const half4*>(E + pl * oplane + int64_t(i) * ld + j);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) v[e] += own * float(old[e]);
-                        }
-                    }
-                    store(i, j, v);
-                }
-    };
-    if constexpr (MODE == kFinal) {
-        auto as = [&](auto type, auto tall) {
-            auto* p = static_cast<decltype(type)*>(t.p) + int64_t(which) * t.rows * t.cols;
-            each([&](int i, int j, const float (&v)[4]) {
-                apply<decltype(type), decltype(tall)::value>(p, t.cols, i, j, cols - j, decay, rate, v);
-            });
-        };
-        const bool tall = t.rows > t.cols;
-        if constexpr (PL == 1) {
-            if (tall) as(__bf16{}, yes);
-            else as(__bf16{}, no);
-        } else if (t.dtype == kF32) {
-            if (tall) as(float{}, yes);
-            else as(float{}, no);
-        } else {
-            if (tall) as(_Float16{}, yes);
-            else as(_Float16{}, no);
-        }
-    } else {
-        each([&](int i, int j, const float (&v)[4]) {
-            half4 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                hi[e] = _Float16(v[e]);
-                lo[e] = _Float16(v[e] - float(hi[e]));
+                for (int pl = 0; pl < PL; ++pl)
+                    if (i < t.rp && j < ld) old[pl][it] = *reinterpret_cast<const half8*>(E + pl * oplane + int64_t(i) * ld + j);
             }
-            *reinterpret_cast<half4*>(out + int64_t(i) * ld + j) = hi;
-            if constexpr (PL == 2) *reinterpret_cast<half4*>(out + oplane + int64_t(i) * ld + j) = lo;
-            if (SYM && ti != tj) {
+        }
+#pragma unroll
+        for (int n = 0; n < MT; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = prod * acc[m][n][4 * q + e];
+                *reinterpret_cast<f32x4*>(part + l32 * LD + 32 * n + 8 * q + 4 * half) = v;
+            }
+        wave_sync();
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+            const int item = it * 64 + lane, r = item / (W / 8), i = i0 + r, jj = item % (W / 8) * 8, j = j0 + jj;
+            const int block = corner ? (jj >> 5) - m : -1;  // 0: the diagonal's; above it, nothing is stored
+            if (i >= t.rp || j >= ld || block > 0) continue;
+            float v[8];
+            if (block < 0) {
+                *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(part + r * LD + jj);
+                *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(part + r * LD + jj + 4);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int c = jj + e - 32 * m;
+                    v[e] = part[max(r, c) * LD + 32 * m + min(r, c)];
+                }
+            }
+            if constexpr (MODE != kGram) {
+#pragma unroll
+                for (int pl = PL - 1; pl >= 0; --pl)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += own * float(old[pl][it][e]);
+                if (columns && block < 0) {
+                    *reinterpret_cast<f32x4*>(part + r * LD + jj) = *reinterpret_cast<const f32x4*>(v);
+                    *reinterpret_cast<f32x4*>(part + r * LD + jj + 4) = *reinterpret_cast<const f32x4*>(v + 4);
+                }
+            }
+            if constexpr (MODE == kFinal) {
+                if (!tall && i < t.r) apply(p + int64_t(i) * t.cols + j, t.c - j, decay, rate, v);
+            } else {
+                put8<PL>(out + int64_t(i) * ld + j, oplane, v);
+            }
+        }
+        wave_sync();
+        if (columns) {
+#pragma unroll
+            for (int it = 0; it < ITEMS; ++it) {
+                const int item = it * 64 + lane, jj = item / 4, j = j0 + jj, r = item % 4 * 8, i = i0 + r;
+                if (i >= t.rp || j >= ld || (corner && (jj >> 5) >= m)) continue;
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = part[(r + e) * LD + jj];
+                if constexpr (MODE == kFinal) {
+                    if (j < t.c) apply(p + int64_t(j) * t.cols + i, t.r - i, decay, rate, v);
+                } else {
+                    put8<PL>(out + int64_t(j) * ld + i, oplane, v);
+                }
+            }
+            wave_sync();
+        }
+    };
+    auto strips = [&](auto type) {
+        strip(type, std::integral_constant<int, 0>());
+        if constexpr (MT > 1) strip(type, std::integral_constant<int, 1>());
+        if constexpr (MT > 2) strip(type, std::integral_constant<int, 2>());
+        if constexpr (MT > 3) strip(type, std::integral_constant<int, 3>());
+    };
+    if constexpr (MODE != kFinal || PL == 1) strips(__bf16{});  // matrices of one plane are bfloat16
+    else if (t.dtype == kF32) strips(float{});
+    else strips(_Float16{});
+}
+
+// ---------------------------------------------------------------------------
+// Small matrices
+// ---------------------------------------------------------------------------
+
+// Rows of a small matrix in LDS: 48 bytes more than their values, so that 16 rows' pieces of 16 bytes meet every bank once.
+inline __host__ __device__ int small_row(int cols) { return 2 * cols + 48; }
+
+// Bytes that X and A of an r x c matrix take there.
+inline int64_t small_bytes(int planes, int64_t r, int64_t c) {
+    const int64_t rq = ceil_div(r, 32) * 32, cq = ceil_div(c, 32) * 32;
+    return planes * rq * (small_row(int(rq)) + 2 * cq + 48);
+}
+
+constexpr int kSmallThreads = 512, kSmallSide = 128;  // the smaller side's limit: four blocks of 32 rows
+constexpr int kSmallLds[] = {48 << 10, (160 << 10) - 512};
+
+// The factors of every step.
+struct Steps {
+    float gram[MNX_MUON_MAX_STEPS], poly_own[MNX_MUON_MAX_STEPS], poly[MNX_MUON_MAX_STEPS], own[MNX_MUON_MAX_STEPS],
+        prod[MNX_MUON_MAX_STEPS];
+    int count;
+};
+
+// A whole matrix in one workgroup, from its gradient to its parameters: X and A (then B) stay in LDS.  The tiled products
+// take eight microseconds a launch however little there is to do, three launches a step.
+//
+// Eight wavefronts share the blocks of 32 x 32 of A and B on and below the diagonal, and the columns of X, 32 at a time: a
+// wavefront's columns of a X + B X read nothing of X but these columns, so they are replaced in place.  Pairs sum hi hi and
+// the two cross products apart, and add them at the end.
+template <int PL, int LDS>
+__global__ void __launch_bounds__(kSmallThreads) k_muon_small(const Mat* __restrict__ table, int count, Momentum h,
+                                                              double eps, Steps st, Apply ap) {
+    __shared__ __attribute__((aligned(16))) char lds[LDS];
+    __shared__ double part[kSmallThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int WAVES = kSmallThreads / 64;
+    const int at = find_mat(table, count, &Mat::stat0, blockIdx.x);
+    const Mat& t = table[at];
+    const int64_t n = int64_t(t.rows) * t.cols, off = int64_t(blockIdx.x - t.stat0) * n;
+    const bool tall = t.rows > t.cols;
+    const int rb = (t.r + 31) / 32, cb = (t.c + 31) / 32;  // blocks of 32
+    const int sx = small_row(32 * cb), sa = small_row(32 * rb);
+    char* const X = lds;
+    char* const A = lds + PL * 32 * rb * sx;
+    const int xplane = 32 * rb * sx, aplane = 32 * rb * sa;
+
+    // momenta and the norm
+    double sum = 0;
+    by_type(t.dtype, [&](auto type) {
+        const auto* g = static_cast<const decltype(type)*>(t.g) + off;
+        for (int64_t i = tid * 4; i < n; i += kSmallThreads * 4) {
+            float v[4], m[4];
+            load4(g + i, n - i, v);
+            if (t.m) {
+                load4(t.m + off + i, n - i, m);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int64_t mirror = int64_t(j + e) * ld + i;
-                    out[mirror] = hi[e];
-                    if constexpr (PL == 2) out[oplane + mirror] = lo[e];
+                    if (h.maximize) v[e] = -v[e];
+                    m[e] = m[e] * h.mu + h.w * v[e];
+                    v[e] = direction(v[e], m[e], h);
+                }
+                store4(t.m + off + i, n - i, m);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum += double(v[e]) * double(v[e]);
+        }
+    });
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    if (lane == 0) part[wave] = sum;
+    __syncthreads();
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) sum += part[w];
+    const Stat stat = stat_of(sqrt(sum), eps);
+
+    // X: u by its own rows, four of their values a thread
+    by_type(t.dtype, [&](auto type) {
+        const auto* g = static_cast<const decltype(type)*>(t.g) + off;
+        const int rows = 32 * (tall ? cb : rb), vecs = 8 * (tall ? rb : cb);
+        for (int it = tid; it < rows * vecs; it += kSmallThreads) {
+            const int i = it / vecs, j = it % vecs * 4, left = i < t.rows ? t.cols - j : 0;
+            float v[4], m[4];
+            load4(g + int64_t(i) * t.cols + j, left, v);
+            if (t.m) load4(t.m + off + int64_t(i) * t.cols + j, left, m);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (t.m) v[e] = direction(h.maximize ? -v[e] : v[e], m[e], h);
+                v[e] = ldexpf(v[e], stat.exponent);
+            }
+            if (!tall) {
+                put4<PL>(reinterpret_cast<_Float16*>(X + i * sx + 2 * j), xplane / 2, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    _Float16* to = reinterpret_cast<_Float16*>(X + (j + e) * sx + 2 * i);
+                    to[0] = _Float16(v[e]);
+                    if constexpr (PL == 2) to[xplane / 2] = _Float16(v[e] - float(to[0]));
                 }
             }
-        });
+        }
+    });
+    __syncthreads();
+
+    auto rows_of = [&](const char* base, int stride, int block, int k) {
+        return *reinterpret_cast<const half8*>(base + (32 * block + l32) * stride + 2 * (k + 8 * half));
+    };
+    auto cols_of = [&](const char* base, int stride, int block, int k) {
+        const char* q = base + (k + 8 * half + ((lane & 15) >> 2)) * stride + 2 * (32 * block + (l32 & 16) + (lane & 3) * 4);
+        return read_tr(reinterpret_cast<const _Float16*>(q), reinterpret_cast<const _Float16*>(q + 4 * stride));
+    };
+    auto zero = [] {
+        f32x16 z;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) z[q] = 0.f;
+        return z;
+    };
+    // block (bi, bj) of the product of S's rows with themselves
+    auto square = [&](const char* S, int stride, int plane, int bi, int bj, int K) {
+        f32x16 big = zero(), small = zero();
+#pragma unroll 4
+        for (int k = 0; k < K; k += 16) {
+            const half8 i = rows_of(S, stride, bi, k), j = rows_of(S, stride, bj, k);
+            if constexpr (PL == 2) {
+                const half8 il = rows_of(S + plane, stride, bi, k), jl = rows_of(S + plane, stride, bj, k);
+                small = mfma(jl, i, small);
+                small = mfma(j, il, small);
+            }
+            big = mfma(j, i, big);
+        }
+        return PL == 2 ? big + small : big;
+    };
+    // the block's values into A, above the diagonal too; `own` of what is there
+    auto into_a = [&](const f32x16& acc, int bi, int bj, float own, float prod) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int i = 32 * bi + l32, j = 32 * bj + 8 * q + 4 * half;
+            _Float16* to = reinterpret_cast<_Float16*>(A + i * sa + 2 * j);
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = prod * acc[4 * q + e];
+            if (own != 0) {
+#pragma unroll
+                for (int pl = PL - 1; pl >= 0; --pl) {
+                    const half4 old = *reinterpret_cast<const half4*>(to + pl * (aplane / 2));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += own * float(old[e]);
+                }
+            }
+            put4<PL>(to, aplane / 2, v);
+            if (bi != bj) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    _Float16* mirror = reinterpret_cast<_Float16*>(A + (j + e) * sa + 2 * i);
+                    const _Float16 hi = _Float16(v[e]);
+                    mirror[0] = hi;
+                    if constexpr (PL == 2) mirror[aplane / 2] = _Float16(v[e] - float(hi));
+                }
+            }
+        }
+    };
+    auto block_of = [](int b, int& bi, int& bj) {  // the b-th on and below the diagonal
+        bi = b >= 6 ? 3 : b >= 3 ? 2 : b >= 1 ? 1 : 0;
+        bj = b - bi * (bi + 1) / 2;
+    };
+    const int blocks = rb * (rb + 1) / 2;
+    float decay = 0, rate = -ap.inv;
+    if (t.m) {
+        const float lr = ap.lr_device ? *ap.lr_device : ap.lr;
+        decay = 1 - lr * ap.wd;
+        rate = lr * t.adjust * ap.inv;
+    }
+#pragma unroll 1
+    for (int step = 0; step < st.count; ++step) {
+        const float rho = step == 0 ? stat.rho : 1.f;
+        for (int b = wave; b < blocks; b += WAVES) {
+            int bi, bj;
+            block_of(b, bi, bj);
+            into_a(square(X, sx, xplane, bi, bj, 32 * cb), bi, bj, 0.f, st.gram[step] * rho * rho);
+        }
+        __syncthreads();
+        {
+            int bi[2], bj[2];
+            f32x16 acc[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int b = wave + k * WAVES;
+                if (b < blocks) {
+                    block_of(b, bi[k], bj[k]);
+                    acc[k] = square(A, sa, aplane, bi[k], bj[k], 32 * rb);
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (wave + k * WAVES < blocks) into_a(acc[k], bi[k], bj[k], st.poly_own[step], st.poly[step]);
+        }
+        __syncthreads();
+        const float own = st.own[step] * rho, prod = st.prod[step] * rho;
+        const bool last = step + 1 == st.count;
+        for (int bj = wave; bj < cb; bj += WAVES) {
+            f32x16 big[4], small[PL == 2 ? 4 : 1];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                big[r] = zero();
+                if constexpr (PL == 2) small[r] = zero();
+            }
+#pragma unroll 2
+            for (int k = 0; k < 32 * rb; k += 16) {
+                const half8 j = cols_of(X, sx, bj, k);
+                half8 jl;
+                if constexpr (PL == 2) jl = cols_of(X + xplane, sx, bj, k);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (r >= rb) continue;
+                    const half8 i = rows_of(A, sa, r, k);
+                    if constexpr (PL == 2) {
+                        const half8 il = rows_of(A + aplane, sa, r, k);
+                        small[r] = mfma(jl, i, small[r]);
+                        small[r] = mfma(j, il, small[r]);
+                    }
+                    big[r] = mfma(j, i, big[r]);
+                }
+            }
+            wave_sync();
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (r >= rb) continue;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int i = 32 * r + l32, j = 32 * bj + 8 * q + 4 * half;
+                    _Float16* to = reinterpret_cast<_Float16*>(X + i * sx + 2 * j);
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = prod * (PL == 2 ? big[r][4 * q + e] + small[PL == 2 ? r : 0][4 * q + e] : big[r][4 * q + e]);
+#pragma unroll
+                    for (int pl = PL - 1; pl >= 0; --pl) {
+                        const half4 old = *reinterpret_cast<const half4*>(to + pl * (xplane / 2));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] += own * float(old[e]);
+                    }
+                    put4<PL>(to, xplane / 2, v);
+                    if (!last || i >= t.r) continue;
+                    by_type(t.dtype, [&](auto type) {
+                        auto* p = static_cast<decltype(type)*>(t.p) + off;
+                        const int step_ = tall ? t.cols : 1;
+                        auto* to_p = p + (tall ? int64_t(j) * t.cols + i : int64_t(i) * t.cols + j);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (j + e < t.c) {
+                                const float o = decay != 0 ? decay * float(to_p[int64_t(e) * step_]) : 0.f;
+                                to_p[int64_t(e) * step_] = decltype(type)(o - rate * v[e]);
+                            }
+                    });
+                }
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -577,6 +983,7 @@ struct Plan {
     uint32_t stats = 0;
     size_t bytes = 0;
     int sym_tile = 128, upd_tile = 128;
+    int64_t lds = 0;
     double* partial = nullptr;
     Stat* stat = nullptr;
     Mat* table = nullptr;
@@ -605,26 +1012,49 @@ inline int64_t tiles_of(const Mat& t, bool sym, int tile) {
     return t.batch * (sym ? ni * (ni + 1) / 2 : ni * nj);
 }
 
-constexpr int kTile[] = {256, 192, 128}, kTiles = 3;
+constexpr int kTile[] = {256, 192, 128, 64}, kTiles = 4;
 
-// The time of a launch, about: rounds of the tiles that the card holds at once (256 CUs; two tiles of 128 a CU), by what a
-// tile takes.
-double cost(const std::vector<Mat>& mats, bool sym, int tile) {
+// The time of a launch, about, in microseconds: a tile's begin and end take 4, a chunk of 64 k 1.95 (256), 1.03 (192), 0.5
+// (128) or 0.13 (64), 1.29 where two of 128 share a CU; the card holds 256 tiles at once (or 512), the longest first.
+double cost(const std::vector<Mat>& mats, int planes, int kind, int tile) {
     double tiles = 0;
-    for (const Mat& t : mats) tiles += double(tiles_of(t, sym, tile));
-    const double slots = tile == 128 ? 512 : 256, each = tile == 256 ? 4.0 : tile == 192 ? 2.4 : 2.2;
-    return std::ceil(tiles / slots) * each;
+    for (const Mat& t : mats) tiles += double(tiles_of(t, kind != kUpdate, tile));
+    const bool two = tile == 128 && tiles > 256;
+    const double slots = two ? 512 : 256;
+    const double chunk = tile == 256 ? 1.95 : tile == 192 ? 1.03 : two ? 1.29 : tile == 128 ? 0.5 : 0.13;
+    double all = 0, longest = 0, shortest = HUGE_VAL;
+    for (const Mat& t : mats) {
+        const double one = 4 + chunk * (planes == 2 ? 3 : 1) * double(kind == kGram ? t.cp : t.rp) / kKC;
+        all += one * double(tiles_of(t, kind != kUpdate, tile));
+        longest = std::max(longest, one);
+        shortest = std::min(shortest, one);
+    }
+    return std::max(longest, std::ceil(all / slots / shortest - 0.01) * shortest);
 }
 
 // float16 numbers that stand for one of X, A and B
 inline int planes_of(int dtype) { return dtype == kBF16 ? 1 : 2; }
 
-// Lays the tensors of `planes` planes out over the workspace (from `base`, which may be null for its size alone).
-int lay_out(const mnx_muon_args& a, int planes, char* base, Plan& plan) {
+// Whether one workgroup takes a whole matrix.  128 x 128 float32 takes 35 us so, 150 with tiles.
+inline bool is_small(int planes, int64_t rows, int64_t cols) {
+    return std::min(rows, cols) <= kSmallSide && std::max(rows, cols) <= 4096 &&
+           small_bytes(planes, std::min(rows, cols), std::max(rows, cols)) <= kSmallLds[1];
+}
+
+// Lays the tensors of `planes` planes, those of small matrices or the others, out over the workspace (from `base`, which may be null for its size alone).
+int lay_out(const mnx_muon_args& a, int planes, bool small, char* base, Plan& plan) {
     Workspace ws{base, 0};
     uint64_t chunk = 0, cast = 0, stat = 0;
-    for (int64_t i = 0; i < a.count; ++i) {
-        if (planes_of(a.dtype[i]) != planes || !a.batch[i] || !a.rows[i] || !a.cols[i]) continue;
+    std::vector<int64_t> order(size_t(a.count));  // the largest first: their tiles take longest
+    std::iota(order.begin(), order.end(), int64_t(0));
+    std::stable_sort(order.begin(), order.end(), [&](int64_t i, int64_t j) {
+        const int64_t x = std::min(a.rows[i], a.cols[i]), y = std::min(a.rows[j], a.cols[j]);
+        return x != y ? x > y : std::max(a.rows[i], a.cols[i]) > std::max(a.rows[j], a.cols[j]);
+    });
+    for (const int64_t i : order) {
+        if (!a.batch[i] || !a.rows[i] || !a.cols[i] || planes_of(a.dtype[i]) != planes ||
+            is_small(planes, a.rows[i], a.cols[i]) != small)
+            continue;
         Mat t{};
         t.rows = int32_t(a.rows[i]);
         t.cols = int32_t(a.cols[i]);
@@ -646,6 +1076,12 @@ int lay_out(const mnx_muon_args& a, int planes, char* base, Plan& plan) {
         t.cast0 = uint32_t(cast);
         const uint64_t b = uint64_t(a.batch[i]);
         stat += b;
+        if (small) {
+            plan.lds = std::max(plan.lds, small_bytes(planes, t.r, t.c));
+            MNX_REQUIRE(stat < (1u << 22), "muon: too many matrices in one call");
+            plan.mat.push_back(t);
+            continue;
+        }
         chunk += b * uint64_t(ceil_div(int64_t(t.rows) * t.cols, kChunk));
         cast += b * uint64_t(t.rp / kCast) * (t.cp / kCast);
         for (_Float16*& x : t.x) x = ws.take<_Float16>(size_t(planes * t.xplane));
@@ -655,19 +1091,32 @@ int lay_out(const mnx_muon_args& a, int planes, char* base, Plan& plan) {
         MNX_REQUIRE(std::max({chunk, cast, stat}) < (1u << 23), "muon: too many matrices in one call");
         plan.mat.push_back(t);
     }
-    for (int kind = 0; kind < 2; ++kind) {
+    if (small) {
+        plan.stats = uint32_t(stat);
+        plan.table = ws.take<Mat>(plan.mat.size());
+        plan.bytes = ws.used;
+        return MNX_OK;
+    }
+    for (int kind : {kGram, kUpdate}) {
         int best = 0;
-        for (int k = 1; k < kTiles; ++k)
-            if (cost(plan.mat, kind == 0, kTile[k]) < cost(plan.mat, kind == 0, kTile[best])) best = k;
-        (kind == 0 ? plan.sym_tile : plan.upd_tile) = kTile[best];
+        double least = HUGE_VAL;
+        for (int k = 0; k < kTiles; ++k) {
+            const double c = cost(plan.mat, planes, kind, kTile[k]);
+            if (c < least) {
+                least = c;
+                best = k;
+            }
+        }
+        (kind == kGram ? plan.sym_tile : plan.upd_tile) = kTile[best];
     }
     uint64_t sym = 0, upd = 0;
     for (Mat& t : plan.mat) {
         t.sym0 = uint32_t(sym);
         t.upd0 = uint32_t(upd);
-        sym += tiles_of(t, true, plan.sym_tile);
-        upd += tiles_of(t, false, plan.upd_tile);
+        sym += uint64_t(tiles_of(t, true, plan.sym_tile));
+        upd += uint64_t(tiles_of(t, false, plan.upd_tile));
     }
+    MNX_REQUIRE(std::max(sym, upd) < (1u << 23), "muon: too many matrices in one call");
     plan.total = {uint32_t(chunk), uint32_t(cast), uint32_t(sym), uint32_t(upd)};
     // the last tiles read past the last matrix
     int64_t past = 0;
@@ -685,19 +1134,18 @@ template <int MODE, int PL>
 int product(const Plan& plan, const Step& s, const Apply& ap, mnx_stream_t stream) {
     constexpr bool SYM = MODE == kGram || MODE == kPoly;
     const int tile = SYM ? plan.sym_tile : plan.upd_tile;
-    const uint32_t units = SYM ? plan.total.sym : plan.total.upd, grid = uint32_t(up(units, 8));
+    const uint32_t units = SYM ? plan.total.sym : plan.total.upd, grid = uint32_t(up(units, 128));
     const int count = int(plan.mat.size());
     const auto kernel = tile == 256 ? k_muon_product<MODE, PL, 256>
-                                    : tile == 192 ? k_muon_product<MODE, PL, 192> : k_muon_product<MODE, PL, 128>;
+                        : tile == 192 ? k_muon_product<MODE, PL, 192>
+                        : tile == 128 ? k_muon_product<MODE, PL, 128> : k_muon_product<MODE, PL, 64>;
     kernel<<<grid, 256, 0, stream>>>(plan.table, count, units, s, plan.stat, ap);
     MNX_CHECK_LAUNCH();
     return MNX_OK;
 }
 
-template <int PL>
-int run(const mnx_muon_args& a, const Plan& plan, const Scales& sc, mnx_stream_t stream) {
+int write_table(const Plan& plan, mnx_stream_t stream) {
     const int count = int(plan.mat.size());
-    if (!count) return MNX_OK;
     for (int at = 0; at < count; at += kTableArgs) {
         TableArgs t;
         t.first = at;
@@ -706,31 +1154,78 @@ int run(const mnx_muon_args& a, const Plan& plan, const Scales& sc, mnx_stream_t
         k_muon_table<<<1, 256, 0, stream>>>(t, plan.table);
         MNX_CHECK_LAUNCH();
     }
+    return MNX_OK;
+}
+
+// The factors of step k's three products.
+struct Factors {
+    Step gram, poly, update;
+};
+Factors factors(const mnx_muon_args& a, const Scales& sc, int k) {
+    const double ca = a.coefficients[0], cb = a.coefficients[1], cc = a.coefficients[2];
+    const double A = sc.a[size_t(k)], B = sc.b[size_t(k)];
+    const int from = k & 1, first = k == 0;
+    const double xs = first ? 4096.0 : sc.x[size_t(k)];  // the first X is stored at 2^12 whatever the bounds say
+    const double to = k + 1 == a.steps ? 1.0 : sc.x[size_t(k) + 1];
+    return {{0.f, float(A / (xs * xs)), from, first},
+            {float(B * cb / A), float(B * cc / (A * A)), from, first},
+            {float(to * ca / xs), float(to / (B * xs)), from, first}};
+}
+
+template <int PL>
+int run(const mnx_muon_args& a, const Plan& plan, const Scales& sc, mnx_stream_t stream) {
+    const int count = int(plan.mat.size());
+    if (!count) return MNX_OK;
+    if (int rc = write_table(plan, stream)) return rc;
     const Momentum h{float(a.momentum), float(1 - a.momentum), a.nesterov, a.maximize};
     k_muon_momentum<<<plan.total.chunk, 256, 0, stream>>>(plan.table, count, h, plan.partial);
     MNX_CHECK_LAUNCH();
-    k_muon_norm<<<plan.stats, 64, 0, stream>>>(plan.table, count, plan.partial, a.eps, plan.stat);
+    k_muon_norm<<<plan.stats, 256, 0, stream>>>(plan.table, count, plan.partial, a.eps, plan.stat);
     MNX_CHECK_LAUNCH();
     k_muon_cast<PL><<<plan.total.cast, 256, 0, stream>>>(plan.table, count, h, plan.stat);
     MNX_CHECK_LAUNCH();
-    const double ca = a.coefficients[0], cb = a.coefficients[1], cc = a.coefficients[2];
-    const Apply none{};
+    const Apply none{}, ap{float(a.lr), a.lr_device, float(a.weight_decay), 1.0f};
     for (int k = 0; k < a.steps; ++k) {
-        const double A = sc.a[k], B = sc.b[k];
-        const int from = k & 1, first = k == 0, last = k + 1 == a.steps;
-        const double xs = first ? 4096.0 : sc.x[k];  // the first X is stored at 2^12 whatever the bounds say
-        const Step gram{0.f, float(A / (xs * xs)), from, first};
-        const Step poly{float(B * cb / A), float(B * cc / (A * A)), from, first};
-        const double to = last ? 1.0 : sc.x[k + 1];
-        const Step update{float(to * ca / xs), float(to / (B * xs)), from, first};
-        if (int rc = product<kGram, PL>(plan, gram, none, stream)) return rc;
-        if (int rc = product<kPoly, PL>(plan, poly, none, stream)) return rc;
-        const Apply ap{float(a.lr), a.lr_device, float(a.weight_decay), 1.0f};
-        if (int rc = last ? product<kFinal, PL>(plan, update, ap, stream) : product<kUpdate, PL>(plan, update, none, stream))
+        const Factors f = factors(a, sc, k);
+        if (int rc = product<kGram, PL>(plan, f.gram, none, stream)) return rc;
+        if (int rc = product<kPoly, PL>(plan, f.poly, none, stream)) return rc;
+        if (int rc = k + 1 == a.steps ? product<kFinal, PL>(plan, f.update, ap, stream)
+                                      : product<kUpdate, PL>(plan, f.update, none, stream))
             return rc;
     }
     return MNX_OK;
 }
+
+template <int PL>
+int run_small(const mnx_muon_args& a, const Plan& plan, const Scales& sc, mnx_stream_t stream) {
+    const int count = int(plan.mat.size());
+    if (!count) return MNX_OK;
+    if (int rc = write_table(plan, stream)) return rc;
+    const Momentum h{float(a.momentum), float(1 - a.momentum), a.nesterov, a.maximize};
+    const Apply ap{float(a.lr), a.lr_device, float(a.weight_decay), 1.0f};
+    Steps st;
+    st.count = a.steps;
+    for (int k = 0; k < a.steps; ++k) {
+        const Factors f = factors(a, sc, k);
+        st.gram[k] = f.gram.prod;
+        st.poly_own[k] = f.poly.own;
+        st.poly[k] = f.poly.prod;
+        st.own[k] = f.update.own;
+        st.prod[k] = f.update.prod;
+    }
+    const auto kernel = plan.lds <= kSmallLds[0] ? k_muon_small<PL, kSmallLds[0]> : k_muon_small<PL, kSmallLds[1]>;
+    kernel<<<plan.stats, kSmallThreads, 0, stream>>>(plan.table, count, h, a.eps, st, ap);
+    MNX_CHECK_LAUNCH();
+    return MNX_OK;
+}
+
+// The tensors of a call by how they are multiplied: each kind's launches follow the last one's, in the same workspace.
+struct Form {
+    int planes;
+    bool small;
+    int (*run)(const mnx_muon_args&, const Plan&, const Scales&, mnx_stream_t);
+};
+constexpr Form kForms[] = {{1, true, run_small<1>}, {2, true, run_small<2>}, {1, false, run<1>}, {2, false, run<2>}};
 
 }  // namespace
 }  // namespace mnx
@@ -743,9 +1238,9 @@ size_t mnx_muon_workspace_bytes(const mnx_muon_args* args) {
     clear_error();
     if (!args || check_args(*args) != MNX_OK) return 0;
     size_t most = 256;
-    for (int planes = 1; planes <= 2; ++planes) {
+    for (const Form& f : kForms) {
         Plan plan;
-        if (lay_out(*args, planes, nullptr, plan) != MNX_OK) return 0;
+        if (lay_out(*args, f.planes, f.small, nullptr, plan) != MNX_OK) return 0;
         most = std::max(most, plan.bytes);
     }
     return most;
@@ -766,14 +1261,15 @@ int mnx_muon_step(const mnx_muon_args* args, mnx_stream_t stream) {
     Scales sc;
     MNX_REQUIRE(bounds(a, sc), "muon: the iteration diverges with coefficients (%g, %g, %g)", a.coefficients[0],
                 a.coefficients[1], a.coefficients[2]);
-    Plan plan[2];
-    for (int planes = 1; planes <= 2; ++planes) {
-        if (int rc = lay_out(a, planes, static_cast<char*>(a.workspace), plan[planes - 1])) return rc;
-        if (!plan[planes - 1].mat.empty() && (!a.workspace || a.workspace_bytes < plan[planes - 1].bytes))
+    Plan plan[4];
+    for (int k = 0; k < 4; ++k) {
+        if (int rc = lay_out(a, kForms[k].planes, kForms[k].small, static_cast<char*>(a.workspace), plan[k])) return rc;
+        if (!plan[k].mat.empty() && (!a.workspace || a.workspace_bytes < plan[k].bytes))
             return set_error(MNX_ERR_WORKSPACE, "muon: workspace too small");
     }
-    if (int rc = run<1>(a, plan[0], sc, stream)) return rc;
-    return run<2>(a, plan[1], sc, stream);
+    for (int k = 0; k < 4; ++k)
+        if (int rc = kForms[k].run(a, plan[k], sc, stream)) return rc;
+    return MNX_OK;
 }
 
 }  // extern "C"
