@@ -45,10 +45,9 @@ struct Mat {
     void* p;         // parameters, or where the orthogonalised matrices go
     const void* g;   // gradients, or the matrices to orthogonalise
     float* m;        // momenta, or null
-    _Float16* x[2];  // [planes][batch][rp][cp]
-    _Float16* a;     // [planes][batch][rp][rp]
+    _Float16* x[2];  // [batch][rp][cp], of pairs: 16 hi, then their 16 lo, along a row
+    _Float16* a;     // [batch][rp][rp]
     _Float16* b;
-    int64_t xplane, aplane;  // elements of a plane
     int32_t rows, cols, r, c, rp, cp, batch, dtype;
     float adjust;    // s
     uint32_t stat0;  // the first matrix's place among the norms
@@ -204,6 +203,12 @@ __global__ void __launch_bounds__(256) k_muon_norm(const Mat* __restrict__ table
     if (threadIdx.x == 0) stats[blockIdx.x] = stat_of(sqrt((part[0] + part[1]) + (part[2] + part[3])), eps);
 }
 
+// Where column j of a row lies, of single numbers or of pairs (lo 16 behind hi).
+template <int PL>
+__device__ __forceinline__ int place(int j) {
+    return PL == 1 ? j : ((j & ~15) << 1) | (j & 15);
+}
+
 template <int PL>
 __device__ __forceinline__ void put4(_Float16* to, int64_t plane, const float (&v)[4]) {
     half4 hi, lo;
@@ -233,7 +238,7 @@ __global__ void __launch_bounds__(256) k_muon_cast(const Mat* __restrict__ table
     const bool tall = t.rows > t.cols;
     const int i0 = tall ? c0 : r0, j0 = tall ? r0 : c0;  // of the tensor's own rows and columns
     const int row = threadIdx.x / 16, col = threadIdx.x % 16 * 4;
-    _Float16* x = t.x[0] + int64_t(which) * t.rp * t.cp + int64_t(r0) * t.cp + c0;
+    _Float16* x = t.x[0] + PL * (int64_t(which) * t.rp * t.cp + int64_t(r0) * t.cp);
     float v[4][4], m[4][4];
     by_type(t.dtype, [&](auto type) {
         const auto* g = static_cast<const decltype(type)*>(t.g) + off;
@@ -253,7 +258,7 @@ __global__ void __launch_bounds__(256) k_muon_cast(const Mat* __restrict__ table
             v[k][e] = ldexpf(v[k][e], s.exponent);
             if (tall) tile[row + 16 * k][col + e] = v[k][e];
         }
-        if (!tall) put4<PL>(x + int64_t(row + 16 * k) * t.cp + col, t.xplane, v[k]);
+        if (!tall) put4<PL>(x + PL * int64_t(row + 16 * k) * t.cp + place<PL>(c0 + col), 16, v[k]);
     }
     if (!tall) return;
     __syncthreads();
@@ -261,7 +266,7 @@ __global__ void __launch_bounds__(256) k_muon_cast(const Mat* __restrict__ table
     for (int k = 0; k < 4; ++k) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[k][e] = tile[col + e][row + 16 * k];
-        put4<PL>(x + int64_t(row + 16 * k) * t.cp + col, t.xplane, v[k]);
+        put4<PL>(x + PL * int64_t(row + 16 * k) * t.cp + place<PL>(c0 + col), 16, v[k]);
     }
 }
 
@@ -324,7 +329,7 @@ __device__ __forceinline__ void apply(T* p, int count, float decay, float rate, 
 }
 
 template <int PL>
-__device__ __forceinline__ void put8(_Float16* to, int64_t plane, const float (&v)[8]) {
+__device__ __forceinline__ void put8(_Float16* to, const float (&v)[8]) {
     half8 hi, lo;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -332,7 +337,7 @@ __device__ __forceinline__ void put8(_Float16* to, int64_t plane, const float (&
         lo[e] = _Float16(v[e] - float(hi[e]));
     }
     *reinterpret_cast<half8*>(to) = hi;
-    if constexpr (PL == 2) *reinterpret_cast<half8*>(to + plane) = lo;
+    if constexpr (PL == 2) *reinterpret_cast<half8*>(to + 16) = lo;
 }
 
 // LDS that one lane wrote is read by others of the wavefront.
@@ -342,17 +347,19 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-constexpr int kKC = 64;  // k of a chunk
+constexpr int kRow = 64;  // numbers of a row's chunk: 64 k, or 32 k of pairs
+
+// Chunks in LDS at a time: as many as leave one workgroup (two of 128) a CU.
+constexpr int stages(int tile) { return tile == 256 ? 2 : tile == 192 ? 3 : tile == 128 ? 2 : 6; }
 
 // A BT x BT tile of one product, the sum over k of I[i][k] J[j][k] (rows of both in memory), or with TR of I[i][k] J[k][j].
-// Four wavefronts share it, a quarter each.  Chunks go from memory straight to LDS, 16 bytes a lane, into two buffers.
-// Within a row of LDS the 16-byte pieces are permuted (by the lanes' source addresses: LDS itself is filled in lane order)
-// so that the reads, 16 bytes of 16 rows or 64 bytes of 4 rows, meet every bank once.
+// Four wavefronts share it, a quarter each.  Chunks go from memory straight to LDS, 16 bytes a lane, several ahead.  Within
+// a row of LDS the 16-byte pieces are permuted (by the lanes' source addresses: LDS itself is filled in lane order) so that
+// the reads, 16 bytes of 16 rows or 32 or 64 bytes of 4 rows, meet every bank once.
 //
-// Operands of the next 16 k are read from LDS between the products of these.  The one barrier of a chunk stands before its
-// last 16 k: by then every read of this buffer has come back and the next chunk has arrived, so behind it half the loads
-// of the chunk after next and the first reads of the next run between those products, the other half of the loads between
-// the next chunk's first ones.
+// Operands are read from LDS between the products of the 32 numbers before, which also cover the loads of chunks to come.
+// One barrier a chunk, before its last products: by then everyone has read all of it (its place is free) and the next
+// chunk has arrived.
 //
 // The last tile of a row or column may reach past the padded matrix: it reads what lies behind it in the workspace (rows
 // and columns of the result that are not stored) and stores none of that.
@@ -362,12 +369,11 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
                                                                         const Stat* __restrict__ stats, Apply ap) {
     constexpr bool SYM = MODE == kGram || MODE == kPoly, TR = !SYM;
     constexpr int W = BT / 2, MT = W / 32;  // a wavefront's part
-    constexpr int SEG = PL == 1 ? 1 : 3;
-    constexpr int FETCH = BT / 32;  // loads a lane of either operand's chunk
-    constexpr int PIECES = BT / 8;  // of a sum's columns
-    constexpr int BUFS = BT == 64 ? 6 : 2;
-    __shared__ _Float16 lds[2 * BUFS * BT * kKC];
-    _Float16 *const sI0 = lds, *const sI1 = sI0 + BT * kKC, *const sJ0 = sI1 + BT * kKC, *const sJ1 = sJ0 + BT * kKC;
+    constexpr int STAGES = stages(BT), SIDE = BT * kRow;  // numbers of an operand's chunk
+    constexpr int FETCH = BT / 32;          // loads a lane of an operand's chunk
+    constexpr int SUMS = kRow / PL;         // k of a chunk
+    constexpr int PIECES = PL * BT / 8;     // of a sum's columns
+    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * STAGES * SIDE];
     const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave & 1, wj = wave >> 1;
@@ -394,14 +400,12 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
     }
     ti = __builtin_amdgcn_readfirstlane(ti);
     tj = __builtin_amdgcn_readfirstlane(tj);
-    const int K = MODE == kGram ? t.cp : t.rp;
-    const _Float16* X = t.x[s.from] + int64_t(which) * t.rp * t.cp;
-    const _Float16* A = t.a + int64_t(which) * t.rp * t.rp;
-    const _Float16* B = t.b + int64_t(which) * t.rp * t.rp;
+    const int K = PL * (MODE == kGram ? t.cp : t.rp);  // numbers of I's rows
+    const _Float16* X = t.x[s.from] + PL * int64_t(which) * t.rp * t.cp;
+    const _Float16* A = t.a + PL * int64_t(which) * t.rp * t.rp;
+    const _Float16* B = t.b + PL * int64_t(which) * t.rp * t.rp;
     const _Float16* I = (MODE == kGram ? X : MODE == kPoly ? A : B) + int64_t(ti) * BT * K;
-    const int64_t iplane = MODE == kGram ? t.xplane : t.aplane;
-    const _Float16* J = TR ? X + tj * BT : (MODE == kGram ? X : A) + int64_t(tj) * BT * K;
-    const int64_t jplane = MODE == kPoly ? t.aplane : t.xplane;
+    const _Float16* J = TR ? X + PL * tj * BT : (MODE == kGram ? X : A) + int64_t(tj) * BT * K;
 
     f32x16 acc[MT][MT];
 #pragma unroll
@@ -411,153 +415,128 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[m][n][q] = 0.f;
 
-    const int per_seg = K / kKC, chunks = SEG * per_seg;
-    // a wavefront fills 1 KB of LDS at a time, every fourth: 8 rows of 64 k, or sums' columns piece after piece
+    const int chunks = K / kRow;  // sides are multiples of 128
+    // a wavefront fills 1 KB of LDS at a time, every fourth: 8 rows of a chunk, or sums' columns piece after piece
     const int frow = wave * 8 + (lane >> 3);
     const uint32_t irow = 2 * (uint32_t(frow) * K + (((lane & 7) ^ ((frow >> 1) & 7)) << 3));  // bytes
-    const int64_t istep = int64_t(32) * K;
+    const int64_t istep = int64_t(32) * K, jld = PL * int64_t(t.cp);
+    // of a piece in the row of sum k: pairs' hi and lo, 32 bytes each of two groups, or 64 bytes
+    auto turn_of = [](int k) {
+        return PL == 2 ? (k & 1) << 1 | (k & 2) << 2 : BT % 128 ? ((k >> 1) & 1) << 2 : (k & 3) << 2;
+    };
     uint32_t jrow[TR ? FETCH : 1];
     if constexpr (TR) {
 #pragma unroll
         for (int n = 0; n < FETCH; ++n) {
             const int piece = (n * 4 + wave) * 64 + lane, k = piece / PIECES, c = piece % PIECES;
-            const int turn = BT % 128 ? ((k >> 1) & 1) << 2 : (k & 3) << 2;
-            jrow[n] = 2 * (uint32_t(k) * t.cp + ((c ^ turn) << 3));
+            jrow[n] = 2 * (uint32_t(k) * uint32_t(jld) + ((c ^ turn_of(k)) << 3));
         }
     }
-    struct Source {
-        const _Float16 *i, *j;
+    // the n-th of chunk c's 2 FETCH loads
+    auto fetch = [&](int c, int n, int stage) {
+        _Float16* to = lds + stage * 2 * SIDE + (n * 4 + wave) * 512;  // J behind I
+        if (n < FETCH) load_lds(I + c * kRow + n * istep, irow, to);
+        else if constexpr (TR) load_lds(J + c * SUMS * jld, jrow[n - FETCH], to);
+        else load_lds(J + c * kRow + (n - FETCH) * istep, irow, to);
     };
-    auto source = [&](int chunk) {
-        Source f{I, J};
-        if constexpr (PL == 2) {
-            const int seg = chunk >= 2 * per_seg ? 2 : chunk >= per_seg ? 1 : 0;
-            chunk -= seg * per_seg;
-            if (seg == 0) f.i += iplane;
-            if (seg == 1) f.j += jplane;
-        }
-        f.i += chunk * kKC;
-        f.j += TR ? int64_t(chunk * kKC) * t.cp : chunk * kKC;
-        return f;
-    };
-    // the n-th of a chunk's 2 FETCH loads
-    auto fetch = [&](const Source& f, int n, _Float16* bi, _Float16* bj) {
-        if (n < FETCH) load_lds(f.i + n * istep, irow, bi + (n * 4 + wave) * 512);
-        else if constexpr (TR) load_lds(f.j, jrow[n - FETCH], bj + ((n - FETCH) * 4 + wave) * 512);
-        else load_lds(f.j + (n - FETCH) * istep, irow, bj + ((n - FETCH) * 4 + wave) * 512);
-    };
+    // operands of 32 numbers: k 0 to 15 and 16 to 31, or hi and lo
     struct Frags {
-        half8 i[MT], j[MT];
+        half8 i[2][MT], j[2][MT];
     };
-    const int ki = (wi * W + l32) * kKC, kj = (wj * W + l32) * kKC, turn = (l32 >> 1) & 7;  // 32 rows on turn alike
-    const int trow = 8 * half + ((lane & 15) >> 2), tcol = wj * W + (l32 & 16) + (lane & 3) * 4;
-    const int tturn = BT % 128 ? ((trow >> 1) & 1) << 2 : (trow & 3) << 2;
-    auto read_i = [&](int m, int ks, const _Float16* bi) {
-        return *reinterpret_cast<const half8*>(bi + ki + m * 32 * kKC + (((2 * ks + half) ^ turn) << 3));
+    const int ki = (wi * W + l32) * kRow, kj = SIDE + (wj * W + l32) * kRow, turn = (l32 >> 1) & 7;  // 32 rows on turn alike
+    const int trow = 8 * half + ((lane & 15) >> 2);
+    auto read_i = [&](int sub, int h, int m, const _Float16* b) {
+        return *reinterpret_cast<const half8*>(b + ki + m * 32 * kRow + (((4 * sub + 2 * h + half) ^ turn) << 3));
     };
-    auto read_j = [&](int n, int ks, const _Float16* bj) {
+    auto read_j = [&](int sub, int h, int n, const _Float16* b) {
         if constexpr (!TR) {
-            return *reinterpret_cast<const half8*>(bj + kj + n * 32 * kKC + (((2 * ks + half) ^ turn) << 3));
-        } else {
-            const int col = tcol + n * 32;
-            const _Float16* q = bj + (16 * ks + trow) * BT + (((col >> 3) ^ tturn) << 3) + (col & 4);
-            return read_tr(q, q + 4 * BT);  // four sums on turn alike
+            return *reinterpret_cast<const half8*>(b + kj + n * 32 * kRow + (((4 * sub + 2 * h + half) ^ turn) << 3));
+        } else {  // four sums on turn alike
+            const int k = trow + 32 / PL * sub + (PL == 1 ? 16 * h : 0), col = wj * W + n * 32 + (l32 & 16);
+            const int in = PL == 1 ? col + (lane & 3) * 4 : 2 * col + 16 * h + (lane & 3) * 4;
+            const _Float16* q = b + SIDE + k * (PL * BT) + (((in >> 3) ^ turn_of(trow)) << 3) + (in & 4);
+            return read_tr(q, q + 4 * PL * BT);
         }
     };
-    // The products of `now`, with the reads of `next` and `loads` between them.
-    auto multiply = [&](const Frags& now, Frags& next, int ks, const _Float16* bi, const _Float16* bj, auto loads) {
+    // The products of `now`, with the reads of `next` (32 numbers of a chunk) and `loads` between them.
+    auto multiply = [&](const Frags& now, Frags& next, int stage, int sub, auto loads) {
+        // k by k, or of pairs lo hi, hi lo, hi hi
+        constexpr int GROUPS = PL == 1 ? 2 : 3, HI[3] = {0, 1, 0}, HJ[3] = {PL == 1 ? 0 : 1, PL == 1 ? 1 : 0, 0};
+        const _Float16* b = lds + stage * 2 * SIDE;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            next.j[m] = read_j(m, ks, bj);
-            next.i[m] = read_i(m, ks, bi);
-            loads(m);
+        for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-            for (int n = 0; n < MT; ++n) acc[m][n] = mfma(now.j[n], now.i[m], acc[m][n]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+            for (int m = 0; m < MT; ++m) {
+                if (g < 2) {
+                    next.j[g][m] = read_j(sub, g, m, b);
+                    next.i[g][m] = read_i(sub, g, m, b);
+                }
+                loads(g * MT + m);
+#pragma unroll
+                for (int n = 0; n < MT; ++n) acc[m][n] = mfma(now.j[HJ[g]][n], now.i[HI[g]][m], acc[m][n]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
     };
-    auto arrived = [] {  // everyone's loads and reads
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    const auto nothing = [](int) {};
+    // half a chunk's loads (the part-th), shared out over the first 2 MT products
+    auto part_of = [&](int c, int part, int stage) {
+        return [=, &fetch](int at) {
+            constexpr int ALL = FETCH, PER = (ALL + 2 * MT - 1) / (2 * MT);
+#pragma unroll
+            for (int n = at * PER; n < (at + 1) * PER; ++n)
+                if (n < ALL) fetch(c, part * ALL + n, stage);
+        };
+    };
+    auto barrier = [] {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
+    auto next_of = [](int stage) { return stage + 1 == STAGES ? 0 : stage + 1; };
     Frags f0, f1;
-    // Chunk c in (bi, bj), its first operands in f0; (oi, oj) takes or holds the next.  REST: the second half of the next
-    // chunk's loads is still to come; MORE: a chunk after next begins.
-    auto body = [&](int c, _Float16* bi, _Float16* bj, _Float16* oi, _Float16* oj, auto rest, auto more) {
-        const auto nothing = [](int) {};
-        if constexpr (rest) {
-            const Source f = source(c + 1);
-            multiply(f0, f1, 1, bi, bj, [&](int m) {
+    int stage = 0, c = 0;
+#pragma unroll 1
+    for (int k = 0; k < min(STAGES, chunks); ++k)
 #pragma unroll
-                for (int n = 0; n < FETCH / MT; ++n) fetch(f, FETCH + m * (FETCH / MT) + n, oi, oj);
-            });
-        } else {
-            multiply(f0, f1, 1, bi, bj, nothing);
-        }
-        multiply(f1, f0, 2, bi, bj, nothing);
-        multiply(f0, f1, 3, bi, bj, nothing);
-        arrived();
-        if constexpr (more) {
-            const Source f = source(c + 2);
-            multiply(f1, f0, 0, oi, oj, [&](int m) {
+        for (int n = 0; n < 2 * FETCH; ++n) fetch(k, n, k);
+    if (chunks >= STAGES) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * FETCH * (STAGES - 1)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    barrier();
 #pragma unroll
-                for (int n = 0; n < FETCH / MT; ++n) fetch(f, m * (FETCH / MT) + n, bi, bj);
-            });
-        } else {
-            multiply(f1, f0, 0, oi, oj, nothing);  // after the last chunk, reads of the one before that nobody uses
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            f0.i[h][m] = read_i(0, h, m, lds);
+            f0.j[h][m] = read_j(0, h, m, lds);
         }
+    // The last products of chunk c, whose operands are in `now`, and the first operands of the next.  MORE: the first part
+    // of chunk c + STAGES goes where c was.
+    auto last_of = [&](const Frags& now, Frags& next, auto more) {
+        // (STAGES - 2) chunks behind the next may still be out
+        if constexpr (decltype(more)::value)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(2 * FETCH * (STAGES - 2)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        barrier();
+        const int free = stage;
+        stage = next_of(stage);
+        if constexpr (decltype(more)::value) multiply(now, next, stage, 0, part_of(c + STAGES, 0, free));
+        else multiply(now, next, stage, 0, nothing);  // after the last chunk it reads what nobody uses
+        ++c;
     };
-    const std::true_type yes;
-    const std::false_type no;
-    if constexpr (BT == 64) {
-        // Few tiles: the latency of a chunk counts, not the products.  Six buffers, and five chunks on their way.
-        auto buf = [&](int c) { return lds + c % BUFS * 2 * BT * kKC; };
-        auto load = [&](int c) {
-            const Source f = source(c);
-#pragma unroll
-            for (int n = 0; n < 2 * FETCH; ++n) fetch(f, n, buf(c), buf(c) + BT * kKC);
-        };
-        for (int c = 0; c < min(BUFS - 1, chunks); ++c) load(c);
-        for (int c = 0; c < chunks; ++c) {
-            // this chunk has come when no more than the later ones' loads are out
-            if (c + BUFS - 1 <= chunks) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(2 * FETCH * (BUFS - 2)) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            if (c + BUFS - 1 < chunks) load(c + BUFS - 1);  // into the buffer of the chunk before, which everyone has read
-            const _Float16 *bi = buf(c), *bj = bi + BT * kKC;
-            Frags f[4];
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-                f[ks].i[0] = read_i(0, ks, bi);
-                f[ks].j[0] = read_j(0, ks, bj);
-            }
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) acc[0][0] = mfma(f[ks].j[0], f[ks].i[0], acc[0][0]);
-        }
-    } else {
-        {
-            const Source f = source(0), g = source(1);
-    #pragma unroll
-            for (int n = 0; n < 2 * FETCH; ++n) fetch(f, n, sI0, sJ0);
-            arrived();
-    #pragma unroll
-            for (int n = 0; n < FETCH; ++n) fetch(g, n, sI1, sJ1);
-    #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                f0.i[m] = read_i(m, 0, sI0);
-                f0.j[m] = read_j(m, 0, sJ0);
-            }
-        }
-        int c = 0;  // chunks are an even number: K is a multiple of 128
-        for (; c + 2 < chunks; c += 2) {
-            body(c, sI0, sJ0, sI1, sJ1, yes, yes);
-            body(c + 1, sI1, sJ1, sI0, sJ0, yes, yes);
-        }
-        body(c, sI0, sJ0, sI1, sJ1, yes, no);
-        body(c + 1, sI1, sJ1, sI0, sJ0, no, no);
+    const std::true_type more;
+    const std::false_type rest;
+    multiply(f0, f1, stage, 1, nothing);
+#pragma unroll 1
+    while (c + STAGES < chunks) {
+        const int free = stage;
+        last_of(f1, f0, more);
+        multiply(f0, f1, stage, 1, part_of(c - 1 + STAGES, 1, free));
     }
+#pragma unroll 1
+    while (c + 1 < chunks) {
+        last_of(f1, f0, rest);
+        multiply(f0, f1, stage, 1, nothing);
+    }
+    last_of(f1, f0, rest);
 
     // The result, 32 rows of a wavefront's part at a time by way of LDS (its own part of it), from where rows and, for the
     // second place of a symmetric one and for tall matrices' parameters, columns leave 8 values a lane.  acc[m][n][q] is
@@ -571,8 +550,8 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
             prod *= rho;
         }
     }
-    const int64_t ld = SYM ? t.rp : t.cp;
-    const int64_t oplane = SYM ? t.aplane : t.xplane;
+    const int width = SYM ? t.rp : t.cp;
+    const int64_t ld = PL * int64_t(width);
     const _Float16* E = MODE == kPoly ? A : X;
     _Float16* out = (MODE == kGram ? t.a : MODE == kPoly ? t.b : t.x[s.from ^ 1]) + int64_t(which) * t.rp * ld;
     float decay = 0, rate = -ap.inv;  // of p and of its change; the result itself has no p
@@ -587,7 +566,7 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
     // too: the two halves' sums run in different orders with pairs, and results would differ with the size of tiles.
     const bool columns = SYM || (MODE == kFinal && tall), corner = SYM && ti == tj && wi == wj;
     constexpr int LD = W + 4, ITEMS = W / 16;  // items of 8 values a lane
-    float* part = reinterpret_cast<float*>(lds + wave * BT * kKC);
+    float* part = reinterpret_cast<float*>(lds + wave * 2 * 32 * LD);
     const int j0 = tj * BT + wj * W;
     __syncthreads();
     if (SYM && ti == tj && wi < wj) return;  // above the diagonal
@@ -602,7 +581,8 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
                 const int item = it * 64 + lane, i = i0 + item / (W / 8), j = j0 + item % (W / 8) * 8;
 #pragma unroll
                 for (int pl = 0; pl < PL; ++pl)
-                    if (i < t.rp && j < ld) old[pl][it] = *reinterpret_cast<const half8*>(E + pl * oplane + int64_t(i) * ld + j);
+                    if (i < t.rp && j < width)
+                        old[pl][it] = *reinterpret_cast<const half8*>(E + int64_t(i) * ld + place<PL>(j) + 16 * pl);
             }
         }
 #pragma unroll
@@ -619,7 +599,7 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
         for (int it = 0; it < ITEMS; ++it) {
             const int item = it * 64 + lane, r = item / (W / 8), i = i0 + r, jj = item % (W / 8) * 8, j = j0 + jj;
             const int block = corner ? (jj >> 5) - m : -1;  // 0: the diagonal's; above it, nothing is stored
-            if (i >= t.rp || j >= ld || block > 0) continue;
+            if (i >= t.rp || j >= width || block > 0) continue;
             float v[8];
             if (block < 0) {
                 *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(part + r * LD + jj);
@@ -644,7 +624,7 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
             if constexpr (MODE == kFinal) {
                 if (!tall && i < t.r) apply(p + int64_t(i) * t.cols + j, t.c - j, decay, rate, v);
             } else {
-                put8<PL>(out + int64_t(i) * ld + j, oplane, v);
+                put8<PL>(out + int64_t(i) * ld + place<PL>(j), v);
             }
         }
         wave_sync();
@@ -652,14 +632,14 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
 #pragma unroll
             for (int it = 0; it < ITEMS; ++it) {
                 const int item = it * 64 + lane, jj = item / 4, j = j0 + jj, r = item % 4 * 8, i = i0 + r;
-                if (i >= t.rp || j >= ld || (corner && (jj >> 5) >= m)) continue;
+                if (i >= t.rp || j >= width || (corner && (jj >> 5) >= m)) continue;
                 float v[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = part[(r + e) * LD + jj];
                 if constexpr (MODE == kFinal) {
                     if (j < t.c) apply(p + int64_t(j) * t.cols + i, t.r - i, decay, rate, v);
                 } else {
-                    put8<PL>(out + int64_t(j) * ld + i, oplane, v);
+                    put8<PL>(out + int64_t(j) * ld + place<PL>(i), v);
                 }
             }
             wave_sync();
@@ -1014,22 +994,39 @@ inline int64_t tiles_of(const Mat& t, bool sym, int tile) {
 
 constexpr int kTile[] = {256, 192, 128, 64}, kTiles = 4;
 
-// The time of a launch, about, in microseconds: a tile's begin and end take 4, a chunk of 64 k 1.95 (256), 1.03 (192), 0.5
-// (128) or 0.13 (64), 1.29 where two of 128 share a CU; the card holds 256 tiles at once (or 512), the longest first.
+// The time of a launch, about, in microseconds.  A tile's begin and end take 4, a chunk of 64 numbers 1.95 (256), 1.1 (192)
+// or 0.23 (64), with one tile a CU; tiles of 128 share a CU two by two, 1.05 a chunk, or 0.6 where they are few; pairs half
+// as much again (a third product).  `mats` are sorted: the longest tiles start first, each on the CU that is free first.
 double cost(const std::vector<Mat>& mats, int planes, int kind, int tile) {
     double tiles = 0;
     for (const Mat& t : mats) tiles += double(tiles_of(t, kind != kUpdate, tile));
     const bool two = tile == 128 && tiles > 256;
     const double slots = two ? 512 : 256;
-    const double chunk = tile == 256 ? 1.95 : tile == 192 ? 1.03 : two ? 1.29 : tile == 128 ? 0.5 : 0.13;
-    double all = 0, longest = 0, shortest = HUGE_VAL;
-    for (const Mat& t : mats) {
-        const double one = 4 + chunk * (planes == 2 ? 3 : 1) * double(kind == kGram ? t.cp : t.rp) / kKC;
-        all += one * double(tiles_of(t, kind != kUpdate, tile));
-        longest = std::max(longest, one);
-        shortest = std::min(shortest, one);
+    double chunk = tile == 256 ? 1.95 : tile == 192 ? 1.1 : two ? 1.05 : tile == 128 ? 0.6 : 0.23;
+    if (planes == 2 && tile != 64) chunk *= 1.5;
+    auto one = [&](const Mat& t) { return 4 + chunk * planes * double(kind == kGram ? t.cp : t.rp) / kRow; };
+    if (tiles > 16 * slots) {  // many rounds: their sum
+        double all = 0;
+        for (const Mat& t : mats) all += one(t) * double(tiles_of(t, kind != kUpdate, tile));
+        return all / slots;
     }
-    return std::max(longest, std::ceil(all / slots / shortest - 0.01) * shortest);
+    std::vector<std::pair<double, double>> free{{0.0, slots}};  // when so many slots are free
+    for (size_t i = 0; i < mats.size();) {
+        const double time = one(mats[i]);
+        double n = 0;
+        for (; i < mats.size() && one(mats[i]) == time; ++i) n += double(tiles_of(mats[i], kind != kUpdate, tile));
+        while (n > 0) {
+            auto at = std::min_element(free.begin(), free.end());
+            const double begin = at->first, some = std::min(n, at->second);
+            n -= some;
+            if ((at->second -= some) == 0) free.erase(at);
+            const double end = begin + time;
+            auto same = std::find_if(free.begin(), free.end(), [&](const auto& f) { return f.first == end; });
+            if (same != free.end()) same->second += some;
+            else free.emplace_back(end, some);
+        }
+    }
+    return std::max_element(free.begin(), free.end())->first;
 }
 
 // float16 numbers that stand for one of X, A and B
@@ -1069,8 +1066,6 @@ int lay_out(const mnx_muon_args& a, int planes, bool small, char* base, Plan& pl
         t.m = a.momenta ? a.momenta[i] : nullptr;
         t.adjust = a.adjust == 0 ? float(std::sqrt(std::max(1.0, double(t.rows) / t.cols)))
                                  : float(0.2 * std::sqrt(double(t.c)));
-        t.xplane = a.batch[i] * t.rp * t.cp;
-        t.aplane = a.batch[i] * t.rp * t.rp;
         t.stat0 = uint32_t(stat);
         t.chunk0 = uint32_t(chunk);
         t.cast0 = uint32_t(cast);
@@ -1084,9 +1079,9 @@ int lay_out(const mnx_muon_args& a, int planes, bool small, char* base, Plan& pl
         }
         chunk += b * uint64_t(ceil_div(int64_t(t.rows) * t.cols, kChunk));
         cast += b * uint64_t(t.rp / kCast) * (t.cp / kCast);
-        for (_Float16*& x : t.x) x = ws.take<_Float16>(size_t(planes * t.xplane));
-        t.a = ws.take<_Float16>(size_t(planes * t.aplane));
-        t.b = ws.take<_Float16>(size_t(planes * t.aplane));
+        for (_Float16*& x : t.x) x = ws.take<_Float16>(size_t(planes * a.batch[i] * t.rp * t.cp));
+        t.a = ws.take<_Float16>(size_t(planes * a.batch[i] * t.rp * t.rp));
+        t.b = ws.take<_Float16>(size_t(planes * a.batch[i] * t.rp * t.rp));
         // a grid has fewer than 2^32 threads
         MNX_REQUIRE(std::max({chunk, cast, stat}) < (1u << 23), "muon: too many matrices in one call");
         plan.mat.push_back(t);
@@ -1120,7 +1115,7 @@ int lay_out(const mnx_muon_args& a, int planes, bool small, char* base, Plan& pl
     plan.total = {uint32_t(chunk), uint32_t(cast), uint32_t(sym), uint32_t(upd)};
     // the last tiles read past the last matrix
     int64_t past = 0;
-    for (const Mat& t : plan.mat) past = std::max<int64_t>(past, int64_t(256) * t.cp);
+    for (const Mat& t : plan.mat) past = std::max<int64_t>(past, int64_t(256) * planes * t.cp);
     if (past) ws.take<_Float16>(size_t(past));
     plan.stats = uint32_t(stat);
     plan.partial = ws.take<double>(size_t(chunk));
