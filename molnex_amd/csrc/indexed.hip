@@ -20,15 +20,13 @@
 // workspace, which a second kernel adds in order: the same bits every time.
 #include "bf16_split.h"
 #include "elem.h"
+#include "tile16.h"
 
 namespace mnx {
 namespace {
 
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef short short4v __attribute__((ext_vector_type(4)));
-typedef short short8v __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+using namespace tile16;
+
 
 constexpr int kThreads = 256;
 constexpr int kBM = 128;
@@ -43,14 +41,6 @@ struct Kind {
     typedef typename Elem<DT>::T T;
     typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
-
-template <int DT>
-__device__ __forceinline__ f32x16 mfma(const short8v& a, const short8v& b, const f32x16& c) {
-    if constexpr (DT == kF16)
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-}
 
 // `left` elements of a vector at p; zeros behind them.
 template <int DT>
@@ -106,11 +96,8 @@ template <int W>
 __device__ __forceinline__ short8v read_sums(const short* lds, int col0, int k0) {
     const int lane = threadIdx.x & 63;
     const int k = k0 + 8 * (lane >> 5) + ((lane & 15) >> 2), col = col0 + (lane & 16) + (lane & 3) * 4;
-    typedef __attribute__((address_space(3))) short4v* P;
     const short* q = lds + by_sums<W>(k, col);
-    const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)q);
-    const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(q + 4 * W));  // k + 4 turns alike
-    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return read_tr(q, q + 4 * W);  // k + 4 turns alike
 }
 
 // Which class workgroup `unit` serves, when a class of n rows has units(n) of them: the class, the unit's number in it,
@@ -157,8 +144,8 @@ __device__ __forceinline__ Found find_class(const Plan& plan, int classes, int u
     return {classes, 0, 0};
 }
 
-template <int DT, int MT, int NT>
-__device__ __forceinline__ void clear(f32x16 (&acc)[MT][NT]) {
+template <int MT, int NT>
+__device__ __forceinline__ void clear_acc(f32x16 (&acc)[MT][NT]) {
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -179,7 +166,7 @@ __device__ __forceinline__ void multiply(const short8v (&a)[Kind<DT>::planes][MT
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-                acc[m][n] = mfma<DT>(a[Z == 6 ? PA[z] : 0][m], b[Z == 6 ? PB[z] : 0][n], acc[m][n]);
+                acc[m][n] = mfma<DT != kF16>(a[Z == 6 ? PA[z] : 0][m], b[Z == 6 ? PB[z] : 0][n], acc[m][n]);
 }
 
 struct RowsArgs {
@@ -255,7 +242,7 @@ __global__ void __launch_bounds__(kThreads) k_indexed_rows(RowsArgs p) {
         }
     };
     f32x16 acc[MT][NT];
-    clear<DT>(acc);
+    clear_acc(acc);
     const int wm = wave & 1, wn = wave >> 1;
     if (K > 0) load(0);
     for (int k0 = 0; k0 < K; k0 += KC) {
@@ -350,7 +337,7 @@ __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
         }
     };
     f32x16 acc[2][2];
-    clear<DT>(acc);
+    clear_acc(acc);
     const int wm = wave & 1, wn = wave >> 1;
     if (begin < end) {
         find_rows(begin);
@@ -401,6 +388,180 @@ __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
         }
 }
 
+// ---------------------------------------------------------------------------
+// 16-bit types whose rows and columns come in pieces of 16 bytes
+// ---------------------------------------------------------------------------
+
+__device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
+
+// The tile's values, 32 rows of a wavefront's part at a time by way of LDS: store(row, column, eight values) for all within
+// rows x cols, numbered in the tile.
+template <int BT, typename Store>
+__device__ __forceinline__ void store_tile(short* lds, const Acc<BT>& acc, int rows, int cols, Store store) {
+    constexpr int W = BT / 2, MT = W / 32, LD = W + 4, ITEMS = W / 16;
+    const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i0 = (wave & 1) * W, j0 = (wave >> 1) * W;
+    float* part = reinterpret_cast<float*>(lds) + wave * 32 * LD;
+    __syncthreads();  // everyone has read its last operands
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int n = 0; n < MT; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[m][n][4 * q + e];
+                *reinterpret_cast<f32x4*>(part + l32 * LD + 32 * n + 8 * q + 4 * half) = v;
+            }
+        wave_sync();
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+            const int item = it * 64 + lane, r = item / (W / 8), jj = item % (W / 8) * 8;
+            const int i = i0 + 32 * m + r, j = j0 + jj;
+            if (i >= rows || j >= cols) continue;
+            float v[8];
+            *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(part + r * LD + jj);
+            *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(part + r * LD + jj + 4);
+            store(i, j, v);
+        }
+        wave_sync();
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* to, const float (&v)[8]) {
+    typedef T Eight __attribute__((ext_vector_type(8)));
+    Eight o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = T(v[e]);
+    *reinterpret_cast<Eight*>(to) = o;
+}
+
+// y or gx, BT rows of one class against BT columns: the loop of tile16.h, rows gathered by the lanes' addresses.  What lies
+// past the sum's end is read as zeros from elsewhere; rows and columns past the tile's repeat the last and are not stored.
+template <int DT, int DIR, int BT>
+__global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_indexed_rows16(RowsArgs p) {
+    using T = typename Elem<DT>::T;
+    constexpr int FETCH = BT / 32;
+    __shared__ __attribute__((aligned(16))) short lds[lds_numbers(BT)];
+    __shared__ int32_t rows[BT];
+    const uint32_t u = unit_of_block();
+    if (u >= p.units) return;
+    const int row_tile = __builtin_amdgcn_readfirstlane(u / uint32_t(p.col_tiles));
+    const int col0 = __builtin_amdgcn_readfirstlane(u % uint32_t(p.col_tiles)) * BT;
+    const int classes = p.plan.classes;
+    const Found f = find_class(p.plan, classes + 1, row_tile, [](int n) { return (n + BT - 1) / BT; }, [](int) { return 0; });
+    if (f.cls > classes) return;
+    const int first = p.plan.start(f.cls) + f.unit * BT;
+    const int count = min(BT, p.plan.start(f.cls + 1) - first);  // at least 1
+    for (int i = threadIdx.x; i < BT; i += 256) rows[i] = p.plan.row(first + min(i, count - 1));
+    __syncthreads();
+    T* out = static_cast<T*>(p.out);
+    Acc<BT> acc;
+    clear<BT>(acc);
+    if (f.cls < classes) {
+        const int K = p.sums, cols = p.cols;
+        const T* A = static_cast<const T*>(p.a);
+        const T* W = static_cast<const T*>(p.w) + int64_t(f.cls) * K * cols;
+        const RowPlace in = row_place();
+        const T* arow[FETCH];
+        uint32_t wrow[FETCH];  // bytes; within a chunk of sums, or from the tile's first column's row
+        int wsum[FETCH];
+#pragma unroll
+        for (int n = 0; n < FETCH; ++n) {
+            arow[n] = A + int64_t(rows[in.row + 32 * n]) * p.lda + in.number;
+            if constexpr (DIR == kForward) {
+                const SumPlace s = sum_place<BT, 1>(n);
+                wsum[n] = s.sum;
+                wrow[n] = 2 * (uint32_t(s.sum) * uint32_t(cols) + uint32_t(min(col0 + s.number, cols - 8)));
+            } else {
+                wsum[n] = in.number;
+                wrow[n] = 2 * (uint32_t(min(in.row + 32 * n, cols - 1 - col0)) * uint32_t(K) + uint32_t(in.number));
+            }
+        }
+        auto load = [&](int c, int n, short* to) {
+            const int k0 = c * kRow;
+            const T* w = W + (DIR == kForward ? int64_t(k0) * cols : int64_t(col0) * K + k0);
+            if (k0 + kRow <= K) {
+                if (n < FETCH) load_lds(arow[n] + k0, to);
+                else load_lds(w, wrow[n - FETCH], to);
+            } else if (n < FETCH) {
+                load_lds(k0 + in.number < K ? static_cast<const void*>(arow[n] + k0) : kZeros, to);
+            } else {
+                const char* from = reinterpret_cast<const char*>(w) + wrow[n - FETCH];
+                load_lds(k0 + wsum[n - FETCH] < K ? static_cast<const void*>(from) : kZeros, to);
+            }
+        };
+        products<BT, 1, false, DIR == kForward, DT == kBF16>(lds, (K + kRow - 1) / kRow, acc, load, [](int) {});
+    }
+    store_tile<BT>(lds, acc, count, p.cols - col0, [&](int i, int j, const float (&v)[8]) {
+        store8(out + int64_t(rows[i]) * p.cols + col0 + j, v);
+    });
+}
+
+constexpr int kIds = 2048;  // rows whose numbers are in LDS at a time
+
+// A BT x BT tile of one class's gradient over one slice of its rows: both operands by sums, their rows gathered by the
+// lanes' addresses; behind the slice's end, zeros from elsewhere.
+template <int DT, int BT>
+__global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_indexed_weights16(WeightArgs p) {
+    using T = typename Elem<DT>::T;
+    constexpr int FETCH = BT / 32;
+    __shared__ __attribute__((aligned(16))) short lds[lds_numbers(BT)];
+    __shared__ int32_t ids[kIds];
+    const uint32_t u = unit_of_block();
+    if (u >= p.units) return;
+    const uint32_t tiles = uint32_t(p.kt) * uint32_t(p.nt);
+    const int slice_at = __builtin_amdgcn_readfirstlane(u / tiles);
+    const int tile = __builtin_amdgcn_readfirstlane(u % tiles);
+    const int tk = tile / p.nt, tn = tile - tk * p.nt;
+    const int k0 = __builtin_amdgcn_readfirstlane(tk) * BT, n0 = __builtin_amdgcn_readfirstlane(tn) * BT;
+    const int slice = p.slice;
+    const Found f = find_class(p.plan, p.plan.classes, slice_at, [=](int n) { return slices(n, slice); },
+                               [=](int n) { return slots(n, slice); });
+    if (f.cls >= p.plan.classes) return;
+    const int lo = p.plan.start(f.cls), n_class = p.plan.count(f.cls);
+    const int begin = lo + f.unit * slice, end = lo + min(n_class, (f.unit + 1) * slice);
+    const T *X = static_cast<const T*>(p.x), *G = static_cast<const T*>(p.g);
+    int sum[FETCH], xcol[FETCH], gcol[FETCH];
+#pragma unroll
+    for (int n = 0; n < FETCH; ++n) {
+        const SumPlace s = sum_place<BT, 1>(n);
+        sum[n] = s.sum;
+        xcol[n] = min(k0 + s.number, p.K - 8);
+        gcol[n] = min(n0 + s.number, p.N - 8);
+    }
+    Acc<BT> acc;
+    clear<BT>(acc);
+    for (int at = begin; at < end; at += kIds) {
+        __syncthreads();
+        const int here = min(kIds, end - at);
+        for (int i = threadIdx.x; i < kIds; i += 256) ids[i] = i < here ? p.plan.row(at + i) : -1;
+        __syncthreads();
+        int row[FETCH];
+        auto ahead = [&](int c) {
+#pragma unroll
+            for (int n = 0; n < FETCH; ++n) row[n] = ids[c * kRow + sum[n]];
+        };
+        auto load = [&](int, int n, short* to) {
+            const int m = n < FETCH ? n : n - FETCH;
+            const T* from = n < FETCH ? X + int64_t(row[m]) * p.ldx + xcol[m] : G + int64_t(row[m]) * p.ldg + gcol[m];
+            load_lds(row[m] >= 0 ? static_cast<const void*>(from) : kZeros, to);
+        };
+        products<BT, 1, true, true, DT == kBF16>(lds, (here + kRow - 1) / kRow, acc, load, ahead);
+    }
+    const bool whole = n_class <= slice;
+    T* out = static_cast<T*>(p.gw) + int64_t(f.cls) * p.K * p.N;
+    float* part = p.part + (whole ? 0 : int64_t(f.extra + f.unit) * p.K * p.N);
+    store_tile<BT>(lds, acc, p.K - k0, p.N - n0, [&](int i, int j, const float (&v)[8]) {
+        const int64_t at = int64_t(k0 + i) * p.N + n0 + j;
+        if (whole) store8(out + at, v);
+        else store8(part + at, v);
+    });
+}
+
 // The partial sums of the classes with several slices, added in order.
 template <int DT>
 __global__ void __launch_bounds__(kThreads) k_indexed_join(WeightArgs p) {
@@ -433,22 +594,39 @@ int check_shape(const char* what, int64_t rows, int32_t classes, int64_t in, int
     return MNX_OK;
 }
 
-template <int DT>
-int rows_product(int dir, RowsArgs p, int64_t rows, mnx_stream_t stream) {
-    const int BN = p.cols <= 64 ? 64 : 128;
+// Whether 16-byte pieces of every row begin at multiples of 16 bytes: the loads of tile16.h.
+inline bool in_pieces(int dtype, const void* p, int64_t ld, int64_t width) {
+    return dtype != kF32 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && width % 8 == 0;
+}
+
+constexpr int64_t kCUs = 256;
+
+template <int DT, int DIR>
+int rows_product(RowsArgs p, mnx_stream_t stream) {
+    const int64_t rows = p.plan.rows, parts = std::min<int64_t>(rows, p.plan.classes + 1);
+    const bool pieces = in_pieces(DT, p.a, p.lda, p.sums) && in_pieces(DT, p.w, p.cols, p.cols) &&
+                        in_pieces(DT, p.out, p.cols, p.cols);
+    int tile = kBM;
+    if (DT != kF32 && pieces) {
+        const int64_t wide = ceil_div(rows, 256) * ceil_div(p.cols, 256), few = ceil_div(rows, 128) * ceil_div(p.cols, 128);
+        tile = few < kCUs || p.cols <= 64 ? 64 : wide >= 4 * kCUs && p.cols > 128 ? 256 : 128;
+    }
+    const int BN = pieces ? tile : p.cols <= 64 ? 64 : 128;
     p.col_tiles = int32_t(ceil_div(p.cols, BN));
-    const int64_t row_tiles = rows / kBM + std::min<int64_t>(rows, p.plan.classes + 1);
-    const int64_t units = row_tiles * p.col_tiles;
+    const int64_t units = (rows / tile + parts) * p.col_tiles;
     MNX_REQUIRE(units < (int64_t(1) << 23), "indexed linear: too many rows and columns for one call");
     p.units = uint32_t(units);
-    const uint32_t grid = uint32_t(ceil_div(units, 8) * 8);
-    if (dir == kForward) {
-        if (BN == 64) k_indexed_rows<DT, kForward, 64><<<grid, kThreads, 0, stream>>>(p);
-        else k_indexed_rows<DT, kForward, 128><<<grid, kThreads, 0, stream>>>(p);
-    } else {
-        if (BN == 64) k_indexed_rows<DT, kGradX, 64><<<grid, kThreads, 0, stream>>>(p);
-        else k_indexed_rows<DT, kGradX, 128><<<grid, kThreads, 0, stream>>>(p);
+    if constexpr (DT != kF32) {
+        if (pieces) {
+            const auto kernel = tile == 256 ? k_indexed_rows16<DT, DIR, 256>
+                                : tile == 128 ? k_indexed_rows16<DT, DIR, 128> : k_indexed_rows16<DT, DIR, 64>;
+            kernel<<<uint32_t(ceil_div(units, 128) * 128), kThreads, 0, stream>>>(p);
+            MNX_CHECK_LAUNCH();
+            return MNX_OK;
+        }
     }
+    const auto kernel = BN == 64 ? k_indexed_rows<DT, DIR, 64> : k_indexed_rows<DT, DIR, 128>;
+    kernel<<<uint32_t(ceil_div(units, 8) * 8), kThreads, 0, stream>>>(p);
     MNX_CHECK_LAUNCH();
     return MNX_OK;
 }
@@ -461,13 +639,29 @@ int64_t slice_rows(int64_t rows, int64_t K, int64_t N) {
 }
 
 template <int DT>
-int weights_product(WeightArgs p, int64_t rows, mnx_stream_t stream) {
-    p.kt = int32_t(ceil_div(p.K, kBM));
-    p.nt = int32_t(ceil_div(p.N, kBM));
-    const int64_t units = (rows / p.slice + p.plan.classes) * p.kt * p.nt;
+int weights_product(WeightArgs p, mnx_stream_t stream) {
+    const int64_t rows = p.plan.rows;
+    const bool pieces = in_pieces(DT, p.x, p.ldx, p.K) && in_pieces(DT, p.g, p.ldg, p.N) && in_pieces(DT, p.gw, p.N, p.N);
+    int tile = kBM;
+    const int64_t parts = rows / p.slice + p.plan.classes;
+    if (DT != kF32 && pieces) {
+        const int64_t wide = ceil_div(p.K, 256) * ceil_div(p.N, 256) * parts;
+        tile = wide >= 4 * kCUs && p.K > 128 && p.N > 128 ? 256 : 128;
+    }
+    p.kt = int32_t(ceil_div(p.K, tile));
+    p.nt = int32_t(ceil_div(p.N, tile));
+    const int64_t units = parts * p.kt * p.nt;
     MNX_REQUIRE(units < (int64_t(1) << 23), "indexed linear: too many classes and columns for one call");
     p.units = uint32_t(units);
-    k_indexed_weights<DT><<<uint32_t(ceil_div(units, 8) * 8), kThreads, 0, stream>>>(p);
+    bool done = false;
+    if constexpr (DT != kF32) {
+        if (pieces) {
+            const auto kernel = tile == 256 ? k_indexed_weights16<DT, 256> : k_indexed_weights16<DT, 128>;
+            kernel<<<uint32_t(ceil_div(units, 128) * 128), kThreads, 0, stream>>>(p);
+            done = true;
+        }
+    }
+    if (!done) k_indexed_weights<DT><<<uint32_t(ceil_div(units, 8) * 8), kThreads, 0, stream>>>(p);
     MNX_CHECK_LAUNCH();
     if (rows > p.slice) {
         const uint32_t blocks = uint32_t(std::min<int64_t>(ceil_div(int64_t(p.K) * p.N, kThreads), 2048));
@@ -495,10 +689,13 @@ int mnx_indexed_linear(const void* a, int64_t lda, int64_t rows, const int32_t* 
     MNX_REQUIRE(a && order && class_start && weight && result, "indexed linear: null pointer");
     RowsArgs p{a, weight, result, lda, Plan{order, class_start, int32_t(rows), classes},
                int32_t(transposed ? out : in), int32_t(transposed ? in : out), 0, 0};
-    const int dir = transposed ? kGradX : kForward;
-    if (dtype == kF32) return rows_product<kF32>(dir, p, rows, stream);
-    if (dtype == kBF16) return rows_product<kBF16>(dir, p, rows, stream);
-    return rows_product<kF16>(dir, p, rows, stream);
+    const auto go = [&](auto type) {
+        constexpr int DT = decltype(type)::value;
+        return transposed ? rows_product<DT, kGradX>(p, stream) : rows_product<DT, kForward>(p, stream);
+    };
+    if (dtype == kF32) return go(std::integral_constant<int, kF32>());
+    if (dtype == kBF16) return go(std::integral_constant<int, kBF16>());
+    return go(std::integral_constant<int, kF16>());
 }
 
 size_t mnx_indexed_linear_wgrad_workspace_bytes(int64_t rows, int32_t classes, int64_t in, int64_t out) {
@@ -524,9 +721,9 @@ int mnx_indexed_linear_wgrad(const void* x, int64_t ldx, const void* grad, int64
     WeightArgs p{x, grad, grad_weight, static_cast<float*>(workspace), ldx, ldg,
                  Plan{order, class_start, int32_t(rows), classes}, int32_t(in), int32_t(out), 0, 0,
                  int32_t(std::min<int64_t>(slice_rows(rows, in, out), INT32_MAX / 2)), 0};
-    if (dtype == kF32) return weights_product<kF32>(p, rows, stream);
-    if (dtype == kBF16) return weights_product<kBF16>(p, rows, stream);
-    return weights_product<kF16>(p, rows, stream);
+    if (dtype == kF32) return weights_product<kF32>(p, stream);
+    if (dtype == kBF16) return weights_product<kBF16>(p, stream);
+    return weights_product<kF16>(p, stream);
 }
 
 }  // extern "C"

@@ -20,6 +20,7 @@
 // that no load or store of the products has a bound to check.  A and B are symmetric: only tiles on and below the
 // diagonal are formed, each stored twice.
 #include "elem.h"
+#include "tile16.h"
 
 #include <cmath>
 #include <numeric>
@@ -29,11 +30,9 @@
 namespace mnx {
 namespace {
 
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+using namespace tile16;
+
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-typedef short short4v __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kPad = 128;  // sides of the padded matrices are multiples of it
 constexpr int kChunk = 4096;  // elements of a matrix that a workgroup of the momentum kernel takes
@@ -292,25 +291,6 @@ __device__ __forceinline__ f32x16 mfma(const half8& a, const half8& b, const f32
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// 16 bytes a lane from base + offset (bytes) to LDS, lane by lane from `to` on (M0).  In assembly, because for the builtin
-// the compiler waits for every such load before the next read of LDS, also of other memory there.  The caller waits
-// (vmcnt) and has a barrier before anyone reads what has come, and before it ends.
-__device__ __forceinline__ void load_lds(const _Float16* base, uint32_t offset, _Float16* to) {
-    const uint32_t m0 = uint32_t(uintptr_t((__attribute__((address_space(3))) _Float16*)to));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(m0), "v"(offset), "s"(base)
-                 : "memory", "m0");
-}
-
-// Four columns (k, k + 4) of the transposed 16-bit read: see read_tr.
-__device__ __forceinline__ half8 read_tr(const _Float16* lo, const _Float16* hi) {
-    typedef __attribute__((address_space(3))) short4v* P;
-    const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)lo), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)hi);
-    const half4 x = __builtin_bit_cast(half4, a), y = __builtin_bit_cast(half4, b);
-    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
 // Eight consecutive parameters (or results) from p on, of which `count` exist.
 template <typename T>
 __device__ __forceinline__ void apply(T* p, int count, float decay, float rate, const float (&v)[8]) {
@@ -340,26 +320,7 @@ __device__ __forceinline__ void put8(_Float16* to, const float (&v)[8]) {
     if constexpr (PL == 2) *reinterpret_cast<half8*>(to + 16) = lo;
 }
 
-// LDS that one lane wrote is read by others of the wavefront.
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-constexpr int kRow = 64;  // numbers of a row's chunk: 64 k, or 32 k of pairs
-
-// Chunks in LDS at a time: as many as leave one workgroup (two of 128) a CU.
-constexpr int stages(int tile) { return tile == 256 ? 2 : tile == 192 ? 3 : tile == 128 ? 2 : 6; }
-
 // A BT x BT tile of one product, the sum over k of I[i][k] J[j][k] (rows of both in memory), or with TR of I[i][k] J[k][j].
-// Four wavefronts share it, a quarter each.  Chunks go from memory straight to LDS, 16 bytes a lane, several ahead.  Within
-// a row of LDS the 16-byte pieces are permuted (by the lanes' source addresses: LDS itself is filled in lane order) so that
-// the reads, 16 bytes of 16 rows or 32 or 64 bytes of 4 rows, meet every bank once.
-//
-// Operands are read from LDS between the products of the 32 numbers before, which also cover the loads of chunks to come.
-// One barrier a chunk, before its last products: by then everyone has read all of it (its place is free) and the next
-// chunk has arrived.
 //
 // The last tile of a row or column may reach past the padded matrix: it reads what lies behind it in the workspace (rows
 // and columns of the result that are not stored) and stores none of that.
@@ -369,16 +330,12 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
                                                                         const Stat* __restrict__ stats, Apply ap) {
     constexpr bool SYM = MODE == kGram || MODE == kPoly, TR = !SYM;
     constexpr int W = BT / 2, MT = W / 32;  // a wavefront's part
-    constexpr int STAGES = stages(BT), SIDE = BT * kRow;  // numbers of an operand's chunk
-    constexpr int FETCH = BT / 32;          // loads a lane of an operand's chunk
-    constexpr int SUMS = kRow / PL;         // k of a chunk
-    constexpr int PIECES = PL * BT / 8;     // of a sum's columns
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * STAGES * SIDE];
+    constexpr int FETCH = BT / 32;
+    __shared__ __attribute__((aligned(16))) short lds[lds_numbers(BT)];
     const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave & 1, wj = wave >> 1;
-    // 16 tiles next to each other run on one XCD (workgroups are dealt to the eight in turn)
-    uint32_t u = (((blockIdx.x >> 7) << 3 | (blockIdx.x & 7)) << 4) | (blockIdx.x >> 3 & 15);
+    uint32_t u = unit_of_block();
     if (u >= units) return;
     const int at = find_mat(table, count, SYM ? &Mat::sym0 : &Mat::upd0, u);
     const Mat& t = table[at];
@@ -407,136 +364,25 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
     const _Float16* I = (MODE == kGram ? X : MODE == kPoly ? A : B) + int64_t(ti) * BT * K;
     const _Float16* J = TR ? X + PL * tj * BT : (MODE == kGram ? X : A) + int64_t(tj) * BT * K;
 
-    f32x16 acc[MT][MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < MT; ++n)
-#pragma unroll
-            for (int q = 0; q < 16; ++q) acc[m][n][q] = 0.f;
-
-    const int chunks = K / kRow;  // sides are multiples of 128
-    // a wavefront fills 1 KB of LDS at a time, every fourth: 8 rows of a chunk, or sums' columns piece after piece
-    const int frow = wave * 8 + (lane >> 3);
-    const uint32_t irow = 2 * (uint32_t(frow) * K + (((lane & 7) ^ ((frow >> 1) & 7)) << 3));  // bytes
+    const RowPlace in = row_place();
+    const uint32_t irow = 2 * (uint32_t(in.row) * K + in.number);  // bytes
     const int64_t istep = int64_t(32) * K, jld = PL * int64_t(t.cp);
-    // of a piece in the row of sum k: pairs' hi and lo, 32 bytes each of two groups, or 64 bytes
-    auto turn_of = [](int k) {
-        return PL == 2 ? (k & 1) << 1 | (k & 2) << 2 : BT % 128 ? ((k >> 1) & 1) << 2 : (k & 3) << 2;
-    };
     uint32_t jrow[TR ? FETCH : 1];
     if constexpr (TR) {
 #pragma unroll
         for (int n = 0; n < FETCH; ++n) {
-            const int piece = (n * 4 + wave) * 64 + lane, k = piece / PIECES, c = piece % PIECES;
-            jrow[n] = 2 * (uint32_t(k) * uint32_t(jld) + ((c ^ turn_of(k)) << 3));
+            const SumPlace at_n = sum_place<BT, PL>(n);
+            jrow[n] = 2 * (uint32_t(at_n.sum) * uint32_t(jld) + at_n.number);
         }
     }
-    // the n-th of chunk c's 2 FETCH loads
-    auto fetch = [&](int c, int n, int stage) {
-        _Float16* to = lds + stage * 2 * SIDE + (n * 4 + wave) * 512;  // J behind I
+    auto load = [&](int c, int n, short* to) {
         if (n < FETCH) load_lds(I + c * kRow + n * istep, irow, to);
-        else if constexpr (TR) load_lds(J + c * SUMS * jld, jrow[n - FETCH], to);
+        else if constexpr (TR) load_lds(J + c * (kRow / PL) * jld, jrow[n - FETCH], to);
         else load_lds(J + c * kRow + (n - FETCH) * istep, irow, to);
     };
-    // operands of 32 numbers: k 0 to 15 and 16 to 31, or hi and lo
-    struct Frags {
-        half8 i[2][MT], j[2][MT];
-    };
-    const int ki = (wi * W + l32) * kRow, kj = SIDE + (wj * W + l32) * kRow, turn = (l32 >> 1) & 7;  // 32 rows on turn alike
-    const int trow = 8 * half + ((lane & 15) >> 2);
-    auto read_i = [&](int sub, int h, int m, const _Float16* b) {
-        return *reinterpret_cast<const half8*>(b + ki + m * 32 * kRow + (((4 * sub + 2 * h + half) ^ turn) << 3));
-    };
-    auto read_j = [&](int sub, int h, int n, const _Float16* b) {
-        if constexpr (!TR) {
-            return *reinterpret_cast<const half8*>(b + kj + n * 32 * kRow + (((4 * sub + 2 * h + half) ^ turn) << 3));
-        } else {  // four sums on turn alike
-            const int k = trow + 32 / PL * sub + (PL == 1 ? 16 * h : 0), col = wj * W + n * 32 + (l32 & 16);
-            const int in = PL == 1 ? col + (lane & 3) * 4 : 2 * col + 16 * h + (lane & 3) * 4;
-            const _Float16* q = b + SIDE + k * (PL * BT) + (((in >> 3) ^ turn_of(trow)) << 3) + (in & 4);
-            return read_tr(q, q + 4 * PL * BT);
-        }
-    };
-    // The products of `now`, with the reads of `next` (32 numbers of a chunk) and `loads` between them.
-    auto multiply = [&](const Frags& now, Frags& next, int stage, int sub, auto loads) {
-        // k by k, or of pairs lo hi, hi lo, hi hi
-        constexpr int GROUPS = PL == 1 ? 2 : 3, HI[3] = {0, 1, 0}, HJ[3] = {PL == 1 ? 0 : 1, PL == 1 ? 1 : 0, 0};
-        const _Float16* b = lds + stage * 2 * SIDE;
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g)
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                if (g < 2) {
-                    next.j[g][m] = read_j(sub, g, m, b);
-                    next.i[g][m] = read_i(sub, g, m, b);
-                }
-                loads(g * MT + m);
-#pragma unroll
-                for (int n = 0; n < MT; ++n) acc[m][n] = mfma(now.j[HJ[g]][n], now.i[HI[g]][m], acc[m][n]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-    };
-    const auto nothing = [](int) {};
-    // half a chunk's loads (the part-th), shared out over the first 2 MT products
-    auto part_of = [&](int c, int part, int stage) {
-        return [=, &fetch](int at) {
-            constexpr int ALL = FETCH, PER = (ALL + 2 * MT - 1) / (2 * MT);
-#pragma unroll
-            for (int n = at * PER; n < (at + 1) * PER; ++n)
-                if (n < ALL) fetch(c, part * ALL + n, stage);
-        };
-    };
-    auto barrier = [] {
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    };
-    auto next_of = [](int stage) { return stage + 1 == STAGES ? 0 : stage + 1; };
-    Frags f0, f1;
-    int stage = 0, c = 0;
-#pragma unroll 1
-    for (int k = 0; k < min(STAGES, chunks); ++k)
-#pragma unroll
-        for (int n = 0; n < 2 * FETCH; ++n) fetch(k, n, k);
-    if (chunks >= STAGES) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * FETCH * (STAGES - 1)) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    barrier();
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            f0.i[h][m] = read_i(0, h, m, lds);
-            f0.j[h][m] = read_j(0, h, m, lds);
-        }
-    // The last products of chunk c, whose operands are in `now`, and the first operands of the next.  MORE: the first part
-    // of chunk c + STAGES goes where c was.
-    auto last_of = [&](const Frags& now, Frags& next, auto more) {
-        // (STAGES - 2) chunks behind the next may still be out
-        if constexpr (decltype(more)::value)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(2 * FETCH * (STAGES - 2)) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        barrier();
-        const int free = stage;
-        stage = next_of(stage);
-        if constexpr (decltype(more)::value) multiply(now, next, stage, 0, part_of(c + STAGES, 0, free));
-        else multiply(now, next, stage, 0, nothing);  // after the last chunk it reads what nobody uses
-        ++c;
-    };
-    const std::true_type more;
-    const std::false_type rest;
-    multiply(f0, f1, stage, 1, nothing);
-#pragma unroll 1
-    while (c + STAGES < chunks) {
-        const int free = stage;
-        last_of(f1, f0, more);
-        multiply(f0, f1, stage, 1, part_of(c - 1 + STAGES, 1, free));
-    }
-#pragma unroll 1
-    while (c + 1 < chunks) {
-        last_of(f1, f0, rest);
-        multiply(f0, f1, stage, 1, nothing);
-    }
-    last_of(f1, f0, rest);
+    Acc<BT> acc;
+    clear<BT>(acc);
+    products<BT, PL, false, TR, false>(lds, K / kRow, acc, load, [](int) {});  // sides are multiples of 128
 
     // The result, 32 rows of a wavefront's part at a time by way of LDS (its own part of it), from where rows and, for the
     // second place of a symmetric one and for tall matrices' parameters, columns leave 8 values a lane.  acc[m][n][q] is
@@ -765,7 +611,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(const Mat* __restr
     };
     auto cols_of = [&](const char* base, int stride, int block, int k) {
         const char* q = base + (k + 8 * half + ((lane & 15) >> 2)) * stride + 2 * (32 * block + (l32 & 16) + (lane & 3) * 4);
-        return read_tr(reinterpret_cast<const _Float16*>(q), reinterpret_cast<const _Float16*>(q + 4 * stride));
+        return __builtin_bit_cast(half8, read_tr(q, q + 4 * stride));
     };
     auto zero = [] {
         f32x16 z;
