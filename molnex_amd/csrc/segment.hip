@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kSegThreads) k_segment_sum_bwd(const float* __
 // element of each node; classes outside [0, S) form class S), giving the node
 // order and class boundaries that the element-indexed linear and the symmetric
 // contraction's weight gradient walk.  One wavefront per segment of
-// kGroupSeg consecutive nodes, 64 nodes per step in ascending order; within a
+// 256 or 1024 consecutive nodes, 64 nodes per step in ascending order; within a
 // step each distinct class present is handled by one ballot (rank = number of
 // lower lanes of the same class), so the order within a class is ascending
 // node id.  Three launches: per-segment class counts, an exclusive scan of
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kSegThreads) k_segment_sum_bwd(const float* __
 // workspace entry is written before it is read: no clearing is needed.
 // ---------------------------------------------------------------------------
 
-constexpr int kGroupSeg = 1024;
+constexpr int kGroupSeg = 1024;  // nodes of a wavefront at most
 constexpr int kGroupScanThreads = 1024;
 
 __device__ __forceinline__ int node_class(const int64_t* __restrict__ cls, int64_t i, int S) {
@@ -193,6 +193,7 @@ __device__ __forceinline__ int node_class(const int64_t* __restrict__ cls, int64
 // The lanes of a wavefront whose class is this lane's (`active` lanes only), by one ballot a bit of the class.
 __device__ __forceinline__ uint64_t same_class(bool active, int c, int bits) {
     uint64_t mask = __ballot(active);
+#pragma unroll 4
     for (int b = 0; b < bits; ++b) {
         const uint64_t set = __ballot(c >> b & 1);
         mask &= c >> b & 1 ? set : ~set;
@@ -230,18 +231,20 @@ __device__ __forceinline__ void load_classes(const int64_t* __restrict__ cls, in
         c[k] = i < e ? node_class(cls, i, S) : -1;
     }
 }
-__device__ __forceinline__ void count_classes(const int (&c)[kGroupSteps], int bits, int32_t* cnt) {
+__device__ __forceinline__ void count_classes(const int (&c)[kGroupSteps], int steps, int bits, int32_t* cnt) {
 #pragma unroll
     for (int k = 0; k < kGroupSteps; ++k) {
+        if (k >= steps) break;
         const uint64_t mask = same_class(c[k] >= 0, c[k], bits);
         if (c[k] >= 0 && first_of(mask)) cnt[c[k]] += __popcll(mask);
         step_done();
     }
 }
-__device__ __forceinline__ void place_classes(const int (&c)[kGroupSteps], int bits, int64_t b, int32_t* base,
-                                              int32_t* __restrict__ order) {
+__device__ __forceinline__ void place_classes(const int (&c)[kGroupSteps], int steps, int bits, int64_t b,
+                                              int32_t* base, int32_t* __restrict__ order) {
 #pragma unroll
     for (int k = 0; k < kGroupSteps; ++k) {
+        if (k >= steps) break;
         const uint64_t mask = same_class(c[k] >= 0, c[k], bits);
         if (c[k] >= 0) {
             const int32_t at = base[c[k]];
@@ -254,22 +257,27 @@ __device__ __forceinline__ void place_classes(const int (&c)[kGroupSteps], int b
 }
 
 __global__ void __launch_bounds__(kWave) k_group_count(const int64_t* __restrict__ cls, int64_t n, int S, int bits,
-                                                       int64_t nseg, int32_t* __restrict__ counts) {
+                                                       int seg_nodes, int64_t nseg, int32_t* __restrict__ counts) {
     extern __shared__ int32_t cnt[];
     const int64_t seg = blockIdx.x;
     for (int s = threadIdx.x; s <= S; s += kWave) cnt[s] = 0;
-    const int64_t b = seg * kGroupSeg;
+    const int64_t b = seg * seg_nodes;
     int c[kGroupSteps];
-    load_classes(cls, b, min(b + kGroupSeg, n), S, c);
+    load_classes(cls, b, min(b + seg_nodes, n), S, c);
     __syncthreads();
-    count_classes(c, bits, cnt);
+    const int steps = int((min(b + seg_nodes, n) - b + kWave - 1) / kWave);
+    count_classes(c, steps, bits, cnt);
     __syncthreads();
     for (int s = threadIdx.x; s <= S; s += kWave) counts[int64_t(s) * nseg + seg] = cnt[s];
 }
 
-// All of it in one workgroup: 16 wavefronts of up to kGroupSeg nodes each, and (S + 1) x 16 counters in LDS.
+// All of it in one workgroup: 16 wavefronts, and (S + 1) x 16 counters in LDS.
 constexpr int kSmallWaves = 16;
-constexpr int kSmallCounters = 8192;
+constexpr int kSmallCounters = 8192, kSmallNodes = 4096;
+
+// Nodes of a wavefront of the three launches: few, so that many run at once (12345 nodes of 89 classes took 19 us at 832
+// each), unless the counters to be summed by one workgroup were many then.
+inline int seg_nodes(int64_t n, int S) { return n * (S + 1) <= int64_t(256) * 16384 ? 256 : kGroupSeg; }
 __global__ void __launch_bounds__(kSmallWaves* kWave) k_group_small(const int64_t* __restrict__ cls, int64_t n, int S,
                                                                    int bits, int32_t* __restrict__ order,
                                                                    int32_t* __restrict__ class_start) {
@@ -283,7 +291,8 @@ __global__ void __launch_bounds__(kSmallWaves* kWave) k_group_small(const int64_
     load_classes(cls, b, min(b + per, n), S, c);
     __syncthreads();
     int32_t* const mine = cnt + wave * (S + 1);
-    count_classes(c, bits, mine);
+    const int steps = __builtin_amdgcn_readfirstlane(int((min(b + per, n) - b + kWave - 1) / kWave));
+    count_classes(c, steps, bits, mine);
     __syncthreads();
     // exclusive sums over (class, wavefront), every thread a run of them
     const int run = (len + kSmallWaves * kWave - 1) / (kSmallWaves * kWave);
@@ -309,7 +318,7 @@ __global__ void __launch_bounds__(kSmallWaves* kWave) k_group_small(const int64_
     for (int s = t; s <= S; s += kSmallWaves * kWave) class_start[s] = cnt[s];
     if (t == 0) class_start[S + 1] = int32_t(n);
     __syncthreads();
-    place_classes(c, bits, b, mine, order);
+    place_classes(c, steps, bits, b, mine, order);
 }
 
 // exclusive scan of counts[(S+1) * nseg] in place (one workgroup); class_start[s] = counts[s * nseg]
@@ -347,16 +356,16 @@ __global__ void __launch_bounds__(kGroupScanThreads) k_group_scan(int32_t* __res
 }
 
 __global__ void __launch_bounds__(kWave) k_group_place(const int64_t* __restrict__ cls, int64_t n, int S, int bits,
-                                                       int64_t nseg, const int32_t* __restrict__ offsets,
-                                                       int32_t* __restrict__ order) {
+                                                       int seg_nodes, int64_t nseg,
+                                                       const int32_t* __restrict__ offsets, int32_t* __restrict__ order) {
     extern __shared__ int32_t base[];
     const int64_t seg = blockIdx.x;
     for (int s = threadIdx.x; s <= S; s += kWave) base[s] = offsets[int64_t(s) * nseg + seg];
-    const int64_t b = seg * kGroupSeg;
+    const int64_t b = seg * seg_nodes;
     int c[kGroupSteps];
-    load_classes(cls, b, min(b + kGroupSeg, n), S, c);
+    load_classes(cls, b, min(b + seg_nodes, n), S, c);
     __syncthreads();
-    place_classes(c, bits, b, base, order);
+    place_classes(c, int((min(b + seg_nodes, n) - b + kWave - 1) / kWave), bits, b, base, order);
 }
 
 }  // namespace
@@ -429,7 +438,7 @@ int mnx_segment_sum_bwd_f32(const float* grad_out, const int64_t* index, const f
 
 size_t mnx_class_groups_workspace_bytes(int64_t num_nodes, int32_t num_classes) {
     if (num_nodes < 0 || num_classes < 0) return 0;
-    return size_t(ceil_div(num_nodes, int64_t(kGroupSeg))) * size_t(num_classes + 1) * sizeof(int32_t) + 256;
+    return size_t(ceil_div(num_nodes, seg_nodes(num_nodes, num_classes))) * size_t(num_classes + 1) * sizeof(int32_t) + 256;
 }
 
 int mnx_class_groups(const int64_t* classes, int64_t num_nodes, int32_t num_classes, int32_t* order,
@@ -442,13 +451,14 @@ int mnx_class_groups(const int64_t* classes, int64_t num_nodes, int32_t num_clas
     MNX_REQUIRE(class_start && (num_nodes == 0 || (classes && order)), "null pointer argument");
     const size_t need = mnx_class_groups_workspace_bytes(num_nodes, num_classes);
     MNX_REQUIRE(workspace && workspace_bytes >= need, "workspace %zu < %zu bytes", workspace_bytes, need);
-    const int64_t nseg = ceil_div(num_nodes, int64_t(kGroupSeg));
+    const int per = seg_nodes(num_nodes, num_classes);
+    const int64_t nseg = ceil_div(num_nodes, per);
     const size_t lds = size_t(num_classes + 1) * sizeof(int32_t);
     int32_t* counts = static_cast<int32_t*>(workspace);
     const int bits = class_bits(int(num_classes));
     // 96 nodes of 5 classes 9.0 us in the three launches, 12345 nodes of 89 160 us (a class at a time there, two barriers
     // each)
-    if (num_nodes > 0 && num_nodes <= kSmallWaves * kGroupSeg && (num_classes + 1) * kSmallWaves <= kSmallCounters) {
+    if (num_nodes > 0 && num_nodes <= kSmallNodes && (num_classes + 1) * kSmallWaves <= kSmallCounters) {
         hipLaunchKernelGGL(k_group_small, dim3(1), dim3(kSmallWaves * kWave), 0, stream, classes, num_nodes,
                            int(num_classes), bits, order, class_start);
         MNX_CHECK_LAUNCH();
@@ -456,7 +466,7 @@ int mnx_class_groups(const int64_t* classes, int64_t num_nodes, int32_t num_clas
     }
     if (nseg > 0) {
         hipLaunchKernelGGL(k_group_count, dim3(unsigned(nseg)), dim3(kWave), lds, stream, classes, num_nodes,
-                           int(num_classes), bits, nseg, counts);
+                           int(num_classes), bits, per, nseg, counts);
         MNX_CHECK_LAUNCH();
     }
     hipLaunchKernelGGL(k_group_scan, dim3(1), dim3(kGroupScanThreads), 0, stream, counts,
@@ -464,7 +474,7 @@ int mnx_class_groups(const int64_t* classes, int64_t num_nodes, int32_t num_clas
     MNX_CHECK_LAUNCH();
     if (nseg > 0) {
         hipLaunchKernelGGL(k_group_place, dim3(unsigned(nseg)), dim3(kWave), lds, stream, classes, num_nodes,
-                           int(num_classes), bits, nseg, counts, order);
+                           int(num_classes), bits, per, nseg, counts, order);
         MNX_CHECK_LAUNCH();
     }
     return MNX_OK;
