@@ -528,9 +528,9 @@ struct Steps {
 // A whole matrix in one workgroup, from its gradient to its parameters: X and A (then B) stay in LDS.  The tiled products
 // take eight microseconds a launch however little there is to do, three launches a step.
 //
-// Eight wavefronts share the blocks of 32 x 32 of A and B on and below the diagonal, and the columns of X, 32 at a time: a
-// wavefront's columns of a X + B X read nothing of X but these columns, so they are replaced in place.  Pairs sum hi hi and
-// the two cross products apart, and add them at the end.
+// Eight wavefronts share the blocks of 32 x 32 of A and B on and below the diagonal, and the columns of X, 32 at a time:
+// such columns of a X + B X read nothing of X but these columns, so they are replaced in place.  Pairs sum hi hi and the
+// cross products apart, and add them at the end.
 template <int PL, int LDS>
 __global__ void __launch_bounds__(kSmallThreads) k_muon_small(const Mat* __restrict__ table, int count, Momentum h,
                                                               double eps, Steps st, Apply ap) {
@@ -549,25 +549,33 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(const Mat* __restr
     char* const A = lds + PL * 32 * rb * sx;
     const int xplane = 32 * rb * sx, aplane = 32 * rb * sa;
 
-    // momenta and the norm
+    // momenta and the norm, four vectors a thread on their way at a time
     double sum = 0;
     by_type(t.dtype, [&](auto type) {
         const auto* g = static_cast<const decltype(type)*>(t.g) + off;
-        for (int64_t i = tid * 4; i < n; i += kSmallThreads * 4) {
-            float v[4], m[4];
-            load4(g + i, n - i, v);
-            if (t.m) {
-                load4(t.m + off + i, n - i, m);
+        for (int64_t i0 = tid * 4; i0 < n; i0 += kSmallThreads * 16) {
+            float v[4][4], m[4][4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (h.maximize) v[e] = -v[e];
-                    m[e] = m[e] * h.mu + h.w * v[e];
-                    v[e] = direction(v[e], m[e], h);
-                }
-                store4(t.m + off + i, n - i, m);
+            for (int k = 0; k < 4; ++k) {
+                const int64_t i = i0 + k * kSmallThreads * 4;
+                load4(g + i, n - i, v[k]);
+                if (t.m) load4(t.m + off + i, n - i, m[k]);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += double(v[e]) * double(v[e]);
+            for (int k = 0; k < 4; ++k) {
+                const int64_t i = i0 + k * kSmallThreads * 4;
+                if (t.m) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (h.maximize) v[k][e] = -v[k][e];
+                        m[k][e] = m[k][e] * h.mu + h.w * v[k][e];
+                        v[k][e] = direction(v[k][e], m[k][e], h);
+                    }
+                    store4(t.m + off + i, n - i, m[k]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += double(v[k][e]) * double(v[k][e]);
+            }
         }
     });
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
@@ -582,24 +590,33 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(const Mat* __restr
     by_type(t.dtype, [&](auto type) {
         const auto* g = static_cast<const decltype(type)*>(t.g) + off;
         const int rows = 32 * (tall ? cb : rb), vecs = 8 * (tall ? rb : cb);
-        for (int it = tid; it < rows * vecs; it += kSmallThreads) {
-            const int i = it / vecs, j = it % vecs * 4, left = i < t.rows ? t.cols - j : 0;
-            float v[4], m[4];
-            load4(g + int64_t(i) * t.cols + j, left, v);
-            if (t.m) load4(t.m + off + int64_t(i) * t.cols + j, left, m);
+        for (int it0 = tid; it0 < rows * vecs; it0 += 4 * kSmallThreads) {
+            float v[4][4], m[4][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (t.m) v[e] = direction(h.maximize ? -v[e] : v[e], m[e], h);
-                v[e] = ldexpf(v[e], stat.exponent);
+            for (int k = 0; k < 4; ++k) {
+                const int it = it0 + k * kSmallThreads, i = it / vecs, j = it % vecs * 4;
+                const int left = i < t.rows ? t.cols - j : 0;
+                load4(g + int64_t(i) * t.cols + j, left, v[k]);
+                if (t.m) load4(t.m + off + int64_t(i) * t.cols + j, left, m[k]);
             }
-            if (!tall) {
-                put4<PL>(reinterpret_cast<_Float16*>(X + i * sx + 2 * j), xplane / 2, v);
-            } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int it = it0 + k * kSmallThreads, i = it / vecs, j = it % vecs * 4;
+                if (it >= rows * vecs) continue;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    _Float16* to = reinterpret_cast<_Float16*>(X + (j + e) * sx + 2 * i);
-                    to[0] = _Float16(v[e]);
-                    if constexpr (PL == 2) to[xplane / 2] = _Float16(v[e] - float(to[0]));
+                    if (t.m) v[k][e] = direction(h.maximize ? -v[k][e] : v[k][e], m[k][e], h);
+                    v[k][e] = ldexpf(v[k][e], stat.exponent);
+                }
+                if (!tall) {
+                    put4<PL>(reinterpret_cast<_Float16*>(X + i * sx + 2 * j), xplane / 2, v[k]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        _Float16* to = reinterpret_cast<_Float16*>(X + (j + e) * sx + 2 * i);
+                        to[0] = _Float16(v[k][e]);
+                        if constexpr (PL == 2) to[xplane / 2] = _Float16(v[k][e] - float(to[0]));
+                    }
                 }
             }
         }
@@ -621,18 +638,18 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(const Mat* __restr
     };
     // block (bi, bj) of the product of S's rows with themselves
     auto square = [&](const char* S, int stride, int plane, int bi, int bj, int K) {
-        f32x16 big = zero(), small = zero();
+        f32x16 big = zero(), low = zero(), high = zero();
 #pragma unroll 4
         for (int k = 0; k < K; k += 16) {
             const half8 i = rows_of(S, stride, bi, k), j = rows_of(S, stride, bj, k);
             if constexpr (PL == 2) {
                 const half8 il = rows_of(S + plane, stride, bi, k), jl = rows_of(S + plane, stride, bj, k);
-                small = mfma(jl, i, small);
-                small = mfma(j, il, small);
+                low = mfma(jl, i, low);
+                high = mfma(j, il, high);
             }
             big = mfma(j, i, big);
         }
-        return PL == 2 ? big + small : big;
+        return PL == 2 ? big + (low + high) : big;
     };
     // the block's values into A, above the diagonal too; `own` of what is there
     auto into_a = [&](const f32x16& acc, int bi, int bj, float own, float prod) {
@@ -702,41 +719,50 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(const Mat* __restr
         __syncthreads();
         const float own = st.own[step] * rho, prod = st.prod[step] * rho;
         const bool last = step + 1 == st.count;
-        for (int bj = wave; bj < cb; bj += WAVES) {
-            f32x16 big[4], small[PL == 2 ? 4 : 1];
+        // with more than two blocks of rows, two wavefronts share 32 columns, and wait for each other before they replace them
+        const int groups = (rb + 1) / 2;
+        for (int item0 = 0; item0 < cb * groups; item0 += WAVES) {
+            const int item = item0 + wave, bj = item / groups, r0 = item % groups * 2;
+            const bool mine = item < cb * groups;
+            f32x16 big[2], small[2];
+            if (mine) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                big[r] = zero();
-                if constexpr (PL == 2) small[r] = zero();
-            }
+                for (int r = 0; r < 2; ++r) big[r] = small[r] = zero();
 #pragma unroll 2
-            for (int k = 0; k < 32 * rb; k += 16) {
-                const half8 j = cols_of(X, sx, bj, k);
-                half8 jl;
-                if constexpr (PL == 2) jl = cols_of(X + xplane, sx, bj, k);
+                for (int k = 0; k < 32 * rb; k += 16) {
+                    const half8 j = cols_of(X, sx, bj, k);
+                    half8 i[2], jl, il[2];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (r >= rb) continue;
-                    const half8 i = rows_of(A, sa, r, k);
+                    for (int r = 0; r < 2; ++r) i[r] = rows_of(A, sa, min(r0 + r, rb - 1), k);
                     if constexpr (PL == 2) {
-                        const half8 il = rows_of(A + aplane, sa, r, k);
-                        small[r] = mfma(jl, i, small[r]);
-                        small[r] = mfma(j, il, small[r]);
+                        jl = cols_of(X + xplane, sx, bj, k);
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) il[r] = rows_of(A + aplane, sa, min(r0 + r, rb - 1), k);
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) small[r] = mfma(jl, i[r], small[r]);
                     }
-                    big[r] = mfma(j, i, big[r]);
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) big[r] = mfma(j, i[r], big[r]);
+                    if constexpr (PL == 2) {
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) small[r] = mfma(j, il[r], small[r]);
+                    }
                 }
             }
-            wave_sync();
+            if (groups > 1) __syncthreads();
+            else wave_sync();
+            if (!mine) continue;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if (r >= rb) continue;
+            for (int r = 0; r < 2; ++r) {
+                if (r0 + r >= rb) continue;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int i = 32 * r + l32, j = 32 * bj + 8 * q + 4 * half;
+                    const int i = 32 * (r0 + r) + l32, j = 32 * bj + 8 * q + 4 * half;
                     _Float16* to = reinterpret_cast<_Float16*>(X + i * sx + 2 * j);
                     float v[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = prod * (PL == 2 ? big[r][4 * q + e] + small[PL == 2 ? r : 0][4 * q + e] : big[r][4 * q + e]);
+                    for (int e = 0; e < 4; ++e)
+                        v[e] = prod * (PL == 2 ? big[r][4 * q + e] + small[r][4 * q + e] : big[r][4 * q + e]);
 #pragma unroll
                     for (int pl = PL - 1; pl >= 0; --pl) {
                         const half4 old = *reinterpret_cast<const half4*>(to + pl * (xplane / 2));
