@@ -179,17 +179,17 @@ struct RowsArgs {
     uint32_t units;
 };
 
-// y or gx: 128 rows of one class against BN columns.
-template <int DT, int DIR, int BN>
+// y or gx: BM rows of one class against BN columns.
+template <int DT, int DIR, int BM, int BN>
 __global__ void __launch_bounds__(kThreads) k_indexed_rows(RowsArgs p) {
     using T = typename Kind<DT>::T;
     constexpr int KC = Kind<DT>::kc, V = Kind<DT>::vec, PL = Kind<DT>::planes;
-    constexpr int NA = kBM * KC / V / kThreads, NB = BN * KC / V / kThreads;  // vectors a thread
+    constexpr int NA = BM * KC / V / kThreads, NB = BN * KC / V / kThreads;  // vectors a thread
     constexpr int VR = KC / V;       // vectors of a row's chunk
     constexpr int VC = BN / V;       // vectors of a sum index's columns
-    constexpr int WN = BN / 2, MT = 2, NT = WN / 32;
-    __shared__ short sA[PL * kBM * KC], sB[PL * BN * KC];
-    __shared__ int32_t rows[kBM];
+    constexpr int WM = BM / 2, WN = BN / 2, MT = WM / 32, NT = WN / 32;
+    __shared__ short sA[PL * BM * KC], sB[PL * BN * KC];
+    __shared__ int32_t rows[BM];
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // Column tiles of the same rows, and then rows of the same class, side by side on one XCD
@@ -197,12 +197,12 @@ __global__ void __launch_bounds__(kThreads) k_indexed_rows(RowsArgs p) {
     if (u >= p.units) return;
     const int row_tile = int(u / uint32_t(p.col_tiles)), col0 = int(u % uint32_t(p.col_tiles)) * BN;
     const int classes = p.plan.classes;
-    const Found f = find_class(p.plan, classes + 1, row_tile, [](int n) { return (n + kBM - 1) / kBM; },
+    const Found f = find_class(p.plan, classes + 1, row_tile, [](int n) { return (n + BM - 1) / BM; },
                                [](int) { return 0; });
     if (f.cls > classes) return;
-    const int first = p.plan.start(f.cls) + f.unit * kBM;
-    const int count = min(kBM, p.plan.start(f.cls + 1) - first);  // at least 1
-    for (int i = tid; i < kBM; i += kThreads) rows[i] = p.plan.row(first + min(i, count - 1));
+    const int first = p.plan.start(f.cls) + f.unit * BM;
+    const int count = min(BM, p.plan.start(f.cls + 1) - first);  // at least 1
+    for (int i = tid; i < BM; i += kThreads) rows[i] = p.plan.row(first + min(i, count - 1));
     __syncthreads();
     const int K = f.cls == classes ? 0 : p.sums;  // zeros for rows out of range
     const T* W = static_cast<const T*>(p.w) + (f.cls == classes ? 0 : int64_t(f.cls) * p.sums * p.cols);
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kThreads) k_indexed_rows(RowsArgs p) {
     auto put = [&]() {
 #pragma unroll
         for (int i = 0; i < NA; ++i)
-            store_vec<DT>(sA, kBM * KC, by_rows<KC>((tid + i * kThreads) / VR, (tid % VR) * V), va[i]);
+            store_vec<DT>(sA, BM * KC, by_rows<KC>((tid + i * kThreads) / VR, (tid % VR) * V), va[i]);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const int it = tid + i * kThreads;
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kThreads) k_indexed_rows(RowsArgs p) {
 #pragma unroll
             for (int pl = 0; pl < PL; ++pl) {
 #pragma unroll
-                for (int m = 0; m < MT; ++m) a[pl][m] = read_rows<KC>(sA + pl * kBM * KC, wm * 64 + m * 32, ks);
+                for (int m = 0; m < MT; ++m) a[pl][m] = read_rows<KC>(sA + pl * BM * KC, wm * WM + m * 32, ks);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
                     b[pl][n] = DIR == kForward ? read_sums<BN>(sB + pl * BN * KC, wn * WN + n * 32, ks)
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kThreads) k_indexed_rows(RowsArgs p) {
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
-            const int r = wm * 64 + m * 32 + 8 * (q / 4) + 4 * half + q % 4;
+            const int r = wm * WM + m * 32 + 8 * (q / 4) + 4 * half + q % 4;
             if (r >= count) continue;
             T* to = out + int64_t(rows[r]) * p.cols;
 #pragma unroll
@@ -296,20 +296,22 @@ struct WeightArgs {
 __device__ __forceinline__ int slices(int n, int slice) { return n > slice ? (n + slice - 1) / slice : 1; }
 __device__ __forceinline__ int slots(int n, int slice) { return n > slice ? (n + slice - 1) / slice : 0; }
 
-// A 128 x 128 tile of one class's gradient over one slice of its rows.
-template <int DT>
+// A 128 x BN tile of one class's gradient over one slice of its rows.
+template <int DT, int BN>
 __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
     using T = typename Kind<DT>::T;
     constexpr int KC = Kind<DT>::kc, V = Kind<DT>::vec, PL = Kind<DT>::planes;
-    constexpr int VC = kBM / V, NV = kBM * KC / V / kThreads, STEP = kThreads / VC;
-    __shared__ short sA[PL * kBM * KC], sB[PL * kBM * KC];
+    constexpr int VA = kBM / V, NA = kBM * KC / V / kThreads, STEP_A = kThreads / VA;
+    constexpr int VB = BN / V, NB = BN * KC / V / kThreads, STEP_B = kThreads / VB;
+    constexpr int WN = BN / 2, NT = WN / 32;
+    __shared__ short sA[PL * kBM * KC], sB[PL * BN * KC];
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t per = (p.units + 7) / 8, u = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if (u >= p.units) return;
     const uint32_t tiles = uint32_t(p.kt) * uint32_t(p.nt);
     const int slice_at = int(u / tiles), tile = int(u % tiles);
-    const int k0 = tile / p.nt * kBM, n0 = tile % p.nt * kBM;
+    const int k0 = tile / p.nt * kBM, n0 = tile % p.nt * BN;
     const int slice = p.slice;
     const Found f = find_class(p.plan, p.plan.classes, slice_at, [=](int n) { return slices(n, slice); },
                                [=](int n) { return slots(n, slice); });
@@ -317,26 +319,31 @@ __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
     const int lo = p.plan.start(f.cls), n_class = p.plan.count(f.cls);
     const int begin = lo + f.unit * slice, end = lo + min(n_class, (f.unit + 1) * slice);
     const T *X = static_cast<const T*>(p.x), *G = static_cast<const T*>(p.g);
-    const int col = (tid % VC) * V, krow = tid / VC;
+    const int acol = (tid % VA) * V, arow = tid / VA, bcol = (tid % VB) * V, brow = tid / VB;
 
-    f32x4 va[NV], vb[NV];
-    int row[NV];
+    f32x4 va[NA], vb[NB];
+    int ra[NA], rb[NB];
     auto find_rows = [&](int r0) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int at = r0 + krow + i * STEP;
-            row[i] = at < end ? p.plan.row(at) : -1;
+        for (int i = 0; i < NA; ++i) {
+            const int at = r0 + arow + i * STEP_A;
+            ra[i] = at < end ? p.plan.row(at) : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int at = r0 + brow + i * STEP_B;
+            rb[i] = at < end ? p.plan.row(at) : -1;
         }
     };
     auto load = [&]() {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int64_t r = max(row[i], 0);
-            va[i] = load_vec<DT>(X + r * p.ldx + k0 + col, row[i] >= 0 ? p.K - k0 - col : 0);
-            vb[i] = load_vec<DT>(G + r * p.ldg + n0 + col, row[i] >= 0 ? p.N - n0 - col : 0);
-        }
+        for (int i = 0; i < NA; ++i)
+            va[i] = load_vec<DT>(X + int64_t(max(ra[i], 0)) * p.ldx + k0 + acol, ra[i] >= 0 ? p.K - k0 - acol : 0);
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+            vb[i] = load_vec<DT>(G + int64_t(max(rb[i], 0)) * p.ldg + n0 + bcol, rb[i] >= 0 ? p.N - n0 - bcol : 0);
     };
-    f32x16 acc[2][2];
+    f32x16 acc[2][NT];
     clear_acc(acc);
     const int wm = wave & 1, wn = wave >> 1;
     if (begin < end) {
@@ -347,10 +354,9 @@ __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
     for (int r0 = begin; r0 < end; r0 += KC) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            store_vec<DT>(sA, kBM * KC, by_sums<kBM>(krow + i * STEP, col), va[i]);
-            store_vec<DT>(sB, kBM * KC, by_sums<kBM>(krow + i * STEP, col), vb[i]);
-        }
+        for (int i = 0; i < NA; ++i) store_vec<DT>(sA, kBM * KC, by_sums<kBM>(arow + i * STEP_A, acol), va[i]);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) store_vec<DT>(sB, BN * KC, by_sums<BN>(brow + i * STEP_B, bcol), vb[i]);
         __syncthreads();
         if (r0 + KC < end) {
             load();
@@ -358,15 +364,15 @@ __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
         }
 #pragma unroll
         for (int ks = 0; ks < KC; ks += 16) {
-            short8v a[PL][2], b[PL][2];
+            short8v a[PL][2], b[PL][NT];
 #pragma unroll
-            for (int pl = 0; pl < PL; ++pl)
+            for (int pl = 0; pl < PL; ++pl) {
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    a[pl][m] = read_sums<kBM>(sA + pl * kBM * KC, wm * 64 + m * 32, ks);
-                    b[pl][m] = read_sums<kBM>(sB + pl * kBM * KC, wn * 64 + m * 32, ks);
-                }
-            multiply<DT, 2, 2>(a, b, acc);
+                for (int m = 0; m < 2; ++m) a[pl][m] = read_sums<kBM>(sA + pl * kBM * KC, wm * 64 + m * 32, ks);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) b[pl][n] = read_sums<BN>(sB + pl * BN * KC, wn * WN + n * 32, ks);
+            }
+            multiply<DT, 2, NT>(a, b, acc);
         }
     }
     const bool whole = n_class <= slice;
@@ -379,8 +385,8 @@ __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
             const int k = k0 + wm * 64 + m * 32 + 8 * (q / 4) + 4 * half + q % 4;
             if (k >= p.K) continue;
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int c = n0 + wn * 64 + n * 32 + l32;
+            for (int n = 0; n < NT; ++n) {
+                const int c = n0 + wn * WN + n * 32 + l32;
                 if (c >= p.N) continue;
                 if (whole) out[int64_t(k) * p.N + c] = T(acc[m][n][q]);
                 else part[int64_t(k) * p.N + c] = acc[m][n][q];
@@ -562,25 +568,45 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_indexed_weights16(We
     });
 }
 
-// The partial sums of the classes with several slices, added in order.
+// The partial sums of the classes with several slices, added in order: a workgroup takes 128 elements, eight shares of the
+// slices (in order again) of 32 threads each.
 template <int DT>
 __global__ void __launch_bounds__(kThreads) k_indexed_join(WeightArgs p) {
-    using T = typename Kind<DT>::T;
+    using T = typename Elem<DT>::T;
+    __shared__ f32x4 share[8][32];
     const int cls = blockIdx.y, slice = p.slice;
     const int n = p.plan.count(cls);
     if (n <= slice) return;
-    // the class's own first unit: the scan's answer for it
-    int before = 0;
+    int before = 0;  // slices of the classes before
     for (int c = int(threadIdx.x & 63); c < cls; c += 64) before += slots(p.plan.count(c), slice);
     for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d);
-    const int count = slots(n, slice);
+    const int count = slots(n, slice), each = (count + 7) / 8;
     const int64_t size = int64_t(p.K) * p.N;
     const float* part = p.part + before * size;
     T* out = static_cast<T*>(p.gw) + cls * size;
-    for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < size; e += int64_t(gridDim.x) * kThreads) {
-        float sum = part[e];
-        for (int s = 1; s < count; ++s) sum += part[s * size + e];
-        out[e] = T(sum);
+    typedef float Four __attribute__((ext_vector_type(4), aligned(4)));
+    const int col = threadIdx.x & 31, group = threadIdx.x >> 5;
+    for (int64_t e0 = int64_t(blockIdx.x) * 128; e0 < size; e0 += int64_t(gridDim.x) * 128) {
+        const int64_t e = e0 + col * 4;
+        f32x4 sum = {0, 0, 0, 0};
+        const int end = min((group + 1) * each, count);
+        if (e + 4 <= size) {
+#pragma unroll 8
+            for (int s = group * each; s < end; ++s) sum += f32x4(*reinterpret_cast<const Four*>(part + s * size + e));
+        } else {
+            for (int s = group * each; s < end; ++s)
+                for (int k = 0; k < 4; ++k)
+                    if (e + k < size) sum[k] += part[s * size + e + k];
+        }
+        share[group][col] = sum;
+        __syncthreads();
+        if (group == 0) {
+#pragma unroll
+            for (int g = 1; g < 8; ++g) sum += share[g][col];
+            for (int k = 0; k < 4; ++k)
+                if (e + k < size) out[e + k] = T(sum[k]);
+        }
+        __syncthreads();
     }
 }
 
@@ -613,6 +639,8 @@ int rows_product(RowsArgs p, mnx_stream_t stream) {
     }
     const int BN = pieces ? tile : p.cols <= 64 ? 64 : 128;
     p.col_tiles = int32_t(ceil_div(p.cols, BN));
+    // three workgroups share a CU: half the rows each where whole ones would leave places free
+    if (!pieces && ceil_div(rows, kBM) * p.col_tiles < 3 * kCUs) tile = kBM / 2;
     const int64_t units = (rows / tile + parts) * p.col_tiles;
     MNX_REQUIRE(units < (int64_t(1) << 23), "indexed linear: too many rows and columns for one call");
     p.units = uint32_t(units);
@@ -625,17 +653,20 @@ int rows_product(RowsArgs p, mnx_stream_t stream) {
             return MNX_OK;
         }
     }
-    const auto kernel = BN == 64 ? k_indexed_rows<DT, DIR, 64> : k_indexed_rows<DT, DIR, 128>;
+    const auto kernel = tile == 64 ? (BN == 64 ? k_indexed_rows<DT, DIR, 64, 64> : k_indexed_rows<DT, DIR, 64, 128>)
+                                   : (BN == 64 ? k_indexed_rows<DT, DIR, 128, 64> : k_indexed_rows<DT, DIR, 128, 128>);
     kernel<<<uint32_t(ceil_div(units, 8) * 8), kThreads, 0, stream>>>(p);
     MNX_CHECK_LAUNCH();
     return MNX_OK;
 }
 
-// Rows of a slice: enough slices for the card where the tiles of one gradient are few.
-int64_t slice_rows(int64_t rows, int64_t K, int64_t N) {
-    const int64_t tiles = ceil_div(K, kBM) * ceil_div(N, kBM);
-    const int64_t want = std::max<int64_t>(1, 1024 / tiles);
-    return std::max<int64_t>(256, ceil_div(ceil_div(std::max<int64_t>(rows, 1), want), 64) * 64);
+// Rows of a slice: enough slices for the card where the tiles of one gradient are few, and none that is eight times the
+// average class.
+int64_t slice_rows(int64_t rows, int64_t K, int64_t N, int64_t classes) {
+    const int64_t tiles = ceil_div(K, kBM) * ceil_div(N, kBM), least = tiles <= 2 ? 128 : 256;
+    const int64_t want = std::max<int64_t>(1, 3 * kCUs / tiles);
+    const int64_t most = std::max(least, 8 * rows / classes);
+    return ceil_div(std::min(most, std::max(least, ceil_div(rows, want))), 64) * 64;
 }
 
 template <int DT>
@@ -648,8 +679,9 @@ int weights_product(WeightArgs p, mnx_stream_t stream) {
         const int64_t wide = ceil_div(p.K, 256) * ceil_div(p.N, 256) * parts;
         tile = wide >= 4 * kCUs && p.K > 128 && p.N > 128 ? 256 : 128;
     }
+    const int cols = !pieces && p.N <= 64 ? 64 : tile;
     p.kt = int32_t(ceil_div(p.K, tile));
-    p.nt = int32_t(ceil_div(p.N, tile));
+    p.nt = int32_t(ceil_div(p.N, cols));
     const int64_t units = parts * p.kt * p.nt;
     MNX_REQUIRE(units < (int64_t(1) << 23), "indexed linear: too many classes and columns for one call");
     p.units = uint32_t(units);
@@ -661,10 +693,13 @@ int weights_product(WeightArgs p, mnx_stream_t stream) {
             done = true;
         }
     }
-    if (!done) k_indexed_weights<DT><<<uint32_t(ceil_div(units, 8) * 8), kThreads, 0, stream>>>(p);
+    if (!done) {
+        const auto kernel = cols == 64 ? k_indexed_weights<DT, 64> : k_indexed_weights<DT, 128>;
+        kernel<<<uint32_t(ceil_div(units, 8) * 8), kThreads, 0, stream>>>(p);
+    }
     MNX_CHECK_LAUNCH();
     if (rows > p.slice) {
-        const uint32_t blocks = uint32_t(std::min<int64_t>(ceil_div(int64_t(p.K) * p.N, kThreads), 2048));
+        const uint32_t blocks = uint32_t(std::min<int64_t>(ceil_div(int64_t(p.K) * p.N, 128), 2048));
         k_indexed_join<DT><<<dim3(blocks, uint32_t(p.plan.classes)), kThreads, 0, stream>>>(p);
         MNX_CHECK_LAUNCH();
     }
@@ -701,7 +736,7 @@ int mnx_indexed_linear(const void* a, int64_t lda, int64_t rows, const int32_t* 
 size_t mnx_indexed_linear_wgrad_workspace_bytes(int64_t rows, int32_t classes, int64_t in, int64_t out) {
     if (check_shape("indexed linear", rows, classes, in, out, kF32)) return 0;
     // a class of several slices has at most twice its share of them
-    const int64_t slice = slice_rows(rows, in, out);
+    const int64_t slice = slice_rows(rows, in, out, classes);
     if (rows <= slice) return 0;
     return size_t(std::min(2 * (rows / slice), rows / slice + classes)) * size_t(in) * size_t(out) * sizeof(float);
 }
@@ -720,7 +755,7 @@ int mnx_indexed_linear_wgrad(const void* x, int64_t ldx, const void* grad, int64
         return set_error(MNX_ERR_WORKSPACE, "indexed linear: workspace too small");
     WeightArgs p{x, grad, grad_weight, static_cast<float*>(workspace), ldx, ldg,
                  Plan{order, class_start, int32_t(rows), classes}, int32_t(in), int32_t(out), 0, 0,
-                 int32_t(std::min<int64_t>(slice_rows(rows, in, out), INT32_MAX / 2)), 0};
+                 int32_t(std::min<int64_t>(slice_rows(rows, in, out, classes), INT32_MAX / 2)), 0};
     if (dtype == kF32) return weights_product<kF32>(p, stream);
     if (dtype == kBF16) return weights_product<kBF16>(p, stream);
     return weights_product<kF16>(p, stream);
