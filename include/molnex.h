@@ -1000,7 +1000,8 @@ int mnx_muon_step(const mnx_muon_args* args, mnx_stream_t stream);
 int mnx_indexed_linear(const void* a, int64_t lda, int64_t rows, const int32_t* order, const int32_t* class_start,
                        int32_t classes, const void* weight, int64_t in, int64_t out, int32_t dtype, int32_t transposed,
                        void* result, mnx_stream_t stream);
-size_t mnx_indexed_linear_wgrad_workspace_bytes(int64_t rows, int32_t classes, int64_t in, int64_t out);
+size_t mnx_indexed_linear_wgrad_workspace_bytes(int64_t rows, int32_t classes, int64_t in, int64_t out,
+                                                int32_t dtype);
 int mnx_indexed_linear_wgrad(const void* x, int64_t ldx, const void* grad, int64_t ldg, int64_t rows,
                              const int32_t* order, const int32_t* class_start, int32_t classes, int64_t in,
                              int64_t out, int32_t dtype, void* grad_weight, void* workspace, size_t workspace_bytes,

@@ -166,7 +166,7 @@ SIGNATURES = {
     "mnx_muon_workspace_bytes": (c_sz, [vp]),
     "mnx_muon_step": (C.c_int, [vp, vp]),
     "mnx_indexed_linear": (C.c_int, [vp, c_i64, c_i64, vp, vp, c_i32, vp, c_i64, c_i64, c_i32, c_i32, vp, vp]),
-    "mnx_indexed_linear_wgrad_workspace_bytes": (c_sz, [c_i64, c_i32, c_i64, c_i64]),
+    "mnx_indexed_linear_wgrad_workspace_bytes": (c_sz, [c_i64, c_i32, c_i64, c_i64, c_i32]),
     "mnx_indexed_linear_wgrad": (C.c_int, [vp, c_i64, vp, c_i64, c_i64, vp, vp, c_i32, c_i64, c_i64, c_i32, vp, vp,
                                             c_sz, vp]),
 }

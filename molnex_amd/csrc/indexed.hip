@@ -22,6 +22,8 @@
 #include "elem.h"
 #include "tile16.h"
 
+#include <cmath>
+
 namespace mnx {
 namespace {
 
@@ -42,7 +44,8 @@ struct Kind {
     typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
-// `left` elements of a vector at p; zeros behind them.
+// `left` elements of a vector at p; zeros behind them.  (The last vector of a row loaded whole and shifted into place would
+// be waited for here: 50k float32 rows of 1024 to 1024 took 1026 us so, 775 as it is.)
 template <int DT>
 __device__ __forceinline__ f32x4 load_vec(const typename Kind<DT>::T* p, int left) {
     constexpr int V = Kind<DT>::vec;
@@ -293,8 +296,13 @@ struct WeightArgs {
     uint32_t units;
 };
 
+// A class of n rows: its slices, those with partial sums, and the rows of each but the last (about the same in all).
 __device__ __forceinline__ int slices(int n, int slice) { return n > slice ? (n + slice - 1) / slice : 1; }
 __device__ __forceinline__ int slots(int n, int slice) { return n > slice ? (n + slice - 1) / slice : 0; }
+__device__ __forceinline__ int slice_length(int n, int slice) {
+    const int count = slices(n, slice);
+    return ((n + count - 1) / count + 63) & ~63;
+}
 
 // A 128 x BN tile of one class's gradient over one slice of its rows.
 template <int DT, int BN>
@@ -317,7 +325,8 @@ __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
                                [=](int n) { return slots(n, slice); });
     if (f.cls >= p.plan.classes) return;
     const int lo = p.plan.start(f.cls), n_class = p.plan.count(f.cls);
-    const int begin = lo + f.unit * slice, end = lo + min(n_class, (f.unit + 1) * slice);
+    const int length = slice_length(n_class, slice);
+    const int begin = lo + f.unit * length, end = lo + min(n_class, (f.unit + 1) * length);
     const T *X = static_cast<const T*>(p.x), *G = static_cast<const T*>(p.g);
     const int acol = (tid % VA) * V, arow = tid / VA, bcol = (tid % VB) * V, brow = tid / VB;
 
@@ -436,13 +445,20 @@ __device__ __forceinline__ void store_tile(short* lds, const Acc<BT>& acc, int r
     }
 }
 
+// Eight values at any alignment, of which `count` exist.
 template <typename T>
-__device__ __forceinline__ void store8(T* to, const float (&v)[8]) {
-    typedef T Eight __attribute__((ext_vector_type(8)));
-    Eight o;
+__device__ __forceinline__ void store8(T* to, int count, const float (&v)[8]) {
+    typedef T Eight __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    if (count >= 8) {
+        Eight o;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = T(v[e]);
-    *reinterpret_cast<Eight*>(to) = o;
+        for (int e = 0; e < 8; ++e) o[e] = T(v[e]);
+        *reinterpret_cast<Eight*>(to) = o;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < count) to[e] = T(v[e]);
+    }
 }
 
 // y or gx, BT rows of one class against BT columns: the loop of tile16.h, rows gathered by the lanes' addresses.  What lies
@@ -503,20 +519,22 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_indexed_rows16(RowsA
         products<BT, 1, false, DIR == kForward, DT == kBF16>(lds, (K + kRow - 1) / kRow, acc, load, [](int) {});
     }
     store_tile<BT>(lds, acc, count, p.cols - col0, [&](int i, int j, const float (&v)[8]) {
-        store8(out + int64_t(rows[i]) * p.cols + col0 + j, v);
+        store8(out + int64_t(rows[i]) * p.cols + col0 + j, p.cols - col0 - j, v);
     });
 }
 
-constexpr int kIds = 2048;  // rows whose numbers are in LDS at a time
+constexpr int kIds = 1536;  // rows whose places are in LDS at a time
 
 // A BT x BT tile of one class's gradient over one slice of its rows: both operands by sums, their rows gathered by the
-// lanes' addresses; behind the slice's end, zeros from elsewhere.
-template <int DT, int BT>
+// lanes' addresses; behind the slice's end, zeros from elsewhere.  NEAR: rows lie within 4 GB, and LDS holds how far, so
+// that an address is one addition (64-bit products of row numbers take as long as the matrix cores here).
+template <int DT, int BT, bool NEAR>
 __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_indexed_weights16(WeightArgs p) {
     using T = typename Elem<DT>::T;
     constexpr int FETCH = BT / 32;
+    constexpr uint32_t NONE = ~0u;
     __shared__ __attribute__((aligned(16))) short lds[lds_numbers(BT)];
-    __shared__ int32_t ids[kIds];
+    __shared__ uint32_t xid[kIds], gid[NEAR ? kIds : 1];  // bytes, or row numbers
     const uint32_t u = unit_of_block();
     if (u >= p.units) return;
     const uint32_t tiles = uint32_t(p.kt) * uint32_t(p.nt);
@@ -529,32 +547,45 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_indexed_weights16(We
                                [=](int n) { return slots(n, slice); });
     if (f.cls >= p.plan.classes) return;
     const int lo = p.plan.start(f.cls), n_class = p.plan.count(f.cls);
-    const int begin = lo + f.unit * slice, end = lo + min(n_class, (f.unit + 1) * slice);
+    const int length = slice_length(n_class, slice);
+    const int begin = lo + f.unit * length, end = lo + min(n_class, (f.unit + 1) * length);
     const T *X = static_cast<const T*>(p.x), *G = static_cast<const T*>(p.g);
-    int sum[FETCH], xcol[FETCH], gcol[FETCH];
+    int sum[FETCH];
+    uint32_t xcol[FETCH], gcol[FETCH];  // bytes; the last piece may reach into the rows' padding
 #pragma unroll
     for (int n = 0; n < FETCH; ++n) {
         const SumPlace s = sum_place<BT, 1>(n);
         sum[n] = s.sum;
-        xcol[n] = min(k0 + s.number, p.K - 8);
-        gcol[n] = min(n0 + s.number, p.N - 8);
+        xcol[n] = 2 * uint32_t(min(k0 + s.number, (p.K - 1) & ~7));
+        gcol[n] = 2 * uint32_t(min(n0 + s.number, (p.N - 1) & ~7));
     }
     Acc<BT> acc;
     clear<BT>(acc);
     for (int at = begin; at < end; at += kIds) {
         __syncthreads();
         const int here = min(kIds, end - at);
-        for (int i = threadIdx.x; i < kIds; i += 256) ids[i] = i < here ? p.plan.row(at + i) : -1;
+        for (int i = threadIdx.x; i < kIds; i += 256) {
+            const int row = i < here ? p.plan.row(at + i) : 0;
+            xid[i] = i < here ? (NEAR ? uint32_t(row) * uint32_t(2 * p.ldx) : uint32_t(row)) : NONE;
+            if constexpr (NEAR) gid[i] = uint32_t(row) * uint32_t(2 * p.ldg);
+        }
         __syncthreads();
-        int row[FETCH];
+        uint32_t xrow[FETCH], grow[FETCH];
         auto ahead = [&](int c) {
 #pragma unroll
-            for (int n = 0; n < FETCH; ++n) row[n] = ids[c * kRow + sum[n]];
+            for (int n = 0; n < FETCH; ++n) {
+                xrow[n] = xid[c * kRow + sum[n]];
+                grow[n] = NEAR ? gid[c * kRow + sum[n]] : xrow[n];
+            }
         };
         auto load = [&](int, int n, short* to) {
-            const int m = n < FETCH ? n : n - FETCH;
-            const T* from = n < FETCH ? X + int64_t(row[m]) * p.ldx + xcol[m] : G + int64_t(row[m]) * p.ldg + gcol[m];
-            load_lds(row[m] >= 0 ? static_cast<const void*>(from) : kZeros, to);
+            const bool of_x = n < FETCH;
+            const int m = of_x ? n : n - FETCH;
+            const T* base = of_x ? X : G;
+            const uint32_t col = of_x ? xcol[m] : gcol[m], row = of_x ? xrow[m] : grow[m];
+            const char* from = reinterpret_cast<const char*>(base);
+            from += NEAR ? uint64_t(row + col) : uint64_t(row) * uint64_t(2 * (of_x ? p.ldx : p.ldg)) + col;
+            load_lds(xrow[m] != NONE ? static_cast<const void*>(from) : kZeros, to);
         };
         products<BT, 1, true, true, DT == kBF16>(lds, (here + kRow - 1) / kRow, acc, load, ahead);
     }
@@ -563,8 +594,9 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_indexed_weights16(We
     float* part = p.part + (whole ? 0 : int64_t(f.extra + f.unit) * p.K * p.N);
     store_tile<BT>(lds, acc, p.K - k0, p.N - n0, [&](int i, int j, const float (&v)[8]) {
         const int64_t at = int64_t(k0 + i) * p.N + n0 + j;
-        if (whole) store8(out + at, v);
-        else store8(part + at, v);
+        const int left = p.N - n0 - j;
+        if (whole) store8(out + at, left, v);
+        else store8(part + at, left, v);
     });
 }
 
@@ -620,9 +652,11 @@ int check_shape(const char* what, int64_t rows, int32_t classes, int64_t in, int
     return MNX_OK;
 }
 
-// Whether 16-byte pieces of every row begin at multiples of 16 bytes: the loads of tile16.h.
-inline bool in_pieces(int dtype, const void* p, int64_t ld, int64_t width) {
-    return dtype != kF32 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && width % 8 == 0;
+// Whether rows are whole pieces of 16 bytes at multiples of 16 bytes: the loads of tile16.h.  `padded`: the last piece may
+// hold what lies between the rows.
+inline bool in_pieces(int dtype, const void* p, int64_t ld, int64_t width, bool padded = false) {
+    return dtype != kF32 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 &&
+           (width % 8 == 0 || (padded && ld == ceil_div(width, 8) * 8));
 }
 
 constexpr int64_t kCUs = 256;
@@ -660,24 +694,45 @@ int rows_product(RowsArgs p, mnx_stream_t stream) {
     return MNX_OK;
 }
 
-// Rows of a slice: enough slices for the card where the tiles of one gradient are few, and none that is eight times the
-// average class.
-int64_t slice_rows(int64_t rows, int64_t K, int64_t N, int64_t classes) {
-    const int64_t tiles = ceil_div(K, kBM) * ceil_div(N, kBM), least = tiles <= 2 ? 128 : 256;
-    const int64_t want = std::max<int64_t>(1, 3 * kCUs / tiles);
-    const int64_t most = std::max(least, 8 * rows / classes);
-    return ceil_div(std::min(most, std::max(least, ceil_div(rows, want))), 64) * 64;
+// Microseconds, about, of a gradient's tiles where every class has `rows` rows cut into `cuts`.
+double weights_time(double rows, double classes, double cuts, double tiles, double slots, double chunk, double ends) {
+    return std::max(classes * cuts * tiles / slots, 1.0) * (std::ceil(rows / cuts / 64) * chunk + ends);
+}
+
+// Rows of a slice.  More slices than classes reach more of the card where tiles are few, and cost their partial sums (at
+// 4 TB/s, written and read).  64 rows take about 6 us by way of registers (float32, odd widths), three workgroups a CU, and
+// 1 with tile16.h, two a CU, or 1.6 where one has its CU to itself.  Where classes stay whole, those of up to two or
+// four times the average do.
+int64_t slice_rows(int64_t rows, int64_t K, int64_t N, int64_t classes, int32_t dtype) {
+    const bool registers = dtype == kF32 || ((K % 8 || N % 8) && (K < 384 || N < 384));
+    const double tiles = double(ceil_div(K, kBM) * ceil_div(N, kBM)), average = std::max(double(rows) / classes, 1.0);
+    double best = 1, least = HUGE_VAL;
+    for (double cuts = 1; cuts <= 1024 && (cuts == 1 || average / cuts >= 64); cuts *= 2) {
+        const double sums = cuts > 1 ? 2 * classes * cuts * double(K) * double(N) * 4 / 4e6 : 0;
+        const double time = registers ? weights_time(average, double(classes), cuts, tiles, 3 * kCUs, 6, 8)
+                                      : weights_time(average, double(classes), cuts, tiles, 2 * kCUs,
+                                                     classes * cuts * tiles <= kCUs ? 1.6 : 1, 6);
+        if (time + sums < least) {
+            least = time + sums;
+            best = cuts;
+        }
+    }
+    return std::max<int64_t>(ceil_div(int64_t((best > 1 ? 1 : registers ? 2 : 4) * average / best), 64) * 64, 128);
 }
 
 template <int DT>
 int weights_product(WeightArgs p, mnx_stream_t stream) {
     const int64_t rows = p.plan.rows;
-    const bool pieces = in_pieces(DT, p.x, p.ldx, p.K) && in_pieces(DT, p.g, p.ldg, p.N) && in_pieces(DT, p.gw, p.N, p.N);
+    const bool pieces = in_pieces(DT, p.x, p.ldx, p.K, true) && in_pieces(DT, p.g, p.ldg, p.N, true);
     int tile = kBM;
     const int64_t parts = rows / p.slice + p.plan.classes;
     if (DT != kF32 && pieces) {
-        const int64_t wide = ceil_div(p.K, 256) * ceil_div(p.N, 256) * parts;
-        tile = wide >= 4 * kCUs && p.K > 128 && p.N > 128 ? 256 : 128;
+        // tiles of 256 take 1.2 us a chunk and 15 more, one a CU, of 128 0.94 and 6, two a CU
+        const double average = double(rows) / p.plan.classes, cuts = std::max(1.0, average / p.slice);
+        const auto time = [&](int64_t side, double slots, double chunk, double ends) {
+            return weights_time(average, p.plan.classes, cuts, double(ceil_div(p.K, side) * ceil_div(p.N, side)), slots, chunk, ends);
+        };
+        if (time(256, kCUs, 1.2, 15) < time(128, 2 * kCUs, 0.94, 6)) tile = 256;
     }
     const int cols = !pieces && p.N <= 64 ? 64 : tile;
     p.kt = int32_t(ceil_div(p.K, tile));
@@ -688,7 +743,9 @@ int weights_product(WeightArgs p, mnx_stream_t stream) {
     bool done = false;
     if constexpr (DT != kF32) {
         if (pieces) {
-            const auto kernel = tile == 256 ? k_indexed_weights16<DT, 256> : k_indexed_weights16<DT, 128>;
+            const bool near = std::max(p.ldx, p.ldg) * rows < (int64_t(1) << 31);  // bytes below 2^32
+            const auto kernel = near ? (tile == 256 ? k_indexed_weights16<DT, 256, true> : k_indexed_weights16<DT, 128, true>)
+                                     : (tile == 256 ? k_indexed_weights16<DT, 256, false> : k_indexed_weights16<DT, 128, false>);
             kernel<<<uint32_t(ceil_div(units, 128) * 128), kThreads, 0, stream>>>(p);
             done = true;
         }
@@ -733,10 +790,10 @@ int mnx_indexed_linear(const void* a, int64_t lda, int64_t rows, const int32_t* 
     return go(std::integral_constant<int, kF16>());
 }
 
-size_t mnx_indexed_linear_wgrad_workspace_bytes(int64_t rows, int32_t classes, int64_t in, int64_t out) {
-    if (check_shape("indexed linear", rows, classes, in, out, kF32)) return 0;
+size_t mnx_indexed_linear_wgrad_workspace_bytes(int64_t rows, int32_t classes, int64_t in, int64_t out, int32_t dtype) {
+    if (check_shape("indexed linear", rows, classes, in, out, dtype)) return 0;
     // a class of several slices has at most twice its share of them
-    const int64_t slice = slice_rows(rows, in, out, classes);
+    const int64_t slice = slice_rows(rows, in, out, classes, dtype);
     if (rows <= slice) return 0;
     return size_t(std::min(2 * (rows / slice), rows / slice + classes)) * size_t(in) * size_t(out) * sizeof(float);
 }
@@ -750,12 +807,12 @@ int mnx_indexed_linear_wgrad(const void* x, int64_t ldx, const void* grad, int64
     MNX_REQUIRE(ldx >= in && ldg >= out, "indexed linear: rows of %lld and %lld values %lld and %lld apart",
                 (long long)in, (long long)out, (long long)ldx, (long long)ldg);
     MNX_REQUIRE(class_start && grad_weight && (rows == 0 || (x && grad && order)), "indexed linear: null pointer");
-    const size_t need = mnx_indexed_linear_wgrad_workspace_bytes(rows, classes, in, out);
+    const size_t need = mnx_indexed_linear_wgrad_workspace_bytes(rows, classes, in, out, dtype);
     if (need && (!workspace || workspace_bytes < need))
         return set_error(MNX_ERR_WORKSPACE, "indexed linear: workspace too small");
     WeightArgs p{x, grad, grad_weight, static_cast<float*>(workspace), ldx, ldg,
                  Plan{order, class_start, int32_t(rows), classes}, int32_t(in), int32_t(out), 0, 0,
-                 int32_t(std::min<int64_t>(slice_rows(rows, in, out, classes), INT32_MAX / 2)), 0};
+                 int32_t(std::min<int64_t>(slice_rows(rows, in, out, classes, dtype), INT32_MAX / 2)), 0};
     if (dtype == kF32) return weights_product<kF32>(p, stream);
     if (dtype == kBF16) return weights_product<kBF16>(p, stream);
     return weights_product<kF16>(p, stream);
