@@ -291,16 +291,19 @@ __device__ __forceinline__ f32x16 mfma(const half8& a, const half8& b, const f32
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// Eight consecutive parameters (or results) from p on, of which `count` exist.
 template <typename T>
-__device__ __forceinline__ void apply(T* p, int count, float decay, float rate, const float (&v)[8]) {
-    typedef T Eight __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+struct Eight {
+    typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
+// Eight consecutive parameters (or results) from p on, of which `count` exist; `old` holds what is there if all do.
+template <typename T>
+__device__ __forceinline__ void apply(T* p, int count, const typename Eight<T>::V& old, float decay, float rate,
+                                      const float (&v)[8]) {
     if (count >= 8) {
-        Eight o = {};
-        if (decay != 0) o = *reinterpret_cast<const Eight*>(p);
+        typename Eight<T>::V o;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = T(decay * float(o[e]) - rate * v[e]);
-        *reinterpret_cast<Eight*>(p) = o;
+        for (int e = 0; e < 8; ++e) o[e] = T((decay != 0 ? decay * float(old[e]) : 0.f) - rate * v[e]);
+        *reinterpret_cast<typename Eight<T>::V*>(p) = o;
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -416,19 +419,36 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
     const int j0 = tj * BT + wj * W;
     __syncthreads();
     if (SYM && ti == tj && wi < wj) return;  // above the diagonal
+    // What a strip reads of E is loaded while the one before it leaves, where there are registers for both
+    constexpr bool EARLY = MODE != kGram && (PL == 1 || BT <= 128);
+    half8 old[EARLY ? 2 : 1][MODE == kGram ? 1 : PL][ITEMS];
+    auto load_old = [&](int m, auto& to) {
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+            const int item = it * 64 + lane;
+            const int i = min(ti * BT + wi * W + 32 * m + item / (W / 8), t.rp - 1), j = min(j0 + item % (W / 8) * 8, width - 8);
+#pragma unroll
+            for (int pl = 0; pl < PL; ++pl)
+                to[pl][it] = *reinterpret_cast<const half8*>(E + int64_t(i) * ld + place<PL>(j) + 16 * pl);
+        }
+    };
+    if constexpr (EARLY) load_old(0, old[0]);
     auto strip = [&](auto type, auto at_m) {
-        constexpr int m = decltype(at_m)::value;
-        auto* p = static_cast<decltype(type)*>(t.p) + off;
+        constexpr int m = decltype(at_m)::value, now = EARLY ? m & 1 : 0;
+        using P = decltype(type);
+        P* const p = static_cast<P*>(t.p) + off;
         const int i0 = ti * BT + wi * W + 32 * m;
-        half8 old[MODE == kGram ? 1 : PL][ITEMS];
-        if constexpr (MODE != kGram) {
+        if constexpr (MODE != kGram && !EARLY) load_old(m, old[0]);
+        typename Eight<P>::V par[MODE == kFinal ? ITEMS : 1];
+        if constexpr (MODE == kFinal) {
 #pragma unroll
             for (int it = 0; it < ITEMS; ++it) {
-                const int item = it * 64 + lane, i = i0 + item / (W / 8), j = j0 + item % (W / 8) * 8;
-#pragma unroll
-                for (int pl = 0; pl < PL; ++pl)
-                    if (i < t.rp && j < width)
-                        old[pl][it] = *reinterpret_cast<const half8*>(E + int64_t(i) * ld + place<PL>(j) + 16 * pl);
+                const int item = it * 64 + lane;
+                const int i = i0 + (tall ? item % 4 * 8 : item / (W / 8)), j = j0 + (tall ? item / 4 : item % (W / 8) * 8);
+                const bool whole = tall ? i + 8 <= t.r && j < t.c : i < t.r && j + 8 <= t.c;
+                if (whole && decay != 0)
+                    par[it] = *reinterpret_cast<const typename Eight<P>::V*>(
+                        p + (tall ? int64_t(j) * t.cols + i : int64_t(i) * t.cols + j));
             }
         }
 #pragma unroll
@@ -440,6 +460,7 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
                 for (int e = 0; e < 4; ++e) v[e] = prod * acc[m][n][4 * q + e];
                 *reinterpret_cast<f32x4*>(part + l32 * LD + 32 * n + 8 * q + 4 * half) = v;
             }
+        if constexpr (EARLY && m + 1 < MT) load_old(m + 1, old[(m + 1) & 1]);
         wave_sync();
 #pragma unroll
         for (int it = 0; it < ITEMS; ++it) {
@@ -461,14 +482,14 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
 #pragma unroll
                 for (int pl = PL - 1; pl >= 0; --pl)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] += own * float(old[pl][it][e]);
+                    for (int e = 0; e < 8; ++e) v[e] += own * float(old[now][pl][it][e]);
                 if (columns && block < 0) {
                     *reinterpret_cast<f32x4*>(part + r * LD + jj) = *reinterpret_cast<const f32x4*>(v);
                     *reinterpret_cast<f32x4*>(part + r * LD + jj + 4) = *reinterpret_cast<const f32x4*>(v + 4);
                 }
             }
             if constexpr (MODE == kFinal) {
-                if (!tall && i < t.r) apply(p + int64_t(i) * t.cols + j, t.c - j, decay, rate, v);
+                if (!tall && i < t.r) apply(p + int64_t(i) * t.cols + j, t.c - j, par[it], decay, rate, v);
             } else {
                 put8<PL>(out + int64_t(i) * ld + place<PL>(j), v);
             }
@@ -483,7 +504,7 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = part[(r + e) * LD + jj];
                 if constexpr (MODE == kFinal) {
-                    if (j < t.c) apply(p + int64_t(j) * t.cols + i, t.r - i, decay, rate, v);
+                    if (j < t.c) apply(p + int64_t(j) * t.cols + i, t.r - i, par[it], decay, rate, v);
                 } else {
                     put8<PL>(out + int64_t(j) * ld + place<PL>(i), v);
                 }
