@@ -165,13 +165,13 @@ __device__ __forceinline__ void products(short* lds, int chunks, Acc<BT>& acc, L
             }
     };
     const auto nothing = [](int) {};
-    // half a chunk's loads (I's or J's), shared out over the first 2 MT products
-    auto part_of = [&](int c, int part, int stage) {
+    // a chunk's loads, shared out over the first 2 MT products
+    auto loads_of = [&](int c, int stage) {
         return [=, &fetch](int at) {
-            constexpr int PER = (FETCH + 2 * MT - 1) / (2 * MT);
+            constexpr int PER = (2 * FETCH + 2 * MT - 1) / (2 * MT);
 #pragma unroll
             for (int n = at * PER; n < (at + 1) * PER; ++n)
-                if (n < FETCH) fetch(c, part * FETCH + n, stage);
+                if (n < 2 * FETCH) fetch(c, n, stage);
         };
     };
     auto barrier = [] {
@@ -196,7 +196,7 @@ __device__ __forceinline__ void products(short* lds, int chunks, Acc<BT>& acc, L
 #pragma unroll
         for (int m = 0; m < MT; ++m) read_both(f0, h, m, 0, 0);
     // The last products of chunk c, whose operands are in `now`, and the first operands of the next.  MORE: chunk
-    // c + STAGES of I goes where c was.
+    // c + STAGES goes where c was.
     auto last_of = [&](const Frags& now, Frags& next, auto more) {
         // (STAGES - 2) chunks behind the next may still be out
         if constexpr (decltype(more)::value)
@@ -205,7 +205,7 @@ __device__ __forceinline__ void products(short* lds, int chunks, Acc<BT>& acc, L
         barrier();
         const int free = stage;
         stage = next_of(stage);
-        if constexpr (decltype(more)::value) multiply(now, next, stage, 0, part_of(c + STAGES, 0, free));
+        if constexpr (decltype(more)::value) multiply(now, next, stage, 0, loads_of(c + STAGES, free));
         else multiply(now, next, stage, 0, nothing);  // after the last chunk it reads what nobody uses
         ++c;
     };
@@ -214,9 +214,8 @@ __device__ __forceinline__ void products(short* lds, int chunks, Acc<BT>& acc, L
     multiply(f0, f1, stage, 1, nothing);
 #pragma unroll 1
     while (c + STAGES < chunks) {
-        const int free = stage;
         last_of(f1, f0, more);
-        multiply(f0, f1, stage, 1, part_of(c - 1 + STAGES, 1, free));
+        multiply(f0, f1, stage, 1, nothing);
         ahead(min(c + STAGES, chunks - 1));
     }
 #pragma unroll 1
