@@ -673,8 +673,9 @@ int rows_product(RowsArgs p, mnx_stream_t stream) {
     }
     const int BN = pieces ? tile : p.cols <= 64 ? 64 : 128;
     p.col_tiles = int32_t(ceil_div(p.cols, BN));
-    // three workgroups share a CU: half the rows each where whole ones would leave places free
-    if (!pieces && ceil_div(rows, kBM) * p.col_tiles < 3 * kCUs) tile = kBM / 2;
+    // half the rows each where whole tiles would leave CUs free: 12345 float16 rows of 77 to 333 13.7 us so, 16.7 with 128;
+    // 50k float32 rows of 128, which fill them, 25 against 22.5
+    if (!pieces && ceil_div(rows, kBM) * p.col_tiles < kCUs) tile = kBM / 2;
     const int64_t units = (rows / tile + parts) * p.col_tiles;
     MNX_REQUIRE(units < (int64_t(1) << 23), "indexed linear: too many rows and columns for one call");
     p.units = uint32_t(units);
@@ -699,17 +700,17 @@ double weights_time(double rows, double classes, double cuts, double tiles, doub
     return std::max(classes * cuts * tiles / slots, 1.0) * (std::ceil(rows / cuts / 64) * chunk + ends);
 }
 
-// Rows of a slice.  More slices than classes reach more of the card where tiles are few, and cost their partial sums (at
-// 4 TB/s, written and read).  64 rows take about 6 us by way of registers (float32, odd widths), three workgroups a CU, and
-// 1 with tile16.h, two a CU, or 1.6 where one has its CU to itself.  Where classes stay whole, those of up to two or
-// four times the average do.
+// Rows of a slice.  More slices than classes reach more of the card where tiles are few, and cost their partial sums
+// (8 TB/s, written and read: mostly through the caches).  64 rows take about 8 us by way of registers (float32, odd
+// widths), three workgroups a CU, and 1 with tile16.h, two a CU, or 1.6 where one has its CU to itself.  Where classes
+// stay whole, those of up to two or four times the average do.
 int64_t slice_rows(int64_t rows, int64_t K, int64_t N, int64_t classes, int32_t dtype) {
     const bool registers = dtype == kF32 || ((K % 8 || N % 8) && (K < 384 || N < 384));
     const double tiles = double(ceil_div(K, kBM) * ceil_div(N, kBM)), average = std::max(double(rows) / classes, 1.0);
     double best = 1, least = HUGE_VAL;
     for (double cuts = 1; cuts <= 1024 && (cuts == 1 || average / cuts >= 64); cuts *= 2) {
-        const double sums = cuts > 1 ? 2 * classes * cuts * double(K) * double(N) * 4 / 4e6 : 0;
-        const double time = registers ? weights_time(average, double(classes), cuts, tiles, 3 * kCUs, 6, 8)
+        const double sums = cuts > 1 ? 2 * classes * cuts * double(K) * double(N) * 4 / 8e6 : 0;
+        const double time = registers ? weights_time(average, double(classes), cuts, tiles, 3 * kCUs, 8, 6)
                                       : weights_time(average, double(classes), cuts, tiles, 2 * kCUs,
                                                      classes * cuts * tiles <= kCUs ? 1.6 : 1, 6);
         if (time + sums < least) {
