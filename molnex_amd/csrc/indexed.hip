@@ -293,6 +293,7 @@ struct WeightArgs {
     int64_t ldx, ldg;
     Plan plan;
     int32_t K, N, kt, nt, slice;
+    int32_t places;  // of partial sums
     uint32_t units;
 };
 
@@ -325,6 +326,8 @@ __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
                                [=](int n) { return slots(n, slice); });
     if (f.cls >= p.plan.classes) return;
     const int lo = p.plan.start(f.cls), n_class = p.plan.count(f.cls);
+    const bool whole = n_class <= slice;
+    if (!whole && f.extra + f.unit >= p.places) return;  // not with a plan of class_groups
     const int length = slice_length(n_class, slice);
     const int begin = lo + f.unit * length, end = lo + min(n_class, (f.unit + 1) * length);
     const T *X = static_cast<const T*>(p.x), *G = static_cast<const T*>(p.g);
@@ -384,7 +387,6 @@ __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
             multiply<DT, 2, NT>(a, b, acc);
         }
     }
-    const bool whole = n_class <= slice;
     T* out = static_cast<T*>(p.gw) + int64_t(f.cls) * p.K * p.N;
     float* part = p.part + (whole ? 0 : int64_t(f.extra + f.unit) * p.K * p.N);
 #pragma unroll
@@ -407,7 +409,7 @@ __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
 // 16-bit types whose rows and columns come in pieces of 16 bytes
 // ---------------------------------------------------------------------------
 
-__device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
+__device__ const __attribute__((aligned(16))) uint32_t kZeros[4] = {0, 0, 0, 0};
 
 // The tile's values, 32 rows of a wavefront's part at a time by way of LDS: store(row, column, eight values) for all within
 // rows x cols, numbered in the tile.
@@ -523,6 +525,8 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_indexed_rows16(RowsA
     });
 }
 
+constexpr int kJoins = 2048;  // workgroups that join a class's partial sums, at most
+
 constexpr int kIds = 1536;  // rows whose places are in LDS at a time
 
 // A BT x BT tile of one class's gradient over one slice of its rows: both operands by sums, their rows gathered by the
@@ -547,6 +551,8 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_indexed_weights16(We
                                [=](int n) { return slots(n, slice); });
     if (f.cls >= p.plan.classes) return;
     const int lo = p.plan.start(f.cls), n_class = p.plan.count(f.cls);
+    const bool whole = n_class <= slice;
+    if (!whole && f.extra + f.unit >= p.places) return;  // not with a plan of class_groups
     const int length = slice_length(n_class, slice);
     const int begin = lo + f.unit * length, end = lo + min(n_class, (f.unit + 1) * length);
     const T *X = static_cast<const T*>(p.x), *G = static_cast<const T*>(p.g);
@@ -589,7 +595,6 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_indexed_weights16(We
         };
         products<BT, 1, true, true, DT == kBF16>(lds, (here + kRow - 1) / kRow, acc, load, ahead);
     }
-    const bool whole = n_class <= slice;
     T* out = static_cast<T*>(p.gw) + int64_t(f.cls) * p.K * p.N;
     float* part = p.part + (whole ? 0 : int64_t(f.extra + f.unit) * p.K * p.N);
     store_tile<BT>(lds, acc, p.K - k0, p.N - n0, [&](int i, int j, const float (&v)[8]) {
@@ -600,51 +605,52 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_indexed_weights16(We
     });
 }
 
-// The partial sums of the classes with several slices, added in order: a workgroup takes 128 elements, eight shares of the
-// slices (in order again) of 32 threads each.
+// The partial sums of the classes with several slices, added in order: a workgroup takes 128 elements of such a class at a
+// time, eight shares of the slices (in order again) of 32 threads each.
 template <int DT>
 __global__ void __launch_bounds__(kThreads) k_indexed_join(WeightArgs p) {
     using T = typename Elem<DT>::T;
     __shared__ f32x4 share[8][32];
-    const int cls = blockIdx.y, slice = p.slice;
-    const int n = p.plan.count(cls);
-    if (n <= slice) return;
-    int before = 0;  // slices of the classes before
-    for (int c = int(threadIdx.x & 63); c < cls; c += 64) before += slots(p.plan.count(c), slice);
-    for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d);
-    const int count = slots(n, slice), each = (count + 7) / 8;
+    const int slice = p.slice, classes = p.plan.classes;
     const int64_t size = int64_t(p.K) * p.N;
-    const float* part = p.part + before * size;
-    T* out = static_cast<T*>(p.gw) + cls * size;
-    typedef float Four __attribute__((ext_vector_type(4), aligned(4)));
+    const int units = int(min((size + 127) / 128, int64_t(kJoins)));  // of a class
     const int col = threadIdx.x & 31, group = threadIdx.x >> 5;
-    for (int64_t e0 = int64_t(blockIdx.x) * 128; e0 < size; e0 += int64_t(gridDim.x) * 128) {
-        const int64_t e = e0 + col * 4;
-        f32x4 sum = {0, 0, 0, 0};
-        const int end = min((group + 1) * each, count);
-        if (e + 4 <= size) {
+    typedef float Four __attribute__((ext_vector_type(4), aligned(4)));
+    for (int u = blockIdx.x;; u += gridDim.x) {
+        const Found f = find_class(p.plan, classes, u, [=](int n) { return n > slice ? units : 0; },
+                                   [=](int n) { return slots(n, slice); });
+        if (f.cls >= classes) return;
+        const int count = min(slots(p.plan.count(f.cls), slice), p.places - f.extra), each = (count + 7) / 8;
+        const float* part = p.part + f.extra * size;
+        T* out = static_cast<T*>(p.gw) + f.cls * size;
+        for (int64_t e0 = int64_t(f.unit) * 128; e0 < size; e0 += int64_t(units) * 128) {
+            const int64_t e = e0 + col * 4;
+            f32x4 sum = {0, 0, 0, 0};
+            const int end = min((group + 1) * each, count);
+            if (e + 4 <= size) {
 #pragma unroll 8
-            for (int s = group * each; s < end; ++s) sum += f32x4(*reinterpret_cast<const Four*>(part + s * size + e));
-        } else {
-            for (int s = group * each; s < end; ++s)
-                for (int k = 0; k < 4; ++k)
-                    if (e + k < size) sum[k] += part[s * size + e + k];
-        }
-        share[group][col] = sum;
-        __syncthreads();
-        if (group == 0) {
+                for (int s = group * each; s < end; ++s) sum += f32x4(*reinterpret_cast<const Four*>(part + s * size + e));
+            } else {
+                for (int s = group * each; s < end; ++s)
+                    for (int k = 0; k < 4; ++k)
+                        if (e + k < size) sum[k] += part[s * size + e + k];
+            }
+            share[group][col] = sum;
+            __syncthreads();
+            if (group == 0) {
 #pragma unroll
-            for (int g = 1; g < 8; ++g) sum += share[g][col];
-            for (int k = 0; k < 4; ++k)
-                if (e + k < size) out[e + k] = T(sum[k]);
+                for (int g = 1; g < 8; ++g) sum += share[g][col];
+                for (int k = 0; k < 4; ++k)
+                    if (e + k < size) out[e + k] = T(sum[k]);
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
 int check_shape(const char* what, int64_t rows, int32_t classes, int64_t in, int64_t out, int32_t dtype) {
     MNX_REQUIRE(elem_valid(dtype), "%s: unknown type %d", what, dtype);
-    MNX_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) - 65536, "%s: %lld rows", what, (long long)rows);
+    MNX_REQUIRE(rows >= 0 && rows <= (int64_t(1) << 30), "%s: %lld rows", what, (long long)rows);  // slices count in 32 bits
     MNX_REQUIRE(classes >= 1 && classes <= MNX_CLASS_GROUPS_MAX_CLASSES, "%s: 1 to %d classes, got %d", what,
                 MNX_CLASS_GROUPS_MAX_CLASSES, classes);
     MNX_REQUIRE(in >= 1 && out >= 1 && in <= MNX_INDEXED_MAX_WIDTH && out <= MNX_INDEXED_MAX_WIDTH,
@@ -721,6 +727,11 @@ int64_t slice_rows(int64_t rows, int64_t K, int64_t N, int64_t classes, int32_t 
     return std::max<int64_t>(ceil_div(int64_t((best > 1 ? 1 : registers ? 2 : 4) * average / best), 64) * 64, 128);
 }
 
+// Slices with partial sums, at most: a class of several has at most twice its share of them.
+int64_t places(int64_t rows, int64_t classes, int64_t slice) {
+    return rows <= slice ? 0 : std::min(2 * (rows / slice), rows / slice + classes);
+}
+
 template <int DT>
 int weights_product(WeightArgs p, mnx_stream_t stream) {
     const int64_t rows = p.plan.rows;
@@ -757,8 +768,10 @@ int weights_product(WeightArgs p, mnx_stream_t stream) {
     }
     MNX_CHECK_LAUNCH();
     if (rows > p.slice) {
-        const uint32_t blocks = uint32_t(std::min<int64_t>(ceil_div(int64_t(p.K) * p.N, 128), 2048));
-        k_indexed_join<DT><<<dim3(blocks, uint32_t(p.plan.classes)), kThreads, 0, stream>>>(p);
+        // the host does not know how many classes have several slices: workgroups for all that could, as far as that goes
+        const int64_t several = std::min<int64_t>(rows / p.slice, p.plan.classes);
+        const int64_t blocks = std::min(ceil_div(int64_t(p.K) * p.N, 128), int64_t(kJoins)) * several;
+        k_indexed_join<DT><<<uint32_t(std::min(blocks, int64_t(2 * kJoins))), kThreads, 0, stream>>>(p);
         MNX_CHECK_LAUNCH();
     }
     return MNX_OK;
@@ -793,10 +806,8 @@ int mnx_indexed_linear(const void* a, int64_t lda, int64_t rows, const int32_t* 
 
 size_t mnx_indexed_linear_wgrad_workspace_bytes(int64_t rows, int32_t classes, int64_t in, int64_t out, int32_t dtype) {
     if (check_shape("indexed linear", rows, classes, in, out, dtype)) return 0;
-    // a class of several slices has at most twice its share of them
-    const int64_t slice = slice_rows(rows, in, out, classes, dtype);
-    if (rows <= slice) return 0;
-    return size_t(std::min(2 * (rows / slice), rows / slice + classes)) * size_t(in) * size_t(out) * sizeof(float);
+    return size_t(places(rows, classes, slice_rows(rows, in, out, classes, dtype))) * size_t(in) * size_t(out) *
+           sizeof(float);
 }
 
 int mnx_indexed_linear_wgrad(const void* x, int64_t ldx, const void* grad, int64_t ldg, int64_t rows,
@@ -813,7 +824,8 @@ int mnx_indexed_linear_wgrad(const void* x, int64_t ldx, const void* grad, int64
         return set_error(MNX_ERR_WORKSPACE, "indexed linear: workspace too small");
     WeightArgs p{x, grad, grad_weight, static_cast<float*>(workspace), ldx, ldg,
                  Plan{order, class_start, int32_t(rows), classes}, int32_t(in), int32_t(out), 0, 0,
-                 int32_t(std::min<int64_t>(slice_rows(rows, in, out, classes, dtype), INT32_MAX / 2)), 0};
+                 int32_t(std::min<int64_t>(slice_rows(rows, in, out, classes, dtype), INT32_MAX / 2)), 0, 0};
+    p.places = int32_t(places(rows, classes, p.slice));
     if (dtype == kF32) return weights_product<kF32>(p, stream);
     if (dtype == kBF16) return weights_product<kBF16>(p, stream);
     return weights_product<kF16>(p, stream);

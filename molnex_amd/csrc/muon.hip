@@ -964,9 +964,9 @@ int lay_out(const mnx_muon_args& a, int planes, bool small, char* base, Plan& pl
         t.cast0 = uint32_t(cast);
         const uint64_t b = uint64_t(a.batch[i]);
         stat += b;
+        MNX_REQUIRE(std::max(b, stat) < (1u << 22), "muon: too many matrices in one call");
         if (small) {
             plan.lds = std::max(plan.lds, small_bytes(planes, t.r, t.c));
-            MNX_REQUIRE(stat < (1u << 22), "muon: too many matrices in one call");
             plan.mat.push_back(t);
             continue;
         }
@@ -976,7 +976,7 @@ int lay_out(const mnx_muon_args& a, int planes, bool small, char* base, Plan& pl
         t.a = ws.take<_Float16>(size_t(planes * a.batch[i] * t.rp * t.rp));
         t.b = ws.take<_Float16>(size_t(planes * a.batch[i] * t.rp * t.rp));
         // a grid has fewer than 2^32 threads
-        MNX_REQUIRE(std::max({chunk, cast, stat}) < (1u << 23), "muon: too many matrices in one call");
+        MNX_REQUIRE(std::max(chunk, cast) < (1u << 23), "muon: too many matrices in one call");
         plan.mat.push_back(t);
     }
     if (small) {

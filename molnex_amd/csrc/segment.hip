@@ -277,7 +277,8 @@ constexpr int kSmallCounters = 8192, kSmallNodes = 4096;
 
 // Nodes of a wavefront of the three launches: few, so that many run at once (12345 nodes of 89 classes took 19 us at 832
 // each), unless the counters to be summed by one workgroup were many then.
-inline int seg_nodes(int64_t n, int S) { return n * (S + 1) <= int64_t(256) * 16384 ? 256 : kGroupSeg; }
+constexpr int64_t kShortCounters = 16384;
+inline int seg_nodes(int64_t n, int S) { return n * (S + 1) <= kShortCounters * 256 ? 256 : kGroupSeg; }
 __global__ void __launch_bounds__(kSmallWaves* kWave) k_group_small(const int64_t* __restrict__ cls, int64_t n, int S,
                                                                    int bits, int32_t* __restrict__ order,
                                                                    int32_t* __restrict__ class_start) {
@@ -438,7 +439,10 @@ int mnx_segment_sum_bwd_f32(const float* grad_out, const int64_t* index, const f
 
 size_t mnx_class_groups_workspace_bytes(int64_t num_nodes, int32_t num_classes) {
     if (num_nodes < 0 || num_classes < 0) return 0;
-    return size_t(ceil_div(num_nodes, seg_nodes(num_nodes, num_classes))) * size_t(num_classes + 1) * sizeof(int32_t) + 256;
+    // no less than fewer nodes would take, by the short runs too
+    const int64_t shorts = std::min(num_nodes, kShortCounters * 256 / (num_classes + 1));
+    const int64_t most = std::max(ceil_div(num_nodes, seg_nodes(num_nodes, num_classes)), ceil_div(shorts, int64_t(256)));
+    return size_t(most) * size_t(num_classes + 1) * sizeof(int32_t) + 256;
 }
 
 int mnx_class_groups(const int64_t* classes, int64_t num_nodes, int32_t num_classes, int32_t* order,
