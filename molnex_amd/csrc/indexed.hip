@@ -22,7 +22,9 @@
 #include "elem.h"
 #include "tile16.h"
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace mnx {
 namespace {
@@ -283,6 +285,127 @@ __global__ void __launch_bounds__(kThreads) k_indexed_rows(RowsArgs p) {
                 if (c < p.cols) to[c] = T(acc[m][n][q]);
             }
         }
+}
+
+constexpr int kFewRows = 16, kFewCols = 32, kFewSums = 512;  // rows and columns of a workgroup, sums of a chunk
+
+// float32 y or gx, up to 16 rows of one class against 32 columns, without the matrix cores: where there are few rows, the
+// weights' way from memory is all there is, and a thread has 16 vectors of them on theirs at a time (the tiles above wait
+// for each chunk of 32 sums).  Forward: eight threads share a row of W, 128 rows of it at a time; gx: 32 threads share a row
+// of W^T.  Sums are float32, 32 shares of each, added in order.  64 rows of 8 classes, 1024 to 1024: 18 us (33.5 MB of
+// weights), 43 with tiles; one row 7.1 and 41.
+template <int DIR>
+__global__ void __launch_bounds__(kThreads) k_indexed_few(RowsArgs p) {
+    constexpr int R = kFewRows, KC = kFewSums, LD = KC + 4;
+    __shared__ __attribute__((aligned(16))) float sx[R * LD];
+    __shared__ int32_t rows[R];
+    const int tid = threadIdx.x;
+    const uint32_t per = (p.units + 7) / 8, u = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (u >= p.units) return;
+    const int row_tile = int(u / uint32_t(p.col_tiles)), col0 = int(u % uint32_t(p.col_tiles)) * kFewCols;
+    const int classes = p.plan.classes;
+    const Found f = find_class(p.plan, classes + 1, row_tile, [](int n) { return (n + R - 1) / R; }, [](int) { return 0; });
+    if (f.cls > classes) return;
+    const int first = p.plan.start(f.cls) + f.unit * R;
+    const int count = min(R, p.plan.start(f.cls + 1) - first);  // at least 1
+    if (tid < R) rows[tid] = p.plan.row(first + min(tid, count - 1));
+    const int K = f.cls == classes ? 0 : p.sums;  // zeros for rows out of range
+    const float* W = static_cast<const float*>(p.w) + (f.cls == classes ? 0 : int64_t(f.cls) * p.sums * p.cols);
+    const float* A = static_cast<const float*>(p.a);
+    float* out = static_cast<float*>(p.out);
+    typedef float Vec __attribute__((ext_vector_type(4), aligned(4)));
+    const bool whole = p.sums % 4 == 0 && (DIR == kGradX || p.cols % 4 == 0);
+    // columns 4 * part, sums 4 * turn + 128 i of a chunk
+    const int part = DIR == kForward ? tid & 7 : tid >> 5, turn = DIR == kForward ? tid >> 3 : tid & 31;
+    auto serve = [&](auto some) {
+        constexpr int RR = decltype(some)::value;  // rows, `count` of them in earnest
+        f32x4 acc[RR];
+#pragma unroll
+        for (int r = 0; r < RR; ++r) acc[r] = f32x4{0, 0, 0, 0};
+        constexpr int NX = RR * KC / 4 / kThreads;  // vectors of x a thread
+        // Every vector is there in full or not at all (`whole`: read without a branch, so that all are on their way at
+        // once), or its end is looked at.
+        auto load = [&](auto all, int k0, Vec(&w)[KC / 128][4], Vec(&x)[NX]) {
+            const auto take = [&](const float* row, int at, int end) {
+                if constexpr (decltype(all)::value) {
+                    const Vec v = *reinterpret_cast<const Vec*>(row + (at < end ? at : 0));
+                    return at < end ? v : Vec{0, 0, 0, 0};
+                } else {
+                    Vec v = {0, 0, 0, 0};
+                    if (at + 4 <= end) {
+                        v = *reinterpret_cast<const Vec*>(row + at);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (at + e < end) v[e] = row[at + e];
+                    }
+                    return v;
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < KC / 128; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int k = k0 + 4 * turn + 128 * i + (DIR == kForward ? e : 0);
+                    const int c = col0 + 4 * part + (DIR == kForward ? 0 : e);
+                    if constexpr (DIR == kForward) w[i][e] = take(W + int64_t(min(k, K - 1)) * p.cols, c, k < K ? p.cols : 0);
+                    else w[i][e] = take(W + int64_t(min(c, p.cols - 1)) * p.sums, k, K);
+                }
+#pragma unroll
+            for (int i = 0; i < NX; ++i) {
+                const int it = tid + i * kThreads;
+                x[i] = take(A + int64_t(rows[it / (KC / 4)]) * p.lda, k0 + it % (KC / 4) * 4, K);
+            }
+        };
+        for (int k0 = 0; k0 < K; k0 += KC) {
+            Vec w[KC / 128][4], x[NX];  // forward: of four sums four columns each; gx: of four columns four sums
+            if (whole) load(std::true_type(), k0, w, x);
+            else load(std::false_type(), k0, w, x);
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < NX; ++i) {
+                const int it = tid + i * kThreads;
+                *reinterpret_cast<f32x4*>(sx + it / (KC / 4) * LD + it % (KC / 4) * 4) = f32x4(x[i]);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < KC / 128; ++i) {
+                if (k0 + 128 * i >= K) break;
+#pragma unroll
+                for (int r = 0; r < RR; ++r) {
+                    const f32x4 v = *reinterpret_cast<const f32x4*>(sx + r * LD + 4 * turn + 128 * i);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[r][c] += v[e] * (DIR == kForward ? w[i][e][c] : w[i][c][e]);
+                }
+            }
+        }
+        // 32 shares of every sum: two by two, then by way of LDS
+        constexpr int OTHER = DIR == kForward ? 32 : 16;  // the lane whose turn is 4 or 16 on
+        const int share = DIR == kForward ? (tid >> 6) * 4 + (turn & 3) : turn & 15;
+        float* sums = sx;  // [16][RR][32]
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RR; ++r) {
+            f32x4 v;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = acc[r][c] + __shfl_xor(acc[r][c], OTHER);
+            if (!(tid & OTHER)) *reinterpret_cast<f32x4*>(sums + (share * RR + r) * kFewCols + 4 * part) = v;
+        }
+        __syncthreads();
+        for (int it = tid; it < RR * kFewCols; it += kThreads) {
+            const int r = it / kFewCols, c = it % kFewCols;
+            float sum = 0;
+#pragma unroll
+            for (int s = 0; s < 16; ++s) sum += sums[(s * RR + r) * kFewCols + c];
+            if (r < count && col0 + c < p.cols) out[int64_t(rows[r]) * p.cols + col0 + c] = sum;
+        }
+    };
+    __syncthreads();
+    if (count <= 4) serve(std::integral_constant<int, 4>());
+    else if (count <= 8) serve(std::integral_constant<int, 8>());
+    else serve(std::integral_constant<int, 16>());
 }
 
 struct WeightArgs {
@@ -676,6 +799,18 @@ int rows_product(RowsArgs p, mnx_stream_t stream) {
     if (DT != kF32 && pieces) {
         const int64_t wide = ceil_div(rows, 256) * ceil_div(p.cols, 256), few = ceil_div(rows, 128) * ceil_div(p.cols, 128);
         tile = few < kCUs || p.cols <= 64 ? 64 : wide >= 4 * kCUs && p.cols > 128 ? 256 : 128;
+    }
+    if constexpr (DT == kF32) {
+        // 256 rows of 5 classes, 128 to 128, 6.9 us so (104 workgroups), 9.5 with tiles; 2048 rows 12.8 (536) and 9.7; 256
+        // rows of 8 classes, 1024 to 1024, 33 (800) and 44; 64 to 64 by tiles always (5.2 us, 6.8 so)
+        const int64_t cols = ceil_div(p.cols, kFewCols), units = (rows / kFewRows + parts) * cols;
+        if (p.sums > 64 && units <= std::clamp(p.sums, 512, 1024)) {
+            p.col_tiles = int32_t(cols);
+            p.units = uint32_t(units);
+            k_indexed_few<DIR><<<uint32_t(ceil_div(units, 8) * 8), kThreads, 0, stream>>>(p);
+            MNX_CHECK_LAUNCH();
+            return MNX_OK;
+        }
     }
     const int BN = pieces ? tile : p.cols <= 64 ? 64 : 128;
     p.col_tiles = int32_t(ceil_div(p.cols, BN));

@@ -38,6 +38,35 @@ def test_sizes_by_way_of_registers(rows, count, width, out, dtype):
     check(x, normal(count, width, out, seed=2, dtype=dtype), z, normal(rows, out, seed=3, dtype=dtype))
 
 
+@pytest.mark.parametrize("rows,count,width,out", [
+    (1, 1, 1024, 1024), (1, 3, 65, 4097), (2, 1, 4096, 33), (4, 2, 128, 128), (5, 1, 66, 31), (8, 8, 512, 520),
+    (9, 1, 511, 513), (16, 1, 513, 64), (17, 1, 1025, 30), (64, 8, 1024, 1024), (33, 40, 100, 96), (500, 7, 129, 128)])
+def test_few_rows(rows, count, width, out):
+    """One to 16 float32 rows of a class and a workgroup; chunks of 512 sums that end inside; unaligned rows."""
+    z = classes(rows, count, seed=rows, outside=0.1 if rows > 2 else 0.0)
+    x, w, g = normal(rows, width, seed=1), normal(count, width, out, seed=2), normal(rows, out, seed=3)
+    check(x, w, z, g)
+    base = normal(rows, width + 3, seed=4)
+    check(base[:, 3:], normal(count * width * out + 1, seed=5)[1:].view(count, width, out), z, g[:, :1].expand(rows, out))
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_few_rows_with_bad_values(bad):
+    """In a class of its own, in weights that no row takes and in rows of no class: the others keep their bits."""
+    rows, count, width, out = 40, 5, 130, 70
+    x, w, g = normal(rows, width, seed=1), normal(count, width, out, seed=2), normal(rows, out, seed=3)
+    z = classes(rows, 3, seed=4)
+    z[7], z[9] = 3, -1
+    want = check(x, w, z, g)
+    x[7], x[9], g[9], w[4] = bad, bad, bad, bad
+    x.requires_grad_()
+    y = F.indexed_linear(x, w, z)
+    gx, = torch.autograd.grad(y, x, g)
+    keep = [k for k in range(rows) if k != 7]
+    assert torch.equal(y[keep], want[0][keep]) and not y[7].isfinite().any()
+    assert torch.equal(gx, want[1])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("width,out", [(391, 405), (392, 405), (391, 400), (640, 384)])
 def test_widths_that_are_copied(width, out, dtype):
