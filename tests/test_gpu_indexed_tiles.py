@@ -16,10 +16,13 @@ BITS16 = [torch.bfloat16, torch.float16]
 @pytest.mark.parametrize("rows,count,width,out", [
     (12_000, 3, 72, 200),     # some hundred tiles of 128
     (70_000, 3, 136, 264),    # thousands
+    (500, 300, 16, 24),
     (140_000, 2, 264, 264),   # tiles of 256, ragged in both
     (40_000, 11, 520, 1032),
     (20_000, 4, 1032, 520),
     (9_000, 1, 1024, 1288),
+    (60_000, 64, 512, 512),   # gradients of the weights by tiles of 256
+    (40_000, 16, 1016, 1024),
     (5_000, 600, 64, 72),     # mostly a few rows a class
     (3, 2, 2048, 2056),
 ])
@@ -29,7 +32,7 @@ def test_sizes_of_16_bits(rows, count, width, out, dtype):
           normal(rows, out, seed=3, dtype=dtype))
 
 
-@pytest.mark.parametrize("rows,count,width,out", [(70_000, 3, 40, 70), (30_000, 2, 257, 130), (5_000, 600, 64, 72),
+@pytest.mark.parametrize("rows,count,width,out", [(70_000, 3, 40, 70), (70_000, 3, 70, 40), (30_000, 2, 257, 130), (5_000, 600, 64, 72),
                                                   (3, 2, 1030, 2051), (33_000, 2, 513, 515)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_sizes_by_way_of_registers(rows, count, width, out, dtype):
@@ -86,16 +89,17 @@ def test_widths_that_are_copied(width, out, dtype):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
-@pytest.mark.parametrize("width,out", [(64, 72), (512, 520)])
-def test_rows_farther_apart_than_4_gb(width, out):
+@pytest.mark.parametrize("dtype", BITS16)
+@pytest.mark.parametrize("count,width,out", [(2, 64, 72), (2, 512, 520), (64, 512, 512)])
+def test_rows_farther_apart_than_4_gb(count, width, out, dtype):
     """Column blocks of a tensor of 2.3e9 elements."""
-    rows, count, ld = 70_000, 2, 32_768
-    base = torch.empty(rows, ld, device=DEV, dtype=torch.bfloat16)
-    x, g = base[:, 128:128 + width], base[:, 30_000:30_000 + out]
+    rows, ld = 120_000, 18_944
+    base = torch.empty(rows, ld, device=DEV, dtype=dtype)
+    x, g = base[:, 128:128 + width], base[:, 18_000:18_000 + out]
     x.copy_(normal(rows, width, seed=1))
     g.copy_(normal(rows, out, seed=2))
     z = classes(rows, count, seed=3)
-    w = normal(count, width, out, seed=4, dtype=torch.bfloat16)
+    w = normal(count, width, out, seed=4, dtype=dtype)
     far = check(x, w, z, g)
     close = check(x.contiguous(), w, z, g.contiguous())
     assert all(torch.equal(a, b) for a, b in zip(far, close))

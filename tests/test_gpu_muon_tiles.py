@@ -57,6 +57,15 @@ def test_a_models_lists_are_as_each_alone(dtype):
         assert torch.equal(p[k], alone[0][k]) and torch.equal(m[k], alone[1][k]), shapes[k]
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,rows,cols", [(64, 512, 512), (32, 900, 1024), (3, 2304, 2304)])
+def test_stacks_of_larger_matrices_are_as_each_alone(batch, rows, cols, dtype):
+    x = normal(batch, rows, cols, seed=batch, dtype=dtype)
+    y = F.orthogonalize(x)
+    for k in (0, batch // 2, batch - 1):
+        assert torch.equal(y[k], F.orthogonalize(x[k]))
+
+
 def test_two_streams_at_once():
     """Each call has its own workspace."""
     pairs = [normal(3, 500, 700, seed=k) for k in range(2)]
