@@ -8,16 +8,24 @@
 // (mnx_class_groups): they are read and written in place, with no sorted copy.  The grid is sized for the worst case
 // (a partial tile per class) and surplus workgroups leave at once, so nothing synchronises.
 //
-// A workgroup forms a 128 x BN tile.  Both operands pass through registers into LDS, the next chunk's loads in flight
-// under this one's products; vectors of 16 bytes at the alignment of one element, so any width and row distance will
-// do.  An operand whose sum index is contiguous in memory lies in LDS by rows and is read 16 bytes a lane; one whose
-// rows are the sum index (W in the forward, x and g in the weights' gradient) lies as it is in memory too and is read
-// with the transposing LDS load.  16-bit types go to the matrix cores as they are; float32 is split into three bfloat16
-// parts on the way into LDS, of whose nine products the six above 2^-24 are formed, smallest first, so that products
-// are as exact as float32's whatever the values' range.  Sums are float32.
+// Three forms, by type and alignment.
 //
-// The weights' gradient sums a class's rows in slices of `slice` rows; a class of several leaves partial sums in the
-// workspace, which a second kernel adds in order: the same bits every time.
+// 16-bit rows and columns of whole 16-byte pieces: k_indexed_rows16 and k_indexed_weights16, the loop of tile16.h, whose
+// loads go straight to LDS from addresses that the lanes gather.
+//
+// Others (float32, odd widths): k_indexed_rows and k_indexed_weights.  Both operands pass through registers into LDS, the
+// next chunk's loads in flight under this one's products; vectors of 16 bytes at the alignment of one element, so any width
+// and row distance will do.  An operand whose sum index is contiguous in memory lies in LDS by rows and is read 16 bytes a
+// lane; one whose rows are the sum index (W in the forward, x and g in the weights' gradient) lies as it is in memory too
+// and is read with the transposing LDS load.  float32 is split into three bfloat16 parts on the way into LDS, of whose nine
+// products the six above 2^-24 are formed, smallest first, so that products are as exact as float32's whatever the values'
+// range (an infinity becomes NaN).
+//
+// Few float32 rows: k_indexed_few, on the vector units.
+//
+// Sums are float32, results rounded once to their type.  The weights' gradient sums a class's rows in slices of about
+// `slice` rows; a class of several leaves partial sums in the workspace, which a second kernel adds in order: the same bits
+// every time.
 #include "bf16_split.h"
 #include "elem.h"
 #include "tile16.h"
@@ -30,7 +38,6 @@ namespace mnx {
 namespace {
 
 using namespace tile16;
-
 
 constexpr int kThreads = 256;
 constexpr int kBM = 128;
@@ -184,7 +191,9 @@ struct RowsArgs {
     uint32_t units;
 };
 
-// y or gx: BM rows of one class against BN columns.
+// y or gx: BM rows of one class against BN columns.  50k float32 rows of 1024 to 1024 take 772 us forward (136 TFLOP/s of
+// float32 products, 815 of the matrix cores') and 656 for gx; 50k of 128 to 128 22 us each way, where the 51 MB of rows
+// take 10: splitting into parts and a chunk's wait for the next one bound it.
 template <int DT, int DIR, int BM, int BN>
 __global__ void __launch_bounds__(kThreads) k_indexed_rows(RowsArgs p) {
     using T = typename Kind<DT>::T;
@@ -417,6 +426,7 @@ struct WeightArgs {
     Plan plan;
     int32_t K, N, kt, nt, slice;
     int32_t places;  // of partial sums
+    int32_t joins;   // workgroups' worth of joining them, at most
     uint32_t units;
 };
 
@@ -428,7 +438,8 @@ __device__ __forceinline__ int slice_length(int n, int slice) {
     return ((n + count - 1) / count + 63) & ~63;
 }
 
-// A 128 x BN tile of one class's gradient over one slice of its rows.
+// A 128 x BN tile of one class's gradient over one slice of its rows.  50k float32 rows of 1024 to 1024 1330 us (79
+// TFLOP/s); 50k of 128 to 128 27 us and 6 for the join: both operands' rows are gathered, split and read transposed.
 template <int DT, int BN>
 __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
     using T = typename Kind<DT>::T;
@@ -588,6 +599,8 @@ __device__ __forceinline__ void store8(T* to, int count, const float (&v)[8]) {
 
 // y or gx, BT rows of one class against BT columns: the loop of tile16.h, rows gathered by the lanes' addresses.  What lies
 // past the sum's end is read as zeros from elsewhere; rows and columns past the tile's repeat the last and are not stored.
+// 100k bfloat16 rows of 64 classes, 1024 to 2048: 560 us, 750 TFLOP/s, 476 for gx (rows in order are no faster: the
+// gather is not what bounds it, the tiles' beginnings and ends are); 20k rows of 512 to 512 22 us, where the 46 MB take 9.
 template <int DT, int DIR, int BT>
 __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_indexed_rows16(RowsArgs p) {
     using T = typename Elem<DT>::T;
@@ -654,7 +667,8 @@ constexpr int kIds = 1536;  // rows whose places are in LDS at a time
 
 // A BT x BT tile of one class's gradient over one slice of its rows: both operands by sums, their rows gathered by the
 // lanes' addresses; behind the slice's end, zeros from elsewhere.  NEAR: rows lie within 4 GB, and LDS holds how far, so
-// that an address is one addition (64-bit products of row numbers take as long as the matrix cores here).
+// that an address is one addition (64-bit products of row numbers take as long as the matrix cores here).  The same 100k
+// rows: 483 us, 870 TFLOP/s, the join of partial sums with it.
 template <int DT, int BT, bool NEAR>
 __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_indexed_weights16(WeightArgs p) {
     using T = typename Elem<DT>::T;
@@ -737,16 +751,31 @@ __global__ void __launch_bounds__(kThreads) k_indexed_join(WeightArgs p) {
     const int slice = p.slice, classes = p.plan.classes;
     const int64_t size = int64_t(p.K) * p.N;
     const int units = int(min((size + 127) / 128, int64_t(kJoins)));  // of a class
-    const int col = threadIdx.x & 31, group = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 63, col = threadIdx.x & 31, group = threadIdx.x >> 5;
     typedef float Four __attribute__((ext_vector_type(4), aligned(4)));
-    for (int u = blockIdx.x;; u += gridDim.x) {
-        const Found f = find_class(p.plan, classes, u, [=](int n) { return n > slice ? units : 0; },
-                                   [=](int n) { return slots(n, slice); });
-        if (f.cls >= classes) return;
-        const int count = min(slots(p.plan.count(f.cls), slice), p.places - f.extra), each = (count + 7) / 8;
-        const float* part = p.part + f.extra * size;
-        T* out = static_cast<T*>(p.gw) + f.cls * size;
-        for (int64_t e0 = int64_t(f.unit) * 128; e0 < size; e0 += int64_t(units) * 128) {
+    for (int u = blockIdx.x; u < p.joins; u += gridDim.x) {
+        // the class: of those with several slices, this many come before it
+        int ahead = u / units, cls = -1, before = 0;
+        for (int base = 0; base < classes && cls < 0; base += 64) {
+            const int c = base + lane, n = c < classes ? p.plan.count(c) : 0;
+            uint64_t several = __ballot(n > slice);
+            const int here = __popcll(several);
+            if (ahead < here) {
+                for (; ahead > 0; --ahead) several &= several - 1;
+                cls = __builtin_ctzll(several);
+                before += lane < cls ? slots(n, slice) : 0;
+                cls += base;
+            } else {
+                ahead -= here;
+                before += slots(n, slice);
+            }
+        }
+        if (cls < 0) return;
+        for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d);
+        const int count = min(slots(p.plan.count(cls), slice), p.places - before), each = (count + 7) / 8;
+        const float* part = p.part + before * size;
+        T* out = static_cast<T*>(p.gw) + cls * size;
+        for (int64_t e0 = int64_t(u % units) * 128; e0 < size; e0 += int64_t(units) * 128) {
             const int64_t e = e0 + col * 4;
             f32x4 sum = {0, 0, 0, 0};
             const int end = min((group + 1) * each, count);
@@ -877,7 +906,8 @@ int weights_product(WeightArgs p, mnx_stream_t stream) {
         // tiles of 256 take 1.2 us a chunk and 15 more, one a CU, of 128 0.94 and 6, two a CU
         const double average = double(rows) / p.plan.classes, cuts = std::max(1.0, average / p.slice);
         const auto time = [&](int64_t side, double slots, double chunk, double ends) {
-            return weights_time(average, p.plan.classes, cuts, double(ceil_div(p.K, side) * ceil_div(p.N, side)), slots, chunk, ends);
+            const double tiles = double(ceil_div(p.K, side) * ceil_div(p.N, side));
+            return weights_time(average, p.plan.classes, cuts, tiles, slots, chunk, ends);
         };
         if (time(256, kCUs, 1.2, 15) < time(128, 2 * kCUs, 0.94, 6)) tile = 256;
     }
@@ -903,10 +933,11 @@ int weights_product(WeightArgs p, mnx_stream_t stream) {
     }
     MNX_CHECK_LAUNCH();
     if (rows > p.slice) {
-        // the host does not know how many classes have several slices: workgroups for all that could, as far as that goes
+        // the host does not know how many classes have several slices: workgroups for all that could, 4096 at most (100k rows
+        // of 64 classes, 1024 to 2048: 5 us, 32 with a workgroup for each part of every class)
         const int64_t several = std::min<int64_t>(rows / p.slice, p.plan.classes);
-        const int64_t blocks = std::min(ceil_div(int64_t(p.K) * p.N, 128), int64_t(kJoins)) * several;
-        k_indexed_join<DT><<<uint32_t(std::min(blocks, int64_t(2 * kJoins))), kThreads, 0, stream>>>(p);
+        p.joins = int32_t(std::min(ceil_div(int64_t(p.K) * p.N, 128), int64_t(kJoins)) * several);
+        k_indexed_join<DT><<<uint32_t(std::min(p.joins, 2 * kJoins)), kThreads, 0, stream>>>(p);
         MNX_CHECK_LAUNCH();
     }
     return MNX_OK;
@@ -959,7 +990,7 @@ int mnx_indexed_linear_wgrad(const void* x, int64_t ldx, const void* grad, int64
         return set_error(MNX_ERR_WORKSPACE, "indexed linear: workspace too small");
     WeightArgs p{x, grad, grad_weight, static_cast<float*>(workspace), ldx, ldg,
                  Plan{order, class_start, int32_t(rows), classes}, int32_t(in), int32_t(out), 0, 0,
-                 int32_t(std::min<int64_t>(slice_rows(rows, in, out, classes, dtype), INT32_MAX / 2)), 0, 0};
+                 int32_t(std::min<int64_t>(slice_rows(rows, in, out, classes, dtype), INT32_MAX / 2)), 0, 0, 0};
     p.places = int32_t(places(rows, classes, p.slice));
     if (dtype == kF32) return weights_product<kF32>(p, stream);
     if (dtype == kBF16) return weights_product<kBF16>(p, stream);

