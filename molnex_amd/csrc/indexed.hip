@@ -772,8 +772,10 @@ __global__ void __launch_bounds__(kThreads) k_indexed_join(WeightArgs p) {
         }
         if (cls < 0) return;
         for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d);
-        const int count = min(slots(p.plan.count(cls), slice), p.places - before), each = (count + 7) / 8;
-        const float* part = p.part + before * size;
+        // (a plan of nonsense may say anything)
+        const int count = before >= 0 && before < p.places ? min(slots(p.plan.count(cls), slice), p.places - before) : 0;
+        const int each = (count + 7) / 8;
+        const float* part = p.part + (count ? before * size : 0);
         T* out = static_cast<T*>(p.gw) + cls * size;
         for (int64_t e0 = int64_t(u % units) * 128; e0 < size; e0 += int64_t(units) * 128) {
             const int64_t e = e0 + col * 4;
