@@ -40,7 +40,7 @@ typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 constexpr int kPad = 128;  // sides of the padded matrices are multiples of it
 constexpr int kChunk = 4096;  // elements of a matrix that a workgroup of the momentum kernel takes
 constexpr int kCast = 64;     // side of the cast kernel's tiles
-constexpr int kTableArgs = 24;
+constexpr int kTableArgs = 34;
 
 // One tensor: `batch` matrices of rows x cols.
 struct Mat {
@@ -60,17 +60,17 @@ struct Prefix {
     uint32_t chunk, cast, sym, upd;
 };
 
-struct TableArgs {
+struct __attribute__((aligned(16))) TableArgs {
     Mat mat[kTableArgs];
     int count, first;
 };
 static_assert(sizeof(TableArgs) <= 3840, "4 KB of arguments");
+static_assert(sizeof(Mat) % 16 == 0 && kTableArgs * sizeof(Mat) <= 256 * 16, "16 bytes a thread");
 
 __global__ void __launch_bounds__(256) k_muon_table(TableArgs t, Mat* __restrict__ table) {
-    const int words = t.count * int(sizeof(Mat) / 4);
-    const uint32_t* from = reinterpret_cast<const uint32_t*>(t.mat);
-    uint32_t* to = reinterpret_cast<uint32_t*>(table + t.first);
-    for (int i = threadIdx.x; i < words; i += 256) to[i] = from[i];
+    typedef uint32_t Piece __attribute__((ext_vector_type(4)));
+    if (threadIdx.x < t.count * (sizeof(Mat) / 16))
+        reinterpret_cast<Piece*>(table + t.first)[threadIdx.x] = reinterpret_cast<const Piece*>(t.mat)[threadIdx.x];
 }
 
 // The last tensor whose first unit is not past `unit`; FIELD is a member of Mat.
@@ -555,6 +555,22 @@ struct Steps {
     int count;
 };
 
+// What k_muon_small reads of a tensor.  Up to 32 of them travel in its arguments, and the launch that writes the table is
+// not needed (64 x 64 float32: 30 us, 33 with it).
+struct SmallMat {
+    void* p;
+    const void* g;
+    float* m;
+    int32_t rows, cols, dtype;
+    float adjust;
+    uint32_t stat0;
+};
+constexpr int kSmallArgs = 32;
+struct SmallList {
+    SmallMat mat[kSmallArgs];
+};
+static_assert(sizeof(SmallList) + sizeof(Steps) <= 3840, "4 KB of arguments");
+
 // A whole matrix in one workgroup, from its gradient to its parameters: X and A (then B) stay in LDS, and one launch does
 // what takes 18 with tiles.  One float32 matrix of 128 x 128 takes 63 us so and 71 with tiles, 64 x 64 33 and 71; 300 of
 // 128 x 128 134 and 252.  It is bound by latency: about 11 us a step at 128 x 128 in pairs, products that depend on the
@@ -563,19 +579,26 @@ struct Steps {
 // Eight wavefronts share the blocks of 32 x 32 of A and B on and below the diagonal, and the columns of X, 32 at a time:
 // such columns of a X + B X read nothing of X but these columns, so they are replaced in place.  Pairs sum hi hi and the
 // cross products apart, and add them at the end.
-template <int PL, int LDS>
-__global__ void __launch_bounds__(kSmallThreads) k_muon_small(const Mat* __restrict__ table, int count, Momentum h,
-                                                              double eps, Steps st, Apply ap) {
+template <int PL, int LDS, bool ARGS>
+__global__ void __launch_bounds__(kSmallThreads) k_muon_small(SmallList list, const Mat* __restrict__ table, int count,
+                                                              Momentum h, double eps, Steps st, Apply ap) {
     __shared__ __attribute__((aligned(16))) char lds[LDS];
     __shared__ double part[kSmallThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     constexpr int WAVES = kSmallThreads / 64;
-    const int at = find_mat(table, count, &Mat::stat0, blockIdx.x);
-    const Mat& t = table[at];
+    SmallMat t;
+    if constexpr (ARGS) {
+        const bool mine = lane < count && list.mat[min(lane, kSmallArgs - 1)].stat0 <= blockIdx.x;
+        t = list.mat[__builtin_amdgcn_readfirstlane(__popcll(__ballot(mine)) - 1)];
+    } else {
+        const Mat& m = table[find_mat(table, count, &Mat::stat0, blockIdx.x)];
+        t = {m.p, m.g, m.m, m.rows, m.cols, m.dtype, m.adjust, m.stat0};
+    }
     const int64_t n = int64_t(t.rows) * t.cols, off = int64_t(blockIdx.x - t.stat0) * n;
     const bool tall = t.rows > t.cols;
-    const int rb = (t.r + 31) / 32, cb = (t.c + 31) / 32;  // blocks of 32
+    const int tr = min(t.rows, t.cols), tc = max(t.rows, t.cols);
+    const int rb = (tr + 31) / 32, cb = (tc + 31) / 32;  // blocks of 32
     const int sx = small_row(32 * cb), sa = small_row(32 * rb);
     char* const X = lds;
     char* const A = lds + PL * 32 * rb * sx;
@@ -802,14 +825,14 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(const Mat* __restr
                         for (int e = 0; e < 4; ++e) v[e] += own * float(old[e]);
                     }
                     put4<PL>(to, xplane / 2, v);
-                    if (!last || i >= t.r) continue;
+                    if (!last || i >= tr) continue;
                     by_type(t.dtype, [&](auto type) {
                         auto* p = static_cast<decltype(type)*>(t.p) + off;
                         const int step_ = tall ? t.cols : 1;
                         auto* to_p = p + (tall ? int64_t(j) * t.cols + i : int64_t(i) * t.cols + j);
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (j + e < t.c) {
+                            if (j + e < tc) {
                                 const float o = decay != 0 ? decay * float(to_p[int64_t(e) * step_]) : 0.f;
                                 to_p[int64_t(e) * step_] = decltype(type)(o - rate * v[e]);
                             }
@@ -1103,7 +1126,16 @@ template <int PL>
 int run_small(const mnx_muon_args& a, const Plan& plan, const Scales& sc, mnx_stream_t stream) {
     const int count = int(plan.mat.size());
     if (!count) return MNX_OK;
-    if (int rc = write_table(plan, stream)) return rc;
+    SmallList list{};
+    const bool args = count <= kSmallArgs;
+    if (args) {
+        for (int i = 0; i < count; ++i) {
+            const Mat& m = plan.mat[size_t(i)];
+            list.mat[i] = {m.p, m.g, m.m, m.rows, m.cols, m.dtype, m.adjust, m.stat0};
+        }
+    } else if (int rc = write_table(plan, stream)) {
+        return rc;
+    }
     const Momentum h{float(a.momentum), float(1 - a.momentum), a.nesterov, a.maximize};
     const Apply ap{float(a.lr), a.lr_device, float(a.weight_decay), 1.0f};
     Steps st;
@@ -1116,8 +1148,9 @@ int run_small(const mnx_muon_args& a, const Plan& plan, const Scales& sc, mnx_st
         st.own[k] = f.update.own;
         st.prod[k] = f.update.prod;
     }
-    const auto kernel = plan.lds <= kSmallLds[0] ? k_muon_small<PL, kSmallLds[0]> : k_muon_small<PL, kSmallLds[1]>;
-    kernel<<<plan.stats, kSmallThreads, 0, stream>>>(plan.table, count, h, a.eps, st, ap);
+    const auto kernel = plan.lds <= kSmallLds[0] ? (args ? k_muon_small<PL, kSmallLds[0], true> : k_muon_small<PL, kSmallLds[0], false>)
+                                                 : (args ? k_muon_small<PL, kSmallLds[1], true> : k_muon_small<PL, kSmallLds[1], false>);
+    kernel<<<plan.stats, kSmallThreads, 0, stream>>>(list, plan.table, count, h, a.eps, st, ap);
     MNX_CHECK_LAUNCH();
     return MNX_OK;
 }

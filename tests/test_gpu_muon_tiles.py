@@ -66,6 +66,22 @@ def test_stacks_of_larger_matrices_are_as_each_alone(batch, rows, cols, dtype):
         assert torch.equal(y[k], F.orthogonalize(x[k]))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("count,low,high", [(32, 3, 70), (33, 3, 70), (90, 8, 128), (33, 130, 200), (34, 130, 200), (35, 130, 200)])
+def test_lists_of_any_length_are_as_each_alone(count, low, high, dtype):
+    """Around the numbers of tensors that fit a launch's arguments."""
+    span = high - low + 1
+    shapes = [(low + 37 * k % span, low + 53 * k % span) for k in range(count)]
+    p = [normal(*s, seed=k, dtype=dtype) for k, s in enumerate(shapes)]
+    g = [normal(*s, seed=500 + k, dtype=dtype) for k, s in enumerate(shapes)]
+    m = [normal(*s, seed=900 + k) for k, s in enumerate(shapes)]
+    alone = [[t.clone() for t in ts] for ts in (p, m)]
+    F.muon_step(p, g, m, lr=0.02)
+    for k in range(count):
+        F.muon_step([alone[0][k]], [g[k]], [alone[1][k]], lr=0.02)
+        assert torch.equal(p[k], alone[0][k]) and torch.equal(m[k], alone[1][k]), shapes[k]
+
+
 def test_two_streams_at_once():
     """Each call has its own workspace."""
     pairs = [normal(3, 500, 700, seed=k) for k in range(2)]
