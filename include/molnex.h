@@ -992,9 +992,9 @@ int mnx_muon_step(const mnx_muon_args* args, mnx_stream_t stream);
 /* classes.  weight [classes][in][out] contiguous; a has `rows` rows lda apart. */
 /*   result[i] = a[i] weight[class of i]          (rows x out), or              */
 /*   result[i] = a[i] weight[class of i]^T        (rows x in) if transposed     */
-/* rows of no class become zero.  wgrad: grad_weight[s] = sum over the rows of  */
-/* class s of x[i]^T grad[i], in a fixed order.  All arrays are of type dtype,  */
-/* sums float32.                                                                */
+/* rows of no class become zero; 2^30 rows at most.  wgrad: grad_weight[s] = sum */
+/* over the rows of class s of x[i]^T grad[i], in a fixed order.  All arrays    */
+/* are of type dtype, sums float32.                                            */
 /* ------------------------------------------------------------------------ */
 #define MNX_INDEXED_MAX_WIDTH 65536
 int mnx_indexed_linear(const void* a, int64_t lda, int64_t rows, const int32_t* order, const int32_t* class_start,

@@ -19,8 +19,9 @@ def indexed_linear(x: Tensor, weight: Tensor, index: Tensor | None = None,
 
     ``groups``: ``class_groups(index, classes)``, kept where the same rows are mapped again (layers, steps); ``index`` is
     not read then and may be left out.  float32, bfloat16 or float16, the same for both; products of float32 values are
-    exact to float32, sums are float32.  Differentiable in backward mode to any order; the weights' gradient is summed
-    in a fixed order.  Nothing synchronises.  Under autocast both go to its type, as for a matrix product."""
+    exact to float32, sums are float32.  An infinite float32 value makes what it reaches NaN.  Differentiable in backward
+    mode to any order; the weights' gradient is summed in a fixed order.  Nothing synchronises.  Under autocast both go
+    to its type, as for a matrix product."""
     order, starts = (None, None) if groups is None else groups
     if torch.is_autocast_enabled("cuda"):
         to = torch.get_autocast_dtype("cuda")

@@ -161,3 +161,21 @@ def test_groups_of_every_form(n, count):
     assert torch.equal(order.long(), key.argsort(stable=True))
     sizes = torch.bincount(key, minlength=count + 1)
     assert starts.tolist() == [0, *sizes.cumsum(0).tolist()]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_opcheck(dtype):
+    """Schemas, fakes, autograd registration and the dispatch of compiled code, of the map, its gradients and the updates."""
+    from torch.library import opcheck
+
+    rows, count = 70, 3
+    x, w, g = (normal(*s, seed=k, dtype=dtype).requires_grad_()
+               for k, s in enumerate([(rows, 24), (count, 24, 16), (rows, 16)]))
+    groups = F.class_groups(classes(rows, count, outside=0.1), count)
+    opcheck(torch.ops.molix.indexed_linear.default, (x, w, *groups, False))
+    opcheck(torch.ops.molix.indexed_linear.default, (g, w, *groups, True))
+    opcheck(torch.ops.molix.indexed_linear_wgrad.default, (x, g, *groups))
+    iteration = (5, 3.4445, -4.7750, 2.0315, 1e-7)
+    opcheck(torch.ops.molix.orthogonalize.default, (w.detach(), *iteration))
+    lists = ([w.detach().clone()], [normal(*w.shape, seed=9, dtype=dtype)], [normal(*w.shape, seed=10)])
+    opcheck(torch.ops.molix.muon_step.default, (*lists, 0.02, 0.95, True, 0.1, *iteration, False, False, None))
