@@ -572,7 +572,7 @@ struct SmallList {
 static_assert(sizeof(SmallList) + sizeof(Steps) <= 3840, "4 KB of arguments");
 
 // A whole matrix in one workgroup, from its gradient to its parameters: X and A (then B) stay in LDS, and one launch does
-// what takes 18 with tiles.  One float32 matrix of 128 x 128 takes 63 us so and 71 with tiles, 64 x 64 33 and 71; 300 of
+// what takes 19 with tiles.  One float32 matrix of 128 x 128 takes 63 us so and 71 with tiles, 64 x 64 33 and 71; 300 of
 // 128 x 128 134 and 252.  It is bound by latency: about 11 us a step at 128 x 128 in pairs, products that depend on the
 // last ones with two wavefronts a SIMD.
 //
