@@ -957,11 +957,12 @@ int mnx_adamw8_moments(const void* const* exp_avgs, const void* const* exp_avg_s
 /*   p = (1 - lr weight_decay) p - lr s X                                      */
 /* s = sqrt(max(1, rows / cols)) with adjust 0, 0.2 sqrt(max(rows, cols)) with */
 /* 1.  Parameters and gradients of one tensor share its dtype, momenta are     */
-/* float32.  bfloat16 matrices are iterated in float16 (scaled, float32 sums),  */
-/* others in pairs of it.  momenta NULL: u = grad, and X itself is        */
-/* written to params.  lr_device (or NULL) holds the learning rate in place of  */
-/* lr.  Coefficients under which singular values of [0, 1] grow past 64 are    */
-/* refused.  A matrix with an infinite or NaN entry becomes NaN.               */
+/* float32.  Matrices of every type are iterated in pairs of scaled float16     */
+/* (22 bits) with float32 sums; a result is rounded to its dtype at the end.    */
+/* momenta NULL: u = grad, and X itself is written to params.  lr_device (or    */
+/* NULL) holds the learning rate in place of lr.  Coefficients under which      */
+/* singular values of [0, 1] grow past 64 are refused.  A matrix with an        */
+/* infinite or NaN entry becomes NaN.                                          */
 /* ------------------------------------------------------------------------ */
 #define MNX_MUON_MAX_SIDE 65536
 #define MNX_MUON_MAX_STEPS 100

@@ -5,15 +5,17 @@
 //   steps times:  A = X X^T,  B = b A + c A A,  X = a X + B X
 //   p = (1 - lr wd) p - lr s X,  s by the matrix's shape
 //
-// Numbers: X, A and B lie in the workspace as float16 scaled by powers of two, and are multiplied on the matrix cores
-// with float32 sums.  Their entries are bounded by the iteration itself (|X|_2 <= max p(s) over the singular values
-// that can occur, about 1.2 with the usual coefficients), so one scale a step, chosen on the host from the
-// coefficients, keeps them inside float16's range with 11 bits each, where bfloat16 would keep 8: every rounding in
-// the chain is 8 times finer at the same rate, and together they stay below bfloat16's own.  The first X is u itself
-// times a power of two, exact for bfloat16 inputs; what remains of 1 / |u| (a factor from 1 to 2) goes into the first
-// step's sums.  For float32 and float16 matrices every number is a pair hi + lo of float16, 22 bits, and a product is
-// the three sums lo hi + hi lo + hi hi, in this order (lo lo is below 2^-22): with single ones a float16 result of
-// 333 x 1234 was off by 1.2e-3, six times its rounding.
+// Numbers: whatever the matrices' type, every number of X, A and B is a pair hi + lo of float16 scaled by powers of two, in
+// the workspace or in LDS, multiplied on the matrix cores with float32 sums.  Their entries are bounded by the iteration
+// itself (|X|_2 <= max p(s) over the singular values that can occur, about 1.2 with the usual coefficients), so one scale
+// a step, chosen on the host from the coefficients, keeps them inside float16's range.  A pair's rounding is half a step of
+// lo, 2^-22 at most and 2e-8 in the mean (float32's own: 2^-24 and 2e-8 to 3e-8), and a product is the three sums lo hi +
+// hi lo + hi hi, in this order (lo lo is below 2^-22, 2e-8 in the mean): measured against float64 the results of float32
+// matrices are as far off as those of float32 products (64 x 64: 7e-7 and 9e-7).  The first X is u itself times a power of
+// two; what remains of 1 / |u| (a factor from 1 to 2) goes into the first step's sums.  Results in bfloat16 and float16 are
+// the float32 ones rounded once.  A single float16 a number (11 bits, a third of the products) is not enough for them: a
+// float16 result of 333 x 1234 was off by 1.2e-3 so, six times its rounding, and a bfloat16 one of 8192 x 4096 by 8.5e-4
+// beside a rounding of 1.7e-3.
 //
 // All matrices of a call share each launch; a table in the workspace, written by a first small kernel from its
 // arguments, tells a workgroup its matrix and tile.  Matrices with a side of at most 128 whose X and A fit LDS take one
@@ -47,7 +49,7 @@ struct Mat {
     void* p;         // parameters, or where the orthogonalised matrices go
     const void* g;   // gradients, or the matrices to orthogonalise
     float* m;        // momenta, or null
-    _Float16* x[2];  // [batch][rp][cp], of pairs: 16 hi, then their 16 lo, along a row
+    _Float16* x[2];  // [batch][rp][cp] pairs: 16 hi, then their 16 lo, along a row
     _Float16* a;     // [batch][rp][rp]
     _Float16* b;
     int32_t rows, cols, r, c, rp, cp, batch, dtype;
@@ -95,7 +97,7 @@ struct Stat {
 
 // u, from the gradient and the momentum after this step.
 __device__ __forceinline__ float direction(float g, float m, const Momentum& h) {
-    return h.nesterov ? h.w * g + h.mu * m : m;
+    return h.nesterov ? __builtin_fmaf(h.mu, m, h.w * g) : m;
 }
 
 // Four consecutive elements, at the alignment of one; `left` of them exist, the others are 0 and not stored.
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(256) k_muon_momentum(const Mat* __restrict__ t
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (h.maximize) v[k][e] = -v[k][e];
-                    m[k][e] = m[k][e] * h.mu + h.w * v[k][e];
+                    m[k][e] = __builtin_fmaf(h.mu, m[k][e], h.w * v[k][e]);
                     v[k][e] = direction(v[k][e], m[k][e], h);
                 }
                 store4(t.m + off + i, n - i, m[k]);
@@ -206,13 +208,11 @@ __global__ void __launch_bounds__(256) k_muon_norm(const Mat* __restrict__ table
     if (threadIdx.x == 0) stats[blockIdx.x] = stat_of(sqrt((part[0] + part[1]) + (part[2] + part[3])), eps);
 }
 
-// Where column j of a row lies, of single numbers or of pairs (lo 16 behind hi).
-template <int PL>
-__device__ __forceinline__ int place(int j) {
-    return PL == 1 ? j : ((j & ~15) << 1) | (j & 15);
-}
+constexpr int kPair = 2;  // numbers of a pair
 
-template <int PL>
+// Where column j's hi of a row lies; its lo is 16 behind.
+__device__ __forceinline__ int place(int j) { return ((j & ~15) << 1) | (j & 15); }
+
 __device__ __forceinline__ void put4(_Float16* to, int64_t plane, const float (&v)[4]) {
     half4 hi, lo;
 #pragma unroll
@@ -221,11 +221,10 @@ __device__ __forceinline__ void put4(_Float16* to, int64_t plane, const float (&
         lo[e] = _Float16(v[e] - float(hi[e]));
     }
     *reinterpret_cast<half4*>(to) = hi;
-    if constexpr (PL == 2) *reinterpret_cast<half4*>(to + plane) = lo;
+    *reinterpret_cast<half4*>(to + plane) = lo;
 }
 
 // u in the products' layout, zeros around it: bytes again, transposed by way of LDS where matrices are tall.
-template <int PL>
 __global__ void __launch_bounds__(256) k_muon_cast(const Mat* __restrict__ table, int count, Momentum h,
                                                    const Stat* __restrict__ stats) {
     __shared__ float tile[kCast][kCast + 1];
@@ -241,7 +240,7 @@ __global__ void __launch_bounds__(256) k_muon_cast(const Mat* __restrict__ table
     const bool tall = t.rows > t.cols;
     const int i0 = tall ? c0 : r0, j0 = tall ? r0 : c0;  // of the tensor's own rows and columns
     const int row = threadIdx.x / 16, col = threadIdx.x % 16 * 4;
-    _Float16* x = t.x[0] + PL * (int64_t(which) * t.rp * t.cp + int64_t(r0) * t.cp);
+    _Float16* x = t.x[0] + kPair * (int64_t(which) * t.rp * t.cp + int64_t(r0) * t.cp);
     float v[4][4], m[4][4];
     by_type(t.dtype, [&](auto type) {
         const auto* g = static_cast<const decltype(type)*>(t.g) + off;
@@ -261,7 +260,7 @@ __global__ void __launch_bounds__(256) k_muon_cast(const Mat* __restrict__ table
             v[k][e] = ldexpf(v[k][e], s.exponent);
             if (tall) tile[row + 16 * k][col + e] = v[k][e];
         }
-        if (!tall) put4<PL>(x + PL * int64_t(row + 16 * k) * t.cp + place<PL>(c0 + col), 16, v[k]);
+        if (!tall) put4(x + kPair * int64_t(row + 16 * k) * t.cp + place(c0 + col), 16, v[k]);
     }
     if (!tall) return;
     __syncthreads();
@@ -269,7 +268,7 @@ __global__ void __launch_bounds__(256) k_muon_cast(const Mat* __restrict__ table
     for (int k = 0; k < 4; ++k) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[k][e] = tile[col + e][row + 16 * k];
-        put4<PL>(x + PL * int64_t(row + 16 * k) * t.cp + place<PL>(c0 + col), 16, v[k]);
+        put4(x + kPair * int64_t(row + 16 * k) * t.cp + place(c0 + col), 16, v[k]);
     }
 }
 
@@ -295,6 +294,14 @@ __device__ __forceinline__ f32x16 mfma(const half8& a, const half8& b, const f32
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
+// A parameter after its step from what decay leaves of it, in the same float32 operations whatever its type: without the
+// empty statement a float16 one would be rounded from the unrounded sum.
+__device__ __forceinline__ float stepped(float left, float v, float rate) {
+    float sum = __builtin_fmaf(-rate, v, left);
+    asm("" : "+v"(sum));
+    return sum;
+}
+
 template <typename T>
 struct Eight {
     typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
@@ -306,16 +313,15 @@ __device__ __forceinline__ void apply(T* p, int count, const typename Eight<T>::
     if (count >= 8) {
         typename Eight<T>::V o;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = T((decay != 0 ? decay * float(old[e]) : 0.f) - rate * v[e]);
+        for (int e = 0; e < 8; ++e) o[e] = T(stepped(decay != 0 ? decay * float(old[e]) : 0.f, v[e], rate));
         *reinterpret_cast<typename Eight<T>::V*>(p) = o;
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (e < count) p[e] = T((decay != 0 ? decay * float(p[e]) : 0.f) - rate * v[e]);
+            if (e < count) p[e] = T(stepped(decay != 0 ? decay * float(p[e]) : 0.f, v[e], rate));
     }
 }
 
-template <int PL>
 __device__ __forceinline__ void put8(_Float16* to, const float (&v)[8]) {
     half8 hi, lo;
 #pragma unroll
@@ -324,7 +330,7 @@ __device__ __forceinline__ void put8(_Float16* to, const float (&v)[8]) {
         lo[e] = _Float16(v[e] - float(hi[e]));
     }
     *reinterpret_cast<half8*>(to) = hi;
-    if constexpr (PL == 2) *reinterpret_cast<half8*>(to + 16) = lo;
+    *reinterpret_cast<half8*>(to + 16) = lo;
 }
 
 // A BT x BT tile of one product, the sum over k of I[i][k] J[j][k] (rows of both in memory), or with TR of I[i][k] J[k][j].
@@ -332,11 +338,11 @@ __device__ __forceinline__ void put8(_Float16* to, const float (&v)[8]) {
 // The last tile of a row or column may reach past the padded matrix: it reads what lies behind it in the workspace (rows
 // and columns of the result that are not stored) and stores none of that.
 //
-// Tiles of 256, one a CU, are bound by the matrix cores at the clock they run at then (a bfloat16 matrix of 8192 x 4096: 243
-// us for B X, 1.13 PFLOP/s, 2.3 ms in all); those of 192 (143 us for A) and 128 by their reads of LDS.  Where a call
-// has fewer tiles than CUs, tiles of 64 and the six chunks they have on their way, 6 to 12 us a launch, 15 launches one
-// after the other.
-template <int MODE, int PL, int BT>
+// Tiles of 256, one a CU, are bound by the matrix cores (a matrix of 8192 x 4096: 640 us for the three products of B X, 1.29
+// PFLOP/s, 5.9 ms in all; a large library product of as many numbers reaches 1.41 here); those of 192 (366 us for A) and
+// 128 by their reads of LDS.  Where a call has fewer tiles than CUs, tiles of 64 and the six chunks they have on their way,
+// 6 to 12 us a launch, 15 launches one after the other.
+template <int MODE, int BT>
 __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const Mat* __restrict__ table, int count,
                                                                         uint32_t units, Step s,
                                                                         const Stat* __restrict__ stats, Apply ap) {
@@ -369,32 +375,32 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
     }
     ti = __builtin_amdgcn_readfirstlane(ti);
     tj = __builtin_amdgcn_readfirstlane(tj);
-    const int K = PL * (MODE == kGram ? t.cp : t.rp);  // numbers of I's rows
-    const _Float16* X = t.x[s.from] + PL * int64_t(which) * t.rp * t.cp;
-    const _Float16* A = t.a + PL * int64_t(which) * t.rp * t.rp;
-    const _Float16* B = t.b + PL * int64_t(which) * t.rp * t.rp;
+    const int K = kPair * (MODE == kGram ? t.cp : t.rp);  // numbers of I's rows
+    const _Float16* X = t.x[s.from] + kPair * int64_t(which) * t.rp * t.cp;
+    const _Float16* A = t.a + kPair * int64_t(which) * t.rp * t.rp;
+    const _Float16* B = t.b + kPair * int64_t(which) * t.rp * t.rp;
     const _Float16* I = (MODE == kGram ? X : MODE == kPoly ? A : B) + int64_t(ti) * BT * K;
-    const _Float16* J = TR ? X + PL * tj * BT : (MODE == kGram ? X : A) + int64_t(tj) * BT * K;
+    const _Float16* J = TR ? X + kPair * tj * BT : (MODE == kGram ? X : A) + int64_t(tj) * BT * K;
 
     const RowPlace in = row_place();
     const uint32_t irow = 2 * (uint32_t(in.row) * K + in.number);  // bytes
-    const int64_t istep = int64_t(32) * K, jld = PL * int64_t(t.cp);
+    const int64_t istep = int64_t(32) * K, jld = kPair * int64_t(t.cp);
     uint32_t jrow[TR ? FETCH : 1];
     if constexpr (TR) {
 #pragma unroll
         for (int n = 0; n < FETCH; ++n) {
-            const SumPlace at_n = sum_place<BT, PL>(n);
+            const SumPlace at_n = sum_place<BT, kPair>(n);
             jrow[n] = 2 * (uint32_t(at_n.sum) * uint32_t(jld) + at_n.number);
         }
     }
     auto load = [&](int c, int n, short* to) {
         if (n < FETCH) load_lds(I + c * kRow + n * istep, irow, to);
-        else if constexpr (TR) load_lds(J + c * (kRow / PL) * jld, jrow[n - FETCH], to);
+        else if constexpr (TR) load_lds(J + c * (kRow / kPair) * jld, jrow[n - FETCH], to);
         else load_lds(J + c * kRow + (n - FETCH) * istep, irow, to);
     };
     Acc<BT> acc;
     clear<BT>(acc);
-    products<BT, PL, false, TR, false>(lds, K / kRow, acc, load, [](int) {});  // sides are multiples of 128
+    products<BT, kPair, false, TR, false>(lds, K / kRow, acc, load, [](int) {});  // sides are multiples of 128
 
     // The result, 32 rows of a wavefront's part at a time by way of LDS (its own part of it), from where rows and, for the
     // second place of a symmetric one and for tall matrices' parameters, columns leave 8 values a lane.  acc[m][n][q] is
@@ -409,7 +415,7 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
         }
     }
     const int width = SYM ? t.rp : t.cp;
-    const int64_t ld = PL * int64_t(width);
+    const int64_t ld = kPair * int64_t(width);
     const _Float16* E = MODE == kPoly ? A : X;
     _Float16* out = (MODE == kGram ? t.a : MODE == kPoly ? t.b : t.x[s.from ^ 1]) + int64_t(which) * t.rp * ld;
     float decay = 0, rate = -ap.inv;  // of p and of its change; the result itself has no p
@@ -429,16 +435,16 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
     __syncthreads();
     if (SYM && ti == tj && wi < wj) return;  // above the diagonal
     // What a strip reads of E is loaded while the one before it leaves, where there are registers for both
-    constexpr bool EARLY = MODE != kGram && (PL == 1 || BT <= 128);
-    half8 old[EARLY ? 2 : 1][MODE == kGram ? 1 : PL][ITEMS];
+    constexpr bool EARLY = MODE != kGram && BT <= 128;
+    half8 old[EARLY ? 2 : 1][MODE == kGram ? 1 : kPair][ITEMS];
     auto load_old = [&](int m, auto& to) {
 #pragma unroll
         for (int it = 0; it < ITEMS; ++it) {
             const int item = it * 64 + lane;
             const int i = min(ti * BT + wi * W + 32 * m + item / (W / 8), t.rp - 1), j = min(j0 + item % (W / 8) * 8, width - 8);
 #pragma unroll
-            for (int pl = 0; pl < PL; ++pl)
-                to[pl][it] = *reinterpret_cast<const half8*>(E + int64_t(i) * ld + place<PL>(j) + 16 * pl);
+            for (int pl = 0; pl < kPair; ++pl)
+                to[pl][it] = *reinterpret_cast<const half8*>(E + int64_t(i) * ld + place(j) + 16 * pl);
         }
     };
     if constexpr (EARLY) load_old(0, old[0]);
@@ -489,7 +495,7 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
             }
             if constexpr (MODE != kGram) {
 #pragma unroll
-                for (int pl = PL - 1; pl >= 0; --pl)
+                for (int pl = kPair - 1; pl >= 0; --pl)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] += own * float(old[now][pl][it][e]);
                 if (columns && block < 0) {
@@ -500,7 +506,7 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
             if constexpr (MODE == kFinal) {
                 if (!tall && i < t.r) apply(p + int64_t(i) * t.cols + j, t.c - j, par[it], decay, rate, v);
             } else {
-                put8<PL>(out + int64_t(i) * ld + place<PL>(j), v);
+                put8(out + int64_t(i) * ld + place(j), v);
             }
         }
         wave_sync();
@@ -515,7 +521,7 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
                 if constexpr (MODE == kFinal) {
                     if (j < t.c) apply(p + int64_t(j) * t.cols + i, t.r - i, par[it], decay, rate, v);
                 } else {
-                    put8<PL>(out + int64_t(j) * ld + place<PL>(i), v);
+                    put8(out + int64_t(j) * ld + place(i), v);
                 }
             }
             wave_sync();
@@ -527,9 +533,8 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
         if constexpr (MT > 2) strip(type, std::integral_constant<int, 2>());
         if constexpr (MT > 3) strip(type, std::integral_constant<int, 3>());
     };
-    if constexpr (MODE != kFinal || PL == 1) strips(__bf16{});  // matrices of one plane are bfloat16
-    else if (t.dtype == kF32) strips(float{});
-    else strips(_Float16{});
+    if constexpr (MODE != kFinal) strips(float{});  // the type is of the parameters
+    else by_type(t.dtype, strips);
 }
 
 // ---------------------------------------------------------------------------
@@ -540,9 +545,9 @@ __global__ void __launch_bounds__(256, BT == 128 ? 2 : 1) k_muon_product(const M
 inline __host__ __device__ int small_row(int cols) { return 2 * cols + 48; }
 
 // Bytes that X and A of an r x c matrix take there.
-inline int64_t small_bytes(int planes, int64_t r, int64_t c) {
+inline int64_t small_bytes(int64_t r, int64_t c) {
     const int64_t rq = ceil_div(r, 32) * 32, cq = ceil_div(c, 32) * 32;
-    return planes * rq * (small_row(int(rq)) + 2 * cq + 48);
+    return kPair * rq * (small_row(int(rq)) + 2 * cq + 48);
 }
 
 constexpr int kSmallThreads = 512, kSmallSide = 128;  // the smaller side's limit: four blocks of 32 rows
@@ -577,9 +582,9 @@ static_assert(sizeof(SmallList) + sizeof(Steps) <= 3840, "4 KB of arguments");
 // last ones with two wavefronts a SIMD.
 //
 // Eight wavefronts share the blocks of 32 x 32 of A and B on and below the diagonal, and the columns of X, 32 at a time:
-// such columns of a X + B X read nothing of X but these columns, so they are replaced in place.  Pairs sum hi hi and the
-// cross products apart, and add them at the end.
-template <int PL, int LDS, bool ARGS>
+// such columns of a X + B X read nothing of X but these columns, so they are replaced in place.  Sums of hi hi and of the
+// cross products run apart, and are added at the end.
+template <int LDS, bool ARGS>
 __global__ void __launch_bounds__(kSmallThreads) k_muon_small(SmallList list, const Mat* __restrict__ table, int count,
                                                               Momentum h, double eps, Steps st, Apply ap) {
     __shared__ __attribute__((aligned(16))) char lds[LDS];
@@ -601,7 +606,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(SmallList list, co
     const int rb = (tr + 31) / 32, cb = (tc + 31) / 32;  // blocks of 32
     const int sx = small_row(32 * cb), sa = small_row(32 * rb);
     char* const X = lds;
-    char* const A = lds + PL * 32 * rb * sx;
+    char* const A = lds + kPair * 32 * rb * sx;
     const int xplane = 32 * rb * sx, aplane = 32 * rb * sa;
 
     // momenta and the norm, four vectors a thread on their way at a time
@@ -623,7 +628,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(SmallList list, co
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         if (h.maximize) v[k][e] = -v[k][e];
-                        m[k][e] = m[k][e] * h.mu + h.w * v[k][e];
+                        m[k][e] = __builtin_fmaf(h.mu, m[k][e], h.w * v[k][e]);
                         v[k][e] = direction(v[k][e], m[k][e], h);
                     }
                     store4(t.m + off + i, n - i, m[k]);
@@ -664,13 +669,13 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(SmallList list, co
                     v[k][e] = ldexpf(v[k][e], stat.exponent);
                 }
                 if (!tall) {
-                    put4<PL>(reinterpret_cast<_Float16*>(X + i * sx + 2 * j), xplane / 2, v[k]);
+                    put4(reinterpret_cast<_Float16*>(X + i * sx + 2 * j), xplane / 2, v[k]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         _Float16* to = reinterpret_cast<_Float16*>(X + (j + e) * sx + 2 * i);
                         to[0] = _Float16(v[k][e]);
-                        if constexpr (PL == 2) to[xplane / 2] = _Float16(v[k][e] - float(to[0]));
+                        to[xplane / 2] = _Float16(v[k][e] - float(to[0]));
                     }
                 }
             }
@@ -697,14 +702,12 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(SmallList list, co
 #pragma unroll 4
         for (int k = 0; k < K; k += 16) {
             const half8 i = rows_of(S, stride, bi, k), j = rows_of(S, stride, bj, k);
-            if constexpr (PL == 2) {
-                const half8 il = rows_of(S + plane, stride, bi, k), jl = rows_of(S + plane, stride, bj, k);
-                low = mfma(jl, i, low);
-                high = mfma(j, il, high);
-            }
+            const half8 il = rows_of(S + plane, stride, bi, k), jl = rows_of(S + plane, stride, bj, k);
+            low = mfma(jl, i, low);
+            high = mfma(j, il, high);
             big = mfma(j, i, big);
         }
-        return PL == 2 ? big + (low + high) : big;
+        return big + (low + high);
     };
     // the block's values into A, above the diagonal too; `own` of what is there
     auto into_a = [&](const f32x16& acc, int bi, int bj, float own, float prod) {
@@ -717,20 +720,20 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(SmallList list, co
             for (int e = 0; e < 4; ++e) v[e] = prod * acc[4 * q + e];
             if (own != 0) {
 #pragma unroll
-                for (int pl = PL - 1; pl >= 0; --pl) {
+                for (int pl = kPair - 1; pl >= 0; --pl) {
                     const half4 old = *reinterpret_cast<const half4*>(to + pl * (aplane / 2));
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] += own * float(old[e]);
                 }
             }
-            put4<PL>(to, aplane / 2, v);
+            put4(to, aplane / 2, v);
             if (bi != bj) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     _Float16* mirror = reinterpret_cast<_Float16*>(A + (j + e) * sa + 2 * i);
                     const _Float16 hi = _Float16(v[e]);
                     mirror[0] = hi;
-                    if constexpr (PL == 2) mirror[aplane / 2] = _Float16(v[e] - float(hi));
+                    mirror[aplane / 2] = _Float16(v[e] - float(hi));
                 }
             }
         }
@@ -786,22 +789,18 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(SmallList list, co
 #pragma unroll 2
                 for (int k = 0; k < 32 * rb; k += 16) {
                     const half8 j = cols_of(X, sx, bj, k);
-                    half8 i[2], jl, il[2];
+                    half8 i[2], il[2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) i[r] = rows_of(A, sa, min(r0 + r, rb - 1), k);
-                    if constexpr (PL == 2) {
-                        jl = cols_of(X + xplane, sx, bj, k);
+                    const half8 jl = cols_of(X + xplane, sx, bj, k);
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) il[r] = rows_of(A + aplane, sa, min(r0 + r, rb - 1), k);
+                    for (int r = 0; r < 2; ++r) il[r] = rows_of(A + aplane, sa, min(r0 + r, rb - 1), k);
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) small[r] = mfma(jl, i[r], small[r]);
-                    }
+                    for (int r = 0; r < 2; ++r) small[r] = mfma(jl, i[r], small[r]);
 #pragma unroll
                     for (int r = 0; r < 2; ++r) big[r] = mfma(j, i[r], big[r]);
-                    if constexpr (PL == 2) {
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) small[r] = mfma(j, il[r], small[r]);
-                    }
+                    for (int r = 0; r < 2; ++r) small[r] = mfma(j, il[r], small[r]);
                 }
             }
             if (groups > 1) __syncthreads();
@@ -817,14 +816,14 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(SmallList list, co
                     float v[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        v[e] = prod * (PL == 2 ? big[r][4 * q + e] + small[r][4 * q + e] : big[r][4 * q + e]);
+                        v[e] = prod * (big[r][4 * q + e] + small[r][4 * q + e]);
 #pragma unroll
-                    for (int pl = PL - 1; pl >= 0; --pl) {
+                    for (int pl = kPair - 1; pl >= 0; --pl) {
                         const half4 old = *reinterpret_cast<const half4*>(to + pl * (xplane / 2));
 #pragma unroll
                         for (int e = 0; e < 4; ++e) v[e] += own * float(old[e]);
                     }
-                    put4<PL>(to, xplane / 2, v);
+                    put4(to, xplane / 2, v);
                     if (!last || i >= tr) continue;
                     by_type(t.dtype, [&](auto type) {
                         auto* p = static_cast<decltype(type)*>(t.p) + off;
@@ -833,8 +832,8 @@ __global__ void __launch_bounds__(kSmallThreads) k_muon_small(SmallList list, co
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             if (j + e < tc) {
-                                const float o = decay != 0 ? decay * float(to_p[int64_t(e) * step_]) : 0.f;
-                                to_p[int64_t(e) * step_] = decltype(type)(o - rate * v[e]);
+                                auto& par = to_p[int64_t(e) * step_];
+                                par = decltype(type)(stepped(decay != 0 ? decay * float(par) : 0.f, v[e], rate));
                             }
                     });
                 }
@@ -921,19 +920,19 @@ inline int64_t tiles_of(const Mat& t, bool sym, int tile) {
 
 constexpr int kTile[] = {256, 192, 128, 64}, kTiles = 4;
 
-// The time of a launch, about, in microseconds, by which the size of its tiles is chosen (64 bfloat16 matrices of 512 x 512:
-// 256; one of 4096 x 4096: 192 for A and B, 256 for B X; one of 2048 x 2048: 128; one of 1024 x 1024: 64).  A tile's begin
-// and end take 4, a chunk of 64 numbers 1.95 (256), 1.1 (192) or 0.23 (64), with one tile a CU; tiles of 128 share a CU two
-// by two, 1.05 a chunk, or 0.6 where they are few; pairs half as much again (a third product).  `mats` are sorted: the
-// longest tiles start first, each on the CU that is free first.
-double cost(const std::vector<Mat>& mats, int planes, int kind, int tile) {
+// The time of a launch, about, in microseconds, by which the size of its tiles is chosen (64 matrices of 512 x 512: 256; one
+// of 4096 x 4096: 192 for A and B, 256 for B X; one of 2048 x 2048: 64 and 128; one of 1024 x 1024: 64).  A tile's begin and
+// end take 4, a chunk of 64 single numbers 1.95 (256), 1.1 (192) or 0.23 (64), with one tile a CU; tiles of 128 share a CU
+// two by two, 1.05 a chunk, or 0.6 where they are few; 32 pairs half as much again (a third product; tiles of 64 wait for
+// memory).  `mats` are sorted: the longest tiles start first, each on the CU that is free first.
+double cost(const std::vector<Mat>& mats, int kind, int tile) {
     double tiles = 0;
     for (const Mat& t : mats) tiles += double(tiles_of(t, kind != kUpdate, tile));
     const bool two = tile == 128 && tiles > 256;
     const double slots = two ? 512 : 256;
     double chunk = tile == 256 ? 1.95 : tile == 192 ? 1.1 : two ? 1.05 : tile == 128 ? 0.6 : 0.23;
-    if (planes == 2 && tile != 64) chunk *= 1.5;
-    auto one = [&](const Mat& t) { return 4 + chunk * planes * double(kind == kGram ? t.cp : t.rp) / kRow; };
+    if (tile != 64) chunk *= 1.5;
+    auto one = [&](const Mat& t) { return 4 + chunk * kPair * double(kind == kGram ? t.cp : t.rp) / kRow; };
     if (tiles > 16 * slots) {  // many rounds: their sum
         double all = 0;
         for (const Mat& t : mats) all += one(t) * double(tiles_of(t, kind != kUpdate, tile));
@@ -958,19 +957,16 @@ double cost(const std::vector<Mat>& mats, int planes, int kind, int tile) {
     return std::max_element(free.begin(), free.end())->first;
 }
 
-// float16 numbers that stand for one of X, A and B
-inline int planes_of(int dtype) { return dtype == kBF16 ? 1 : 2; }
-
-// Whether one workgroup takes a whole matrix (at most LDS holds: with pairs 128 x 128 or 64 x 512).  300 bfloat16
-// matrices of 128 x 300 take 153 us so and 230 with tiles, 300 float32 ones of 32 x 256 63 and 298.
-inline bool is_small(int planes, int64_t rows, int64_t cols) {
+// Whether one workgroup takes a whole matrix (at most LDS holds: 128 x 128 or 64 x 512).  300 matrices of 32 x 256 take
+// 63 us so and 298 with tiles.
+inline bool is_small(int64_t rows, int64_t cols) {
     return std::min(rows, cols) <= kSmallSide && std::max(rows, cols) <= 4096 &&
-           small_bytes(planes, std::min(rows, cols), std::max(rows, cols)) <= kSmallLds[1];
+           small_bytes(std::min(rows, cols), std::max(rows, cols)) <= kSmallLds[1];
 }
 
-// Lays the tensors of `planes` planes, those of small matrices or the others, out over the workspace (from `base`, which
-// may be null for its size alone).
-int lay_out(const mnx_muon_args& a, int planes, bool small, char* base, Plan& plan) {
+// Lays the tensors of small matrices, or the others, out over the workspace (from `base`, which may be null for its size
+// alone).
+int lay_out(const mnx_muon_args& a, bool small, char* base, Plan& plan) {
     Workspace ws{base, 0};
     uint64_t chunk = 0, cast = 0, stat = 0;
     std::vector<int64_t> order(size_t(a.count));  // the largest first: their tiles take longest
@@ -980,9 +976,7 @@ int lay_out(const mnx_muon_args& a, int planes, bool small, char* base, Plan& pl
         return x != y ? x > y : std::max(a.rows[i], a.cols[i]) > std::max(a.rows[j], a.cols[j]);
     });
     for (const int64_t i : order) {
-        if (!a.batch[i] || !a.rows[i] || !a.cols[i] || planes_of(a.dtype[i]) != planes ||
-            is_small(planes, a.rows[i], a.cols[i]) != small)
-            continue;
+        if (!a.batch[i] || !a.rows[i] || !a.cols[i] || is_small(a.rows[i], a.cols[i]) != small) continue;
         Mat t{};
         t.rows = int32_t(a.rows[i]);
         t.cols = int32_t(a.cols[i]);
@@ -1004,15 +998,15 @@ int lay_out(const mnx_muon_args& a, int planes, bool small, char* base, Plan& pl
         stat += b;
         MNX_REQUIRE(std::max(b, stat) < (1u << 22), "muon: too many matrices in one call");
         if (small) {
-            plan.lds = std::max(plan.lds, small_bytes(planes, t.r, t.c));
+            plan.lds = std::max(plan.lds, small_bytes(t.r, t.c));
             plan.mat.push_back(t);
             continue;
         }
         chunk += b * uint64_t(ceil_div(int64_t(t.rows) * t.cols, kChunk));
         cast += b * uint64_t(t.rp / kCast) * (t.cp / kCast);
-        for (_Float16*& x : t.x) x = ws.take<_Float16>(size_t(planes * a.batch[i] * t.rp * t.cp));
-        t.a = ws.take<_Float16>(size_t(planes * a.batch[i] * t.rp * t.rp));
-        t.b = ws.take<_Float16>(size_t(planes * a.batch[i] * t.rp * t.rp));
+        for (_Float16*& x : t.x) x = ws.take<_Float16>(size_t(kPair * a.batch[i] * t.rp * t.cp));
+        t.a = ws.take<_Float16>(size_t(kPair * a.batch[i] * t.rp * t.rp));
+        t.b = ws.take<_Float16>(size_t(kPair * a.batch[i] * t.rp * t.rp));
         // a grid has fewer than 2^32 threads
         MNX_REQUIRE(std::max(chunk, cast) < (1u << 23), "muon: too many matrices in one call");
         plan.mat.push_back(t);
@@ -1027,7 +1021,7 @@ int lay_out(const mnx_muon_args& a, int planes, bool small, char* base, Plan& pl
         int best = 0;
         double least = HUGE_VAL;
         for (int k = 0; k < kTiles; ++k) {
-            const double c = cost(plan.mat, planes, kind, kTile[k]);
+            const double c = cost(plan.mat, kind, kTile[k]);
             if (c < least) {
                 least = c;
                 best = k;
@@ -1046,7 +1040,7 @@ int lay_out(const mnx_muon_args& a, int planes, bool small, char* base, Plan& pl
     plan.total = {uint32_t(chunk), uint32_t(cast), uint32_t(sym), uint32_t(upd)};
     // the last tiles read past the last matrix
     int64_t past = 0;
-    for (const Mat& t : plan.mat) past = std::max<int64_t>(past, int64_t(256) * planes * t.cp);
+    for (const Mat& t : plan.mat) past = std::max<int64_t>(past, int64_t(256) * kPair * t.cp);
     if (past) ws.take<_Float16>(size_t(past));
     plan.stats = uint32_t(stat);
     plan.partial = ws.take<double>(size_t(chunk));
@@ -1056,15 +1050,15 @@ int lay_out(const mnx_muon_args& a, int planes, bool small, char* base, Plan& pl
     return MNX_OK;
 }
 
-template <int MODE, int PL>
+template <int MODE>
 int product(const Plan& plan, const Step& s, const Apply& ap, mnx_stream_t stream) {
     constexpr bool SYM = MODE == kGram || MODE == kPoly;
     const int tile = SYM ? plan.sym_tile : plan.upd_tile;
     const uint32_t units = SYM ? plan.total.sym : plan.total.upd, grid = uint32_t(up(units, 128));
     const int count = int(plan.mat.size());
-    const auto kernel = tile == 256 ? k_muon_product<MODE, PL, 256>
-                        : tile == 192 ? k_muon_product<MODE, PL, 192>
-                        : tile == 128 ? k_muon_product<MODE, PL, 128> : k_muon_product<MODE, PL, 64>;
+    const auto kernel = tile == 256 ? k_muon_product<MODE, 256>
+                        : tile == 192 ? k_muon_product<MODE, 192>
+                        : tile == 128 ? k_muon_product<MODE, 128> : k_muon_product<MODE, 64>;
     kernel<<<grid, 256, 0, stream>>>(plan.table, count, units, s, plan.stat, ap);
     MNX_CHECK_LAUNCH();
     return MNX_OK;
@@ -1098,7 +1092,6 @@ Factors factors(const mnx_muon_args& a, const Scales& sc, int k) {
             {float(to * ca / xs), float(to / (B * xs)), from, first}};
 }
 
-template <int PL>
 int run(const mnx_muon_args& a, const Plan& plan, const Scales& sc, mnx_stream_t stream) {
     const int count = int(plan.mat.size());
     if (!count) return MNX_OK;
@@ -1108,21 +1101,20 @@ int run(const mnx_muon_args& a, const Plan& plan, const Scales& sc, mnx_stream_t
     MNX_CHECK_LAUNCH();
     k_muon_norm<<<plan.stats, 256, 0, stream>>>(plan.table, count, plan.partial, a.eps, plan.stat);
     MNX_CHECK_LAUNCH();
-    k_muon_cast<PL><<<plan.total.cast, 256, 0, stream>>>(plan.table, count, h, plan.stat);
+    k_muon_cast<<<plan.total.cast, 256, 0, stream>>>(plan.table, count, h, plan.stat);
     MNX_CHECK_LAUNCH();
     const Apply none{}, ap{float(a.lr), a.lr_device, float(a.weight_decay), 1.0f};
     for (int k = 0; k < a.steps; ++k) {
         const Factors f = factors(a, sc, k);
-        if (int rc = product<kGram, PL>(plan, f.gram, none, stream)) return rc;
-        if (int rc = product<kPoly, PL>(plan, f.poly, none, stream)) return rc;
-        if (int rc = k + 1 == a.steps ? product<kFinal, PL>(plan, f.update, ap, stream)
-                                      : product<kUpdate, PL>(plan, f.update, none, stream))
+        if (int rc = product<kGram>(plan, f.gram, none, stream)) return rc;
+        if (int rc = product<kPoly>(plan, f.poly, none, stream)) return rc;
+        if (int rc = k + 1 == a.steps ? product<kFinal>(plan, f.update, ap, stream)
+                                      : product<kUpdate>(plan, f.update, none, stream))
             return rc;
     }
     return MNX_OK;
 }
 
-template <int PL>
 int run_small(const mnx_muon_args& a, const Plan& plan, const Scales& sc, mnx_stream_t stream) {
     const int count = int(plan.mat.size());
     if (!count) return MNX_OK;
@@ -1148,8 +1140,8 @@ int run_small(const mnx_muon_args& a, const Plan& plan, const Scales& sc, mnx_st
         st.own[k] = f.update.own;
         st.prod[k] = f.update.prod;
     }
-    const auto kernel = plan.lds <= kSmallLds[0] ? (args ? k_muon_small<PL, kSmallLds[0], true> : k_muon_small<PL, kSmallLds[0], false>)
-                                                 : (args ? k_muon_small<PL, kSmallLds[1], true> : k_muon_small<PL, kSmallLds[1], false>);
+    const auto kernel = plan.lds <= kSmallLds[0] ? (args ? k_muon_small<kSmallLds[0], true> : k_muon_small<kSmallLds[0], false>)
+                                                 : (args ? k_muon_small<kSmallLds[1], true> : k_muon_small<kSmallLds[1], false>);
     kernel<<<plan.stats, kSmallThreads, 0, stream>>>(list, plan.table, count, h, a.eps, st, ap);
     MNX_CHECK_LAUNCH();
     return MNX_OK;
@@ -1157,11 +1149,10 @@ int run_small(const mnx_muon_args& a, const Plan& plan, const Scales& sc, mnx_st
 
 // The tensors of a call by how they are multiplied: each kind's launches follow the last one's, in the same workspace.
 struct Form {
-    int planes;
     bool small;
     int (*run)(const mnx_muon_args&, const Plan&, const Scales&, mnx_stream_t);
 };
-constexpr Form kForms[] = {{1, true, run_small<1>}, {2, true, run_small<2>}, {1, false, run<1>}, {2, false, run<2>}};
+constexpr Form kForms[] = {{true, run_small}, {false, run}};
 
 }  // namespace
 }  // namespace mnx
@@ -1176,7 +1167,7 @@ size_t mnx_muon_workspace_bytes(const mnx_muon_args* args) {
     size_t most = 256;
     for (const Form& f : kForms) {
         Plan plan;
-        if (lay_out(*args, f.planes, f.small, nullptr, plan) != MNX_OK) return 0;
+        if (lay_out(*args, f.small, nullptr, plan) != MNX_OK) return 0;
         most = std::max(most, plan.bytes);
     }
     return most;
@@ -1197,13 +1188,13 @@ int mnx_muon_step(const mnx_muon_args* args, mnx_stream_t stream) {
     Scales sc;
     MNX_REQUIRE(bounds(a, sc), "muon: the iteration diverges with coefficients (%g, %g, %g)", a.coefficients[0],
                 a.coefficients[1], a.coefficients[2]);
-    Plan plan[4];
-    for (int k = 0; k < 4; ++k) {
-        if (int rc = lay_out(a, kForms[k].planes, kForms[k].small, static_cast<char*>(a.workspace), plan[k])) return rc;
+    Plan plan[2];
+    for (int k = 0; k < 2; ++k) {
+        if (int rc = lay_out(a, kForms[k].small, static_cast<char*>(a.workspace), plan[k])) return rc;
         if (!plan[k].mat.empty() && (!a.workspace || a.workspace_bytes < plan[k].bytes))
             return set_error(MNX_ERR_WORKSPACE, "muon: workspace too small");
     }
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < 2; ++k)
         if (int rc = kForms[k].run(a, plan[k], sc, stream)) return rc;
     return MNX_OK;
 }

@@ -13,8 +13,8 @@ class Muon(torch.optim.Optimizer):
     two axes is a stack of matrices (``nn.IndexedLinear``'s weight: one a class).  Vectors, embeddings and the like
     belong to another optimizer (``AdamW``).
 
-    Momenta are float32 whatever the parameters' type, and an update is orthogonalised to the accuracy of its
-    parameter's type (``molix.F.orthogonalize``).  ``lr`` may be a tensor on the device: nothing synchronises, and a
+    Momenta are float32 whatever the parameters' type, and so are the updates, orthogonalised as ``molix.F.orthogonalize``
+    does it; only the new parameters are rounded to their type.  ``lr`` may be a tensor on the device: nothing synchronises, and a
     step can be captured in a graph once the momenta exist (after a first step)."""
 
     def __init__(self, params, lr: float | Tensor = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95,
