@@ -1186,11 +1186,15 @@ std::vector<Tensor> tensors(PyObject* o, const char* what, bool& overridden) {
     return got;
 }
 
-OptTensor tensor_or_none(PyObject* o, const char* what, bool& overridden) {
+OptTensor tensor_or_none(PyObject* o, const char* what) {
     if (o == Py_None) return std::nullopt;
     TORCH_CHECK_TYPE(THPVariable_Check(o), what, ": a tensor or None, got ", Py_TYPE(o)->tp_name);
-    overridden |= has_torch_function(o);
     return THPVariable_Unpack(o);
+}
+OptTensor tensor_or_none(PyObject* o, const char* what, bool& overridden) {
+    OptTensor t = tensor_or_none(o, what);
+    if (t.has_value()) overridden |= has_torch_function(o);
+    return t;
 }
 
 double number(PyObject* o) {
@@ -1326,17 +1330,13 @@ PyObject* py_moments(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// (x, weight, index, order, starts): molix.F.indexed_linear of rows; index or the plan (order, starts) may be None
+// (x, weight, index, order, starts): molix.F.indexed_linear of rows; index or the plan (order, starts) may be None.  The
+// caller has handed over calls that __torch_function__ takes.
 PyObject* py_indexed_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == 5, "indexed_linear: 5 arguments, got ", n);
-    if (mode_on()) Py_RETURN_NOTIMPLEMENTED;
-    bool overridden = false;
-    const OptTensor x = tensor_or_none(a[0], "x", overridden), w = tensor_or_none(a[1], "weight", overridden);
-    const OptTensor z = tensor_or_none(a[2], "index", overridden);
-    const OptTensor order = tensor_or_none(a[3], "groups", overridden);
-    const OptTensor starts = tensor_or_none(a[4], "groups", overridden);
-    if (overridden) Py_RETURN_NOTIMPLEMENTED;
+    const OptTensor x = tensor_or_none(a[0], "x"), w = tensor_or_none(a[1], "weight"), z = tensor_or_none(a[2], "index");
+    const OptTensor order = tensor_or_none(a[3], "groups"), starts = tensor_or_none(a[4], "groups");
     TORCH_CHECK_TYPE(given(x) && given(w) && (given(z) || (given(order) && given(starts))),
                      "indexed_linear: x, weight and an index or groups");
     TORCH_CHECK(!transformed(), "molix::indexed_linear does not run inside torch.func's transforms");

@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
-from torch.overrides import handle_torch_function
+from torch.overrides import handle_torch_function, has_torch_function_variadic
 
 from ...kernels import class_groups
 from ...training import DTYPES, _host
@@ -23,6 +23,10 @@ def indexed_linear(x: Tensor, weight: Tensor, index: Tensor | None = None,
     mode to any order; the weights' gradient is summed in a fixed order.  Nothing synchronises.  Under autocast both go
     to its type, as for a matrix product."""
     order, starts = (None, None) if groups is None else groups
+    compiling = torch.compiler.is_compiling()
+    if not compiling and has_torch_function_variadic(x, weight, index, order, starts):
+        return handle_torch_function(indexed_linear, (x, weight, index, order, starts), x, weight, index=index,
+                                     groups=groups)
     if torch.is_autocast_enabled("cuda"):
         to = torch.get_autocast_dtype("cuda")
         x, weight = (t.to(to) if t.is_cuda and t.dtype in DTYPES else t for t in (x, weight))
@@ -33,13 +37,10 @@ def indexed_linear(x: Tensor, weight: Tensor, index: Tensor | None = None,
                              f"{None if index is None else tuple(index.shape)}")
         lead, x = x.shape[:-1], x.reshape(-1, x.shape[-1])
         index = None if index is None else index.reshape(-1)
-    if torch.compiler.is_compiling():
+    if compiling:
         if order is None:
             order, starts = class_groups(index, weight.shape[0])
         y = torch.ops.molix.indexed_linear(x, weight, order, starts, False)
     else:
         y = _host.indexed_linear(x, weight, index, order, starts)
-        if y is NotImplemented:
-            return handle_torch_function(indexed_linear, (x, weight, index, order, starts), x, weight, index=index,
-                                         groups=groups)
     return y if lead is None else y.reshape(*lead, y.shape[-1])

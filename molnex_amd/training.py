@@ -310,6 +310,7 @@ def muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weigh
     if torch.compiler.is_compiling():
         torch.ops.molix.muon_step(params, grads, momenta, *args)
     elif _host.muon(params, grads, momenta, *args) is NotImplemented:
-        _handed_over(muon_step, (params, grads, momenta, (lr_tensor,)), params, grads, momenta, lr=lr,
-                     momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
-                     coefficients=coefficients, eps=eps, adjust=adjust, maximize=maximize)
+        return _handed_over(muon_step, (params, grads, momenta, (lr_tensor,)), params, grads, momenta, lr=lr,
+                            momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                            coefficients=coefficients, eps=eps, adjust=adjust, maximize=maximize)
+    return None
