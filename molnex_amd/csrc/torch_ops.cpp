@@ -1161,6 +1161,19 @@ bool has_torch_function(PyObject* o) {
 
 bool mode_on() { return at::impl::torch_function_mode_enabled(); }
 
+// Whether something looks at the ops of a call with these tensors on their way to the kernels and may repeat or replace
+// them: dispatch modes, tracers, fake and functional tensors.  All of the work has to be registered ops then.
+bool watched(std::initializer_list<const OptTensor*> tensors) {
+    using c10::DispatchKey;
+    constexpr c10::DispatchKeySet watchers({DispatchKey::Python, DispatchKey::PythonTLSSnapshot, DispatchKey::PythonDispatcher,
+                                            DispatchKey::PreDispatch, DispatchKey::Tracer, DispatchKey::Functionalize});
+    const auto tls = c10::impl::tls_local_dispatch_key_set();
+    c10::DispatchKeySet keys = tls.included_;
+    for (const OptTensor* t : tensors)
+        if (given(*t)) keys = keys | (*t)->key_set();
+    return (keys - tls.excluded_).has_any(watchers);
+}
+
 // The tensors of a list; `overridden` where one of them has __torch_function__.
 std::vector<Tensor> tensors(PyObject* o, const char* what, bool& overridden) {
     PyObject* seq = PySequence_Fast(o, "");
@@ -1331,7 +1344,7 @@ PyObject* py_moments(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // (x, weight, index, order, starts): molix.F.indexed_linear of rows; index or the plan (order, starts) may be None.  The
-// caller has handed over calls that __torch_function__ takes.
+// caller has handed over calls that __torch_function__ takes.  None where the grouping has to be an op of its own.
 PyObject* py_indexed_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == 5, "indexed_linear: 5 arguments, got ", n);
@@ -1345,7 +1358,7 @@ PyObject* py_indexed_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Released r;
         if (given(order) && given(starts)) {
             y = indexed_linear_op().call(*x, *w, *order, *starts, false);
-        } else {
+        } else if (!watched({&x, &w, &z})) {
             check_rows("indexed_linear", "x", *x);
             TORCH_CHECK_VALUE(z->dim() == 1 && z->size(0) == x->size(0) && z->device() == x->device() &&
                                   at::isIntegralType(z->scalar_type(), false),
@@ -1358,6 +1371,7 @@ PyObject* py_indexed_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
             y = indexed_linear_op().call(*x, *w, o, s, false);
         }
     }
+    if (!y.defined()) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(y));
     END_HANDLE_TH_ERRORS
 }

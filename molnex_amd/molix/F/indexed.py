@@ -11,6 +11,8 @@ from ...training import DTYPES, _host
 
 __all__ = ["class_groups", "indexed_linear"]
 
+_INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8, torch.uint16, torch.uint32, torch.uint64)
+
 
 def indexed_linear(x: Tensor, weight: Tensor, index: Tensor | None = None,
                    groups: tuple[Tensor, Tensor] | None = None) -> Tensor:
@@ -37,10 +39,13 @@ def indexed_linear(x: Tensor, weight: Tensor, index: Tensor | None = None,
                              f"{None if index is None else tuple(index.shape)}")
         lead, x = x.shape[:-1], x.reshape(-1, x.shape[-1])
         index = None if index is None else index.reshape(-1)
-    if compiling:
+    y = None if compiling else _host.indexed_linear(x, weight, index, order, starts)
+    if y is None:  # every op is seen: by a compiler, a tracer, a dispatch mode or fake tensors
         if order is None:
+            if index is None or index.shape != x.shape[:1] or index.device != x.device or index.dtype not in _INTEGERS:
+                raise ValueError("indexed_linear: index of integers, one a row, on x's device; got "
+                                 + ("None" if index is None else f"{index.dtype} {tuple(index.shape)} on {index.device}")
+                                 + f" for x {tuple(x.shape)}")
             order, starts = class_groups(index, weight.shape[0])
         y = torch.ops.molix.indexed_linear(x, weight, order, starts, False)
-    else:
-        y = _host.indexed_linear(x, weight, index, order, starts)
     return y if lead is None else y.reshape(*lead, y.shape[-1])
