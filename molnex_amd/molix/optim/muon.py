@@ -71,12 +71,27 @@ class Muon(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """Also takes ``torch.optim.Muon``'s state: momenta become contiguous float32 (the base class would give them the
         parameters' type)."""
-        saved = state_dict["state"]
-        super().load_state_dict(state_dict)
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, p in zip(ids, [p for g in self.param_groups for p in g["params"]]):
-            if i in saved and "momentum_buffer" in saved[i]:
-                m = saved[i]["momentum_buffer"]
+        fitted: dict = {}
+
+        def fit(_, final):  # after the other hooks that may replace it
+            saved = [i for g in final["param_groups"] for i in g["params"]]
+            params = [p for g in self.param_groups for p in g["params"]]
+            for i, p in zip(saved, params):
+                m = final["state"].get(i, {}).get("momentum_buffer")
+                if m is None or len(saved) != len(params):
+                    continue
                 if m.shape != p.shape:
                     raise ValueError(f"Muon: saved momentum of shape {tuple(m.shape)}, its parameter {tuple(p.shape)}")
-                self.state[p]["momentum_buffer"] = torch.empty(p.shape, dtype=torch.float32, device=p.device).copy_(m)
+                fitted[p] = torch.empty(p.shape, dtype=torch.float32, device=p.device).copy_(m)
+
+        def put(_):  # before the other hooks that look at the outcome
+            for p, m in fitted.items():
+                self.state[p]["momentum_buffer"] = m
+
+        hooks = [self.register_load_state_dict_pre_hook(fit),
+                 self.register_load_state_dict_post_hook(put, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
