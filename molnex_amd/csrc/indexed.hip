@@ -18,8 +18,10 @@
 // and row distance will do.  An operand whose sum index is contiguous in memory lies in LDS by rows and is read 16 bytes a
 // lane; one whose rows are the sum index (W in the forward, x and g in the weights' gradient) lies as it is in memory too
 // and is read with the transposing LDS load.  float32 is split into three bfloat16 parts on the way into LDS, of whose nine
-// products the six above 2^-24 are formed, smallest first, so that products are as exact as float32's whatever the values'
-// range (an infinity becomes NaN).
+// products the six above 2^-24 are formed, smallest first: a product x w is off by 6 2^-24 |x w| at most, and where a value
+// is so small (below 2^-109) that its parts become subnormal, by 2^-133 (|x| + |w|) more.  Infinities and values that
+// bfloat16's largest does not reach (within 2^-8 of float32's) make sums of parts NaN; sums that come out infinite or NaN
+// are formed again from the values themselves, in the order of the rows, with float32 operations.
 //
 // Few float32 rows: k_indexed_few, on the vector units.
 //
@@ -191,6 +193,16 @@ struct RowsArgs {
     uint32_t units;
 };
 
+// Sum k of `n` products of float32 values, at a(k) and b(k).
+template <typename A, typename B>
+__device__ __forceinline__ float plain_sum(int n, A a, B b) {
+    float sum = 0;
+#pragma unroll 1
+    for (int k = 0; k < n && sum == sum; ++k) sum = __builtin_fmaf(*a(k), *b(k), sum);
+    return sum;
+}
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < HUGE_VALF; }
+
 // y or gx: BM rows of one class against BN columns.  50k float32 rows of 1024 to 1024 take 772 us forward (136 TFLOP/s of
 // float32 products, 815 of the matrix cores') and 656 for gx; 50k of 128 to 128 22 us each way, where the 51 MB of rows
 // take 10: splitting into parts and a chunk's wait for the next one bound it.
@@ -281,6 +293,7 @@ __global__ void __launch_bounds__(kThreads) k_indexed_rows(RowsArgs p) {
     }
     // acc[m][n][q]: row 32 m + 8 (q / 4) + 4 half + q % 4, column 32 n + l32 of the wave's tile
     T* out = static_cast<T*>(p.out);
+    float sound = 0;  // NaN: some sum is not finite
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -292,8 +305,23 @@ __global__ void __launch_bounds__(kThreads) k_indexed_rows(RowsArgs p) {
             for (int n = 0; n < NT; ++n) {
                 const int c = col0 + wn * WN + n * 32 + l32;
                 if (c < p.cols) to[c] = T(acc[m][n][q]);
+                if constexpr (DT == kF32) sound = __builtin_fmaf(acc[m][n][q], 0.f, sound);
             }
         }
+    if constexpr (DT == kF32) {
+        if (sound == 0) return;
+#pragma unroll 1
+        for (int e = 0; e < MT * NT * 16; ++e) {
+            const int q = e / NT % 16, r = wm * WM + e / (NT * 16) * 32 + 8 * (q / 4) + 4 * half + q % 4;
+            const int c = col0 + wn * WN + e % NT * 32 + l32;
+            if (r >= count || c >= p.cols) continue;
+            T* to = out + int64_t(rows[r]) * p.cols + c;
+            const T *a = A + int64_t(rows[r]) * p.lda, *w = W + (DIR == kForward ? c : int64_t(c) * p.sums);
+            if (!finite(*to))
+                *to = plain_sum(K, [=](int k) { return a + k; },
+                                [=](int k) { return w + (DIR == kForward ? int64_t(k) * p.cols : k); });
+        }
+    }
 }
 
 constexpr int kFewRows = 16, kFewCols = 32, kFewSums = 512;  // rows and columns of a workgroup, sums of a chunk
@@ -523,6 +551,7 @@ __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
     }
     T* out = static_cast<T*>(p.gw) + int64_t(f.cls) * p.K * p.N;
     float* part = p.part + (whole ? 0 : int64_t(f.extra + f.unit) * p.K * p.N);
+    float sound = 0;  // NaN: some sum is not finite
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -535,8 +564,23 @@ __global__ void __launch_bounds__(kThreads) k_indexed_weights(WeightArgs p) {
                 if (c >= p.N) continue;
                 if (whole) out[int64_t(k) * p.N + c] = T(acc[m][n][q]);
                 else part[int64_t(k) * p.N + c] = acc[m][n][q];
+                if constexpr (DT == kF32) sound = __builtin_fmaf(acc[m][n][q], 0.f, sound);
             }
         }
+    if constexpr (DT == kF32) {
+        if (sound == 0) return;
+        float* sums = whole ? out : part;
+#pragma unroll 1
+        for (int e = 0; e < 2 * NT * 16; ++e) {
+            const int q = e / NT % 16, k = k0 + wm * 64 + e / (NT * 16) * 32 + 8 * (q / 4) + 4 * half + q % 4;
+            const int c = n0 + wn * WN + e % NT * 32 + l32;
+            if (k >= p.K || c >= p.N) continue;
+            float* to = sums + int64_t(k) * p.N + c;
+            if (!finite(*to))
+                *to = plain_sum(end - begin, [=](int i) { return X + int64_t(p.plan.row(begin + i)) * p.ldx + k; },
+                                [=](int i) { return G + int64_t(p.plan.row(begin + i)) * p.ldg + c; });
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------
