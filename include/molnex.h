@@ -962,7 +962,8 @@ int mnx_adamw8_moments(const void* const* exp_avgs, const void* const* exp_avg_s
 /* momenta NULL: u = grad, and X itself is written to params.  lr_device (or    */
 /* NULL) holds the learning rate in place of lr.  Coefficients under which      */
 /* singular values of [0, 1] grow past 64 are refused.  A matrix with an        */
-/* infinite or NaN entry becomes NaN.                                          */
+/* infinite or NaN entry becomes NaN.  A call takes fewer than 2^22 matrices    */
+/* with a side of up to 128, fewer of larger ones.                             */
 /* ------------------------------------------------------------------------ */
 #define MNX_MUON_MAX_SIDE 65536
 #define MNX_MUON_MAX_STEPS 100

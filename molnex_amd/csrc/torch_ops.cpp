@@ -671,7 +671,7 @@ void adamw8_moments(at::TensorList exp_avgs, at::TensorList exp_avg_sqs, at::Ten
 // Orthogonalised updates
 // ---------------------------------------------------------------------------
 
-// A list's workspace is at most this, or one tensor's: longer lists take several calls.
+// A call's workspace is at most this, or one matrix's: longer lists and larger stacks take several calls.
 constexpr size_t kMuonWorkspace = size_t(4) << 30;
 
 // Whether memory that is written overlaps other memory of the call.  Tensors with gaps may interleave: of those only
@@ -738,37 +738,52 @@ struct MuonLists {
         batch.push_back(from.numel() ? from.numel() / (from.size(-2) * from.size(-1)) : 0);
         dtype.push_back(dtype_of(from.scalar_type()));
     }
+    // One half of the tensors, or of the matrices of a single one.
+    MuonLists half(bool second) const {
+        MuonLists l;
+        const size_t count = p.size(), lo = second ? count / 2 : 0, hi = second ? count : count / 2;
+        if (count == 1) {
+            const int64_t skip = second ? batch[0] / 2 : 0, n = skip * rows[0] * cols[0];
+            const int64_t bytes = n * (dtype[0] == MNX_F32 ? 4 : 2);
+            l = *this;
+            l.p[0] = static_cast<char*>(p[0]) + bytes;
+            l.g[0] = static_cast<const char*>(g[0]) + bytes;
+            if (m[0]) l.m[0] = m[0] + n;
+            l.batch[0] = second ? batch[0] - skip : batch[0] / 2;
+            return l;
+        }
+        const auto take = [&](const auto& from, auto& to) { to.assign(from.begin() + lo, from.begin() + hi); };
+        take(p, l.p);
+        take(g, l.g);
+        take(m, l.m);
+        take(batch, l.batch);
+        take(rows, l.rows);
+        take(cols, l.cols);
+        take(dtype, l.dtype);
+        return l;
+    }
 };
 
 void muon_call(const char* name, const MuonLists& l, bool momenta, mnx_muon_args a, const Tensor& like) {
-    const auto part = [&](size_t at, size_t count) {
-        a.count = int64_t(count);
-        a.params = l.p.data() + at;
-        a.grads = l.g.data() + at;
-        a.momenta = momenta ? l.m.data() + at : nullptr;
-        a.batch = l.batch.data() + at;
-        a.rows = l.rows.data() + at;
-        a.cols = l.cols.data() + at;
-        a.dtype = l.dtype.data() + at;
-        const size_t bytes = mnx_muon_workspace_bytes(&a);
-        TORCH_CHECK(bytes, "molix::", name, ": ", mnx_last_error());
-        return bytes;
-    };
-    const auto step = [&](size_t at, size_t count) {
-        a.workspace_bytes = part(at, count);
-        Tensor ws = at::empty({int64_t(a.workspace_bytes)}, like.options().dtype(at::kByte).requires_grad(false));
-        a.workspace = out(ws);
-        check(mnx_muon_step(&a, stream_of(like)), name);
-    };
     const size_t count = l.p.size();
     if (!count) return;
-    if (part(0, count) <= kMuonWorkspace) return step(0, count);
-    for (size_t at = 0; at < count;) {
-        size_t n = 1, bytes = part(at, 1);
-        while (at + n < count && (bytes += part(at + n, 1)) <= kMuonWorkspace) ++n;
-        step(at, n);
-        at += n;
+    a.count = int64_t(count);
+    a.params = l.p.data();
+    a.grads = l.g.data();
+    a.momenta = momenta ? l.m.data() : nullptr;
+    a.batch = l.batch.data();
+    a.rows = l.rows.data();
+    a.cols = l.cols.data();
+    a.dtype = l.dtype.data();
+    a.workspace_bytes = mnx_muon_workspace_bytes(&a);  // 0: also for more matrices than a call takes
+    if ((!a.workspace_bytes || a.workspace_bytes > kMuonWorkspace) && (count > 1 || l.batch[0] > 1)) {
+        for (bool second : {false, true}) muon_call(name, l.half(second), momenta, a, like);
+        return;
     }
+    TORCH_CHECK(a.workspace_bytes, "molix::", name, ": ", mnx_last_error());
+    Tensor ws = at::empty({int64_t(a.workspace_bytes)}, like.options().dtype(at::kByte).requires_grad(false));
+    a.workspace = out(ws);
+    check(mnx_muon_step(&a, stream_of(like)), name);
 }
 
 mnx_muon_args muon_args(const Iteration& it) {
