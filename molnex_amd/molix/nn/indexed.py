@@ -11,7 +11,8 @@ from ..F.indexed import indexed_linear
 
 class IndexedLinear(nn.Module):
     """``molix.F.indexed_linear`` with its weight (num_classes, in_features, out_features), drawn as ``nn.Linear`` draws
-    (uniform to 1 / sqrt(in_features)).  GPU tensors only."""
+    (uniform to 1 / sqrt(in_features)).  A class's matrix is (in, out), the transpose of ``nn.Linear``'s.  GPU tensors
+    only."""
 
     def __init__(self, num_classes: int, in_features: int, out_features: int, *, device=None, dtype=None):
         super().__init__()

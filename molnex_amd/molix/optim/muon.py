@@ -5,13 +5,19 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from ...training import NEWTON_SCHULZ, muon_step
+from ...training import MUON_MAX_SIDE, NEWTON_SCHULZ, muon_step
 
 
 class Muon(torch.optim.Optimizer):
     """Muon for the matrices of a model on the GPU, with the arguments of ``torch.optim.Muon``.  A parameter of more than
-    two axes is a stack of matrices (``nn.IndexedLinear``'s weight: one a class).  Vectors, embeddings and the like
-    belong to another optimizer (``AdamW``).
+    two axes is a stack of matrices (``nn.IndexedLinear``'s weight: one a class).  Vectors and embeddings belong to another
+    optimizer (``AdamW``), and so do weights that hold several matrices in one row, (1, n) or (classes, n), as those of
+    the equivariant ``Linear`` and of ``ElementUpdate`` do: such a row is one matrix here, and is only normalised.
+    Sides are at most 65536.
+
+    ``adjust_lr_fn`` takes a weight's rows for its outputs, as ``torch.nn.Linear`` has them: "original" raises the rate by
+    sqrt(rows / columns) where there are more rows.  ``nn.IndexedLinear``'s matrices are (in, out), so it raises that of
+    layers that narrow; "match_rms_adamw" is the same for both.
 
     Momenta are float32 whatever the parameters' type, and so are the updates, orthogonalised as ``molix.F.orthogonalize``
     does it; only the new parameters are rounded to their type.  ``lr`` may be a tensor on the device: nothing synchronises, and a
@@ -36,9 +42,10 @@ class Muon(torch.optim.Optimizer):
             raise ValueError(f"Muon: adjust_lr_fn {group['adjust_lr_fn']!r}, one of original, match_rms_adamw")
         super().add_param_group(param_group)
         for p in self.param_groups[-1]["params"]:
-            if p.dim() < 2:
+            if p.dim() < 2 or max(p.shape[-2:]) > MUON_MAX_SIDE:
                 self.param_groups.pop()
-                raise ValueError(f"Muon: parameters are matrices or stacks of them, got {tuple(p.shape)}")
+                raise ValueError(f"Muon: parameters are matrices or stacks of them with sides of at most {MUON_MAX_SIDE}, "
+                                 f"got {tuple(p.shape)}")
 
     def __setstate__(self, state) -> None:
         super().__setstate__(state)

@@ -266,6 +266,7 @@ def adamw8_relayout(exp_avg: Tensor, exp_avg_sq: Tensor, bases: Tensor, like: Te
 
 
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+MUON_MAX_SIDE = 1 << 16
 
 
 def orthogonalize(x: Tensor, *, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7) -> Tensor:
