@@ -996,7 +996,10 @@ int mnx_muon_step(const mnx_muon_args* args, mnx_stream_t stream);
 /*   result[i] = a[i] weight[class of i]^T        (rows x in) if transposed     */
 /* rows of no class become zero; 2^30 rows at most.  wgrad: grad_weight[s] = sum */
 /* over the rows of class s of x[i]^T grad[i], in a fixed order.  All arrays    */
-/* are of type dtype, sums float32.                                            */
+/* are of type dtype, sums float32.  wgrad reads 16-bit rows that begin at      */
+/* multiples of 16 bytes, ldx (ldg) apart, with ldx the width rounded up to a   */
+/* multiple of 8, up to that distance: behind the last row, too, these bytes    */
+/* have to be the caller's.  What they hold does not matter.                    */
 /* ------------------------------------------------------------------------ */
 #define MNX_INDEXED_MAX_WIDTH 65536
 int mnx_indexed_linear(const void* a, int64_t lda, int64_t rows, const int32_t* order, const int32_t* class_start,

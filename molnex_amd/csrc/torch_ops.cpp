@@ -945,14 +945,26 @@ Tensor indexed_linear(const Tensor& x, const Tensor& weight, const Tensor& order
     return y;
 }
 
-// Rows of whole pieces of 16 bytes (what pads them is of no interest), for the products by the tile.
+// 16-bit rows `ld` apart, the width rounded up to whole pieces of 16 bytes, are read with what pads them.
+int64_t pieces_of(const Tensor& t) { return (t.size(1) + 7) / 8 * 8; }
+bool padding_exists(const Tensor& t) {
+    return size_t(t.storage_offset() + t.size(0) * t.stride(0)) * t.element_size() <= t.storage().nbytes();
+}
+
+// Rows of whole pieces (what pads them is of no interest), for the products by the tile.
 Tensor in_pieces(const Tensor& t) {
-    const int64_t width = t.size(1), ld = (width + 7) / 8 * 8;
+    const int64_t width = t.size(1), ld = pieces_of(t);
     if (t.stride(1) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 &&
-        (t.stride(0) == ld || (width % 8 == 0 && t.stride(0) % 8 == 0)))
+        ((t.stride(0) == ld && padding_exists(t)) || (width % 8 == 0 && t.stride(0) % 8 == 0)))
         return t;
     Tensor padded = at::empty({t.size(0), ld}, t.options().requires_grad(false)).narrow(1, 0, width);
     return padded.copy_(t);
+}
+// Rows as they are, unless those that are read with their padding end before it.
+Tensor in_place(const Tensor& t) {
+    const bool ends = t.scalar_type() != at::kFloat && t.size(0) && t.size(1) % 8 && t.stride(0) == pieces_of(t) &&
+                      !padding_exists(t);
+    return ends ? t.contiguous() : t;
 }
 
 Tensor indexed_linear_wgrad(const Tensor& x, const Tensor& grad, const Tensor& order, const Tensor& starts) {
@@ -967,7 +979,7 @@ Tensor indexed_linear_wgrad(const Tensor& x, const Tensor& grad, const Tensor& o
     const int64_t in = x.size(1), cols = grad.size(1);
     // 50001 rows of 1001 and 999 bfloat16 values take 566 us as they are; rows of 250 are not worth the copies
     const bool copies = x.scalar_type() != at::kFloat && in >= 384 && cols >= 384 && n.rows > 0;
-    const Rows a(copies ? in_pieces(x.detach()) : x, in), g(copies ? in_pieces(grad.detach()) : grad, cols);
+    const Rows a(copies ? in_pieces(x.detach()) : in_place(x), in), g(copies ? in_pieces(grad.detach()) : in_place(grad), cols);
     Tensor gw = at::empty({n.classes, in, cols}, x.options().requires_grad(false)), ws;
     const size_t bytes = mnx_indexed_linear_wgrad_workspace_bytes(n.rows, n.classes, in, cols, dtype_of(x.scalar_type()));
     if (bytes) ws = at::empty({int64_t(bytes)}, x.options().dtype(at::kByte).requires_grad(false));
