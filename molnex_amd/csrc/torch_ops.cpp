@@ -1131,8 +1131,6 @@ TORCH_LIBRARY_IMPL(molix, CUDA, m) {
 TORCH_LIBRARY_IMPL(molix, CPU, m) {  // these say that they run on the GPU only
     m.impl("indexed_linear", indexed_linear);
     m.impl("indexed_linear_wgrad", indexed_linear_wgrad);
-    m.impl("indexed_linear", indexed_linear);
-    m.impl("indexed_linear_wgrad", indexed_linear_wgrad);
     m.impl("orthogonalize", orthogonalize);
     m.impl("muon_step", muon_step);
 }
