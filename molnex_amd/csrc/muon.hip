@@ -10,12 +10,12 @@
 // itself (|X|_2 <= max p(s) over the singular values that can occur, about 1.2 with the usual coefficients), so one scale
 // a step, chosen on the host from the coefficients, keeps them inside float16's range.  A pair's rounding is half a step of
 // lo, 2^-22 at most and 2e-8 in the mean (float32's own: 2^-24 and 2e-8 to 3e-8), and a product is the three sums lo hi +
-// hi lo + hi hi, in this order (lo lo is below 2^-22, 2e-8 in the mean): measured against float64 the results of float32
-// matrices are as far off as those of float32 products (64 x 64: 7e-7 and 9e-7).  The first X is u itself times a power of
-// two; what remains of 1 / |u| (a factor from 1 to 2) goes into the first step's sums.  Results in bfloat16 and float16 are
-// the float32 ones rounded once.  A single float16 a number (11 bits, a third of the products) is not enough for them: a
-// float16 result of 333 x 1234 was off by 1.2e-3 so, six times its rounding, and a bfloat16 one of 8192 x 4096 by 8.5e-4
-// beside a rounding of 1.7e-3.
+// hi lo + hi hi, in this order (lo lo is below 2^-22, 2e-8 in the mean): against float64 the results of float32 matrices are
+// about as far off as with torch's float32 products (8192 x 4096: 2.3e-6 of the norm, 3.5e-6 there; 64 x 64: 0.6e-6 to
+// 2.4e-6, 1.0e-6 there).  The first X is u itself times a power of two; what remains of 1 / |u| (a factor from 1 to 2) goes
+// into the first step's sums.  Results in bfloat16 and float16 are the float32 ones rounded.  A single float16 a number (11
+// bits, a third of the products) is not enough for them: a float16 result of 333 x 1234 was off by 1.2e-3 so, six times its
+// rounding, and a bfloat16 one of 8192 x 4096 by 8.5e-4 beside a rounding of 1.7e-3.
 //
 // All matrices of a call share each launch; a table in the workspace, written by a first small kernel from its
 // arguments, tells a workgroup its matrix and tile.  Matrices with a side of at most 128 whose X and A fit LDS take one
@@ -135,7 +135,7 @@ __device__ __forceinline__ void by_type(int dtype, F f) {
 }
 
 // Momenta, and a partial sum of squares for each chunk of a matrix (float64: squares of any float32).  Bound by bytes: a
-// stack of 64 bfloat16 matrices of 512 x 1024, 65 us for 336 MB.
+// stack of 64 bfloat16 matrices of 512 x 1024, 65 us for 336 MB (5.2 TB/s).
 __global__ void __launch_bounds__(256) k_muon_momentum(const Mat* __restrict__ table, int count, Momentum h,
                                                        double* __restrict__ partial) {
     const uint32_t unit = blockIdx.x;
@@ -577,9 +577,9 @@ struct SmallList {
 static_assert(sizeof(SmallList) + sizeof(Steps) <= 3840, "4 KB of arguments");
 
 // A whole matrix in one workgroup, from its gradient to its parameters: X and A (then B) stay in LDS, and one launch does
-// what takes 19 with tiles.  One float32 matrix of 128 x 128 takes 63 us so and 71 with tiles, 64 x 64 33 and 71; 300 of
-// 128 x 128 134 and 252.  It is bound by latency: about 11 us a step at 128 x 128 in pairs, products that depend on the
-// last ones with two wavefronts a SIMD.
+// what takes 19 with tiles.  One matrix of 128 x 128 takes 61 us so and 74 with tiles, 64 x 64 30 and 74; 300 of 128 x 128
+// 123 and 269.  It is bound by latency: about 11 us a step at 128 x 128, products that depend on the last ones with two
+// wavefronts a SIMD.
 //
 // Eight wavefronts share the blocks of 32 x 32 of A and B on and below the diagonal, and the columns of X, 32 at a time:
 // such columns of a X + B X read nothing of X but these columns, so they are replaced in place.  Sums of hi hi and of the
@@ -958,7 +958,7 @@ double cost(const std::vector<Mat>& mats, int kind, int tile) {
 }
 
 // Whether one workgroup takes a whole matrix (at most LDS holds: 128 x 128 or 64 x 512).  300 matrices of 32 x 256 take
-// 63 us so and 298 with tiles.
+// 59 us so and 298 with tiles.
 inline bool is_small(int64_t rows, int64_t cols) {
     return std::min(rows, cols) <= kSmallSide && std::max(rows, cols) <= 4096 &&
            small_bytes(std::min(rows, cols), std::max(rows, cols)) <= kSmallLds[1];

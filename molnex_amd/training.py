@@ -276,8 +276,9 @@ def orthogonalize(x: Tensor, *, steps: int = 5, coefficients=NEWTON_SCHULZ, eps:
     1.2, those that began below 0.002 excepted).  A matrix of zeros stays so; one with an infinite or NaN entry becomes
     NaN; coefficients under which the iteration grows past 64 are refused.
 
-    float32, bfloat16 or float16.  All are iterated in pairs of scaled float16 (22 bits, as exact in the mean as float32's
-    24) with float32 sums, and 16-bit results are the float32 ones rounded.  Not differentiable.  GPU tensors only."""
+    float32, bfloat16 or float16.  All are iterated in pairs of scaled float16 (22 bits) with float32 sums, and 16-bit
+    results are the float32 ones rounded; these are off by 1e-6 to 3e-6 of their norm, as with float32 products.  Not
+    differentiable.  GPU tensors only."""
     a, b, c = coefficients
     if torch.compiler.is_compiling():
         return torch.ops.molix.orthogonalize(x, steps, a, b, c, eps)
