@@ -339,7 +339,7 @@ __device__ __forceinline__ void put8(_Float16* to, const float (&v)[8]) {
 // and columns of the result that are not stored) and stores none of that.
 //
 // Tiles of 256, one a CU, are bound by the matrix cores (a matrix of 8192 x 4096: 640 us for the three products of B X, 1.29
-// PFLOP/s, 5.9 ms in all; a large library product of as many numbers reaches 1.41 here); those of 192 (366 us for A) and
+// PFLOP/s, 5.8 ms in all; a large library product of as many numbers reaches 1.41 here); those of 192 (366 us for A) and
 // 128 by their reads of LDS.  Where a call has fewer tiles than CUs, tiles of 64 and the six chunks they have on their way,
 // 6 to 12 us a launch, 15 launches one after the other.
 template <int MODE, int BT>
