@@ -23,8 +23,8 @@ def indexed_linear(x: Tensor, weight: Tensor, index: Tensor | None = None,
     not read then and may be left out.  float32, bfloat16 or float16, the same for both; sums are float32.  Products of
     float32 values x w are exact to 6 2^-24 |x w|, and where a value is below 2^-109 (1.5e-33) to 2^-133 (|x| + |w|) more;
     few rows (some hundreds of workgroups' worth) are multiplied in float32 itself.  Infinities and NaN do what they do in
-    float32 operations.  Differentiable in backward mode to any order; the weights' gradient is summed in a fixed order.  Nothing synchronises.  Under autocast both go
-    to its type, as for a matrix product."""
+    float32 operations.  Differentiable in backward mode to any order; the weights' gradient is summed in a fixed order.
+    Nothing synchronises.  Under autocast both go to its type, as for a matrix product."""
     order, starts = (None, None) if groups is None else groups
     compiling = torch.compiler.is_compiling()
     if not compiling and has_torch_function_variadic(x, weight, index, order, starts):

@@ -11,17 +11,17 @@ from ...training import MUON_MAX_SIDE, NEWTON_SCHULZ, muon_step
 class Muon(torch.optim.Optimizer):
     """Muon for the matrices of a model on the GPU, with the arguments of ``torch.optim.Muon``.  A parameter of more than
     two axes is a stack of matrices (``nn.IndexedLinear``'s weight: one a class).  Vectors and embeddings belong to another
-    optimizer (``AdamW``), and so do weights that hold several matrices in one row, (1, n) or (classes, n), as those of
-    the equivariant ``Linear`` and of ``ElementUpdate`` do: such a row is one matrix here, and is only normalised.
-    Sides are at most 65536.
+    optimizer (``AdamW``), and so do weights that hold several matrices in one row, as those of the equivariant
+    ``Linear``, (1, n), and of ``ElementUpdate``, (classes, n): the first are only normalised here, the others' rows made
+    orthogonal to each other.  Sides are at most 65536.
 
     ``adjust_lr_fn`` takes a weight's rows for its outputs, as ``torch.nn.Linear`` has them: "original" raises the rate by
     sqrt(rows / columns) where there are more rows.  ``nn.IndexedLinear``'s matrices are (in, out), so it raises that of
     layers that narrow; "match_rms_adamw" is the same for both.
 
     Momenta are float32 whatever the parameters' type, and so are the updates, orthogonalised as ``molix.F.orthogonalize``
-    does it; only the new parameters are rounded to their type.  ``lr`` may be a tensor on the device: nothing synchronises, and a
-    step can be captured in a graph once the momenta exist (after a first step)."""
+    does it; only the new parameters are rounded to their type.  ``lr`` may be a tensor on the device: nothing
+    synchronises, and a step can be captured in a graph once the momenta exist (after a first step)."""
 
     def __init__(self, params, lr: float | Tensor = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95,
                  nesterov: bool = True, ns_coefficients: tuple[float, float, float] = NEWTON_SCHULZ, eps: float = 1e-7,
