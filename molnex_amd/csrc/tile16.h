@@ -46,10 +46,15 @@ __device__ __forceinline__ f32x16 mfma(const short8v& a, const short8v& b, const
 // 16 bytes a lane to LDS, lane by lane from `to` on (M0); from base + offset (bytes), or from an address a lane.  In
 // assembly, because for the builtin the compiler waits for every such load before the next read of LDS, also of other
 // memory there.  The caller waits (vmcnt) and has a barrier before anyone reads what has come, and before it ends.
+//
+// A load must not begin within five wait states of a vector instruction's write of its scalar base (a lane that was read,
+// say), and the compiler does not look into the statement: the base passes through a scalar move, which waits by itself, and
+// is the state that M0 needs, too.
 __device__ __forceinline__ void load_lds(const void* base, uint32_t offset, void* to) {
     const uint32_t m0 = uint32_t(uintptr_t((__attribute__((address_space(3))) char*)to));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
+    const void* from;
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
+                 : "=&s"(from)
                  : "s"(m0), "v"(offset), "s"(base)
                  : "memory", "m0");
 }
